@@ -268,6 +268,81 @@ int krn_b200_attn_decode_fp8_paged_noalloc(const void* q, const void* k_pages, c
                                            int64_t max_pages_per_seq, int64_t max_context, float scale_log2,
                                            void* stream);
 
+/* ---- The paged 8-bit cache with one scale per (page, kv head): plan, append, attention -------------------------------
+ *
+ * A pool holds e4m3 codes [num_pages, page_size, kv_heads, d] for K and for V (page_size 16, 32, 64, 128 or 256; d
+ * contiguous, the other strides multiples of 16 bytes) and f32 scales [num_pages, kv_heads] for each; a value is code *
+ * scale. A token's slot is page * page_size + its offset in the page. The three entries are the cache's part of a serving
+ * step: the plan takes pages for the tokens that arrive, the append writes them, attention reads the cache. None of
+ * them has a counterpart in the reference (roadmap item "Paged attention"); codes are rounded by its narrowing rule, nearest
+ * even and saturating (src/krn/compiler/narrow.py:94-105). */
+
+/* Entries a run list needs for `rows` rows of `batch` requests: min(rows, rows / page_size + 2 * batch). */
+int64_t krn_b200_cache_runs(int64_t rows, int64_t batch, int64_t page_size);
+
+/* Block tables and slot maps of a step, from request lengths alone.
+ *   context_len  int32 [batch]: tokens each request holds; clamped into [0, max_pages * page_size]
+ *   new_len      int32 [batch]: tokens it brings (0: none), < 0: it is finished and gives its pages back
+ *   page_table   int32 [batch, max_pages], row pitch table_pitch: entries of pages taken are WRITTEN, others left alone
+ *   free_pages   int32 [capacity]: ring of free page ids; the live ones are positions taken, ..., given - 1, modulo the
+ *                capacity. Pages given back are WRITTEN behind them and handed out from the next step on
+ *   pool_state   int64 [3]: taken, given (pages ever taken from and given to the ring), third word not read
+ *   context_out  int32 [batch]: context_len + new_len; 0 for a finished request
+ *   row_start    int32 [batch + 1]: first row of each request in the step's packed rows
+ *   slot_map     int64 [rows]: the slot of every row; -1 behind the last request
+ *   runs         int32 [runs_len], runs_len >= krn_b200_cache_runs(...): the rows where a page's run of new tokens begins,
+ *                in order, then -1
+ *   state_out    int64 [3]: the new taken, given, and what was refused
+ * A step that asks for more pages than are free, for more table entries than a row has or for more rows than slot_map
+ * holds is refused whole: state_out[2] has bit 0 set, nothing is taken, row_start and the contexts are those of a step
+ * without new tokens; finished requests still give their pages back. Bit 1: more pages came back than the ring has room
+ * for (a page was given back twice): none was accepted. A page id outside [0, num_pages) gets slot -1, and the status word
+ * reports KRN_B200_ERR_DEVICE_INDEX. Outputs must not share memory with inputs (page_table and free_pages are both).
+ * batch is at most 8192. */
+int krn_b200_cache_plan(const int32_t* context_len, const int32_t* new_len, int32_t* page_table, int32_t* free_pages,
+                        const int64_t* pool_state, int32_t* context_out, int32_t* row_start, int64_t* slot_map, int32_t* runs,
+                        int64_t* state_out, int64_t batch, int64_t max_pages, int64_t table_pitch, int64_t capacity,
+                        int64_t page_size, int64_t num_pages, int64_t rows, int64_t runs_len, void* stream);
+
+/* Quantise the step's keys and values into the pool.
+ *   k, v         bf16 or f16 (`type`) [rows, kv_heads, d]; *_strides: element strides of rows and heads, multiples of 8
+ *   slot_map, runs  as krn_b200_cache_plan makes them: rows of one page are consecutive, in slot order, and no two runs
+ *                share a page (two that do race on its scale). Rows with slot -1 and runs past the rows are skipped; a slot
+ *                beyond the pool is skipped and reported (KRN_B200_ERR_DEVICE_INDEX)
+ *   *_page_strides  element (= byte) strides of pages, tokens and heads of a pool
+ * For each run and head the page's scale becomes max(scale, least power of two 2^k, k >= -100, with all of the run's finite
+ * magnitudes <= 448 * 2^k); a run that begins at a page's offset 0 ignores the scale the page had. Codes the page holds
+ * already are rounded again to the new scale where it grew. Infinities become +-448 codes and NaN NaN codes; neither has a
+ * say in the scale. */
+int krn_b200_cache_append(int type, const void* k, const void* v, const int64_t* slot_map, const int32_t* runs, void* k_pages,
+                          void* v_pages, float* k_scale, float* v_scale, int64_t rows, int64_t runs_len, int64_t kv_heads,
+                          int64_t d, int64_t page_size, int64_t num_pages, const int64_t* k_strides, const int64_t* v_strides,
+                          const int64_t* k_page_strides, const int64_t* v_page_strides, void* stream);
+
+/* Bytes of caller workspace krn_b200_cache_attn needs for these extents. */
+int64_t krn_b200_cache_attn_workspace_bytes(int64_t batch, int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t d,
+                                            int64_t max_new, int64_t max_context);
+
+/* Attention of packed query rows over the pool: row i of the n rows of a request with a context of c tokens (the new ones
+ * included, already in the cache) stands at position c - n + i and sees keys 0 .. c - n + i.
+ *   q, o         bf16 or f16 (`type`) [rows, q_heads, d]; *_strides: element strides of rows and heads, multiples of 8;
+ *                q_heads % kv_heads == 0, at most 128 q heads per kv head
+ *   row_start    int32 [batch + 1], context_len int32 [batch]: as krn_b200_cache_plan makes them. Contexts are clamped into
+ *                [0, max_context]; rows of o behind row_start[batch] are left as they were; a row that sees no key gets zeros
+ *   max_new      no request has more rows than this; one that has is not computed and reported
+ *                (KRN_B200_ERR_DEVICE_INDEX). It chooses the kernels, as max_context does
+ *   page ids outside [0, num_pages) are never fetched: their tokens read as zeros, and the status word reports
+ *                KRN_B200_ERR_DEVICE_INDEX; entries past a request's context are never looked at
+ *   scale_log2   log2(e) * softmax scale
+ *   workspace    at least krn_b200_cache_attn_workspace_bytes(...) bytes, 16-byte aligned; needs no preparation. Calls that
+ *                may overlap on the GPU need one each */
+int krn_b200_cache_attn(int type, const void* q, const void* k_pages, const void* v_pages, const float* k_scale,
+                        const float* v_scale, const int32_t* page_table, const int32_t* context_len, const int32_t* row_start,
+                        void* o, int64_t batch, int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t d, int64_t page_size,
+                        int64_t num_pages, int64_t max_pages, int64_t table_pitch, int64_t max_new, int64_t max_context,
+                        const int64_t* q_strides, const int64_t* o_strides, const int64_t* k_page_strides,
+                        const int64_t* v_page_strides, float scale_log2, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* Copy this rank's column block C_local[M, n_local] into columns [col0, col0 + n_local) of the row-major
  * C_full[M, N] (ld in elements, elem_bytes 2 or 4). Used after the NCCL all-gather of GEMM output column
  * blocks to lay the gathered slabs out as one row-major matrix. No counterpart in the reference (it has no

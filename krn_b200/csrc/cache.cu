@@ -1,0 +1,543 @@
+// The paged 8-bit cache: the step's plan (block tables and slot maps from request lengths) and the append that quantises
+// new keys and values into pages with one power-of-two scale per (page, kv head).
+//
+// A pool is codes e4m3 [num_pages, page_size, kv_heads, d] for K and for V and f32 scales [num_pages, kv_heads] for each;
+// value = code * scale. A token's slot is page * page_size + offset in the page.
+//
+// The reference has neither (its roadmap lists paged attention); the rounding to e4m3 is its narrowing rule, nearest even
+// and saturating (src/krn/compiler/narrow.py:94-105).
+#include "host.cuh"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+namespace krnb {
+namespace {
+
+constexpr int kErrDeviceIndex = 6;  // mirrors KRN_B200_ERR_DEVICE_INDEX in include/krn_b200.h
+
+enum Site { kSitePlanPage = 41, kSiteAppendSlot = 42 };
+
+// ---- plan ----------------------------------------------------------------------------------------------------------
+
+constexpr int kPlanThreads = 512;
+constexpr int kPlanWarps = kPlanThreads / 32;
+constexpr int kMaxBatch = 8192;             // three prefixes of the batch sit in shared memory
+constexpr uint32_t kSaturated = 1u << 30;   // sums stop here: above every bound they are compared with
+
+struct PlanParams {
+  const int32_t* context_len;  // [batch]
+  const int32_t* new_len;      // [batch], < 0: finished
+  int32_t* page_table;         // [batch, max_pages], new entries are written
+  int32_t* free_pages;         // ring [capacity], pages of finished requests are written
+  const int64_t* pool_state;   // taken, given, -
+  int32_t* context_out;        // [batch]
+  int32_t* row_start;          // [batch + 1]
+  int64_t* slot_map;           // [rows]
+  int32_t* runs;               // [runs_len]
+  int64_t* state_out;          // taken, given, refused
+  int64_t table_pitch;
+  int batch, max_pages, page_shift, rows, runs_len, num_pages, capacity;
+};
+
+__device__ __forceinline__ uint32_t add_saturated(uint32_t a, uint32_t b) { return min(a + b, kSaturated); }
+
+// What one request asks of the step.
+struct Request {
+  int context, rows;         // tokens it holds, rows it brings
+  int have;                  // pages it holds
+  uint32_t need, lead, back; // pages it takes, page runs of its rows, pages it gives back
+  bool wide;                 // its pages would not fit its row of the table
+};
+
+__device__ __forceinline__ Request request_at(const PlanParams& p, int i) {
+  Request r;
+  const int brings = p.new_len[i];
+  const long long most = (long long)p.max_pages << p.page_shift;
+  r.context = int(min((long long)max(p.context_len[i], 0), most));
+  r.rows = min(max(brings, 0), p.rows + 1);  // one more than there is room for is refused all the same
+  const int page = 1 << p.page_shift;
+  const long long length = (long long)r.context + r.rows;
+  const int after = int((length + page - 1) >> p.page_shift);
+  r.have = (r.context + page - 1) >> p.page_shift;
+  r.need = uint32_t(after - r.have);
+  r.lead = r.rows > 0 ? uint32_t(((length - 1) >> p.page_shift) - (r.context >> p.page_shift) + 1) : 0u;
+  r.back = brings < 0 ? uint32_t(r.have) : 0u;
+  r.wide = after > p.max_pages;
+  return r;
+}
+
+// Exclusive prefix of four sums over the block's threads in thread order, on top of `carry`, which moves on by their
+// totals. `scratch` holds 4 * kPlanWarps values.
+__device__ __forceinline__ void block_prefix(uint32_t (&v)[4], uint32_t (&carry)[4], uint32_t* scratch) {
+  const int warp = threadIdx.x >> 5;
+  const uint32_t lane = lane_id();
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t below = __shfl_up_sync(0xffffffffu, v[k], o);
+      if (lane >= uint32_t(o)) v[k] = add_saturated(v[k], below);
+    }
+    if (lane == 31) scratch[k * kPlanWarps + warp] = v[k];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    uint32_t before = carry[k], total = carry[k];
+    for (int w = 0; w < kPlanWarps; ++w) {
+      const uint32_t s = scratch[k * kPlanWarps + w];
+      if (w < warp) before = add_saturated(before, s);
+      total = add_saturated(total, s);
+    }
+    const uint32_t inclusive_before = __shfl_up_sync(0xffffffffu, v[k], 1);
+    v[k] = add_saturated(before, lane == 0 ? 0u : inclusive_before);
+    carry[k] = total;
+  }
+  __syncthreads();  // scratch is free again
+}
+
+// One launch, no communication between blocks: every block scans all request lengths by itself (a few loads per thread)
+// and then fills its own part of the slot map, the run list and the table. Bound by latency: launch, one pass over the
+// lengths, a binary search per row.
+__global__ void __launch_bounds__(kPlanThreads) cache_plan_kernel(PlanParams p, DeviceStatus* status) {
+  extern __shared__ uint32_t plan_smem[];
+  uint32_t* start = plan_smem;                 // [batch + 1] first row of each request
+  uint32_t* first = start + p.batch + 1;       // [batch] first page taken from (finished: given back to) the ring
+  uint32_t* run = first + p.batch;             // [batch] first entry of the run list
+  uint32_t* scratch = run + p.batch;           // [4 * kPlanWarps]
+  const int page = 1 << p.page_shift;
+
+  // totals first: a step that does not fit takes nothing
+  uint32_t carry[4] = {0, 0, 0, 0};
+  bool wide = false;
+  for (int base = 0; base < p.batch; base += kPlanThreads) {
+    const int i = base + int(threadIdx.x);
+    uint32_t v[4] = {0, 0, 0, 0};
+    if (i < p.batch) {
+      const Request r = request_at(p, i);
+      wide |= r.wide;
+      v[0] = uint32_t(r.rows);
+      v[1] = r.need;
+      v[2] = r.lead;
+      v[3] = r.back;
+    }
+    const bool gives = v[3] != 0;
+    block_prefix(v, carry, scratch);
+    if (i < p.batch) {
+      start[i] = v[0];
+      first[i] = gives ? v[3] : v[1];
+      run[i] = v[2];
+    }
+  }
+  const long long taken = p.pool_state[0], given = p.pool_state[1];
+  const long long available = max(0ll, min(given - taken, (long long)p.capacity));
+  const bool any_wide = __syncthreads_or(wide) != 0;
+  const bool refused = any_wide || carry[0] > uint32_t(p.rows) || (long long)carry[1] > available;
+  const bool overfull = available + carry[3] > p.capacity;  // pages given back that the ring has no room for
+  const uint32_t rows = refused ? 0u : carry[0], runs = refused ? 0u : carry[2];
+  if (threadIdx.x == 0) start[p.batch] = rows;
+  __syncthreads();
+
+  const int here = blockIdx.x * kPlanThreads + threadIdx.x, stride = gridDim.x * kPlanThreads;
+  if (here == 0) {
+    p.state_out[0] = taken + (refused ? 0u : carry[1]);
+    p.state_out[1] = given + (overfull ? 0u : carry[3]);
+    p.state_out[2] = (refused ? 1 : 0) | (overfull ? 2 : 0);
+  }
+  for (int i = here; i <= p.batch; i += stride) {
+    p.row_start[i] = refused ? 0 : int(start[i]);
+    if (i < p.batch) {
+      const Request r = request_at(p, i);
+      p.context_out[i] = p.new_len[i] < 0 ? (overfull ? r.context : 0) : r.context + (refused ? 0 : r.rows);
+    }
+  }
+  for (int i = here; i < p.runs_len; i += stride) {
+    if (i >= int(runs)) p.runs[i] = -1;
+  }
+
+  // rows: request by binary search, page from the table or from the ring
+  const long long taken_at = ((taken % p.capacity) + p.capacity) % p.capacity;
+  const long long given_at = ((given % p.capacity) + p.capacity) % p.capacity;
+  for (int r = here; r < p.rows; r += stride) {
+    if (r >= int(rows)) {
+      p.slot_map[r] = -1;
+      continue;
+    }
+    int low = 0, high = p.batch;  // the last request that starts at or before r and is not empty
+    while (high - low > 1) {
+      const int mid = (low + high) >> 1;
+      if (start[mid] <= uint32_t(r)) low = mid; else high = mid;
+    }
+    const long long most = (long long)p.max_pages << p.page_shift;
+    const int context = int(min((long long)max(p.context_len[low], 0), most));
+    const int have = (context + page - 1) >> p.page_shift;
+    const int pos = context + r - int(start[low]);
+    const int at = pos >> p.page_shift;
+    int id;
+    if (at < have) {
+      id = p.page_table[low * p.table_pitch + at];
+    } else {
+      long long spot = taken_at + first[low] + (at - have);
+      if (spot >= p.capacity) spot -= p.capacity;
+      id = p.free_pages[spot];
+    }
+    const bool lead = r == int(start[low]) || (pos & (page - 1)) == 0;
+    if (lead) {
+      const int entry = int(run[low]) + at - (context >> p.page_shift);
+      if (entry < p.runs_len) p.runs[entry] = r;
+      if (at >= have) p.page_table[low * p.table_pitch + at] = id;
+    }
+    const bool good = uint32_t(id) < uint32_t(p.num_pages);
+    if (!good) report_failure(status, kErrDeviceIndex, kSitePlanPage, uint32_t(id) & 0x7fffffffu);
+    p.slot_map[r] = good ? ((long long)id << p.page_shift) + (pos & (page - 1)) : -1;
+  }
+
+  // pages of finished requests, a warp each: handed out from the next step on
+  if (!overfull) {
+    for (int i = here >> 5; i < p.batch; i += stride >> 5) {
+      if (p.new_len[i] >= 0) continue;
+      const Request r = request_at(p, i);
+      for (int j = int(lane_id()); j < r.have; j += 32) {
+        long long spot = given_at + first[i] + j;
+        if (spot >= p.capacity) spot -= p.capacity;
+        p.free_pages[spot] = p.page_table[i * p.table_pitch + j];
+      }
+    }
+  }
+}
+
+size_t plan_smem_bytes(int64_t batch) { return size_t(3 * batch + 1 + 4 * kPlanWarps) * 4; }
+
+// ---- append ----------------------------------------------------------------------------------------------------------
+
+constexpr int kLeastExponent = -100;  // of a page's scale: a page of zeros, and of values that e4m3 * 2^-100 cannot tell from it
+
+struct AppendSide {
+  const uint16_t* x;   // [rows, heads, d] bf16 or f16
+  long long x_row, x_head;
+  uint8_t* pages;      // [num_pages, page_size, heads, d]
+  long long page_pitch, token_pitch, head_pitch;
+  float* scale;        // [num_pages, heads]
+};
+
+struct AppendParams {
+  AppendSide side[2];      // K, V
+  const int64_t* slot_map; // [rows]
+  const int32_t* runs;     // [runs_len]
+  int rows, runs_len, heads, page_shift, num_pages;
+};
+
+template <bool BF16>
+__device__ __forceinline__ float2 unpack(uint32_t w) {
+  if constexpr (BF16) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  } else {
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  }
+}
+
+// |x|, or 0 where x is not finite: infinities and NaN have no say in a page's scale.
+__device__ __forceinline__ float finite_size(float x) {
+  const float a = fabsf(x);
+  return a <= 3.4028234663852886e38f ? a : 0.f;
+}
+
+// The least power of two 2^k, k >= kLeastExponent, with a <= 448 * 2^k, read off a's exponent: 448 = 1.75 * 2^8.
+__device__ __forceinline__ float scale_of(float a) {
+  const uint32_t bits = __float_as_uint(a);
+  int k = int(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+  k = max(k, kLeastExponent);
+  return __uint_as_float(uint32_t(k + 127) << 23);
+}
+
+// Two values over `scale` to e4m3, nearest even, saturated; infinities become +-448, NaN stays NaN. Multiplying by the
+// reciprocal of a power of two is the division itself; a page that some other program filled may have any scale.
+struct Divisor {
+  float scale, inverse;
+  bool exact;
+  __device__ __forceinline__ uint32_t two(float2 v) const {
+    const float a = exact ? v.x * inverse : v.x / scale, b = exact ? v.y * inverse : v.y / scale;
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(b), "f"(a));
+    return r;
+  }
+};
+
+__device__ __forceinline__ uint32_t rescale_two(uint32_t codes, float ratio) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(uint16_t(codes)));
+  const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h));
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(v.y * ratio), "f"(v.x * ratio));
+  return r;
+}
+
+struct Run {
+  int row, count, offset, page;
+};
+
+// Entry `u` of the run list: rows [row, row + count) fill slots `offset`, ... of `page`. False where there is none.
+__device__ __forceinline__ bool run_at(const AppendParams& p, int u, Run& run, DeviceStatus* status) {
+  const int row = p.runs[u];
+  if (uint32_t(row) >= uint32_t(p.rows)) return false;
+  const long long slot = p.slot_map[row];
+  if (slot < 0) return false;
+  const long long page = slot >> p.page_shift;
+  if (page >= p.num_pages) {
+    report_failure(status, kErrDeviceIndex, kSiteAppendSlot, uint32_t(row));
+    return false;
+  }
+  run.row = row;
+  run.page = int(page);
+  run.offset = int(slot & ((1 << p.page_shift) - 1));
+  const int most = min((1 << p.page_shift) - run.offset, p.rows - row);
+  int count = 1;
+  for (int base = 0; base < most; base += 32) {
+    const int i = base + int(lane_id());
+    const bool same = i < most && p.slot_map[row + i] == slot + i;
+    const uint32_t mask = __ballot_sync(0xffffffffu, same);
+    if (mask != 0xffffffffu) {
+      count = base + __ffs(int(~mask)) - 1;
+      break;
+    }
+    count = base + 32;
+  }
+  run.count = min(count, most);
+  return true;
+}
+
+// A thread group of `Threads` owns one (run, kv head, K or V): no two groups share a page's scale, so the new scale, the
+// page's old codes and its new ones are settled without atomics, and the result does not depend on any order.
+//   1. the group reads its rows once (16 bytes a thread and pass; up to kHeld passes stay in registers) and takes the
+//      largest finite magnitude;
+//   2. scale = max(old, least power of two that fits); a run that begins a page ignores what the page held;
+//   3. where the scale grew, the codes already in the page are brought to it (a power-of-two ratio: only what falls below
+//      e4m3's normal range is rounded again);
+//   4. the rows go out as codes, 8 bytes a thread.
+// Bound by HBM for prompts (2 bytes in, 1 out per value) and by launch and load latency for single tokens.
+constexpr int kHeld = 8;
+
+template <int D, bool BF16, int Threads>
+__global__ void __launch_bounds__(128) cache_append_kernel(AppendParams p, DeviceStatus* status) {
+  constexpr int kLanes = D / 8;                // threads per row
+  constexpr int kRows = Threads / kLanes;      // rows per pass
+  constexpr int kGroups = 128 / Threads;       // (run, head, side) items per block
+  __shared__ float peak[4];
+  const int tid = threadIdx.x % Threads;
+  const long long item = (long long)blockIdx.x * kGroups + threadIdx.x / Threads;
+  const int per_run = 2 * p.heads;
+  const int u = int(item / per_run), which = int(item % per_run);
+  if (u >= p.runs_len) return;
+  Run run;
+  if (!run_at(p, u, run, status)) return;
+  const AppendSide& side = p.side[which >= p.heads ? 1 : 0];
+  const int head = which >= p.heads ? which - p.heads : which;
+  const int lane = tid % kLanes, row0 = tid / kLanes;
+  const uint16_t* x = side.x + (long long)run.row * side.x_row + head * side.x_head + lane * 8;
+
+  uint4 held[kHeld];
+  float a = 0.f;
+  auto take = [&](const uint4& w) {
+    const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 v = unpack<BF16>(words[e]);
+      a = fmaxf(a, fmaxf(finite_size(v.x), finite_size(v.y)));
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    const int row = row0 + i * kRows;
+    held[i] = make_uint4(0, 0, 0, 0);
+    if (row < run.count) held[i] = *reinterpret_cast<const uint4*>(x + row * side.x_row);
+  }
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) take(held[i]);
+  for (int row = row0 + kHeld * kRows; row < run.count; row += kRows) take(*reinterpret_cast<const uint4*>(x + row * side.x_row));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+  if constexpr (Threads > 32) {
+    if (lane_id() == 0) peak[threadIdx.x >> 5] = a;
+    __syncthreads();
+    a = fmaxf(fmaxf(peak[0], peak[1]), fmaxf(peak[2], peak[3]));
+  }
+
+  float* at = side.scale + (long long)run.page * p.heads + head;
+  const float old = run.offset > 0 ? *at : 0.f;
+  const float now = fmaxf(old, scale_of(a));
+  uint8_t* page = side.pages + run.page * side.page_pitch + head * side.head_pitch;
+  if (now != old && run.offset > 0) {
+    const float ratio = old / now;
+    for (int i = tid; i < run.offset * (D / 16); i += Threads) {
+      uint4* spot = reinterpret_cast<uint4*>(page + (i / (D / 16)) * side.token_pitch + (i % (D / 16)) * 16);
+      uint4 w = *spot;
+      w.x = rescale_two(w.x, ratio) | rescale_two(w.x >> 16, ratio) << 16;
+      w.y = rescale_two(w.y, ratio) | rescale_two(w.y >> 16, ratio) << 16;
+      w.z = rescale_two(w.z, ratio) | rescale_two(w.z >> 16, ratio) << 16;
+      w.w = rescale_two(w.w, ratio) | rescale_two(w.w >> 16, ratio) << 16;
+      *spot = w;
+    }
+  }
+  const Divisor by = {now, 1.0f / now, (__float_as_uint(now) & 0x7fffffu) == 0};
+  auto put = [&](const uint4& w, int row) {
+    uint2 codes;
+    codes.x = by.two(unpack<BF16>(w.x)) | by.two(unpack<BF16>(w.y)) << 16;
+    codes.y = by.two(unpack<BF16>(w.z)) | by.two(unpack<BF16>(w.w)) << 16;
+    *reinterpret_cast<uint2*>(page + (run.offset + row) * side.token_pitch + lane * 8) = codes;
+  };
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    const int row = row0 + i * kRows;
+    if (row < run.count) put(held[i], row);
+  }
+  for (int row = row0 + kHeld * kRows; row < run.count; row += kRows) put(*reinterpret_cast<const uint4*>(x + row * side.x_row), row);
+  // every thread has read the old scale before it is replaced
+  if constexpr (Threads > 32) __syncthreads(); else __syncwarp();
+  if (tid == 0 && now != old) *at = now;
+}
+
+template <int D, bool BF16, int Threads>
+int launch_append(const AppendParams& p, DeviceStatus* status, cudaStream_t stream) {
+  const long long items = (long long)p.runs_len * 2 * p.heads;
+  const long long blocks = (items + 128 / Threads - 1) / (128 / Threads);
+  cache_append_kernel<D, BF16, Threads><<<unsigned(blocks), 128, 0, stream>>>(p, status);
+  KRNB_CUDA(cudaGetLastError());
+  return KRN_B200_OK;
+}
+
+bool page_size_ok(int64_t page_size) { return page_size >= 16 && page_size <= 256 && (page_size & (page_size - 1)) == 0; }
+
+int shift_of(int64_t page_size) {
+  int s = 0;
+  while ((int64_t(1) << s) < page_size) ++s;
+  return s;
+}
+
+}  // namespace
+}  // namespace krnb
+
+extern "C" int64_t krn_b200_cache_runs(int64_t rows, int64_t batch, int64_t page_size) {
+  if (rows <= 0 || batch <= 0 || page_size <= 0) return 0;
+  // a request of n rows touches at most (n + page_size - 2) / page_size + 1 pages, and at most n
+  const int64_t bound = rows / page_size + 2 * batch;
+  return rows < bound ? rows : bound;
+}
+
+extern "C" int krn_b200_cache_plan(const int32_t* context_len, const int32_t* new_len, int32_t* page_table,
+                                   int32_t* free_pages, const int64_t* pool_state, int32_t* context_out, int32_t* row_start,
+                                   int64_t* slot_map, int32_t* runs, int64_t* state_out, int64_t batch, int64_t max_pages,
+                                   int64_t table_pitch, int64_t capacity, int64_t page_size, int64_t num_pages, int64_t rows,
+                                   int64_t runs_len, void* stream_handle) {
+  using namespace krnb;
+  if (!page_size_ok(page_size)) {
+    return fail(KRN_B200_ERR_UNSUPPORTED, "page size %lld is not available on sm_100a: pages are 16, 32, 64, 128 or 256 tokens. "
+                "Instead: use one of them", (long long)page_size);
+  }
+  if (batch < 0 || max_pages <= 0 || capacity <= 0 || num_pages <= 0 || rows < 0 || table_pitch < max_pages) {
+    return fail(KRN_B200_ERR_INVALID_ARGUMENT, "bad extents (batch %lld, %lld table entries at pitch %lld, ring of %lld, %lld "
+                "pages, %lld rows)", (long long)batch, (long long)max_pages, (long long)table_pitch, (long long)capacity,
+                (long long)num_pages, (long long)rows);
+  }
+  if (batch > kMaxBatch) {
+    return fail(KRN_B200_ERR_UNSUPPORTED, "a plan for %lld requests is not available: their prefix sums sit in shared memory, "
+                "at most %d fit. Instead: plan the batch in parts", (long long)batch, kMaxBatch);
+  }
+  if (rows >= int64_t(kSaturated) || capacity >= int64_t(kSaturated) || num_pages >= INT32_MAX ||
+      max_pages * page_size >= int64_t(kSaturated)) {
+    return fail(KRN_B200_ERR_UNSUPPORTED, "extents too large for this kernel's 32-bit sums");
+  }
+  if (runs_len < krn_b200_cache_runs(rows, batch, page_size) || runs_len > INT32_MAX) {
+    return fail(KRN_B200_ERR_INVALID_ARGUMENT, "a run list of %lld entries is too short: %lld needed", (long long)runs_len,
+                (long long)krn_b200_cache_runs(rows, batch, page_size));
+  }
+  if (batch == 0) return fail(KRN_B200_ERR_INVALID_ARGUMENT, "a plan needs at least one request");
+  if (context_len == nullptr || new_len == nullptr || page_table == nullptr || free_pages == nullptr || pool_state == nullptr ||
+      context_out == nullptr || row_start == nullptr || state_out == nullptr || (rows > 0 && slot_map == nullptr) ||
+      (runs_len > 0 && runs == nullptr)) {
+    return fail(KRN_B200_ERR_INVALID_ARGUMENT, "null tensor address");
+  }
+  if (context_out == context_len || context_out == new_len || state_out == pool_state) {
+    return fail(KRN_B200_ERR_INVALID_ARGUMENT, "the plan's outputs must not share memory with its inputs: blocks read the "
+                "lengths while others write");
+  }
+  DeviceContext* ctx = current_context();
+  if (ctx == nullptr) return KRN_B200_ERR_CUDA;
+  if (int rc = require_sm100(ctx)) return rc;
+  PlanParams p = {context_len, new_len, page_table, free_pages, pool_state, context_out, row_start, slot_map, runs, state_out,
+                  table_pitch, int(batch), int(max_pages), shift_of(page_size), int(rows), int(runs_len), int(num_pages),
+                  int(capacity)};
+  const size_t smem = plan_smem_bytes(batch);
+  KRNB_CUDA(cudaFuncSetAttribute(cache_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(plan_smem_bytes(kMaxBatch))));
+  const int64_t wanted = (rows + kPlanThreads - 1) / kPlanThreads;
+  const int blocks = int(wanted < 1 ? 1 : wanted > ctx->sm_count ? ctx->sm_count : wanted);
+  cache_plan_kernel<<<blocks, kPlanThreads, smem, static_cast<cudaStream_t>(stream_handle)>>>(p, ctx->status_dev);
+  KRNB_CUDA(cudaGetLastError());
+  return KRN_B200_OK;
+}
+
+extern "C" int krn_b200_cache_append(int type, const void* k, const void* v, const int64_t* slot_map, const int32_t* runs,
+                                     void* k_pages, void* v_pages, float* k_scale, float* v_scale, int64_t rows,
+                                     int64_t runs_len, int64_t heads, int64_t d, int64_t page_size, int64_t num_pages,
+                                     const int64_t* k_strides, const int64_t* v_strides, const int64_t* k_page_strides,
+                                     const int64_t* v_page_strides, void* stream_handle) {
+  using namespace krnb;
+  if (type != KRN_B200_BF16 && type != KRN_B200_F16) {
+    return fail(KRN_B200_ERR_UNSUPPORTED, "cache append of element type %d is not available on sm_100a: keys and values come in "
+                "16 bits. Instead: pass bf16 or f16 tensors", type);
+  }
+  if (d != 64 && d != 128) {
+    return fail(KRN_B200_ERR_UNSUPPORTED, "head dimension %lld is not available on sm_100a. Instead: use d = 64 or d = 128",
+                (long long)d);
+  }
+  if (!page_size_ok(page_size)) {
+    return fail(KRN_B200_ERR_UNSUPPORTED, "page size %lld is not available on sm_100a: pages are 16, 32, 64, 128 or 256 tokens. "
+                "Instead: use one of them", (long long)page_size);
+  }
+  if (rows < 0 || runs_len < 0 || heads <= 0 || num_pages <= 0) {
+    return fail(KRN_B200_ERR_INVALID_ARGUMENT, "bad extents (%lld rows, %lld runs, %lld heads, %lld pages)", (long long)rows,
+                (long long)runs_len, (long long)heads, (long long)num_pages);
+  }
+  if (rows == 0 || runs_len == 0) return KRN_B200_OK;
+  if (rows > INT32_MAX / 2 || num_pages >= INT32_MAX || heads > 65535 || runs_len * 2 * heads > INT32_MAX) {
+    return fail(KRN_B200_ERR_UNSUPPORTED, "extents too large for this kernel's 32-bit indices");
+  }
+  if (k == nullptr || v == nullptr || slot_map == nullptr || runs == nullptr || k_pages == nullptr || v_pages == nullptr ||
+      k_scale == nullptr || v_scale == nullptr || k_strides == nullptr || v_strides == nullptr || k_page_strides == nullptr ||
+      v_page_strides == nullptr) {
+    return fail(KRN_B200_ERR_INVALID_ARGUMENT, "null tensor address");
+  }
+  if (!aligned16(k) || !aligned16(v) || !aligned16(k_pages) || !aligned16(v_pages) || k_strides[0] % 8 || k_strides[1] % 8 ||
+      v_strides[0] % 8 || v_strides[1] % 8) {
+    return fail(KRN_B200_ERR_INVALID_ARGUMENT, "rows are read 16 bytes at a time: addresses and strides must be multiples of 16 bytes");
+  }
+  for (int i = 0; i < 3; ++i) {
+    if (k_page_strides[i] % 16 || v_page_strides[i] % 16 || k_page_strides[i] <= 0 || v_page_strides[i] <= 0) {
+      return fail(KRN_B200_ERR_INVALID_ARGUMENT, "the strides of a page pool must be positive multiples of 16 bytes");
+    }
+  }
+  DeviceContext* ctx = current_context();
+  if (ctx == nullptr) return KRN_B200_ERR_CUDA;
+  if (int rc = require_sm100(ctx)) return rc;
+  AppendParams p;
+  p.side[0] = {static_cast<const uint16_t*>(k), k_strides[0], k_strides[1], static_cast<uint8_t*>(k_pages), k_page_strides[0],
+               k_page_strides[1], k_page_strides[2], k_scale};
+  p.side[1] = {static_cast<const uint16_t*>(v), v_strides[0], v_strides[1], static_cast<uint8_t*>(v_pages), v_page_strides[0],
+               v_page_strides[1], v_page_strides[2], v_scale};
+  p.slot_map = slot_map;
+  p.runs = runs;
+  p.rows = int(rows);
+  p.runs_len = int(runs_len);
+  p.heads = int(heads);
+  p.page_shift = shift_of(page_size);
+  p.num_pages = int(num_pages);
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_handle);
+  const bool bf16 = type == KRN_B200_BF16;
+  // a warp per (run, head) where runs hold a few rows, a block where they are whole pages
+  if (rows < 4 * runs_len) {
+    if (d == 128) return bf16 ? launch_append<128, true, 32>(p, ctx->status_dev, stream) : launch_append<128, false, 32>(p, ctx->status_dev, stream);
+    return bf16 ? launch_append<64, true, 32>(p, ctx->status_dev, stream) : launch_append<64, false, 32>(p, ctx->status_dev, stream);
+  }
+  if (d == 128) return bf16 ? launch_append<128, true, 128>(p, ctx->status_dev, stream) : launch_append<128, false, 128>(p, ctx->status_dev, stream);
+  return bf16 ? launch_append<64, true, 128>(p, ctx->status_dev, stream) : launch_append<64, false, 128>(p, ctx->status_dev, stream);
+}

@@ -223,5 +223,113 @@ def decode_attention(q: Any, k_pages: Any, v_pages: Any, page_table: Any, contex
     return out
 
 
-__all__ = ["DeviceTensor", "QMatrix", "attention", "decode_attention", "decode_attention_workspace", "matmul", "matmul_fp8_blockscaled",
-           "matmul_nt", "matmul_q", "quantize", "quantize_host"]
+@dataclass(frozen=True)
+class PagedCache:
+    """A paged 8-bit key/value cache on the device: e4m3 codes [pages, page size, kv heads, d] and one f32 scale per
+    (page, kv head), for keys and for values; a value is code * scale. Pages are 16, 32, 64, 128 or 256 tokens, d is 64 or
+    128. The d axis is contiguous; the other strides are free (multiples of 16 bytes), so the two pools may be halves of one
+    allocation or kept head by head."""
+
+    k_pages: Any
+    v_pages: Any
+    k_scale: Any
+    v_scale: Any
+
+    @property
+    def page_size(self) -> int:
+        return self.k_pages.shape[1]
+
+    @property
+    def num_pages(self) -> int:
+        return self.k_pages.shape[0]
+
+
+def paged_cache(num_pages: int, page_size: int, kv_heads: int, d: int, device: Any = None) -> PagedCache:
+    """An empty cache on `device` (a torch device; default: the current one)."""
+    import torch
+
+    device = torch.device("cuda", torch.cuda.current_device()) if device is None else device
+    codes = [torch.zeros((num_pages, page_size, kv_heads, d), dtype=torch.uint8, device=device) for _ in range(2)]
+    scales = [torch.zeros((num_pages, kv_heads), dtype=torch.float32, device=device) for _ in range(2)]
+    return PagedCache(*codes, *scales)
+
+
+@dataclass(frozen=True)
+class CachePlan:
+    """What `plan_cache` says of a step: the requests' new contexts (int32 [batch]), the first row of each request in the
+    step's packed rows (int32 [batch + 1]), the slot of every row (int64 [rows], page * page size + offset; -1 behind the
+    last request), the rows where a page's run of new tokens begins (int32, -1 behind the last) and the pool's state
+    (int64 [3]: pages ever taken, ever given, what was refused: 1 = the step did not fit and nothing was taken, 2 = pages
+    came back that the ring has no room for)."""
+
+    context_len: Any
+    row_start: Any
+    slot_map: Any
+    runs: Any
+    pool_state: Any
+
+
+def cache_plan(batch: int, rows: int, page_size: int, device: Any = None) -> CachePlan:
+    """Memory for the plans of steps of `batch` requests with at most `rows` new tokens together."""
+    import torch
+
+    device = torch.device("cuda", torch.cuda.current_device()) if device is None else device
+
+    def empty(n: int, dtype: Any) -> Any:
+        return torch.empty(n, dtype=dtype, device=device)
+
+    return CachePlan(empty(batch, torch.int32), empty(batch + 1, torch.int32), empty(rows, torch.int64),
+                     empty(calls.cache_runs(rows, batch, page_size), torch.int32), empty(3, torch.int64))
+
+
+def plan_cache(context_len: Any, new_len: Any, page_table: Any, free_pages: Any, pool_state: Any, plan: CachePlan, *,
+               page_size: int, num_pages: int, stream: Any = None) -> CachePlan:
+    """Plan a step on the GPU from request lengths: `new_len[b] >= 0` tokens arrive for request b, which holds
+    `context_len[b]`; `new_len[b] < 0` says that it is finished. Pages are taken in order from the ring `free_pages`, whose
+    live entries are positions `pool_state[0]` to `pool_state[1]` (modulo its length), and written into `page_table`
+    [batch, entries]; the pages of finished requests go back to the ring's end and are handed out from the next step on.
+    Fills `plan`, whose `context_len` and `pool_state` are the next step's inputs (with another plan: outputs never share
+    memory with inputs). A step that does not fit is refused whole: `plan.pool_state[2]` is then not 0 and no row has a
+    slot."""
+    calls.cache_plan(_raw(context_len), _raw(new_len), _raw(page_table), _raw(free_pages), _raw(pool_state),
+                     _raw(plan.context_len), _raw(plan.row_start), _raw(plan.slot_map), _raw(plan.runs), _raw(plan.pool_state),
+                     page_size, num_pages, _stream(stream))
+    return plan
+
+
+def append_cache(k: Any, v: Any, slot_map: Any, runs: Any, cache: PagedCache, stream: Any = None) -> PagedCache:
+    """Quantise the step's keys and values [rows, kv heads, d] (bf16 or f16) into the cache at the plan's `slot_map` and
+    `runs`. A page's scale is a power of two, the least that holds its largest finite magnitude within e4m3's 448, and only
+    grows while the page fills: the codes the page holds already are then rounded again to the new scale, which a power of
+    two leaves exact but for values below e4m3's normal range. Rows of one page must be consecutive and in slot order, as
+    `plan_cache` lays them out."""
+    calls.cache_append(_raw(k), _raw(v), _raw(slot_map), _raw(runs), _raw(cache.k_pages), _raw(cache.v_pages),
+                       _raw(cache.k_scale), _raw(cache.v_scale), _stream(stream))
+    return cache
+
+
+def cache_attention_workspace(batch: int, rows: int, q_heads: int, kv_heads: int, d: int, *, max_new: int,
+                              max_context: int) -> int:
+    """Bytes of workspace that `cache_attention` needs for these extents."""
+    return calls.cache_attention_workspace_bytes(batch, rows, q_heads, kv_heads, d, max_new, max_context)
+
+
+def cache_attention(q: Any, cache: PagedCache, page_table: Any, context_len: Any, row_start: Any, out: Any, *, max_new: int,
+                    max_context: int, workspace: Any, scale: float | None = None, stream: Any = None) -> Any:
+    """Attention of packed query rows [rows, q heads, d] (bf16 or f16) over the cache: row i of the n rows of request b
+    (rows `row_start[b]` to `row_start[b + 1]`) stands at position `context_len[b]` - n + i and sees the keys up to it, its
+    own included: one row a request for plain decoding, a few for drafted tokens, many for a prompt or a chunk of one, mixed
+    in one call. `scale` defaults to 1/sqrt(d). `max_new` is the most rows any request has (one with more is not computed
+    and reported), contexts are clamped to `max_context`. Rows that see no key get zeros; rows behind the last request are
+    left as they were."""
+    d = q.shape[-1]
+    scale = (1.0 / math.sqrt(d)) if scale is None else scale
+    calls.cache_attention(_raw(q), _raw(cache.k_pages), _raw(cache.v_pages), _raw(cache.k_scale), _raw(cache.v_scale),
+                          _raw(page_table), _raw(context_len), _raw(row_start), _raw(out), scale * math.log2(math.e), max_new,
+                          max_context, _raw(workspace), _stream(stream))
+    return out
+
+
+__all__ = ["CachePlan", "DeviceTensor", "PagedCache", "QMatrix", "append_cache", "attention", "cache_attention",
+           "cache_attention_workspace", "cache_plan", "decode_attention", "decode_attention_workspace", "matmul",
+           "matmul_fp8_blockscaled", "matmul_nt", "matmul_q", "paged_cache", "plan_cache", "quantize", "quantize_host"]
