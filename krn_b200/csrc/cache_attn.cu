@@ -15,7 +15,7 @@ namespace {
 
 constexpr int kErrDeviceIndex = 6;  // mirrors KRN_B200_ERR_DEVICE_INDEX in include/krn_b200.h
 
-enum Site { kSitePage = 51, kSiteRows = 52 };
+enum Site { kSitePage = 51, kSiteRows = 52, kSiteTile = 53 };
 
 struct PoolSide {
   const uint8_t* pages;
@@ -32,8 +32,636 @@ struct CacheAttnParams {
   const int32_t* context_len;
   const int32_t* row_start;
   int batch, rows, q_heads, kv_heads, group, page_shift, num_pages, max_new, max_context;
+  int few;  // a request with at most this many rows (new tokens x q heads of a kv head) is streamed, one with more is tiled
   float scale_log2;
 };
+
+template <bool BF16>
+__device__ __forceinline__ float2 unpack(uint32_t w) {
+  if constexpr (BF16) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  } else {
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  }
+}
+
+// ---- few rows: a stream of keys per warp ---------------------------------------------------------------------------------
+
+constexpr int kTile = 32;          // tokens a warp takes at a time
+constexpr int kWarps = 8;
+constexpr int kStages = 3;         // tiles a warp has in flight or in work
+constexpr int kMaxBlocks = 160;    // bounds the workspace; a B200 has 148 SMs
+constexpr int kMaxBatch = 8192;    // tile counts of the batch sit in shared memory
+constexpr float kLeastScale = 7.70371977754894341e-34f;  // 2^-110: value scales below it are held against it
+
+// Partial results of the pieces of split segments, 2 + d floats (m, l, the unnormalised output) for each of `rows`.
+struct StreamParams {
+  CacheAttnParams a;
+  int32_t* tiles;    // [batch + 1] exclusive prefix of the requests' tile counts, written for the join
+  float* partial;
+  int slot_rows;     // rows a partial slot holds
+};
+
+__device__ __forceinline__ uint32_t halves_of(uint32_t codes) {  // two e4m3 codes in the low 16 bits
+  uint32_t h2;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"(uint16_t(codes)));
+  return h2;
+}
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint4 ld_shared_16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+
+__device__ __forceinline__ uint2 ld_shared_8(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+  return v;
+}
+
+__device__ __forceinline__ float ld_shared_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+  return v;
+}
+
+// 4 bytes global -> shared that complete on `bar` with one arrival; zeros when `take` is false.
+__device__ __forceinline__ void copy_scale(uint32_t dst, const float* src, bool take, uint32_t bar) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(take ? 4 : 0) : "memory");
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+// Tiles of one (request, kv head): none for a request without rows or with more than this path takes, at least one
+// otherwise, so that rows that see no key get their zeros.
+__device__ __forceinline__ int tiles_of(const StreamParams& p, int b) {
+  const int n = p.a.row_start[b + 1] - p.a.row_start[b];
+  if (n <= 0 || n > p.a.max_new || (long long)n * p.a.group > p.a.few) return 0;
+  const int context = max(0, min(p.a.context_len[b], p.a.max_context));
+  return max(1, (context + kTile - 1) / kTile);
+}
+
+// First tile of warp `w` of `warps` when `total` tiles are dealt evenly and in order.
+__device__ __forceinline__ int first_tile(int w, int warps, int total) { return int((long long)w * total / warps); }
+
+// Warps that share the tiles: one per tile while there are warps left.
+__device__ __forceinline__ int warps_used(int total, int warps) { return max(1, min(warps, total)); }
+
+// One (request, kv head) and where a warp stands in it.
+struct Segment {
+  int b, g, tile, tiles;  // current tile, tiles of the segment
+};
+
+__device__ __forceinline__ Segment segment_at(const int32_t* tiles, int batch, int kv_heads, int at) {
+  int low = 0, high = batch;
+  while (high - low > 1) {
+    const int mid = (low + high) >> 1;
+    if (tiles[mid] * kv_heads <= at) low = mid; else high = mid;
+  }
+  Segment s;
+  s.b = low;
+  s.tiles = tiles[low + 1] - tiles[low];
+  const int rest = at - tiles[low] * kv_heads;
+  s.g = rest / s.tiles;
+  s.tile = rest - s.g * s.tiles;
+  return s;
+}
+
+__device__ __forceinline__ void step(Segment& s, const int32_t* tiles, int batch, int kv_heads) {
+  if (++s.tile < s.tiles) return;
+  s.tile = 0;
+  if (++s.g < kv_heads) return;
+  s.g = 0;
+  do {
+    ++s.b;
+  } while (s.b < batch && tiles[s.b + 1] == tiles[s.b]);
+  if (s.b < batch) s.tiles = tiles[s.b + 1] - tiles[s.b];
+}
+
+template <int D>
+struct StreamLayout {
+  static constexpr int kSide = kTile * D;                 // one of K and V, bytes
+  static constexpr int kStage = 2 * kSide;
+  static constexpr int kRing = kWarps * kStages * kStage;
+  static constexpr int kScales = kWarps * kStages * 16;   // ks, ks, vs, vs of a tile's two 16-token groups
+  static constexpr int kBars = kWarps * kStages * 8;
+  static int bytes(int batch) { return 1024 + kRing + kScales + kBars + 16 + 4 * (batch + 1 + kWarps); }
+};
+
+// Few query rows against many keys: bound by HBM. The (request, kv head) segments of the batch, cut into tiles of 32
+// tokens, form one line; every warp of the grid takes an equal stretch of it and works alone, with a ring of TMA tiles of
+// its own, no block barrier after the start. NT * 8 rows (a request's new tokens x the q heads of the kv head) share a tile:
+//   S^T[token, row] = K Q^T   (M = 16 tokens, N = 8 rows, K = 16 columns of d; K's codes become f16 exactly, q is f16 with a
+//                              power-of-two factor per row)
+//   running maximum and sum per row in f32; P^T = exp2(S - m) times the page's value scale, f16
+//   O^T[d, row] += V^T P^T    (M = 16 columns of d, K = 16 tokens; P^T turns from accumulator to operand by movmatrix)
+// Value scales enter P relative to the largest seen so far, R, and P carries 2^15: a weight keeps f16's eleven bits down to
+// 2^-29 of the largest one. A warp whose stretch covers a whole segment writes its output; pieces of split segments go to
+// the workspace and cache_join_kernel joins them.
+template <int D, bool BF16, int NT>
+__global__ void __launch_bounds__(kWarps * 32, 1)
+cache_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, StreamParams p,
+                    DeviceStatus* status) {
+  using L = StreamLayout<D>;
+  constexpr int kSteps = D / 16;       // MMA steps over d
+  constexpr int kWords = D / 16;       // 32-bit words of a K row that a thread holds
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (base - raw);
+  const CacheAttnParams& a = p.a;
+  const int warp = threadIdx.x >> 5;
+  const int lane = int(lane_id());
+  const int r = lane >> 2, q4 = lane & 3;
+  const uint32_t ring = base + warp * kStages * L::kStage;
+  const uint32_t scales = base + L::kRing + warp * kStages * 16;
+  const uint32_t bars = base + L::kRing + L::kScales + warp * kStages * 8;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kRing + L::kScales + L::kBars);
+  int32_t* tiles = reinterpret_cast<int32_t*>(smem + L::kRing + L::kScales + L::kBars + 16);
+  int32_t* sums = tiles + a.batch + 1;
+
+  if (lane == 0) {
+    for (int s = 0; s < kStages; ++s) mbar_init(bars + 8 * s, 5);  // the TMA bytes' arrival and four scales
+    fence_mbar_init();
+  }
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    prefetch_tensormap(&map_k);
+    prefetch_tensormap(&map_v);
+  }
+  // ---- every block counts the batch's tiles for itself
+  int carry = 0;
+  for (int first = 0; first < a.batch; first += kWarps * 32) {
+    const int b = first + int(threadIdx.x);
+    int v = b < a.batch ? tiles_of(p, b) : 0;
+    const int own = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int below = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += below;
+    }
+    if (lane == 31) sums[warp] = v;
+    __syncthreads();
+    int before = carry, total = carry;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const int s = sums[w];
+      if (w < warp) before += s;
+      total += s;
+    }
+    if (b < a.batch) tiles[b] = before + v - own;
+    carry = total;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) tiles[a.batch] = carry;
+  __syncthreads();
+  if (blockIdx.x == 0) {
+    for (int b = threadIdx.x; b <= a.batch; b += kWarps * 32) p.tiles[b] = tiles[b];
+    for (int b = threadIdx.x; b < a.batch; b += kWarps * 32) {
+      const int n = a.row_start[b + 1] - a.row_start[b];
+      if (n > a.max_new) report_failure(status, kErrDeviceIndex, kSiteRows, uint32_t(n));
+    }
+  }
+  // consecutive stretches lie on different blocks, so a few of them use as many SMs
+  const int warps = warps_used(carry * a.kv_heads, int(gridDim.x) * kWarps);
+  const int me = warp * int(gridDim.x) + int(blockIdx.x);
+  const int begin = me < warps ? first_tile(me, warps, carry * a.kv_heads) : 0;
+  const int end = me < warps ? first_tile(me + 1, warps, carry * a.kv_heads) : 0;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (begin >= end) return;
+
+  const int page_mask = (1 << a.page_shift) - 1;
+  const int box = min(kTile, page_mask + 1);  // tokens of one copy
+  int bad_page = 0;
+
+  // ---- the stretch's tiles in order: page ids come 32 at a time, one per lane
+  Segment ahead = segment_at(tiles, a.batch, a.kv_heads, begin);
+  int ids = 0, ids_b = -1, ids_first = 0, ahead_pages = 0;
+  auto issue = [&](int number) {  // tile `number` of the stretch into its stage
+    const int stage = number % kStages;
+    const uint32_t bar = bars + 8 * stage, dst = ring + stage * L::kStage;
+    const int token = ahead.tile * kTile;
+    const int first_page = token >> a.page_shift;
+    if (ahead.b != ids_b || first_page < ids_first || first_page + 1 >= ids_first + 32) {
+      ids_b = ahead.b;
+      ids_first = first_page;
+      const int context = max(0, min(a.context_len[ahead.b], a.max_context));
+      ahead_pages = (context + page_mask) >> a.page_shift;
+      ids = first_page + lane < ahead_pages ? a.page_table[ahead.b * a.table_pitch + first_page + lane] : 0;
+    }
+    // sub-tile 0 / 1: tokens 0..15 / 16..31 for 16-token pages; else one copy of 32 tokens
+    const int part = box == kTile ? 0 : (lane & 1);
+    int page = __shfl_sync(0xffffffffu, ids, first_page + part - ids_first);
+    const bool there = first_page + part < ahead_pages;
+    const bool good = there && uint32_t(page) < uint32_t(a.num_pages);
+    if (there && !good) {
+      bad_page = page | int(0x80000000);
+      page = a.num_pages;  // one past the pool: TMA fills zeros
+    }
+    const int copies = kTile / box;
+    const int there_parts = min(copies, ahead_pages - first_page);
+    if (lane == 0) mbar_arrive_expect_tx(bar, uint32_t(max(0, there_parts)) * 2u * uint32_t(box) * D);
+    __syncwarp();
+    if (lane < 4) {
+      const bool keys = lane < 2;
+      if (there && (lane & 1) < copies) {
+        tma_load_4d(dst + (keys ? 0 : L::kSide) + part * box * D, keys ? &map_k : &map_v, 0, ahead.g, token & page_mask, page, bar);
+      }
+      const float* source = keys ? a.k.scale : a.v.scale;
+      copy_scale(scales + stage * 16 + lane * 4, source + (good ? (long long)page * a.kv_heads + ahead.g : 0), good, bar);
+    }
+    step(ahead, tiles, a.batch, a.kv_heads);
+  };
+  const int count = end - begin;
+  for (int i = 0; i < min(count, kStages); ++i) issue(i);
+
+  Segment at = segment_at(tiles, a.batch, a.kv_heads, begin);
+  float acc[kSteps][NT][4], m[NT][2], l[NT][2], row_scale[NT][2];
+  uint32_t query[NT][kSteps][2];
+  int limit[NT][2], context = 0, rows = 0, row0 = 0, nearest = 0;
+  float top = kLeastScale, from_top = 0.f;
+  int piece = 0;  // first tile of the current piece within its segment
+  bool ok = true;
+
+  for (int i = 0; i < count; ++i) {
+    if (i == 0 || at.tile == 0) {
+      // ---- a new piece: its rows of q as f16 with a power-of-two factor, and how far each row sees
+      piece = at.tile;
+      row0 = a.row_start[at.b];
+      const int n = a.row_start[at.b + 1] - row0;
+      rows = n * a.group;
+      context = max(0, min(a.context_len[at.b], a.max_context));
+      nearest = context - n + 1;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const int mine = t * 8 + r;
+        uint4 w[D / 32];
+        float size = 0.f;
+        const bool live = mine < rows && row0 + mine / a.group < a.rows;
+        const uint16_t* src = a.q + (row0 + mine / a.group) * a.q_row + (at.g * a.group + mine % a.group) * a.q_head + q4 * (D / 4);
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          w[c] = live ? *reinterpret_cast<const uint4*>(src + c * 8) : make_uint4(0, 0, 0, 0);
+          const uint32_t words[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 v = unpack<BF16>(words[e]);
+            size = fmaxf(size, fmaxf(fabsf(v.x), fabsf(v.y)));
+          }
+        }
+        size = fmaxf(size, __shfl_xor_sync(0xffffffffu, size, 1));
+        size = fmaxf(size, __shfl_xor_sync(0xffffffffu, size, 2));
+        // the row's largest magnitude comes to lie in [2^14, 2^15)
+        const int up = max(-113, min(126, 14 - (int(__float_as_uint(size) >> 23) - 127)));
+        const float by = __uint_as_float(uint32_t(up + 127) << 23);
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          const uint32_t words[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 v = unpack<BF16>(words[e]);
+            query[t][c * 2 + e / 2][e & 1] = pack_f16x2(v.x * by, v.y * by);
+          }
+        }
+        const float back = __uint_as_float(uint32_t(127 - up) << 23) * a.scale_log2;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int row = t * 8 + 2 * q4 + e;  // the rows whose scores this thread holds
+          row_scale[t][e] = __shfl_sync(0xffffffffu, back, (2 * q4 + e) * 4);
+          limit[t][e] = row < rows ? nearest + row / a.group : context;
+          m[t][e] = -INFINITY;
+          l[t][e] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < kSteps; ++c)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[c][t][e] = 0.f;
+      top = kLeastScale;
+      from_top = 32768.0f / kLeastScale;
+    }
+
+    const int stage = i % kStages;
+    const uint32_t keys = ring + stage * L::kStage, values = keys + L::kSide;
+    if (!__all_sync(0xffffffffu, mbar_wait(bars + 8 * stage, (i / kStages) & 1, abort_flag, status, kSiteTile))) {
+      ok = false;
+      break;
+    }
+    const int token0 = at.tile * kTile;
+
+    // ---- scores: a thread's words of K are 32 (d = 64: 16) consecutive bytes of rows r and r + 8; q holds the same columns
+    float s[2][NT][4];
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      uint32_t ka[kWords], kb[kWords];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int row = g * 16 + half * 8 + r;
+        uint32_t(&k)[kWords] = half == 0 ? ka : kb;
+        if constexpr (D == 128) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const uint4 v = ld_shared_16(keys + row * 128 + (((q4 * 2 + c) ^ (row & 7)) << 4));
+            k[c * 4] = v.x, k[c * 4 + 1] = v.y, k[c * 4 + 2] = v.z, k[c * 4 + 3] = v.w;
+          }
+        } else {
+          const uint4 v = ld_shared_16(keys + row * 64 + ((q4 ^ ((row >> 1) & 3)) << 4));
+          k[0] = v.x, k[1] = v.y, k[2] = v.z, k[3] = v.w;
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[g][t][e] = 0.f;
+#pragma unroll
+      for (int c = 0; c < kSteps; ++c) {
+        const uint32_t a0 = halves_of(ka[c]), a2 = halves_of(ka[c] >> 16), a1 = halves_of(kb[c]), a3 = halves_of(kb[c] >> 16);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) mma_f16(s[g][t], a0, a1, a2, a3, query[t][c][0], query[t][c][1]);
+      }
+    }
+
+    // ---- softmax: the thread's tokens are g * 16 + r and + 8, its rows 2 * q4 and + 1 of each eight
+    const bool edge = token0 + kTile > nearest;  // some row does not see all of the tile
+    float high[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) high[t][0] = high[t][1] = -INFINITY;
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const float ks = ld_shared_f32(scales + stage * 16 + (box == kTile ? 0 : g) * 4);
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[g][t][e] *= ks * row_scale[t][e & 1];
+          if (edge && token0 + g * 16 + r + (e >> 1) * 8 >= limit[t][e & 1]) s[g][t][e] = -INFINITY;
+          high[t][e & 1] = fmaxf(high[t][e & 1], s[g][t][e]);
+        }
+    }
+    const float vs0 = ld_shared_f32(scales + stage * 16 + 8);
+    const float vs1 = box == kTile ? vs0 : ld_shared_f32(scales + stage * 16 + 12);
+    const float new_top = fmaxf(top, fmaxf(fabsf(vs0), fabsf(vs1)));
+    bool moved = new_top != top;
+    float m_new[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) high[t][e] = fmaxf(high[t][e], __shfl_xor_sync(0xffffffffu, high[t][e], o));
+        m_new[t][e] = fmaxf(m[t][e], high[t][e]);
+        moved |= m_new[t][e] != m[t][e];
+      }
+    if (__any_sync(0xffffffffu, moved)) {
+      const float shrink = top / new_top;
+      top = new_top;
+      from_top = 32768.0f / new_top;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        float corr[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float c = m[t][e] == -INFINITY ? 0.f : ex2_approx(m[t][e] - m_new[t][e]);
+          m[t][e] = m_new[t][e];
+          l[t][e] *= c;
+          corr[e] = c * shrink;
+        }
+#pragma unroll
+        for (int c = 0; c < kSteps; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[c][t][e] *= corr[e & 1];
+      }
+    }
+    uint32_t weight[2][NT][2];
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const float vs = (g == 0 ? vs0 : vs1) * from_top;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        float w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          w[e] = m[t][e & 1] == -INFINITY ? 0.f : ex2_approx(s[g][t][e] - m[t][e & 1]);
+          l[t][e & 1] += w[e];
+        }
+        weight[g][t][0] = transposed(pack_f16x2(w[0] * vs, w[1] * vs));
+        weight[g][t][1] = transposed(pack_f16x2(w[2] * vs, w[3] * vs));
+      }
+    }
+
+    // ---- output: a thread's columns of V are 16 (d = 64: 8) consecutive ones of tokens 2 * q4, + 1, + 8, + 9
+    const bool tail = token0 + kTile > context;  // what lies behind the context may be any bits
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      uint32_t v[4][D / 32];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int row = g * 16 + 2 * q4 + (e & 1) + (e >> 1) * 8;
+        if constexpr (D == 128) {
+          const uint4 x = ld_shared_16(values + row * 128 + ((r ^ (row & 7)) << 4));
+          v[e][0] = x.x, v[e][1] = x.y, v[e][2] = x.z, v[e][3] = x.w;
+        } else {
+          const uint2 x = ld_shared_8(values + row * 64 + (((r >> 1) ^ ((row >> 1) & 3)) << 4) + (r & 1) * 8);
+          v[e][0] = x.x, v[e][1] = x.y;
+        }
+        if (tail && token0 + row >= context) {
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) v[e][c] = 0;
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        const uint32_t x0 = __byte_perm(v[0][c], v[1][c], 0x5140), x1 = __byte_perm(v[0][c], v[1][c], 0x7362);
+        const uint32_t y0 = __byte_perm(v[2][c], v[3][c], 0x5140), y1 = __byte_perm(v[2][c], v[3][c], 0x7362);
+        const uint32_t a0 = halves_of(x0), a1 = halves_of(x0 >> 16), a2 = halves_of(y0), a3 = halves_of(y0 >> 16);
+        const uint32_t b0 = halves_of(x1), b1 = halves_of(x1 >> 16), b2 = halves_of(y1), b3 = halves_of(y1 >> 16);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          mma_f16(acc[2 * c][t], a0, a1, a2, a3, weight[g][t][0], weight[g][t][1]);
+          mma_f16(acc[2 * c + 1][t], b0, b1, b2, b3, weight[g][t][0], weight[g][t][1]);
+        }
+      }
+    }
+    __syncwarp();
+    if (i + kStages < count) issue(i + kStages);
+
+    // ---- the end of a piece
+    if (at.tile + 1 == at.tiles || i + 1 == count) {
+      const bool whole = piece == 0 && at.tile + 1 == at.tiles;
+      const int slot = 2 * me + (i - (at.tile - piece) == 0 ? 0 : 1);
+      const float unit = top * (1.0f / 32768.0f);
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float total = l[t][e];
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+          const int row = t * 8 + 2 * q4 + e;
+          if (row >= rows || row0 + row / a.group >= a.rows) continue;
+          if (whole) {
+            const float by = total > 0.f ? unit / total : 0.f;
+            uint16_t* out = a.o + (row0 + row / a.group) * a.o_row + (at.g * a.group + row % a.group) * a.o_head + r * (D / 8);
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c) {
+              uint32_t w[4];
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                const float y0 = acc[c * 4 + x][t][e] * by, y1 = acc[c * 4 + x][t][2 + e] * by;
+                w[x] = BF16 ? pack_bf16x2(y0, y1) : pack_f16x2(y0, y1);
+              }
+              *reinterpret_cast<uint4*>(out + c * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          } else {
+            float* out = p.partial + ((long long)slot * p.slot_rows + row) * (D + 4);
+            if (r == 0) *reinterpret_cast<float2*>(out) = make_float2(m[t][e], total);
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+              *reinterpret_cast<float4*>(out + 4 + r * (D / 8) + c * 4) =
+                  make_float4(acc[c * 2][t][e] * unit, acc[c * 2][t][2 + e] * unit, acc[c * 2 + 1][t][e] * unit,
+                              acc[c * 2 + 1][t][2 + e] * unit);
+            }
+          }
+        }
+    }
+    step(at, tiles, a.batch, a.kv_heads);
+  }
+  if (bad_page != 0) report_failure(status, kErrDeviceIndex, kSitePage, uint32_t(bad_page) & 0x7fffffffu);
+  if (!ok) {  // let this warp's own copies land before the block's memory goes
+    for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+  }
+}
+
+// Joins the pieces of split segments: a block per (segment, row), its warps take the pieces in turn,
+//   o = sum 2^(m_i - M) acc_i / sum 2^(m_i - M) l_i.
+// Launched as a programmatic dependent of the stream kernel, so that its launch overlaps that kernel's end.
+constexpr int kJoinWarps = 4;
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kJoinWarps * 32) cache_join_kernel(StreamParams p, int warps_of_grid) {
+  constexpr int kCols = D / 32;
+  __shared__ float shared[kJoinWarps][D + 2];
+  const CacheAttnParams& a = p.a;
+  const int b = blockIdx.x / a.kv_heads, g = blockIdx.x % a.kv_heads, row = blockIdx.y;
+  const int warp = threadIdx.x >> 5, lane = int(lane_id());
+  const int row0 = a.row_start[b], n = a.row_start[b + 1] - row0;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int tiles = p.tiles[b + 1] - p.tiles[b], total = p.tiles[a.batch] * a.kv_heads;
+  if (tiles == 0 || row >= n * a.group || row0 + row / a.group >= a.rows) return;
+  const int warps = warps_used(total, warps_of_grid);
+  const int first = p.tiles[b] * a.kv_heads + g * tiles, last = first + tiles - 1;
+  const int w0 = int(((long long)(first + 1) * warps - 1) / total), w1 = int(((long long)(last + 1) * warps - 1) / total);
+  if (w0 == w1) return;  // one warp had it all and has written it
+  float m = -INFINITY, l = 0.f, acc[kCols];
+#pragma unroll
+  for (int c = 0; c < kCols; ++c) acc[c] = 0.f;
+  for (int w = w0 + warp; w <= w1; w += kJoinWarps) {
+    const int slot = 2 * w + (first > first_tile(w, warps, total) ? 1 : 0);
+    const float* from = p.partial + ((long long)slot * p.slot_rows + row) * (D + 4);
+    const float2 ml = *reinterpret_cast<const float2*>(from);
+    float x[kCols];
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) x[c] = from[4 + c * 32 + lane];
+    const float m_new = fmaxf(m, ml.x);
+    const float old = m == -INFINITY ? 0.f : exp2f(m - m_new), now = ml.x == -INFINITY ? 0.f : exp2f(ml.x - m_new);
+    m = m_new;
+    l = l * old + ml.y * now;
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) acc[c] = acc[c] * old + x[c] * now;
+  }
+  if (lane == 0) {
+    shared[warp][0] = m;
+    shared[warp][1] = l;
+  }
+#pragma unroll
+  for (int c = 0; c < kCols; ++c) shared[warp][2 + c * 32 + lane] = acc[c];
+  __syncthreads();
+  if (threadIdx.x >= D / 2) return;
+  float top = -INFINITY;
+  for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, shared[w][0]);
+  float den = 0.f, y0 = 0.f, y1 = 0.f;
+  for (int w = 0; w < kJoinWarps; ++w) {
+    const float by = shared[w][0] == -INFINITY ? 0.f : exp2f(shared[w][0] - top);
+    den += by * shared[w][1];
+    y0 += by * shared[w][2 + 2 * threadIdx.x];
+    y1 += by * shared[w][3 + 2 * threadIdx.x];
+  }
+  const float by = den > 0.f ? 1.0f / den : 0.f;
+  uint32_t* out = reinterpret_cast<uint32_t*>(a.o + (row0 + row / a.group) * a.o_row + (g * a.group + row % a.group) * a.o_head);
+  out[threadIdx.x] = BF16 ? pack_bf16x2(y0 * by, y1 * by) : pack_f16x2(y0 * by, y1 * by);
+}
+
+int encode_pool(CUtensorMap* map, const PoolSide& side, int64_t d, int64_t kv_heads, int64_t page_size, int64_t num_pages,
+                uint32_t tokens) {
+  uint64_t dims[4] = {uint64_t(d), uint64_t(kv_heads), uint64_t(page_size), uint64_t(num_pages)};
+  uint64_t strides[3] = {uint64_t(side.head_pitch), uint64_t(side.token_pitch), uint64_t(side.page_pitch)};
+  uint32_t box[4] = {uint32_t(d), 1, tokens, 1};
+  return encode_tensor_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, side.pages, dims, strides, box,
+                           d == 128 ? Swizzle::k128B : Swizzle::k64B);
+}
+
+template <int D, bool BF16, int NT>
+int launch_stream(const DeviceContext* ctx, const StreamParams& p, int64_t page_size, cudaStream_t stream) {
+  const CacheAttnParams& a = p.a;
+  CUtensorMap map_k, map_v;
+  const uint32_t box = uint32_t(page_size < kTile ? page_size : kTile);
+  if (int rc = encode_pool(&map_k, a.k, D, a.kv_heads, page_size, a.num_pages, box)) return rc;
+  if (int rc = encode_pool(&map_v, a.v, D, a.kv_heads, page_size, a.num_pages, box)) return rc;
+  auto kernel = cache_stream_kernel<D, BF16, NT>;
+  KRNB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, StreamLayout<D>::bytes(kMaxBatch)));
+  const int64_t tiles = int64_t(a.batch) * a.kv_heads * ((a.max_context + kTile - 1) / kTile);
+  const int most = ctx->sm_count < kMaxBlocks ? ctx->sm_count : kMaxBlocks;
+  const int blocks = int(tiles < most ? tiles : most);
+  kernel<<<blocks, kWarps * 32, StreamLayout<D>::bytes(a.batch), stream>>>(map_k, map_v, p, ctx->status_dev);
+  KRNB_CUDA(cudaGetLastError());
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(unsigned(a.batch) * unsigned(a.kv_heads), unsigned(p.slot_rows), 1);
+  config.blockDim = dim3(kJoinWarps * 32, 1, 1);
+  config.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attr;
+  config.numAttrs = 1;
+  KRNB_CUDA(cudaLaunchKernelEx(&config, cache_join_kernel<D, BF16>, p, blocks * kWarps));
+  return KRN_B200_OK;
+}
+
+// Rows of a streamed request: all of them where every request has few; where some have many, those with one new token
+// (or the few that fit beside it) are streamed and the rest is tiled.
+int64_t slot_rows(int64_t max_new, int64_t group) {
+  if (max_new * group <= 32) return max_new * group;
+  return group <= 8 ? 8 : group <= 16 ? 16 : group <= 32 ? 32 : 0;
+}
+
+int64_t prefix_bytes(int64_t batch) { return (batch + 1 + 3) / 4 * 16; }
+
+int64_t stream_workspace(int64_t batch, int64_t d, int64_t rows) {
+  return prefix_bytes(batch) + 2 * int64_t(kMaxBlocks) * kWarps * rows * (d + 4) * 4;
+}
+
+template <int D, bool BF16>
+int launch_stream_rows(const DeviceContext* ctx, const StreamParams& p, int64_t page_size, cudaStream_t stream) {
+  if (p.slot_rows <= 8) return launch_stream<D, BF16, 1>(ctx, p, page_size, stream);
+  if (p.slot_rows <= 16) return launch_stream<D, BF16, 2>(ctx, p, page_size, stream);
+  return launch_stream<D, BF16, 4>(ctx, p, page_size, stream);
+}
 
 template <bool BF16>
 __device__ __forceinline__ float widen(uint16_t w) {
@@ -62,6 +690,7 @@ __global__ void __launch_bounds__(128) cache_attn_kernel(CacheAttnParams p, Devi
     report_failure(status, kErrDeviceIndex, kSiteRows, uint32_t(n));
     return;
   }
+  if ((long long)n * p.group <= p.few) return;
   const int visible = context - n + (row - p.row_start[b]) + 1;
   const int g = h / p.group;
   float q[kCols], acc[kCols];
@@ -106,8 +735,10 @@ int launch(const CacheAttnParams& p, DeviceStatus* status, cudaStream_t stream) 
 
 extern "C" int64_t krn_b200_cache_attn_workspace_bytes(int64_t batch, int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t d,
                                                        int64_t max_new, int64_t max_context) {
-  (void)batch, (void)rows, (void)q_heads, (void)kv_heads, (void)d, (void)max_new, (void)max_context;
-  return 16;
+  using namespace krnb;
+  if (batch <= 0 || rows <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0 || d <= 0 || max_new <= 0) return 16;
+  (void)max_context;
+  return stream_workspace(batch, d, slot_rows(max_new, q_heads / kv_heads));
 }
 
 extern "C" int krn_b200_cache_attn(int type, const void* q, const void* k_pages, const void* v_pages, const float* k_scale,
@@ -145,7 +776,11 @@ extern "C" int krn_b200_cache_attn(int type, const void* q, const void* k_pages,
                 (long long)max_pages);
   }
   if (batch == 0 || rows == 0) return KRN_B200_OK;
-  if (batch > 65535 || kv_heads > 65535 || rows > INT32_MAX / 256 || rows * q_heads > INT32_MAX / 2 ||
+  if (batch > kMaxBatch) {
+    return fail(KRN_B200_ERR_UNSUPPORTED, "a batch of %lld requests is not available: their tile counts sit in shared memory, at "
+                "most %d fit. Instead: split the batch", (long long)batch, kMaxBatch);
+  }
+  if (batch * kv_heads * ((max_context + kTile - 1) / kTile) > INT32_MAX / 2 || kv_heads > 65535 || rows > INT32_MAX / 256 || rows * q_heads > INT32_MAX / 2 ||
       max_context > INT32_MAX / 2 || num_pages >= INT32_MAX) {
     return fail(KRN_B200_ERR_UNSUPPORTED, "extents too large for this kernel's 32-bit indices");
   }
@@ -198,6 +833,18 @@ extern "C" int krn_b200_cache_attn(int type, const void* q, const void* k_pages,
   p.scale_log2 = scale_log2;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_handle);
   const bool bf16 = type == KRN_B200_BF16;
+  StreamParams sp;
+  p.few = int(slot_rows(max_new, p.group));
+  sp.a = p;
+  sp.tiles = static_cast<int32_t*>(workspace);
+  sp.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + prefix_bytes(batch));
+  sp.slot_rows = p.few;
+  int rc = KRN_B200_OK;
+  if (p.few == 0) rc = KRN_B200_OK;
+  else if (d == 128) rc = bf16 ? launch_stream_rows<128, true>(ctx, sp, page_size, stream) : launch_stream_rows<128, false>(ctx, sp, page_size, stream);
+  else rc = bf16 ? launch_stream_rows<64, true>(ctx, sp, page_size, stream) : launch_stream_rows<64, false>(ctx, sp, page_size, stream);
+  if (rc) return rc;
+  if (max_new * p.group <= p.few) return KRN_B200_OK;
   if (d == 128) return bf16 ? launch<128, true>(p, ctx->status_dev, stream) : launch<128, false>(p, ctx->status_dev, stream);
   return bf16 ? launch<64, true>(p, ctx->status_dev, stream) : launch<64, false>(p, ctx->status_dev, stream);
 }

@@ -132,7 +132,9 @@ int encode_tensor_map(CUtensorMap* map, CUtensorMapDataType type, int rank, cons
   }
   CUresult res = encode(map, type, static_cast<cuuint32_t>(rank), const_cast<void*>(base), gdims, gstrides, gbox,
                         estrides, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        swizzle == Swizzle::k128B ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                        swizzle == Swizzle::k128B  ? CU_TENSOR_MAP_SWIZZLE_128B
+                        : swizzle == Swizzle::k64B ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                   : CU_TENSOR_MAP_SWIZZLE_NONE,
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (res != CUDA_SUCCESS) {
     return fail(KRN_B200_ERR_INVALID_ARGUMENT,

@@ -54,7 +54,7 @@ int require_sm100(const DeviceContext* ctx);
 
 // ---- TMA descriptors -----------------------------------------------------------------------------------
 
-enum class Swizzle { kNone, k128B };
+enum class Swizzle { kNone, k64B, k128B };
 
 // Encode a tiled tensor map of `rank` dims. dims/strides innermost first; strides in bytes for dims 1..rank-1.
 int encode_tensor_map(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base, const uint64_t* dims,

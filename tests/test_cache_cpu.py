@@ -120,7 +120,8 @@ def attention_status(**change) -> int:
     (dict(q_heads=258), native.ERR_UNSUPPORTED, "129 q heads per kv head"),
     (dict(max_context=129), native.ERR_INVALID_ARGUMENT, "does not fit 2 pages"),
     (dict(max_new=0), native.ERR_INVALID_ARGUMENT, "bad extents"),
-    (dict(batch=65536), native.ERR_UNSUPPORTED, "32-bit"),
+    (dict(batch=8193), native.ERR_UNSUPPORTED, "at most 8192"),
+    (dict(batch=8192, width=1 << 24, pitch=1 << 24, max_context=1 << 30), native.ERR_UNSUPPORTED, "32-bit"),
     (dict(o=None), native.ERR_INVALID_ARGUMENT, "null"),
     (dict(q=8), native.ERR_INVALID_ARGUMENT, "16 bytes"),
     (dict(q_strides=_strides(1028, 128)), native.ERR_INVALID_ARGUMENT, "16 bytes"),

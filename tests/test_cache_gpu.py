@@ -663,7 +663,7 @@ def test_refusals_on_the_device(cuda) -> None:
     cache = ops.PagedCache(*(torch.from_numpy(x).cuda() for x in (*case["codes"], *case["scales"])))
     table, context, start = (torch.from_numpy(case[x]).cuda() for x in ("table", "context", "start"))
     q = case["q"]
-    workspace = torch.empty(1 << 22, dtype=torch.uint8, device="cuda")
+    workspace = torch.empty(1 << 26, dtype=torch.uint8, device="cuda")
 
     def call(q=q, out=None, table=table, context=context, start=start, **more):
         given = dict(max_new=1, max_context=100, workspace=workspace) | more
