@@ -1,49 +1,14 @@
 // Attention over the paged 8-bit cache with one scale per (page, kv head): rows of q packed by request, row i of a request
 // with n rows and a context of c tokens stands at position c - n + i and sees the keys up to it.
 //
-// One warp per (row, q head): each lane holds d / 32 columns, a key's score is a shuffle sum, one pass over the keys with a
-// running maximum and sum.
-#include "host.cuh"
-
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
+// Two paths: requests with few rows (new tokens x q heads of a kv head) are streamed, a warp per stretch of keys, here;
+// prompts and chunks of prompts go to tensor-core tiles (cache_attn_tile.cu).
+#include "cache_attn.cuh"
 
 #include <cmath>
 
 namespace krnb {
 namespace {
-
-constexpr int kErrDeviceIndex = 6;  // mirrors KRN_B200_ERR_DEVICE_INDEX in include/krn_b200.h
-
-enum Site { kSitePage = 51, kSiteRows = 52, kSiteTile = 53 };
-
-struct PoolSide {
-  const uint8_t* pages;
-  const float* scale;  // [num_pages, kv_heads]
-  long long page_pitch, token_pitch, head_pitch;
-};
-
-struct CacheAttnParams {
-  const uint16_t* q;
-  uint16_t* o;
-  long long q_row, q_head, o_row, o_head, table_pitch;
-  PoolSide k, v;
-  const int32_t* page_table;
-  const int32_t* context_len;
-  const int32_t* row_start;
-  int batch, rows, q_heads, kv_heads, group, page_shift, num_pages, max_new, max_context;
-  int few;  // a request with at most this many rows (new tokens x q heads of a kv head) is streamed, one with more is tiled
-  float scale_log2;
-};
-
-template <bool BF16>
-__device__ __forceinline__ float2 unpack(uint32_t w) {
-  if constexpr (BF16) {
-    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-  } else {
-    return __half22float2(*reinterpret_cast<const __half2*>(&w));
-  }
-}
 
 // ---- few rows: a stream of keys per warp ---------------------------------------------------------------------------------
 
@@ -61,12 +26,6 @@ struct StreamParams {
   float* partial;
   int slot_rows;     // rows a partial slot holds
 };
-
-__device__ __forceinline__ uint32_t halves_of(uint32_t codes) {  // two e4m3 codes in the low 16 bits
-  uint32_t h2;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"(uint16_t(codes)));
-  return h2;
-}
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
@@ -110,7 +69,7 @@ __device__ __forceinline__ void copy_scale(uint32_t dst, const float* src, bool 
 // otherwise, so that rows that see no key get their zeros.
 __device__ __forceinline__ int tiles_of(const StreamParams& p, int b) {
   const int n = p.a.row_start[b + 1] - p.a.row_start[b];
-  if (n <= 0 || n > p.a.max_new || (long long)n * p.a.group > p.a.few) return 0;
+  if (!rows_ok(p.a, b, n) || (long long)n * p.a.group > p.a.few) return 0;
   const int context = max(0, min(p.a.context_len[b], p.a.max_context));
   return max(1, (context + kTile - 1) / kTile);
 }
@@ -516,7 +475,7 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           const int row = t * 8 + 2 * q4 + e;
           if (row >= rows || row0 + row / a.group >= a.rows) continue;
           if (whole) {
-            const float by = total > 0.f ? unit / total : 0.f;
+            const float by = total == 0.f ? 0.f : unit / total;
             uint16_t* out = a.o + (row0 + row / a.group) * a.o_row + (at.g * a.group + row % a.group) * a.o_head + r * (D / 8);
 #pragma unroll
             for (int c = 0; c < D / 64; ++c) {
@@ -602,18 +561,9 @@ __global__ void __launch_bounds__(kJoinWarps * 32) cache_join_kernel(StreamParam
     y0 += by * shared[w][2 + 2 * threadIdx.x];
     y1 += by * shared[w][3 + 2 * threadIdx.x];
   }
-  const float by = den > 0.f ? 1.0f / den : 0.f;
+  const float by = den == 0.f ? 0.f : 1.0f / den;
   uint32_t* out = reinterpret_cast<uint32_t*>(a.o + (row0 + row / a.group) * a.o_row + (g * a.group + row % a.group) * a.o_head);
   out[threadIdx.x] = BF16 ? pack_bf16x2(y0 * by, y1 * by) : pack_f16x2(y0 * by, y1 * by);
-}
-
-int encode_pool(CUtensorMap* map, const PoolSide& side, int64_t d, int64_t kv_heads, int64_t page_size, int64_t num_pages,
-                uint32_t tokens) {
-  uint64_t dims[4] = {uint64_t(d), uint64_t(kv_heads), uint64_t(page_size), uint64_t(num_pages)};
-  uint64_t strides[3] = {uint64_t(side.head_pitch), uint64_t(side.token_pitch), uint64_t(side.page_pitch)};
-  uint32_t box[4] = {uint32_t(d), 1, tokens, 1};
-  return encode_tensor_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, side.pages, dims, strides, box,
-                           d == 128 ? Swizzle::k128B : Swizzle::k64B);
 }
 
 template <int D, bool BF16, int NT>
@@ -621,8 +571,9 @@ int launch_stream(const DeviceContext* ctx, const StreamParams& p, int64_t page_
   const CacheAttnParams& a = p.a;
   CUtensorMap map_k, map_v;
   const uint32_t box = uint32_t(page_size < kTile ? page_size : kTile);
-  if (int rc = encode_pool(&map_k, a.k, D, a.kv_heads, page_size, a.num_pages, box)) return rc;
-  if (int rc = encode_pool(&map_v, a.v, D, a.kv_heads, page_size, a.num_pages, box)) return rc;
+  const Swizzle swizzle = D == 128 ? Swizzle::k128B : Swizzle::k64B;
+  if (int rc = encode_pool(&map_k, a.k, D, a.kv_heads, page_size, a.num_pages, box, swizzle)) return rc;
+  if (int rc = encode_pool(&map_v, a.v, D, a.kv_heads, page_size, a.num_pages, box, swizzle)) return rc;
   auto kernel = cache_stream_kernel<D, BF16, NT>;
   KRNB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, StreamLayout<D>::bytes(kMaxBatch)));
   const int64_t tiles = int64_t(a.batch) * a.kv_heads * ((a.max_context + kTile - 1) / kTile);
@@ -663,73 +614,6 @@ int launch_stream_rows(const DeviceContext* ctx, const StreamParams& p, int64_t 
   return launch_stream<D, BF16, 4>(ctx, p, page_size, stream);
 }
 
-template <bool BF16>
-__device__ __forceinline__ float widen(uint16_t w) {
-  if constexpr (BF16) return __uint_as_float(uint32_t(w) << 16);
-  return __half2float(__ushort_as_half(w));
-}
-
-__device__ __forceinline__ float from_e4m3(uint32_t code) {
-  uint32_t h2;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"(uint16_t(code)));
-  return __half2float(__ushort_as_half(uint16_t(h2 & 0xffffu)));
-}
-
-template <int D, bool BF16>
-__global__ void __launch_bounds__(128) cache_attn_kernel(CacheAttnParams p, DeviceStatus* status) {
-  constexpr int kCols = D / 32;
-  const int lane = int(lane_id());
-  const int row = blockIdx.x, h = blockIdx.y * 4 + (threadIdx.x >> 5);
-  if (h >= p.q_heads) return;
-  int b = 0;
-  while (b < p.batch && p.row_start[b + 1] <= row) ++b;
-  if (b >= p.batch || p.row_start[b] > row) return;  // behind the last request
-  const int n = p.row_start[b + 1] - p.row_start[b];
-  const int context = max(0, min(p.context_len[b], p.max_context));
-  if (n > p.max_new) {
-    report_failure(status, kErrDeviceIndex, kSiteRows, uint32_t(n));
-    return;
-  }
-  if ((long long)n * p.group <= p.few) return;
-  const int visible = context - n + (row - p.row_start[b]) + 1;
-  const int g = h / p.group;
-  float q[kCols], acc[kCols];
-  for (int c = 0; c < kCols; ++c) {
-    q[c] = widen<BF16>(p.q[row * p.q_row + h * p.q_head + lane * kCols + c]) * p.scale_log2;
-    acc[c] = 0.f;
-  }
-  float m = -INFINITY, l = 0.f;
-  for (int j = 0; j < visible; ++j) {
-    const int page = p.page_table[b * p.table_pitch + (j >> p.page_shift)];
-    const bool good = uint32_t(page) < uint32_t(p.num_pages);
-    if (!good) report_failure(status, kErrDeviceIndex, kSitePage, uint32_t(page) & 0x7fffffffu);
-    const int at = j & ((1 << p.page_shift) - 1);
-    float s = 0.f;
-    const uint8_t* key = p.k.pages + page * p.k.page_pitch + at * p.k.token_pitch + g * p.k.head_pitch + lane * kCols;
-    const uint8_t* val = p.v.pages + page * p.v.page_pitch + at * p.v.token_pitch + g * p.v.head_pitch + lane * kCols;
-    for (int c = 0; c < kCols; ++c) s += good ? q[c] * from_e4m3(key[c]) : 0.f;
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (good) s *= p.k.scale[(long long)page * p.kv_heads + g];
-    const float m_new = fmaxf(m, s), corr = exp2f(m - m_new), w = exp2f(s - m_new);
-    m = m_new;
-    l = l * corr + w;
-    const float wv = good ? w * p.v.scale[(long long)page * p.kv_heads + g] : 0.f;
-    for (int c = 0; c < kCols; ++c) acc[c] = acc[c] * corr + (good ? wv * from_e4m3(val[c]) : 0.f);
-  }
-  for (int c = 0; c < kCols; ++c) {
-    const float y = l > 0.f ? acc[c] / l : 0.f;
-    p.o[row * p.o_row + h * p.o_head + lane * kCols + c] =
-        BF16 ? uint16_t(pack_bf16x2(y, 0.f) & 0xffffu) : uint16_t(pack_f16x2(y, 0.f) & 0xffffu);
-  }
-}
-
-template <int D, bool BF16>
-int launch(const CacheAttnParams& p, DeviceStatus* status, cudaStream_t stream) {
-  cache_attn_kernel<D, BF16><<<dim3(unsigned(p.rows), unsigned((p.q_heads + 3) / 4)), 128, 0, stream>>>(p, status);
-  KRNB_CUDA(cudaGetLastError());
-  return KRN_B200_OK;
-}
-
 }  // namespace
 }  // namespace krnb
 
@@ -737,8 +621,9 @@ extern "C" int64_t krn_b200_cache_attn_workspace_bytes(int64_t batch, int64_t ro
                                                        int64_t max_new, int64_t max_context) {
   using namespace krnb;
   if (batch <= 0 || rows <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0 || d <= 0 || max_new <= 0) return 16;
-  (void)max_context;
-  return stream_workspace(batch, d, slot_rows(max_new, q_heads / kv_heads));
+  const int64_t few = slot_rows(max_new, q_heads / kv_heads);
+  return stream_workspace(batch, d, few) +
+         (max_new * (q_heads / kv_heads) <= few ? 0 : tile_workspace(batch, rows, q_heads, kv_heads, d, few, max_context));
 }
 
 extern "C" int krn_b200_cache_attn(int type, const void* q, const void* k_pages, const void* v_pages, const float* k_scale,
@@ -839,12 +724,13 @@ extern "C" int krn_b200_cache_attn(int type, const void* q, const void* k_pages,
   sp.tiles = static_cast<int32_t*>(workspace);
   sp.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + prefix_bytes(batch));
   sp.slot_rows = p.few;
-  int rc = KRN_B200_OK;
-  if (p.few == 0) rc = KRN_B200_OK;
-  else if (d == 128) rc = bf16 ? launch_stream_rows<128, true>(ctx, sp, page_size, stream) : launch_stream_rows<128, false>(ctx, sp, page_size, stream);
-  else rc = bf16 ? launch_stream_rows<64, true>(ctx, sp, page_size, stream) : launch_stream_rows<64, false>(ctx, sp, page_size, stream);
-  if (rc) return rc;
+  if (p.few > 0) {
+    int rc;
+    if (d == 128) rc = bf16 ? launch_stream_rows<128, true>(ctx, sp, page_size, stream) : launch_stream_rows<128, false>(ctx, sp, page_size, stream);
+    else rc = bf16 ? launch_stream_rows<64, true>(ctx, sp, page_size, stream) : launch_stream_rows<64, false>(ctx, sp, page_size, stream);
+    if (rc) return rc;
+  }
   if (max_new * p.group <= p.few) return KRN_B200_OK;
-  if (d == 128) return bf16 ? launch<128, true>(p, ctx->status_dev, stream) : launch<128, false>(p, ctx->status_dev, stream);
-  return bf16 ? launch<64, true>(p, ctx->status_dev, stream) : launch<64, false>(p, ctx->status_dev, stream);
+  float* partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + stream_workspace(batch, d, p.few));
+  return launch_tiles(ctx, p, bf16, d, page_size, partial, stream);
 }

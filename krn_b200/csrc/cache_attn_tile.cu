@@ -1,0 +1,755 @@
+// Attention of many query rows (prompts, chunks of prompts) over the paged 8-bit cache: tensor-core tiles.
+//
+// A block owns two tiles of 128 query rows of one (request, kv head): 128 / group consecutive tokens of each q head that
+// shares the kv head, so K and V are fetched once for the whole group. It runs over the keys in tiles of 128:
+//
+//   warp 0        TMA producer: K codes into a ring of kKStages tiles, V codes into a ring of two;
+//   warp 1        MMA issuer: S_t = Q_t K^T (kind::f8f6f4) on the cache's bytes as they are, O_t += P_t V (kind::f16);
+//   warps 2, 3    turn a V tile into f16, times its pages' scales: 16-bit P needs a 16-bit V;
+//   warps 4..11   softmax of the two query tiles, a thread per row; then the output.
+//
+// Q is split into e4m3 parts, each the rounded remainder of the ones before (a power-of-two factor puts the row's largest
+// magnitude into [128, 256)): two parts hold bf16's 8 significant bits exactly, three hold f16's 11, but for elements below
+// 2^-9 of the row's largest, where the remainder is under 2^-17 of it. S is the sum over the parts, and two e4m3 products
+// take the tensor cores as long as one of 16 bits, so K needs no conversion at all.
+//
+// A page's key scale multiplies its columns of S in f32, before the maximum. Its value scale multiplies V, relative to the
+// largest one that this block meets and times 2^7 (448 * 2^7 is within f16): for scales that are powers of two V stays
+// exact down to 2^-22 of the largest; any other scale costs two roundings of 2^-12.
+//
+// Tensor memory (512 columns): S0 | S1 | O0 | O1, 128 columns each; P_t (f16) lies over the first 64 columns of S_t.
+#include "cache_attn.cuh"
+
+#include <cmath>
+
+namespace krnb {
+namespace {
+
+constexpr int kTileQ = 128;
+constexpr int kTileKV = 128;
+constexpr int kThreads = 384;
+constexpr int kSMs = 148;                 // blocks that run at once: fewer are split over the keys
+constexpr float kRescaleThreshold = 8.0f;
+constexpr float kNone = -3.0e38f;         // reference maximum of a row that has seen no key
+
+struct TileParams {
+  CacheAttnParams a;
+  float* partial;  // [splits, rows, q_heads, d + 4]: m, l, the unnormalised output
+  int tokens;      // tokens of a query tile: 128 / group
+  int splits;
+};
+
+template <int D, int Parts>
+struct Layout {
+  static constexpr int kKStages = D == 128 && Parts == 3 ? 2 : 3;
+  static constexpr int kPerRow = 128 / D;                               // parts in a 128-byte row of Q
+  static constexpr int kQBlocks = (Parts + kPerRow - 1) / kPerRow;
+  static constexpr int kQBytes = kQBlocks * kTileQ * 128;               // one query tile
+  static constexpr int kRawBytes = kTileKV * D;                         // a tile of codes
+  static constexpr int kHalfBytes = kTileKV * D * 2;                    // a tile of V in f16
+  static constexpr int kBlockBytes = 128 * 128;                         // [128 rows x 128 bytes]
+  static constexpr int kOffK = 2 * kQBytes;
+  static constexpr int kOffRaw = kOffK + kKStages * kRawBytes;
+  static constexpr int kOffHalf = kOffRaw + 2 * kRawBytes;
+  static constexpr int kOffTail = kOffHalf + 2 * kHalfBytes;
+  static constexpr int kSmemBytes = kOffTail + 512 + 1024;
+};
+
+__device__ __forceinline__ void tie(uint32_t (&r)[32]) {
+  asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                   "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                   "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :: "memory");
+}
+
+// K-major operand rows of 64 bytes, 64-byte swizzle (what TMA writes with that mode): 8-row groups are 512 bytes apart.
+__device__ __forceinline__ uint64_t desc_kmajor_sw64(uint32_t smem_addr) {
+  uint64_t desc = 0;
+  desc |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
+  desc |= static_cast<uint64_t>(1) << 16;
+  desc |= static_cast<uint64_t>(512 >> 4) << 32;
+  desc |= static_cast<uint64_t>(1) << 46;
+  desc |= static_cast<uint64_t>(4) << 61;
+  return desc;
+}
+
+__device__ __forceinline__ void st_shared_16(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+
+__device__ __forceinline__ uint4 ld_shared_16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+
+__device__ __forceinline__ uint32_t times(uint32_t a, uint32_t b) {  // f16x2
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// Blocks of two query tiles that request b has on this path.
+__device__ __forceinline__ int blocks_of(const TileParams& p, int b) {
+  const int n = p.a.row_start[b + 1] - p.a.row_start[b];
+  if (!rows_ok(p.a, b, n) || (long long)n * p.a.group <= p.a.few) return 0;
+  return (n + 2 * p.tokens - 1) / (2 * p.tokens);
+}
+
+// Page ids of the 16-token groups of key tiles, one group per lane of 8, two tiles ahead, and the groups' scales one ahead:
+// a loader that hides both loads behind the tile in work. Groups without a page in the pool have the scale `none`.
+struct ScaleAhead {
+  const int32_t* table;
+  const float* scale;
+  int shift, pages, num_pages, heads, head, lane;
+  float none;
+  int id;
+  float next;
+  __device__ __forceinline__ int id_at(int tile) const {
+    const int at = (tile * kTileKV + (lane & 7) * 16) >> shift;
+    return at < pages ? table[at] : -1;
+  }
+  __device__ __forceinline__ float scale_at(int page) const {
+    return uint32_t(page) < uint32_t(num_pages) ? scale[(long long)page * heads + head] : none;
+  }
+  __device__ __forceinline__ void start(int tile) {
+    next = scale_at(id_at(tile));
+    id = id_at(tile + 1);
+  }
+  // The scale of group lane & 7 of `tile`; afterwards those of tile + 1 are under way.
+  __device__ __forceinline__ float take(int tile) {
+    const float now = next;
+    next = scale_at(id);
+    id = id_at(tile + 2);
+    return now;
+  }
+};
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kThreads, 1)
+cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, TileParams p,
+                  DeviceStatus* status) {
+  constexpr int Parts = BF16 ? 2 : 3;
+  using L = Layout<D, Parts>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (base - raw);
+  const CacheAttnParams& a = p.a;
+
+  const uint32_t q_addr = base, k_addr = base + L::kOffK, raw_addr = base + L::kOffRaw, half_addr = base + L::kOffHalf;
+  uint8_t* tail = smem + L::kOffTail;
+  const uint32_t bars = smem_u32(tail);
+  const uint32_t q_full = bars, k_full = bars + 8, k_empty = bars + 32, raw_full = bars + 56, raw_empty = bars + 72;
+  const uint32_t v_full = bars + 88, v_empty = bars + 104, s_full = bars + 120, p_full = bars + 136, o_full = bars + 152;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail + 168);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + 172);
+  int32_t* found = reinterpret_cast<int32_t*>(tail + 176);  // request, block of it, blocks of it
+  int32_t* sums = reinterpret_cast<int32_t*>(tail + 192);   // [12]
+  float* tops = reinterpret_cast<float*>(tail + 256);       // [12]
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = int(lane_id());
+
+  // ---- which request: blocks of the batch's requests in order, the last (longest) block of a request first
+  const int g = int(blockIdx.x) % a.kv_heads, wanted = int(blockIdx.x) / a.kv_heads;
+  if (threadIdx.x == 0) {
+    found[0] = -1;
+    *abort_flag = 0;
+  }
+  int carry = 0;
+  for (int first = 0; first < a.batch; first += kThreads) {
+    const int b = first + int(threadIdx.x);
+    const int own = b < a.batch ? blocks_of(p, b) : 0;
+    if (blockIdx.x == 0 && blockIdx.y == 0 && b < a.batch && a.row_start[b + 1] - a.row_start[b] > a.max_new) {
+      report_failure(status, kErrDeviceIndex, kSiteRows, uint32_t(a.row_start[b + 1] - a.row_start[b]));
+    }
+    int v = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int below = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += below;
+    }
+    __syncthreads();
+    if (lane == 31) sums[warp] = v;
+    __syncthreads();
+    int before = carry, total = carry;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) {
+      const int s = sums[w];
+      if (w < warp) before += s;
+      total += s;
+    }
+    const int start = before + v - own;
+    if (wanted >= start && wanted < start + own) {
+      found[0] = b;
+      found[1] = own - 1 - (wanted - start);
+    }
+    carry = total;
+    if (carry > wanted) break;
+  }
+  __syncthreads();
+  const int b = found[0];
+  if (b < 0) return;  // the whole block: the grid is sized by a bound
+  const int row0 = a.row_start[b], n = a.row_start[b + 1] - row0;
+  const int context = max(0, min(a.context_len[b], a.max_context));
+  const int token0 = found[1] * 2 * p.tokens;  // first token of query tile 0
+  const int32_t* table = a.page_table + b * a.table_pitch;
+  const int pages = (context + (1 << a.page_shift) - 1) >> a.page_shift;
+
+  // ---- key tiles: up to the position of a query tile's last token, this split's share of them
+  int counts[2];
+  int most = 0;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int last = min(n, token0 + (t + 1) * p.tokens) - 1;  // last token of the tile
+    const int keys = token0 + t * p.tokens < n ? max(0, min(context, context - n + last + 1)) : 0;
+    counts[t] = (keys + kTileKV - 1) / kTileKV;
+    most = max(most, counts[t]);
+  }
+  const int j0 = int((long long)most * blockIdx.y / p.splits), j1 = int((long long)most * (blockIdx.y + 1) / p.splits);
+  const int n0 = max(0, min(counts[0], j1) - j0), n1 = max(0, min(counts[1], j1) - j0);
+  const int count = max(n0, n1);
+
+  // ---- the largest value scale of these keys; ids outside the pool are reported
+  {
+    float top = 0.f;
+    const int first = (j0 * kTileKV) >> a.page_shift, last = min(pages, (((j0 + count) * kTileKV - 1) >> a.page_shift) + 1);
+    for (int at = first + int(threadIdx.x); at < last; at += kThreads) {
+      const int page = table[at];
+      if (uint32_t(page) < uint32_t(a.num_pages)) {
+        top = fmaxf(top, fabsf(a.v.scale[(long long)page * a.kv_heads + g]));
+      } else {
+        report_failure(status, kErrDeviceIndex, kSitePage, uint32_t(page) & 0x7fffffffu);
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (lane == 0) tops[warp] = top;
+  }
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 8);
+    for (int i = 0; i < 3; ++i) {
+      mbar_init(k_full + 8 * i, 1);
+      mbar_init(k_empty + 8 * i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(raw_full + 8 * i, 1);
+      mbar_init(raw_empty + 8 * i, 2);
+      mbar_init(v_full + 8 * i, 2);
+      mbar_init(v_empty + 8 * i, 1);
+      mbar_init(s_full + 8 * i, 1);
+      mbar_init(p_full + 8 * i, 4);
+      mbar_init(o_full + 8 * i, 1);
+    }
+    fence_mbar_init();
+    prefetch_tensormap(&map_k);
+    prefetch_tensormap(&map_v);
+  }
+  if (warp == 1) {
+    tmem_alloc<1>(smem_u32(tmem_slot), 512);
+    tmem_relinquish<1>();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  float top = 0x1p-110f;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) top = fmaxf(top, tops[w]);
+
+  if (warp < 4) reg_dealloc<56>();
+  if (warp == 0) {
+    // ---------------------------------------------------------------- TMA producer
+    const int box = min(kTileKV, 1 << a.page_shift), copies = kTileKV / box;
+    int ids = 0, ids_first = -64;
+    for (int j = 0; j < count; ++j) {
+      const int token = (j0 + j) * kTileKV, first_page = token >> a.page_shift;
+      if (first_page + copies > ids_first + 32) {
+        ids_first = first_page;
+        ids = first_page + lane < pages ? table[first_page + lane] : 0;
+      }
+      int page = __shfl_sync(0xffffffffu, ids, (first_page + lane - ids_first) & 31);
+      if (uint32_t(page) >= uint32_t(a.num_pages)) page = a.num_pages;  // one past the pool: TMA fills zeros
+      const int there = min(copies, pages - first_page);
+      const uint32_t bytes = uint32_t(there) * uint32_t(box) * D;
+      const int stage = j % L::kKStages, v_stage = j & 1;
+      bool ok = true;
+      if (lane == 0) ok = mbar_wait(k_empty + 8 * stage, ((j / L::kKStages) & 1) ^ 1u, abort_flag, status, kSiteKeys);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      if (lane == 0) mbar_arrive_expect_tx(k_full + 8 * stage, bytes);
+      __syncwarp();
+      if (lane < there) {
+        tma_load_4d(k_addr + stage * L::kRawBytes + lane * box * D, &map_k, 0, g, token & ((1 << a.page_shift) - 1), page,
+                    k_full + 8 * stage);
+      }
+      if (lane == 0) ok = mbar_wait(raw_empty + 8 * v_stage, ((j >> 1) & 1) ^ 1u, abort_flag, status, kSiteValues);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      if (lane == 0) mbar_arrive_expect_tx(raw_full + 8 * v_stage, bytes);
+      __syncwarp();
+      if (lane < there) {
+        tma_load_4d(raw_addr + v_stage * L::kRawBytes + lane * box * D, &map_v, 0, g, token & ((1 << a.page_shift) - 1), page,
+                    raw_full + 8 * v_stage);
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- MMA issuer
+    if (count > 0) {
+      const bool leader = elect_one();
+      const uint32_t idesc_s = umma_idesc(kFmtE4M3, kFmtE4M3, kTileQ, kTileKV, 0, 0);
+      const uint32_t idesc_pv = umma_idesc(kFmtF16, kFmtF16, kTileQ, D, 0, 1);
+      const int nt[2] = {n0, n1};
+      const uint64_t q_desc = umma_desc_kmajor_sw128(0);
+      const uint64_t k_desc = D == 128 ? umma_desc_kmajor_sw128(0) : desc_kmajor_sw64(0);
+      const uint64_t v_desc = umma_desc_mnmajor_sw128(0, L::kBlockBytes, 1024);
+      const uint32_t q_hi = uint32_t(q_desc >> 32), k_hi = uint32_t(k_desc >> 32), v_hi = uint32_t(v_desc >> 32);
+      const uint32_t q_lo = uint32_t(q_desc) + (q_addr >> 4), k_lo = uint32_t(k_desc) + (k_addr >> 4);
+      const uint32_t v_lo = uint32_t(v_desc) + (half_addr >> 4);
+
+      // S_t = sum over Q's parts: D / 32 instructions of K = 32 columns each
+      auto issue_s = [&](int t, int stage) {
+        const uint32_t qa = q_lo + t * (L::kQBytes >> 4);
+        const uint32_t ka = k_lo + stage * (L::kRawBytes >> 4);
+        if (leader) {
+#pragma unroll
+          for (int part = 0; part < Parts; ++part) {
+#pragma unroll
+            for (int ks = 0; ks < D / 32; ++ks) {
+              const uint32_t off = ((part / L::kPerRow) * L::kBlockBytes + (part % L::kPerRow) * D + ks * 32) >> 4;
+              umma_ss_halves<1, true>(tmem_base + t * 128, qa + off, q_hi, ka + ks * 2, k_hi, idesc_s, part + ks > 0 ? 1u : 0u);
+            }
+          }
+          umma_commit(s_full + 8 * t);
+        }
+        __syncwarp();
+      };
+      // O_t += P_t V: 8 instructions of K = 16 keys; P_t from tensor memory, V with d contiguous in 64-column blocks
+      auto issue_pv = [&](int t, int stage, bool accumulate) {
+        const uint32_t va = v_lo + stage * (L::kHalfBytes >> 4);
+        if (leader) {
+#pragma unroll
+          for (int ks = 0; ks < kTileKV / 16; ++ks) {
+            umma_ts_f16_halves(tmem_base + 256 + t * 128, tmem_base + t * 128 + ks * 8, va + ks * (2048 >> 4), v_hi, idesc_pv,
+                               (accumulate || ks > 0) ? 1u : 0u);
+          }
+        }
+        __syncwarp();
+      };
+      auto wait = [&](uint32_t bar, uint32_t parity, int site) {
+        return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, site)) != 0;
+      };
+      bool ok = wait(q_full, 0, kSiteQuery) && wait(k_full, 0, kSiteScores);
+      if (ok) {
+        tc_fence_after();
+        for (int t = 0; t < 2; ++t)
+          if (nt[t] > 0) issue_s(t, 0);
+        if (leader) umma_commit(k_empty);
+      }
+      int k_stage = 0;          // stage and phase of the K tile behind the one in work
+      uint32_t k_phase = 0;
+      for (int j = 0; j < count && ok; ++j) {
+        const int stage = j & 1;
+        if (++k_stage == L::kKStages) {
+          k_stage = 0;
+          k_phase ^= 1u;
+        }
+        if (!wait(v_full + 8 * stage, (j >> 1) & 1, kSiteScores)) break;
+        bool next_k_ready = false;
+        for (int t = 0; t < 2 && ok; ++t) {
+          if (j >= nt[t]) continue;
+          if (!wait(p_full + 8 * t, j & 1, kSiteWeights)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          issue_pv(t, stage, j > 0);
+          if (j + 1 < nt[t]) {
+            if (!next_k_ready) {
+              if (!wait(k_full + 8 * k_stage, k_phase, kSiteScores)) {
+                ok = false;
+                break;
+              }
+              tc_fence_after();
+              next_k_ready = true;
+            }
+            issue_s(t, k_stage);
+          } else {
+            if (leader) umma_commit(o_full + 8 * t);
+          }
+        }
+        if (!ok) break;
+        if (leader) {
+          umma_commit(v_empty + 8 * stage);
+          if (j + 1 < count) umma_commit(k_empty + 8 * k_stage);
+        }
+        __syncwarp();
+      }
+    }
+  } else if (warp < 4) {
+    // ---------------------------------------------------------------- V to f16
+    constexpr int kLanes = D / 16;               // threads per row, 16 codes each
+    constexpr int kRows = 64 / kLanes;           // rows per pass of the two warps
+    const int tid = int(threadIdx.x) - 64;
+    const int row0_of = tid / kLanes, c = tid % kLanes;
+    ScaleAhead scales = {table, a.v.scale, a.page_shift, pages, a.num_pages, a.kv_heads, g, lane, 0.f, 0, 0.f};
+    if (count > 0) scales.start(j0);
+    const float unit = 128.0f / top;
+    // the two 16-byte halves of a thread's 16 columns, in an order that spreads a row over all banks
+    const int turn = (c >> 2) & 1;
+    for (int j = 0; j < count; ++j) {
+      const int stage = j & 1;
+      const float factor = scales.take(j0 + j) * unit;
+      const uint32_t mine = pack_f16x2(factor, factor);
+      bool ok = mbar_wait(raw_full + 8 * stage, (j >> 1) & 1, abort_flag, status, kSiteValues) &&
+                mbar_wait(v_empty + 8 * stage, ((j >> 1) & 1) ^ 1u, abort_flag, status, kSiteRoom);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      const int valid = context - (j0 + j) * kTileKV;  // rows behind the context may hold any bits
+      const uint32_t from = raw_addr + stage * L::kRawBytes, to = half_addr + stage * L::kHalfBytes;
+#pragma unroll 4
+      for (int i = 0; i < kTileKV / kRows; ++i) {
+        const int row = i * kRows + row0_of;
+        uint4 w = ld_shared_16(from + row * D + c * 16);
+        if (row >= valid) w = make_uint4(0, 0, 0, 0);
+        const uint32_t by = __shfl_sync(0xffffffffu, mine, (i * kRows) >> 4);
+        const uint32_t x[8] = {times(halves_of(w.x), by), times(halves_of(w.x >> 16), by), times(halves_of(w.y), by),
+                               times(halves_of(w.y >> 16), by), times(halves_of(w.z), by), times(halves_of(w.z >> 16), by),
+                               times(halves_of(w.w), by), times(halves_of(w.w >> 16), by)};
+        const uint32_t at = to + (c >> 2) * L::kBlockBytes + row * 128;
+        const uint32_t even = uint32_t((2 * c) & 7), x7 = uint32_t(row & 7);
+        if (turn == 0) {
+          st_shared_16(at + ((even ^ x7) << 4), x[0], x[1], x[2], x[3]);
+          st_shared_16(at + (((even + 1) ^ x7) << 4), x[4], x[5], x[6], x[7]);
+        } else {
+          st_shared_16(at + (((even + 1) ^ x7) << 4), x[4], x[5], x[6], x[7]);
+          st_shared_16(at + ((even ^ x7) << 4), x[0], x[1], x[2], x[3]);
+        }
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(v_full + 8 * stage);
+        mbar_arrive(raw_empty + 8 * stage);
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------- Q, softmax, output
+    reg_alloc<224>();
+    const int t = (warp - 4) >> 2;
+    const int quarter = warp & 3;
+    const int nt = t == 0 ? n0 : n1;
+    const int row_in_tile = quarter * 32 + lane;
+    const int token = token0 + t * p.tokens + row_in_tile / a.group;
+    const bool live = row_in_tile < p.tokens * a.group && token < n && row0 + token < a.rows;
+    const int head = g * a.group + row_in_tile % a.group;
+    const uint32_t lane_base = tmem_base + (uint32_t(quarter * 32) << 16);
+    const uint32_t s_tmem = lane_base + t * 128;
+    const uint32_t o_tmem = lane_base + 256 + t * 128;
+    float row_scale;
+
+    // ---- this thread's row of Q as e4m3 parts
+    {
+      const uint16_t* src = a.q + (long long)(row0 + token) * a.q_row + (long long)head * a.q_head;
+      uint4 w[D / 8];
+      float size = 0.f;
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) w[c] = live ? *reinterpret_cast<const uint4*>(src + c * 8) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) {
+        const uint32_t words[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 v = unpack<BF16>(words[e]);
+          size = fmaxf(size, fmaxf(fabsf(v.x), fabsf(v.y)));
+        }
+      }
+      const int up = max(-120, min(126, 7 - (int(__float_as_uint(size) >> 23) - 127)));
+      const float by = copysignf(__uint_as_float(uint32_t(up + 127) << 23), a.scale_log2);
+      row_scale = __uint_as_float(uint32_t(127 - up) << 23) * fabsf(a.scale_log2);
+      if (size > 3.4028234663852886e38f) row_scale = __int_as_float(0x7fffffff);  // no factor brings an infinity back
+      const uint32_t row_addr = q_addr + t * L::kQBytes + row_in_tile * 128;
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c) {
+        float v[16];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint4& x = w[2 * c + (e >> 2)];
+          const float2 y = unpack<BF16>((e & 3) == 0 ? x.x : (e & 3) == 1 ? x.y : (e & 3) == 2 ? x.z : x.w);
+          v[2 * e] = y.x * by;
+          v[2 * e + 1] = y.y * by;
+        }
+#pragma unroll
+        for (int part = 0; part < Parts; ++part) {
+          uint32_t code[4];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            uint16_t two;
+            asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(two) : "f"(v[2 * e + 1]), "f"(v[2 * e]));
+            const uint32_t h = halves_of(two);
+            const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&h));
+            v[2 * e] -= back.x;
+            v[2 * e + 1] -= back.y;
+            code[e >> 1] = (e & 1) ? code[e >> 1] | uint32_t(two) << 16 : uint32_t(two);
+          }
+          const uint32_t chunk = uint32_t((part % L::kPerRow) * (D / 16) + c);
+          st_shared_16(row_addr + (part / L::kPerRow) * L::kBlockBytes + ((chunk ^ (uint32_t(row_in_tile) & 7u)) << 4), code[0],
+                       code[1], code[2], code[3]);
+        }
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+    }
+
+    const int sees = live ? max(0, min(context, context - n + token + 1)) : 0;  // keys of this row
+    ScaleAhead scales = {table, a.k.scale, a.page_shift, pages, a.num_pages, a.kv_heads, g, lane, 1.f, 0, 0.f};
+    if (nt > 0) scales.start(j0);
+    float m_ref = kNone, l = 0.f;
+    bool ok = true;
+
+    for (int j = 0; j < nt; ++j) {
+      const float scale_lane = scales.take(j0 + j);
+      float scale[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float x = __shfl_sync(0xffffffffu, scale_lane, i) * row_scale;
+        scale[i] = x < 0x1p-126f ? 0x1p-126f : x;  // never 0: a masked score is -inf times this
+      }
+      if (!__all_sync(0xffffffffu, mbar_wait(s_full + 8 * t, j & 1, abort_flag, status, kSiteScores))) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      uint32_t s[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld_32x32(s_tmem + c * 32, s[c]);
+      tmem_ld_wait(s[0]);
+      tie(s[1]);
+      tie(s[2]);
+      tie(s[3]);
+
+      const int visible = sees - (j0 + j) * kTileKV;
+      if (visible < kTileKV) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          if (i >= visible) s[0][i] = 0xff800000u;
+          if (32 + i >= visible) s[1][i] = 0xff800000u;
+          if (64 + i >= visible) s[2][i] = 0xff800000u;
+          if (96 + i >= visible) s[3][i] = 0xff800000u;
+        }
+      }
+      float m_new = m_ref;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        float mx = __uint_as_float(s[c >> 1][(c & 1) * 16]);
+#pragma unroll
+        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, __uint_as_float(s[c >> 1][(c & 1) * 16 + i]));
+        if (c * 16 < visible) m_new = fmaxf(m_new, mx * scale[c]);  // a group out of sight has no scale
+      }
+      if (j == 0) {
+        m_ref = m_new;
+      } else {
+        const bool moved = m_new - m_ref > kRescaleThreshold;
+        if (__any_sync(0xffffffffu, moved)) {
+          // S_t(j) was issued after P_t(j-1) V(j-1), so O_t is complete and idle until p_full is signalled
+          const float corr = moved ? ex2_approx(m_ref - m_new) : 1.0f;
+          l *= corr;
+          if (moved) m_ref = m_new;
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld_32x32(o_tmem + c * 32, o);
+            tmem_ld_wait(o);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+            tmem_st_32x32(o_tmem + c * 32, o);
+          }
+        }
+      }
+      // p = exp2(s * scale - m_ref), summed in f32 before the rounding to f16
+      const float2 shift2 = make_float2(-m_ref, -m_ref);
+      float2 sum[4];
+      uint32_t packed[2][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) sum[c] = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float by = scale[2 * c + (i >> 3)];
+          const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[c][2 * i]), __uint_as_float(s[c][2 * i + 1])),
+                                      make_float2(by, by), shift2);
+          const float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+          sum[c] = __fadd2_rn(sum[c], e);
+          packed[c >> 1][(c & 1) * 16 + i] = pack_f16x2(e.x, e.y);
+        }
+      }
+      const float2 all = __fadd2_rn(__fadd2_rn(sum[0], sum[1]), __fadd2_rn(sum[2], sum[3]));
+      l += all.x + all.y;
+      tmem_st_32x32(s_tmem, packed[0]);       // keys 0..63  -> columns 0..31
+      tmem_st_32x32(s_tmem + 32, packed[1]);  // keys 64..127 -> columns 32..63
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_full + 8 * t);
+    }
+
+    // ---- O_t over l, or a split's share of it
+    if (nt > 0 && ok) ok = __all_sync(0xffffffffu, mbar_wait(o_full + 8 * t, 0, abort_flag, status, kSiteOutput));
+    if (ok) {
+      tc_fence_after();
+      const bool split = p.splits > 1;
+      float* share = p.partial + (((long long)blockIdx.y * a.rows + row0 + token) * a.q_heads + head) * (D + 4);
+      uint16_t* out = a.o + (long long)(row0 + token) * a.o_row + (long long)head * a.o_head;
+      const float unit = top * (1.0f / 128.0f);
+      const float by = split ? unit : l == 0.f ? 0.f : unit / l;
+      if (split && live) *reinterpret_cast<float2*>(share) = make_float2(nt > 0 ? m_ref : kNone, l);
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        __syncwarp();
+        if (nt > 0) {
+          tmem_ld_32x32(o_tmem + c * 32, o);
+          tmem_ld_wait(o);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0;
+        }
+        if (live && split) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            *reinterpret_cast<float4*>(share + 4 + c * 32 + i * 4) =
+                make_float4(__uint_as_float(o[4 * i]) * by, __uint_as_float(o[4 * i + 1]) * by,
+                            __uint_as_float(o[4 * i + 2]) * by, __uint_as_float(o[4 * i + 3]) * by);
+          }
+        } else if (live) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float x = l == 0.f ? 0.f : __uint_as_float(o[8 * i + 2 * e]) * by;
+              const float y = l == 0.f ? 0.f : __uint_as_float(o[8 * i + 2 * e + 1]) * by;
+              w[e] = BF16 ? pack_bf16x2(x, y) : pack_f16x2(x, y);
+            }
+            *reinterpret_cast<uint4*>(out + c * 32 + i * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+      }
+    }
+  }
+
+  // ------------------------------------------------------------------ teardown
+  if (*abort_flag != 0) {
+    for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc<1>(tmem_base, 512);
+  }
+}
+
+// Joins the splits, a warp per (row, q head). Rows of requests that were streamed, and rows behind the last request, are
+// not touched.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(128) cache_tile_join_kernel(TileParams p) {
+  constexpr int kCols = D / 32;
+  const CacheAttnParams& a = p.a;
+  const int row = blockIdx.x, head = blockIdx.y * 4 + (threadIdx.x >> 5), lane = int(lane_id());
+  if (head >= a.q_heads || row >= a.row_start[a.batch]) return;
+  int low = 0, high = a.batch;  // the last request that starts at or before the row
+  while (high - low > 1) {
+    const int mid = (low + high) >> 1;
+    if (a.row_start[mid] <= row) low = mid; else high = mid;
+  }
+  if (blocks_of(p, low) == 0) return;
+  const float* from = p.partial + ((long long)row * a.q_heads + head) * (D + 4);
+  const long long stride = (long long)a.rows * a.q_heads * (D + 4);
+  float m = kNone, l = 0.f, acc[kCols];
+#pragma unroll
+  for (int c = 0; c < kCols; ++c) acc[c] = 0.f;
+  for (int s = 0; s < p.splits; ++s) {
+    const float2 ml = *reinterpret_cast<const float2*>(from + s * stride);
+    if (ml.y == 0.f) continue;  // no key of this split was seen
+    const float m_new = fmaxf(m, ml.x);
+    const float old = exp2f(m - m_new), now = exp2f(ml.x - m_new);
+    m = m_new;
+    l = l * old + ml.y * now;
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) acc[c] = acc[c] * old + from[s * stride + 4 + c * 32 + lane] * now;
+  }
+  const float by = l == 0.f ? 0.f : 1.0f / l;
+  uint16_t* out = a.o + (long long)row * a.o_row + (long long)head * a.o_head;
+#pragma unroll
+  for (int c = 0; c < kCols; ++c) {
+    const float y = acc[c] * by;
+    out[c * 32 + lane] = uint16_t((BF16 ? pack_bf16x2(y, 0.f) : pack_f16x2(y, 0.f)) & 0xffffu);
+  }
+}
+
+// Blocks that the grid needs at most: every tiled request has more than `few` rows.
+int64_t blocks_bound(int64_t batch, int64_t rows, int64_t group, int64_t few) {
+  const int64_t least = few / group + 1, tokens = 2 * (kTileQ / group);
+  const int64_t requests = rows / least < batch ? rows / least : batch;
+  return rows / tokens + requests;
+}
+
+// Shares of the keys: as many as fill the GPU where there are few blocks, none shorter than four key tiles.
+int64_t splits_of(int64_t blocks, int64_t max_context) {
+  if (blocks <= 0) return 1;
+  const int64_t room = kSMs / blocks, tiles = (max_context + 4 * kTileKV - 1) / (4 * kTileKV);
+  const int64_t splits = room < tiles ? room : tiles;
+  return splits < 1 ? 1 : splits;
+}
+
+template <int D, bool BF16>
+int launch(const DeviceContext* ctx, const TileParams& p, int64_t page_size, int64_t blocks, cudaStream_t stream) {
+  const CacheAttnParams& a = p.a;
+  using L = Layout<D, BF16 ? 2 : 3>;
+  CUtensorMap map_k, map_v;
+  const uint32_t box = uint32_t(page_size < kTileKV ? page_size : kTileKV);
+  const Swizzle swizzle = D == 128 ? Swizzle::k128B : Swizzle::k64B;
+  if (int rc = encode_pool(&map_k, a.k, D, a.kv_heads, page_size, a.num_pages, box, swizzle)) return rc;
+  if (int rc = encode_pool(&map_v, a.v, D, a.kv_heads, page_size, a.num_pages, box, Swizzle::kNone)) return rc;
+  auto kernel = cache_tile_kernel<D, BF16>;
+  KRNB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmemBytes));
+  // setmaxnreg.inc blocks until the CTA's register pool can cover it: 128 x (R - 56) must reach 256 x (224 - R)
+  cudaFuncAttributes attributes;
+  KRNB_CUDA(cudaFuncGetAttributes(&attributes, kernel));
+  if ((attributes.numRegs - 56) * 128 < (224 - attributes.numRegs) * 256) {
+    return fail(KRN_B200_ERR_UNSUPPORTED, "cache attention kernel was built with %d registers per thread; the register "
+                "re-partitioning needs at least 168", attributes.numRegs);
+  }
+  kernel<<<dim3(unsigned(blocks * a.kv_heads), unsigned(p.splits)), kThreads, L::kSmemBytes, stream>>>(map_k, map_v, p,
+                                                                                                    ctx->status_dev);
+  KRNB_CUDA(cudaGetLastError());
+  if (p.splits > 1) {
+    cache_tile_join_kernel<D, BF16><<<dim3(unsigned(a.rows), unsigned((a.q_heads + 3) / 4)), 128, 0, stream>>>(p);
+    KRNB_CUDA(cudaGetLastError());
+  }
+  return KRN_B200_OK;
+}
+
+}  // namespace
+
+int64_t tile_workspace(int64_t batch, int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t d, int64_t few, int64_t max_context) {
+  const int64_t splits = splits_of(blocks_bound(batch, rows, q_heads / kv_heads, few) * kv_heads, max_context);
+  return splits > 1 ? splits * rows * q_heads * (d + 4) * 4 : 0;
+}
+
+int launch_tiles(const DeviceContext* ctx, const CacheAttnParams& a, bool bf16, int64_t d, int64_t page_size, float* partial,
+                 cudaStream_t stream) {
+  TileParams p;
+  p.a = a;
+  p.partial = partial;
+  p.tokens = kTileQ / a.group;
+  const int64_t blocks = blocks_bound(a.batch, a.rows, a.group, a.few);
+  if (blocks == 0) return KRN_B200_OK;
+  p.splits = int(splits_of(blocks * a.kv_heads, a.max_context));
+  if (d == 128) return bf16 ? launch<128, true>(ctx, p, page_size, blocks, stream) : launch<128, false>(ctx, p, page_size, blocks, stream);
+  return bf16 ? launch<64, true>(ctx, p, page_size, blocks, stream) : launch<64, false>(ctx, p, page_size, blocks, stream);
+}
+
+}  // namespace krnb

@@ -111,7 +111,8 @@ def attention(q, k_codes, v_codes, k_scale, v_scale, table, context, start, *, p
       delta = scale * 2^-8 * sum |q k| (largest over the keys) and a weight by exp(2 delta) - 1;
     * f32 sums of up to a few hundred products and the exponential: below 2^-14 of delta's sum and 2^-20 of a weight;
     * a weight is rounded to f16, at most 2^-11 of it, or 2^-25 of the largest: 2^-11 A, and with up to 2^17 keys of
-      equal weight 2^-8 ulp-sized terms stay below another 2^-11 A."""
+      equal weight 2^-8 ulp-sized terms stay below another 2^-11 A;
+    * a page's value scale, relative to the largest, is rounded to f16 and so is its product with a value: 2^-11 A each."""
     rows, q_heads, d = q.shape
     heads = k_codes.shape[2]
     out = np.array(untouched, np.float64)
@@ -139,5 +140,5 @@ def attention(q, k_codes, v_codes, k_scale, v_scale, table, context, start, *, p
                 a = w[seen[i]] @ np.abs(v[seen[i]])
                 out[start[b] + i, h] = w[seen[i]] @ v[seen[i]]
                 delta = moved[i] * (2.0 ** -8 + 2.0 ** -14)
-                bound[start[b] + i, h] = a * (math.expm1(2 * delta) + 2.0 ** -10 + 2.0 ** -18)
+                bound[start[b] + i, h] = a * (math.expm1(2 * delta) + 4 * 2.0 ** -11 + 2.0 ** -17)
     return out, bound
