@@ -468,7 +468,13 @@ extern "C" int krn_b200_cache_plan(const int32_t* context_len, const int32_t* ne
                   table_pitch, int(batch), int(max_pages), shift_of(page_size), int(rows), int(runs_len), int(num_pages),
                   int(capacity)};
   const size_t smem = plan_smem_bytes(batch);
-  KRNB_CUDA(cudaFuncSetAttribute(cache_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(plan_smem_bytes(kMaxBatch))));
+  static OncePerDevice ready;
+  if (int rc = ready(ctx->device, [] {
+        KRNB_CUDA(cudaFuncSetAttribute(cache_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(plan_smem_bytes(kMaxBatch))));
+        return KRN_B200_OK;
+      })) {
+    return rc;
+  }
   const int64_t wanted = (rows + kPlanThreads - 1) / kPlanThreads;
   const int blocks = int(wanted < 1 ? 1 : wanted > ctx->sm_count ? ctx->sm_count : wanted);
   cache_plan_kernel<<<blocks, kPlanThreads, smem, static_cast<cudaStream_t>(stream_handle)>>>(p, ctx->status_dev);

@@ -575,7 +575,13 @@ int launch_stream(const DeviceContext* ctx, const StreamParams& p, int64_t page_
   if (int rc = encode_pool(&map_k, a.k, D, a.kv_heads, page_size, a.num_pages, box, swizzle)) return rc;
   if (int rc = encode_pool(&map_v, a.v, D, a.kv_heads, page_size, a.num_pages, box, swizzle)) return rc;
   auto kernel = cache_stream_kernel<D, BF16, NT>;
-  KRNB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, StreamLayout<D>::bytes(kMaxBatch)));
+  static OncePerDevice ready;
+  if (int rc = ready(ctx->device, [&] {
+        KRNB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, StreamLayout<D>::bytes(kMaxBatch)));
+        return KRN_B200_OK;
+      })) {
+    return rc;
+  }
   const int64_t tiles = int64_t(a.batch) * a.kv_heads * ((a.max_context + kTile - 1) / kTile);
   const int most = ctx->sm_count < kMaxBlocks ? ctx->sm_count : kMaxBlocks;
   const int blocks = int(tiles < most ? tiles : most);

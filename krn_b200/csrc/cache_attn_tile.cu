@@ -714,13 +714,19 @@ int launch(const DeviceContext* ctx, const TileParams& p, int64_t page_size, int
   if (int rc = encode_pool(&map_k, a.k, D, a.kv_heads, page_size, a.num_pages, box, swizzle)) return rc;
   if (int rc = encode_pool(&map_v, a.v, D, a.kv_heads, page_size, a.num_pages, box, Swizzle::kNone)) return rc;
   auto kernel = cache_tile_kernel<D, BF16>;
-  KRNB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmemBytes));
-  // setmaxnreg.inc blocks until the CTA's register pool can cover it: 128 x (R - 56) must reach 256 x (224 - R)
-  cudaFuncAttributes attributes;
-  KRNB_CUDA(cudaFuncGetAttributes(&attributes, kernel));
-  if ((attributes.numRegs - 56) * 128 < (224 - attributes.numRegs) * 256) {
-    return fail(KRN_B200_ERR_UNSUPPORTED, "cache attention kernel was built with %d registers per thread; the register "
-                "re-partitioning needs at least 168", attributes.numRegs);
+  static OncePerDevice ready;
+  if (int rc = ready(ctx->device, [&] {
+        KRNB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmemBytes));
+        // setmaxnreg.inc blocks until the CTA's register pool can cover it: 128 x (R - 56) must reach 256 x (224 - R)
+        cudaFuncAttributes attributes;
+        KRNB_CUDA(cudaFuncGetAttributes(&attributes, kernel));
+        if ((attributes.numRegs - 56) * 128 < (224 - attributes.numRegs) * 256) {
+          return fail(KRN_B200_ERR_UNSUPPORTED, "cache attention kernel was built with %d registers per thread; the register "
+                      "re-partitioning needs at least 168", attributes.numRegs);
+        }
+        return KRN_B200_OK;
+      })) {
+    return rc;
   }
   kernel<<<dim3(unsigned(blocks * a.kv_heads), unsigned(p.splits)), kThreads, L::kSmemBytes, stream>>>(map_k, map_v, p,
                                                                                                     ctx->status_dev);

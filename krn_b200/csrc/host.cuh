@@ -6,6 +6,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 
@@ -51,6 +52,24 @@ DeviceContext* existing_context();
 
 // Refuse anything that is not a compute-capability 10.x device.
 int require_sm100(const DeviceContext* ctx);
+
+// Runs `set_up` (a function that returns a status) the first time a device is met: kernel attributes stay set, and asking
+// the runtime for them again costs a launch of a few microseconds a good part of its time. Two threads that meet a device
+// together both run it.
+class OncePerDevice {
+ public:
+  template <class SetUp>
+  int operator()(int device, SetUp set_up) {
+    const uint64_t bit = uint64_t(1) << (device & 63);
+    if (done_.load(std::memory_order_acquire) & bit) return KRN_B200_OK;
+    if (int rc = set_up()) return rc;
+    done_.fetch_or(bit, std::memory_order_release);
+    return KRN_B200_OK;
+  }
+
+ private:
+  std::atomic<uint64_t> done_{0};
+};
 
 // ---- TMA descriptors -----------------------------------------------------------------------------------
 

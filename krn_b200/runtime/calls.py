@@ -270,74 +270,105 @@ def attention_decode_fp8_paged_noalloc(q: Any, k_pages: Any, v_pages: Any, page_
     native.check(status, "paged FP8 decode attention (built-in scratch)")
 
 
-def _on_device(feature: str, **tensors: Any) -> None:
-    """Every tensor lives on the current CUDA device: an address of host memory or of another GPU never reaches a kernel."""
-    import torch
-
-    current = torch.cuda.current_device() if torch.cuda.is_available() else None
-    for name, tensor in tensors.items():
-        if not getattr(tensor, "is_cuda", False):
-            raise ValueError(f"{feature}: `{name}` must be a CUDA tensor")
-        if tensor.device.index != current:
-            raise ValueError(f"{feature}: `{name}` is on {tensor.device}, the current device is cuda:{current}")
+_Strides2, _Strides3 = ctypes.c_int64 * 2, ctypes.c_int64 * 3
 
 
-def _vector(feature: str, name: str, tensor: Any, dtype: str, length: int | None = None) -> int:
-    """The address of a contiguous rank-1 tensor of `dtype` (and of `length` elements)."""
-    if str(tensor.dtype) != "torch." + dtype:
-        raise TypeError(f"{feature}: `{name}` must be {dtype}, got {tensor.dtype}")
-    if tensor.dim() != 1 or (tensor.shape[0] > 1 and tensor.stride(0) != 1):
-        raise ValueError(f"{feature}: `{name}` must be a contiguous vector, got shape {tuple(tensor.shape)}")
-    if length is not None and tensor.shape[0] != length:
-        raise ValueError(f"{feature}: `{name}` has {tensor.shape[0]} elements, {length} expected")
-    return tensor.data_ptr()
+class _Place:
+    """Checks of one call's tensors and their addresses. Every tensor lives on the current CUDA device: an address of host
+    memory or of another GPU never reaches a kernel. These run before every launch of kernels of a few microseconds, so
+    they ask a tensor for as little as they can."""
 
+    __slots__ = ("feature", "torch", "device")
 
-def _table(feature: str, name: str, tensor: Any, batch: int) -> tuple[int, int, int]:
-    """(address, entries per row, row pitch) of an int32 page table [batch, entries]."""
-    if str(tensor.dtype) != "torch.int32":
-        raise TypeError(f"{feature}: `{name}` must be int32, got {tensor.dtype}")
-    if tensor.dim() != 2 or tensor.shape[0] != batch or (tensor.shape[1] > 1 and tensor.stride(1) != 1):
-        raise ValueError(f"{feature}: `{name}` must be [{batch}, entries] with contiguous rows, got shape {tuple(tensor.shape)}")
-    entries = tensor.shape[1]
-    return tensor.data_ptr(), entries, tensor.stride(0) if batch > 1 else max(entries, 1)
+    def __init__(self, feature: str) -> None:
+        import torch
 
+        self.feature, self.torch, self.device = feature, torch, -2
 
-def _outer_strides(feature: str, name: str, tensor: Any, written: bool) -> Any:
-    """Element strides of the outer axes of a tensor whose last axis is contiguous; an axis of one element counts as packed.
-    A tensor that is written must not overlap itself."""
-    shape, strides = tuple(tensor.shape), list(tensor.stride())
-    if shape[-1] > 1 and strides[-1] != 1:
-        raise ValueError(f"{feature}: the last axis of `{name}` must be contiguous")
-    for i in range(len(shape) - 1):
-        if shape[i] <= 1:
-            strides[i] = shape[-1]
-    if written:
-        room = shape[-1]
-        for stride, size in sorted((strides[i], shape[i]) for i in range(len(shape) - 1) if shape[i] > 1):
-            if stride < room:
-                raise ValueError(f"{feature}: `{name}` is written and must not overlap itself (shape {shape}, strides {tuple(tensor.stride())})")
-            room = stride * (size - 1) + room
-    return (ctypes.c_int64 * (len(shape) - 1))(*strides[:-1])
+    def address(self, name: str, tensor: Any) -> int:
+        place = tensor.get_device() if hasattr(tensor, "get_device") else -1
+        if place != self.device:
+            if place < 0:
+                raise ValueError(f"{self.feature}: `{name}` must be a CUDA tensor")
+            self.device = self.torch.cuda.current_device()
+            if place != self.device:
+                raise ValueError(f"{self.feature}: `{name}` is on cuda:{place}, the current device is cuda:{self.device}")
+        return tensor.data_ptr()
 
+    def vector(self, name: str, tensor: Any, dtype: Any, length: int = -1) -> int:
+        """A contiguous rank-1 tensor of `dtype` (and of `length` elements)."""
+        address = self.address(name, tensor)
+        if tensor.dtype is not dtype:
+            raise TypeError(f"{self.feature}: `{name}` must be {str(dtype)[6:]}, got {tensor.dtype}")
+        if tensor.dim() != 1 or not tensor.is_contiguous():
+            raise ValueError(f"{self.feature}: `{name}` must be a contiguous vector, got shape {tuple(tensor.shape)}")
+        if length >= 0 and tensor.numel() != length:
+            raise ValueError(f"{self.feature}: `{name}` has {tensor.numel()} elements, {length} expected")
+        return address
 
-_BYTES = ("torch.uint8", "torch.float8_e4m3fn")
+    def table(self, name: str, tensor: Any, batch: int) -> tuple[int, int, int]:
+        """(address, entries per row, row pitch) of an int32 page table [batch, entries]."""
+        address = self.address(name, tensor)
+        if tensor.dtype is not self.torch.int32:
+            raise TypeError(f"{self.feature}: `{name}` must be int32, got {tensor.dtype}")
+        shape = tensor.shape
+        if len(shape) != 2 or shape[0] != batch or (shape[1] > 1 and tensor.stride(1) != 1):
+            raise ValueError(f"{self.feature}: `{name}` must be [{batch}, entries] with contiguous rows, got shape {tuple(shape)}")
+        return address, shape[1], tensor.stride(0) if batch > 1 else max(shape[1], 1)
 
+    def element(self, name: str, tensor: Any) -> int:
+        """The element type of keys, values and queries."""
+        torch, dtype = self.torch, tensor.dtype
+        if dtype is torch.bfloat16:
+            return native.BF16
+        if dtype is torch.float16:
+            return native.F16
+        return _type_of(tensor)
 
-def _pool(feature: str, k_pages: Any, v_pages: Any, k_scale: Any, v_scale: Any, written: bool) -> tuple[Any, Any]:
-    """Checks of a paged cache: codes [pages, page size, kv heads, d], scales [pages, kv heads]; the pools' byte strides."""
-    shape = tuple(k_pages.shape)
-    if len(shape) != 4 or tuple(v_pages.shape) != shape:
-        raise ValueError(f"{feature}: page pools are [pages, page size, kv heads, d], got {shape} and {tuple(v_pages.shape)}")
-    for name, pages in (("k_pages", k_pages), ("v_pages", v_pages)):
-        if str(pages.dtype) not in _BYTES:
-            raise TypeError(f"{feature}: `{name}` holds e4m3 codes (float8_e4m3fn or uint8), got {pages.dtype}")
-    for name, scale in (("k_scale", k_scale), ("v_scale", v_scale)):
-        if str(scale.dtype) != "torch.float32":
-            raise TypeError(f"{feature}: `{name}` must be float32, got {scale.dtype}")
-        if tuple(scale.shape) != (shape[0], shape[2]) or not scale.is_contiguous():
-            raise ValueError(f"{feature}: `{name}` must be contiguous [{shape[0]}, {shape[2]}], got {tuple(scale.shape)}")
-    return _outer_strides(feature, "k_pages", k_pages, written), _outer_strides(feature, "v_pages", v_pages, written)
+    def pool(self, cache: tuple[Any, Any, Any, Any], written: bool) -> tuple[tuple[int, ...], Any, Any]:
+        """Checks of a paged cache: codes [pages, page size, kv heads, d], scales [pages, kv heads]; the four addresses and
+        the pools' byte strides."""
+        torch, feature = self.torch, self.feature
+        k_pages, v_pages, k_scale, v_scale = cache
+        addresses = (self.address("k_pages", k_pages), self.address("v_pages", v_pages), self.address("k_scale", k_scale),
+                     self.address("v_scale", v_scale))
+        shape = k_pages.shape
+        if len(shape) != 4 or v_pages.shape != shape:
+            raise ValueError(f"{feature}: page pools are [pages, page size, kv heads, d], got {tuple(shape)} and {tuple(v_pages.shape)}")
+        for name, pages in (("k_pages", k_pages), ("v_pages", v_pages)):
+            if pages.dtype is not torch.uint8 and pages.dtype is not torch.float8_e4m3fn:
+                raise TypeError(f"{feature}: `{name}` holds e4m3 codes (float8_e4m3fn or uint8), got {pages.dtype}")
+        for name, scale in (("k_scale", k_scale), ("v_scale", v_scale)):
+            if scale.dtype is not torch.float32:
+                raise TypeError(f"{feature}: `{name}` must be float32, got {scale.dtype}")
+            if scale.shape != (shape[0], shape[2]) or not scale.is_contiguous():
+                raise ValueError(f"{feature}: `{name}` must be contiguous [{shape[0]}, {shape[2]}], got {tuple(scale.shape)}")
+        return addresses, self.strides("k_pages", k_pages, written), self.strides("v_pages", v_pages, written)
+
+    def strides(self, name: str, tensor: Any, written: bool) -> Any:
+        """Element strides of the outer axes of a tensor whose last axis is contiguous; an axis of one element counts as
+        packed. A tensor that is written must not overlap itself."""
+        shape, strides = tensor.shape, tensor.stride()
+        outer = len(shape) - 1
+        of = _Strides2 if outer == 2 else _Strides3
+        if tensor.is_contiguous() and 1 not in shape:
+            return of(*strides[:outer])
+        if shape[outer] > 1 and strides[outer] != 1:
+            raise ValueError(f"{self.feature}: the last axis of `{name}` must be contiguous")
+        strides = [strides[i] if shape[i] > 1 else shape[outer] for i in range(outer)]
+        if written:
+            room = shape[outer]
+            for stride, size in sorted((strides[i], shape[i]) for i in range(outer) if shape[i] > 1):
+                if stride < room:
+                    raise ValueError(f"{self.feature}: `{name}` is written and must not overlap itself (shape {tuple(shape)}, "
+                                     f"strides {tuple(tensor.stride())})")
+                room = stride * (size - 1) + room
+        return of(*strides)
+
+    def stream(self, stream: Any) -> Any:
+        """As `_stream`, without the objects that torch makes around its current stream."""
+        raw = getattr(self.torch._C, "_cuda_getCurrentRawStream", None)
+        return raw(self.device) if stream is None and raw is not None else _stream(stream)
 
 
 def cache_runs(rows: int, batch: int, page_size: int) -> int:
@@ -348,42 +379,37 @@ def cache_plan(context_len: Any, new_len: Any, page_table: Any, free_pages: Any,
                row_start: Any, slot_map: Any, runs: Any, state_out: Any, page_size: int, num_pages: int,
                stream: Any = None) -> None:
     """Pages, slots and page runs of a step's new tokens from request lengths (see krn_b200_cache_plan)."""
-    feature = "cache plan"
-    _on_device(feature, context_len=context_len, new_len=new_len, page_table=page_table, free_pages=free_pages,
-               pool_state=pool_state, context_out=context_out, row_start=row_start, slot_map=slot_map, runs=runs,
-               state_out=state_out)
+    at = _Place("cache plan")
+    int32, int64 = at.torch.int32, at.torch.int64
+    context = at.vector("context_len", context_len, int32)
     batch = context_len.shape[0]
-    lengths = _vector(feature, "context_len", context_len, "int32"), _vector(feature, "new_len", new_len, "int32", batch)
-    table, entries, pitch = _table(feature, "page_table", page_table, batch)
-    ring, state = _vector(feature, "free_pages", free_pages, "int32"), _vector(feature, "pool_state", pool_state, "int64", 3)
-    outputs = (_vector(feature, "context_out", context_out, "int32", batch), _vector(feature, "row_start", row_start, "int32", batch + 1),
-               _vector(feature, "slot_map", slot_map, "int64"), _vector(feature, "runs", runs, "int32"),
-               _vector(feature, "state_out", state_out, "int64", 3))
+    brings = at.vector("new_len", new_len, int32, batch)
+    table, entries, pitch = at.table("page_table", page_table, batch)
     status = native.library().krn_b200_cache_plan(
-        *lengths, table, ring, state, *outputs, batch, entries, pitch, free_pages.shape[0], page_size, num_pages,
-        slot_map.shape[0], runs.shape[0], _stream(stream))
-    native.check(status, feature)
+        context, brings, table, at.vector("free_pages", free_pages, int32), at.vector("pool_state", pool_state, int64, 3),
+        at.vector("context_out", context_out, int32, batch), at.vector("row_start", row_start, int32, batch + 1),
+        at.vector("slot_map", slot_map, int64), at.vector("runs", runs, int32), at.vector("state_out", state_out, int64, 3), batch,
+        entries, pitch, free_pages.shape[0], page_size, num_pages, slot_map.shape[0], runs.shape[0], at.stream(stream))
+    native.check(status, at.feature)
 
 
 def cache_append(k: Any, v: Any, slot_map: Any, runs: Any, k_pages: Any, v_pages: Any, k_scale: Any, v_scale: Any,
                  stream: Any = None) -> None:
     """Quantise rows of keys and values [rows, kv heads, d] into the pool (see krn_b200_cache_append)."""
-    feature = "cache append"
-    _on_device(feature, k=k, v=v, slot_map=slot_map, runs=runs, k_pages=k_pages, v_pages=v_pages, k_scale=k_scale,
-               v_scale=v_scale)
-    k_page_strides, v_page_strides = _pool(feature, k_pages, v_pages, k_scale, v_scale, True)
+    at = _Place("cache append")
+    keys, values = at.address("k", k), at.address("v", v)
+    pool, k_page_strides, v_page_strides = at.pool((k_pages, v_pages, k_scale, v_scale), True)
     num_pages, page_size, heads, d = k_pages.shape
-    if k.dim() != 3 or tuple(k.shape) != tuple(v.shape) or tuple(k.shape[1:]) != (heads, d):
-        raise ValueError(f"{feature}: k {tuple(k.shape)} and v {tuple(v.shape)} do not match a pool of {heads} heads of {d}")
-    if _type_of(k) != _type_of(v):
-        raise TypeError(f"{feature}: k and v must have the same element type")
-    rows = min(k.shape[0], slot_map.shape[0])
+    shape = k.shape
+    if len(shape) != 3 or v.shape != shape or shape[1] != heads or shape[2] != d:
+        raise ValueError(f"{at.feature}: k {tuple(k.shape)} and v {tuple(v.shape)} do not match a pool of {heads} heads of {d}")
+    if k.dtype is not v.dtype:
+        raise TypeError(f"{at.feature}: k and v must have the same element type")
+    slots, starts = at.vector("slot_map", slot_map, at.torch.int64), at.vector("runs", runs, at.torch.int32)
     status = native.library().krn_b200_cache_append(
-        _type_of(k), k.data_ptr(), v.data_ptr(), _vector(feature, "slot_map", slot_map, "int64"),
-        _vector(feature, "runs", runs, "int32"), k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-        rows, runs.shape[0], heads, d, page_size, num_pages, _outer_strides(feature, "k", k, False),
-        _outer_strides(feature, "v", v, False), k_page_strides, v_page_strides, _stream(stream))
-    native.check(status, feature)
+        at.element("k", k), keys, values, slots, starts, *pool, min(shape[0], slot_map.shape[0]), runs.shape[0], heads, d, page_size,
+        num_pages, at.strides("k", k, False), at.strides("v", v, False), k_page_strides, v_page_strides, at.stream(stream))
+    native.check(status, at.feature)
 
 
 def cache_attention_workspace_bytes(batch: int, rows: int, q_heads: int, kv_heads: int, d: int, max_new: int,
@@ -395,24 +421,25 @@ def cache_attention(q: Any, k_pages: Any, v_pages: Any, k_scale: Any, v_scale: A
                     row_start: Any, o: Any, scale_log2: float, max_new: int, max_context: int, workspace: Any,
                     stream: Any = None) -> None:
     """Attention of packed query rows [rows, q heads, d] over the pool (see krn_b200_cache_attn)."""
-    feature = "cache attention"
-    _on_device(feature, q=q, k_pages=k_pages, v_pages=v_pages, k_scale=k_scale, v_scale=v_scale, page_table=page_table,
-               context_len=context_len, row_start=row_start, out=o, workspace=workspace)
-    k_page_strides, v_page_strides = _pool(feature, k_pages, v_pages, k_scale, v_scale, False)
+    at = _Place("cache attention")
+    queries, out, scratch = at.address("q", q), at.address("out", o), at.address("workspace", workspace)
+    pool, k_page_strides, v_page_strides = at.pool((k_pages, v_pages, k_scale, v_scale), False)
     num_pages, page_size, heads, d = k_pages.shape
-    if q.dim() != 3 or q.shape[2] != d or tuple(o.shape) != tuple(q.shape):
-        raise ValueError(f"{feature}: q {tuple(q.shape)} and out {tuple(o.shape)} do not match a pool of heads of {d}")
-    if _type_of(q) != _type_of(o):
-        raise TypeError(f"{feature}: q and out must have the same element type")
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != d or o.shape != shape:
+        raise ValueError(f"{at.feature}: q {tuple(q.shape)} and out {tuple(o.shape)} do not match a pool of heads of {d}")
+    if q.dtype is not o.dtype:
+        raise TypeError(f"{at.feature}: q and out must have the same element type")
+    context = at.vector("context_len", context_len, at.torch.int32)
     batch = context_len.shape[0]
-    table, entries, pitch = _table(feature, "page_table", page_table, batch)
+    table, entries, pitch = at.table("page_table", page_table, batch)
+    k_at, v_at, k_scale_at, v_scale_at = pool
     status = native.library().krn_b200_cache_attn(
-        _type_of(q), q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), table,
-        _vector(feature, "context_len", context_len, "int32"), _vector(feature, "row_start", row_start, "int32", batch + 1),
-        o.data_ptr(), batch, q.shape[0], q.shape[1], heads, d, page_size, num_pages, entries, pitch, max_new, max_context,
-        _outer_strides(feature, "q", q, False), _outer_strides(feature, "out", o, True), k_page_strides, v_page_strides,
-        scale_log2, workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream(stream))
-    native.check(status, feature)
+        at.element("q", q), queries, k_at, v_at, k_scale_at, v_scale_at, table, context,
+        at.vector("row_start", row_start, at.torch.int32, batch + 1), out, batch, shape[0], shape[1], heads, d, page_size, num_pages,
+        entries, pitch, max_new, max_context, at.strides("q", q, False), at.strides("out", o, True), k_page_strides, v_page_strides,
+        scale_log2, scratch, workspace.nbytes, at.stream(stream))
+    native.check(status, at.feature)
 
 
 def scatter_columns(slabs: Any, c_full: Any, ranks: int, stream: Any = None) -> None:

@@ -156,37 +156,41 @@ def test_host_tensors_are_refused() -> None:
         ops.cache_attention(x, cache, table, lengths, plan.row_start, x, max_new=1, max_context=64, workspace=x)
 
 
-def test_layout_checks() -> None:
-    """The stride checks behind the calls, on host tensors."""
+def test_layout_checks(monkeypatch) -> None:
+    """The checks behind the calls, on host tensors that pass for the device's."""
     import torch
 
+    at = calls._Place("t")
+    monkeypatch.setattr(calls._Place, "address", lambda self, name, tensor: tensor.data_ptr())
     x = torch.zeros(6, 4, 128)
-    assert list(calls._outer_strides("t", "x", x, True)) == [512, 128]
-    assert list(calls._outer_strides("t", "x", x.transpose(0, 1), True)) == [128, 512]
-    assert list(calls._outer_strides("t", "x", x[:, :1], True)) == [512, 128]
-    assert list(calls._outer_strides("t", "x", torch.zeros(6, 1, 128).as_strided((6, 1, 128), (128, 7, 1)), True)) == [128, 128]
-    assert list(calls._outer_strides("t", "x", x[:1].expand(6, 4, 128), False)) == [0, 128]
+    assert list(at.strides("x", x, True)) == [512, 128]
+    assert list(at.strides("x", x.transpose(0, 1), True)) == [128, 512]
+    assert list(at.strides("x", x[:, :1], True)) == [512, 128]
+    assert list(at.strides("x", torch.zeros(6, 1, 128).as_strided((6, 1, 128), (128, 7, 1)), True)) == [128, 128]
+    assert list(at.strides("x", x[:1].expand(6, 4, 128), False)) == [0, 128]
     with pytest.raises(ValueError, match="must not overlap"):
-        calls._outer_strides("t", "x", x[:1].expand(6, 4, 128), True)
+        at.strides("x", x[:1].expand(6, 4, 128), True)
     with pytest.raises(ValueError, match="must not overlap"):
-        calls._outer_strides("t", "x", torch.zeros(4096).as_strided((6, 4, 128), (256, 128, 1)), True)
+        at.strides("x", torch.zeros(4096).as_strided((6, 4, 128), (256, 128, 1)), True)
     with pytest.raises(ValueError, match="last axis"):
-        calls._outer_strides("t", "x", torch.zeros(6, 4, 256)[..., ::2], False)
+        at.strides("x", torch.zeros(6, 4, 256)[..., ::2], False)
     codes, scale = torch.zeros(3, 16, 2, 64, dtype=torch.uint8), torch.zeros(3, 2)
-    assert list(calls._pool("t", codes, codes, scale, scale, True)[0]) == [2048, 128, 64]
+    assert list(at.pool((codes, codes, scale, scale), True)[1]) == [2048, 128, 64]
     with pytest.raises(TypeError, match="e4m3"):
-        calls._pool("t", codes.to(torch.int8), codes, scale, scale, True)
+        at.pool((codes.to(torch.int8), codes, scale, scale), True)
     with pytest.raises(TypeError, match="float32"):
-        calls._pool("t", codes, codes, scale.double(), scale, True)
+        at.pool((codes, codes, scale.double(), scale), True)
     with pytest.raises(ValueError, match=r"contiguous \[3, 2\]"):
-        calls._pool("t", codes, codes, scale.t().contiguous().t(), scale, True)
+        at.pool((codes, codes, scale.t().contiguous().t(), scale), True)
     with pytest.raises(ValueError, match="page pools"):
-        calls._pool("t", codes, codes[:2], scale, scale, True)
+        at.pool((codes, codes[:2], scale, scale), True)
     with pytest.raises(TypeError, match="int32"):
-        calls._table("t", "page_table", torch.zeros(2, 4, dtype=torch.int64), 2)
+        at.table("page_table", torch.zeros(2, 4, dtype=torch.int64), 2)
     with pytest.raises(ValueError, match=r"\[3, entries\]"):
-        calls._table("t", "page_table", torch.zeros(2, 4, dtype=torch.int32), 3)
+        at.table("page_table", torch.zeros(2, 4, dtype=torch.int32), 3)
     with pytest.raises(ValueError, match="5 expected"):
-        calls._vector("t", "x", torch.zeros(4, dtype=torch.int32), "int32", 5)
+        at.vector("x", torch.zeros(4, dtype=torch.int32), torch.int32, 5)
     with pytest.raises(ValueError, match="contiguous vector"):
-        calls._vector("t", "x", torch.zeros(8, dtype=torch.int32)[::2], "int32")
+        at.vector("x", torch.zeros(8, dtype=torch.int32)[::2], torch.int32)
+    with pytest.raises(TypeError, match="must be int32, got torch.int64"):
+        at.vector("x", torch.zeros(8, dtype=torch.int64), torch.int32)
