@@ -74,37 +74,32 @@ __device__ __forceinline__ int tiles_of(const StreamParams& p, int b) {
   return max(1, (context + kTile - 1) / kTile);
 }
 
-// First tile of warp `w` of `warps` when `total` tiles are dealt evenly and in order.
-__device__ __forceinline__ int first_tile(int w, int warps, int total) { return int((long long)w * total / warps); }
+// The line of the batch's tiles, dealt evenly and in order to `parts` stretches: the first tile of stretch `part`.
+__device__ __forceinline__ int first_tile(int part, int parts, int total) { return int((long long)part * total / parts); }
 
-// Warps that share the tiles: one per tile while there are warps left.
-__device__ __forceinline__ int warps_used(int total, int warps) { return max(1, min(warps, total)); }
+// The stretch that holds tile `at`.
+__device__ __forceinline__ int stretch_of(int at, int parts, int total) { return int(((long long)(at + 1) * parts - 1) / total); }
 
-// One (request, kv head) and where a warp stands in it.
-struct Segment {
-  int b, g, tile, tiles;  // current tile, tiles of the segment
+// Stretches: one warp for each and kv head, one tile at least.
+__device__ __forceinline__ int stretches(int total, int warps, int kv_heads) { return max(1, min(warps / kv_heads, total)); }
+
+// Where a warp stands in the line.
+struct Spot {
+  int b, tile, tiles;  // request, tile of it, tiles it has
 };
 
-__device__ __forceinline__ Segment segment_at(const int32_t* tiles, int batch, int kv_heads, int at) {
+__device__ __forceinline__ Spot spot_at(const int32_t* tiles, int batch, int at) {
   int low = 0, high = batch;
   while (high - low > 1) {
     const int mid = (low + high) >> 1;
-    if (tiles[mid] * kv_heads <= at) low = mid; else high = mid;
+    if (tiles[mid] <= at) low = mid; else high = mid;
   }
-  Segment s;
-  s.b = low;
-  s.tiles = tiles[low + 1] - tiles[low];
-  const int rest = at - tiles[low] * kv_heads;
-  s.g = rest / s.tiles;
-  s.tile = rest - s.g * s.tiles;
-  return s;
+  return {low, at - tiles[low], tiles[low + 1] - tiles[low]};
 }
 
-__device__ __forceinline__ void step(Segment& s, const int32_t* tiles, int batch, int kv_heads) {
+__device__ __forceinline__ void step(Spot& s, const int32_t* tiles, int batch) {
   if (++s.tile < s.tiles) return;
   s.tile = 0;
-  if (++s.g < kv_heads) return;
-  s.g = 0;
   do {
     ++s.b;
   } while (s.b < batch && tiles[s.b + 1] == tiles[s.b]);
@@ -121,9 +116,11 @@ struct StreamLayout {
   static int bytes(int batch) { return 1024 + kRing + kScales + kBars + 16 + 4 * (batch + 1 + kWarps); }
 };
 
-// Few query rows against many keys: bound by HBM. The (request, kv head) segments of the batch, cut into tiles of 32
-// tokens, form one line; every warp of the grid takes an equal stretch of it and works alone, with a ring of TMA tiles of
-// its own, no block barrier after the start. NT * 8 rows (a request's new tokens x the q heads of the kv head) share a tile:
+// Few query rows against many keys: bound by HBM. The contexts of the batch, cut into tiles of 32 tokens, form one line;
+// it is dealt in equal stretches, and a warp takes one stretch for one kv head and works alone, with a ring of TMA tiles of
+// its own, no block barrier after the start. Neighbouring warps take the kv heads of one stretch, so that a token's heads,
+// which lie side by side in a page, are fetched at about the same time. NT * 8 rows (a request's new tokens x the q heads
+// of the kv head) share a tile:
 //   S^T[token, row] = K Q^T   (M = 16 tokens, N = 8 rows, K = 16 columns of d; K's codes become f16 exactly, q is f16 with a
 //                              power-of-two factor per row)
 //   running maximum and sum per row in f32; P^T = exp2(S - m) times the page's value scale, f16
@@ -195,311 +192,314 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       if (n > a.max_new) report_failure(status, kErrDeviceIndex, kSiteRows, uint32_t(n));
     }
   }
-  // consecutive stretches lie on different blocks, so a few of them use as many SMs
-  const int warps = warps_used(carry * a.kv_heads, int(gridDim.x) * kWarps);
-  const int me = warp * int(gridDim.x) + int(blockIdx.x);
-  const int begin = me < warps ? first_tile(me, warps, carry * a.kv_heads) : 0;
-  const int end = me < warps ? first_tile(me + 1, warps, carry * a.kv_heads) : 0;
+  const int total = carry, grid_warps = int(gridDim.x) * kWarps;
+  const int parts = stretches(total, grid_warps, a.kv_heads);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (begin >= end) return;
+  if (total == 0) return;
 
   const int page_mask = (1 << a.page_shift) - 1;
   const int box = min(kTile, page_mask + 1);  // tokens of one copy
   int bad_page = 0;
 
-  // ---- the stretch's tiles in order: page ids come 32 at a time, one per lane
-  Segment ahead = segment_at(tiles, a.batch, a.kv_heads, begin);
-  int ids = 0, ids_b = -1, ids_first = 0, ahead_pages = 0;
-  auto issue = [&](int number) {  // tile `number` of the stretch into its stage
-    const int stage = number % kStages;
-    const uint32_t bar = bars + 8 * stage, dst = ring + stage * L::kStage;
-    const int token = ahead.tile * kTile;
-    const int first_page = token >> a.page_shift;
-    if (ahead.b != ids_b || first_page < ids_first || first_page + 1 >= ids_first + 32) {
-      ids_b = ahead.b;
-      ids_first = first_page;
-      const int context = max(0, min(a.context_len[ahead.b], a.max_context));
-      ahead_pages = (context + page_mask) >> a.page_shift;
-      ids = first_page + lane < ahead_pages ? a.page_table[ahead.b * a.table_pitch + first_page + lane] : 0;
-    }
-    // sub-tile 0 / 1: tokens 0..15 / 16..31 for 16-token pages; else one copy of 32 tokens
-    const int part = box == kTile ? 0 : (lane & 1);
-    int page = __shfl_sync(0xffffffffu, ids, first_page + part - ids_first);
-    const bool there = first_page + part < ahead_pages;
-    const bool good = there && uint32_t(page) < uint32_t(a.num_pages);
-    if (there && !good) {
-      bad_page = page | int(0x80000000);
-      page = a.num_pages;  // one past the pool: TMA fills zeros
-    }
-    const int copies = kTile / box;
-    const int there_parts = min(copies, ahead_pages - first_page);
-    if (lane == 0) mbar_arrive_expect_tx(bar, uint32_t(max(0, there_parts)) * 2u * uint32_t(box) * D);
-    __syncwarp();
-    if (lane < 4) {
-      const bool keys = lane < 2;
-      if (there && (lane & 1) < copies) {
-        tma_load_4d(dst + (keys ? 0 : L::kSide) + part * box * D, keys ? &map_k : &map_v, 0, ahead.g, token & page_mask, page, bar);
-      }
-      const float* source = keys ? a.k.scale : a.v.scale;
-      copy_scale(scales + stage * 16 + lane * 4, source + (good ? (long long)page * a.kv_heads + ahead.g : 0), good, bar);
-    }
-    step(ahead, tiles, a.batch, a.kv_heads);
-  };
-  const int count = end - begin;
-  for (int i = 0; i < min(count, kStages); ++i) issue(i);
-
-  Segment at = segment_at(tiles, a.batch, a.kv_heads, begin);
-  float acc[kSteps][NT][4], m[NT][2], l[NT][2], row_scale[NT][2];
-  uint32_t query[NT][kSteps][2];
-  int limit[NT][2], context = 0, rows = 0, row0 = 0, nearest = 0;
-  float top = kLeastScale, from_top = 0.f;
-  int piece = 0;  // first tile of the current piece within its segment
   bool ok = true;
+  int done = 0;  // tiles of earlier units: the ring goes on
+  for (int unit = int(blockIdx.x) * kWarps + warp; unit < parts * a.kv_heads && ok; unit += grid_warps) {
+    const int part = unit / a.kv_heads, g = unit - part * a.kv_heads;
+    const int begin = first_tile(part, parts, total), count = first_tile(part + 1, parts, total) - begin;
 
-  for (int i = 0; i < count; ++i) {
-    if (i == 0 || at.tile == 0) {
-      // ---- a new piece: its rows of q as f16 with a power-of-two factor, and how far each row sees
-      piece = at.tile;
-      row0 = a.row_start[at.b];
-      const int n = a.row_start[at.b + 1] - row0;
-      rows = n * a.group;
-      context = max(0, min(a.context_len[at.b], a.max_context));
-      nearest = context - n + 1;
+    // ---- the stretch's tiles in order: page ids come 32 at a time, one per lane
+    Spot ahead = spot_at(tiles, a.batch, begin);
+    int ids = 0, ids_b = -1, ids_first = 0, ahead_pages = 0;
+    auto issue = [&](int number) {  // tile `number` of the stretch into its stage
+      const int stage = (done + number) % kStages;
+      const uint32_t bar = bars + 8 * stage, dst = ring + stage * L::kStage;
+      const int token = ahead.tile * kTile;
+      const int first_page = token >> a.page_shift;
+      if (ahead.b != ids_b || first_page < ids_first || first_page + 1 >= ids_first + 32) {
+        ids_b = ahead.b;
+        ids_first = first_page;
+        const int context = max(0, min(a.context_len[ahead.b], a.max_context));
+        ahead_pages = (context + page_mask) >> a.page_shift;
+        ids = first_page + lane < ahead_pages ? a.page_table[ahead.b * a.table_pitch + first_page + lane] : 0;
+      }
+      // sub-tile 0 / 1: tokens 0..15 / 16..31 for 16-token pages; else one copy of 32 tokens
+      const int sub = box == kTile ? 0 : (lane & 1);
+      int page = __shfl_sync(0xffffffffu, ids, first_page + sub - ids_first);
+      const bool there = first_page + sub < ahead_pages;
+      const bool good = there && uint32_t(page) < uint32_t(a.num_pages);
+      if (there && !good) {
+        bad_page = page | int(0x80000000);
+        page = a.num_pages;  // one past the pool: TMA fills zeros
+      }
+      const int copies = kTile / box;
+      const int there_parts = min(copies, ahead_pages - first_page);
+      if (lane == 0) mbar_arrive_expect_tx(bar, uint32_t(max(0, there_parts)) * 2u * uint32_t(box) * D);
+      __syncwarp();
+      if (lane < 4) {
+        const bool keys = lane < 2;
+        if (there && (lane & 1) < copies) {
+          tma_load_4d(dst + (keys ? 0 : L::kSide) + sub * box * D, keys ? &map_k : &map_v, 0, g, token & page_mask, page, bar);
+        }
+        const float* source = keys ? a.k.scale : a.v.scale;
+        copy_scale(scales + stage * 16 + lane * 4, source + (good ? (long long)page * a.kv_heads + g : 0), good, bar);
+      }
+      step(ahead, tiles, a.batch);
+    };
+    for (int i = 0; i < min(count, kStages); ++i) issue(i);
+
+    Spot at = spot_at(tiles, a.batch, begin);
+    float acc[kSteps][NT][4], m[NT][2], l[NT][2], row_scale[NT][2];
+    uint32_t query[NT][kSteps][2];
+    int limit[NT][2], context = 0, rows = 0, row0 = 0, nearest = 0;
+    float top = kLeastScale, from_top = 0.f;
+    int piece = 0;  // first tile of the current piece within its request
+
+    for (int i = 0; i < count; ++i) {
+      if (i == 0 || at.tile == 0) {
+        // ---- a new piece: its rows of q as f16 with a power-of-two factor, and how far each row sees
+        piece = at.tile;
+        row0 = a.row_start[at.b];
+        const int n = a.row_start[at.b + 1] - row0;
+        rows = n * a.group;
+        context = max(0, min(a.context_len[at.b], a.max_context));
+        nearest = context - n + 1;
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const int mine = t * 8 + r;
-        uint4 w[D / 32];
-        float size = 0.f;
-        const bool live = mine < rows && row0 + mine / a.group < a.rows;
-        const uint16_t* src = a.q + (row0 + mine / a.group) * a.q_row + (at.g * a.group + mine % a.group) * a.q_head + q4 * (D / 4);
+        for (int t = 0; t < NT; ++t) {
+          const int mine = t * 8 + r;
+          uint4 w[D / 32];
+          float size = 0.f;
+          const bool live = mine < rows && row0 + mine / a.group < a.rows;
+          const uint16_t* src = a.q + (row0 + mine / a.group) * a.q_row + (g * a.group + mine % a.group) * a.q_head + q4 * (D / 4);
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          w[c] = live ? *reinterpret_cast<const uint4*>(src + c * 8) : make_uint4(0, 0, 0, 0);
-          const uint32_t words[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
+          for (int c = 0; c < D / 32; ++c) {
+            w[c] = live ? *reinterpret_cast<const uint4*>(src + c * 8) : make_uint4(0, 0, 0, 0);
+            const uint32_t words[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 v = unpack<BF16>(words[e]);
-            size = fmaxf(size, fmaxf(fabsf(v.x), fabsf(v.y)));
+            for (int e = 0; e < 4; ++e) {
+              const float2 v = unpack<BF16>(words[e]);
+              size = fmaxf(size, fmaxf(fabsf(v.x), fabsf(v.y)));
+            }
           }
-        }
-        size = fmaxf(size, __shfl_xor_sync(0xffffffffu, size, 1));
-        size = fmaxf(size, __shfl_xor_sync(0xffffffffu, size, 2));
-        // the row's largest magnitude comes to lie in [2^14, 2^15)
-        const int up = max(-113, min(126, 14 - (int(__float_as_uint(size) >> 23) - 127)));
-        const float by = __uint_as_float(uint32_t(up + 127) << 23);
+          size = fmaxf(size, __shfl_xor_sync(0xffffffffu, size, 1));
+          size = fmaxf(size, __shfl_xor_sync(0xffffffffu, size, 2));
+          // the row's largest magnitude comes to lie in [2^14, 2^15)
+          const int up = max(-113, min(126, 14 - (int(__float_as_uint(size) >> 23) - 127)));
+          const float by = __uint_as_float(uint32_t(up + 127) << 23);
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          const uint32_t words[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
+          for (int c = 0; c < D / 32; ++c) {
+            const uint32_t words[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 v = unpack<BF16>(words[e]);
-            query[t][c * 2 + e / 2][e & 1] = pack_f16x2(v.x * by, v.y * by);
+            for (int e = 0; e < 4; ++e) {
+              const float2 v = unpack<BF16>(words[e]);
+              query[t][c * 2 + e / 2][e & 1] = pack_f16x2(v.x * by, v.y * by);
+            }
           }
-        }
-        const float back = __uint_as_float(uint32_t(127 - up) << 23) * a.scale_log2;
+          const float back = __uint_as_float(uint32_t(127 - up) << 23) * a.scale_log2;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int row = t * 8 + 2 * q4 + e;  // the rows whose scores this thread holds
-          row_scale[t][e] = __shfl_sync(0xffffffffu, back, (2 * q4 + e) * 4);
-          limit[t][e] = row < rows ? nearest + row / a.group : context;
-          m[t][e] = -INFINITY;
-          l[t][e] = 0.f;
-        }
-      }
-#pragma unroll
-      for (int c = 0; c < kSteps; ++c)
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[c][t][e] = 0.f;
-      top = kLeastScale;
-      from_top = 32768.0f / kLeastScale;
-    }
-
-    const int stage = i % kStages;
-    const uint32_t keys = ring + stage * L::kStage, values = keys + L::kSide;
-    if (!__all_sync(0xffffffffu, mbar_wait(bars + 8 * stage, (i / kStages) & 1, abort_flag, status, kSiteTile))) {
-      ok = false;
-      break;
-    }
-    const int token0 = at.tile * kTile;
-
-    // ---- scores: a thread's words of K are 32 (d = 64: 16) consecutive bytes of rows r and r + 8; q holds the same columns
-    float s[2][NT][4];
-#pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      uint32_t ka[kWords], kb[kWords];
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int row = g * 16 + half * 8 + r;
-        uint32_t(&k)[kWords] = half == 0 ? ka : kb;
-        if constexpr (D == 128) {
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const uint4 v = ld_shared_16(keys + row * 128 + (((q4 * 2 + c) ^ (row & 7)) << 4));
-            k[c * 4] = v.x, k[c * 4 + 1] = v.y, k[c * 4 + 2] = v.z, k[c * 4 + 3] = v.w;
+          for (int e = 0; e < 2; ++e) {
+            const int row = t * 8 + 2 * q4 + e;  // the rows whose scores this thread holds
+            row_scale[t][e] = __shfl_sync(0xffffffffu, back, (2 * q4 + e) * 4);
+            limit[t][e] = row < rows ? nearest + row / a.group : context;
+            m[t][e] = -INFINITY;
+            l[t][e] = 0.f;
           }
-        } else {
-          const uint4 v = ld_shared_16(keys + row * 64 + ((q4 ^ ((row >> 1) & 3)) << 4));
-          k[0] = v.x, k[1] = v.y, k[2] = v.z, k[3] = v.w;
-        }
-      }
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[g][t][e] = 0.f;
-#pragma unroll
-      for (int c = 0; c < kSteps; ++c) {
-        const uint32_t a0 = halves_of(ka[c]), a2 = halves_of(ka[c] >> 16), a1 = halves_of(kb[c]), a3 = halves_of(kb[c] >> 16);
-#pragma unroll
-        for (int t = 0; t < NT; ++t) mma_f16(s[g][t], a0, a1, a2, a3, query[t][c][0], query[t][c][1]);
-      }
-    }
-
-    // ---- softmax: the thread's tokens are g * 16 + r and + 8, its rows 2 * q4 and + 1 of each eight
-    const bool edge = token0 + kTile > nearest;  // some row does not see all of the tile
-    float high[NT][2];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) high[t][0] = high[t][1] = -INFINITY;
-#pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      const float ks = ld_shared_f32(scales + stage * 16 + (box == kTile ? 0 : g) * 4);
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[g][t][e] *= ks * row_scale[t][e & 1];
-          if (edge && token0 + g * 16 + r + (e >> 1) * 8 >= limit[t][e & 1]) s[g][t][e] = -INFINITY;
-          high[t][e & 1] = fmaxf(high[t][e & 1], s[g][t][e]);
-        }
-    }
-    const float vs0 = ld_shared_f32(scales + stage * 16 + 8);
-    const float vs1 = box == kTile ? vs0 : ld_shared_f32(scales + stage * 16 + 12);
-    const float new_top = fmaxf(top, fmaxf(fabsf(vs0), fabsf(vs1)));
-    bool moved = new_top != top;
-    float m_new[NT][2];
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) high[t][e] = fmaxf(high[t][e], __shfl_xor_sync(0xffffffffu, high[t][e], o));
-        m_new[t][e] = fmaxf(m[t][e], high[t][e]);
-        moved |= m_new[t][e] != m[t][e];
-      }
-    if (__any_sync(0xffffffffu, moved)) {
-      const float shrink = top / new_top;
-      top = new_top;
-      from_top = 32768.0f / new_top;
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        float corr[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float c = m[t][e] == -INFINITY ? 0.f : ex2_approx(m[t][e] - m_new[t][e]);
-          m[t][e] = m_new[t][e];
-          l[t][e] *= c;
-          corr[e] = c * shrink;
         }
 #pragma unroll
         for (int c = 0; c < kSteps; ++c)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[c][t][e] *= corr[e & 1];
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[c][t][e] = 0.f;
+        top = kLeastScale;
+        from_top = 32768.0f / kLeastScale;
       }
-    }
-    uint32_t weight[2][NT][2];
-#pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      const float vs = (g == 0 ? vs0 : vs1) * from_top;
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        float w[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          w[e] = m[t][e & 1] == -INFINITY ? 0.f : ex2_approx(s[g][t][e] - m[t][e & 1]);
-          l[t][e & 1] += w[e];
-        }
-        weight[g][t][0] = transposed(pack_f16x2(w[0] * vs, w[1] * vs));
-        weight[g][t][1] = transposed(pack_f16x2(w[2] * vs, w[3] * vs));
-      }
-    }
 
-    // ---- output: a thread's columns of V are 16 (d = 64: 8) consecutive ones of tokens 2 * q4, + 1, + 8, + 9
-    const bool tail = token0 + kTile > context;  // what lies behind the context may be any bits
-#pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      uint32_t v[4][D / 32];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int row = g * 16 + 2 * q4 + (e & 1) + (e >> 1) * 8;
-        if constexpr (D == 128) {
-          const uint4 x = ld_shared_16(values + row * 128 + ((r ^ (row & 7)) << 4));
-          v[e][0] = x.x, v[e][1] = x.y, v[e][2] = x.z, v[e][3] = x.w;
-        } else {
-          const uint2 x = ld_shared_8(values + row * 64 + (((r >> 1) ^ ((row >> 1) & 3)) << 4) + (r & 1) * 8);
-          v[e][0] = x.x, v[e][1] = x.y;
-        }
-        if (tail && token0 + row >= context) {
-#pragma unroll
-          for (int c = 0; c < D / 32; ++c) v[e][c] = 0;
-        }
+      const int stage = (done + i) % kStages;
+      const uint32_t keys = ring + stage * L::kStage, values = keys + L::kSide;
+      if (!__all_sync(0xffffffffu, mbar_wait(bars + 8 * stage, ((done + i) / kStages) & 1, abort_flag, status, kSiteTile))) {
+        ok = false;
+        break;
       }
-#pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        const uint32_t x0 = __byte_perm(v[0][c], v[1][c], 0x5140), x1 = __byte_perm(v[0][c], v[1][c], 0x7362);
-        const uint32_t y0 = __byte_perm(v[2][c], v[3][c], 0x5140), y1 = __byte_perm(v[2][c], v[3][c], 0x7362);
-        const uint32_t a0 = halves_of(x0), a1 = halves_of(x0 >> 16), a2 = halves_of(y0), a3 = halves_of(y0 >> 16);
-        const uint32_t b0 = halves_of(x1), b1 = halves_of(x1 >> 16), b2 = halves_of(y1), b3 = halves_of(y1 >> 16);
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          mma_f16(acc[2 * c][t], a0, a1, a2, a3, weight[g][t][0], weight[g][t][1]);
-          mma_f16(acc[2 * c + 1][t], b0, b1, b2, b3, weight[g][t][0], weight[g][t][1]);
-        }
-      }
-    }
-    __syncwarp();
-    if (i + kStages < count) issue(i + kStages);
+      const int token0 = at.tile * kTile;
 
-    // ---- the end of a piece
-    if (at.tile + 1 == at.tiles || i + 1 == count) {
-      const bool whole = piece == 0 && at.tile + 1 == at.tiles;
-      const int slot = 2 * me + (i - (at.tile - piece) == 0 ? 0 : 1);
-      const float unit = top * (1.0f / 32768.0f);
+      // ---- scores: a thread's words of K are 32 (d = 64: 16) consecutive bytes of rows r and r + 8; q holds the same columns
+      float s[2][NT][4];
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        uint32_t ka[kWords], kb[kWords];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int row = g * 16 + half * 8 + r;
+          uint32_t(&k)[kWords] = half == 0 ? ka : kb;
+          if constexpr (D == 128) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const uint4 v = ld_shared_16(keys + row * 128 + (((q4 * 2 + c) ^ (row & 7)) << 4));
+              k[c * 4] = v.x, k[c * 4 + 1] = v.y, k[c * 4 + 2] = v.z, k[c * 4 + 3] = v.w;
+            }
+          } else {
+            const uint4 v = ld_shared_16(keys + row * 64 + ((q4 ^ ((row >> 1) & 3)) << 4));
+            k[0] = v.x, k[1] = v.y, k[2] = v.z, k[3] = v.w;
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[g][t][e] = 0.f;
+#pragma unroll
+        for (int c = 0; c < kSteps; ++c) {
+          const uint32_t a0 = halves_of(ka[c]), a2 = halves_of(ka[c] >> 16), a1 = halves_of(kb[c]), a3 = halves_of(kb[c] >> 16);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) mma_f16(s[g][t], a0, a1, a2, a3, query[t][c][0], query[t][c][1]);
+        }
+      }
+
+      // ---- softmax: the thread's tokens are g * 16 + r and + 8, its rows 2 * q4 and + 1 of each eight
+      const bool edge = token0 + kTile > nearest;  // some row does not see all of the tile
+      float high[NT][2];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) high[t][0] = high[t][1] = -INFINITY;
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const float ks = ld_shared_f32(scales + stage * 16 + (box == kTile ? 0 : g) * 4);
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            s[g][t][e] *= ks * row_scale[t][e & 1];
+            if (edge && token0 + g * 16 + r + (e >> 1) * 8 >= limit[t][e & 1]) s[g][t][e] = -INFINITY;
+            high[t][e & 1] = fmaxf(high[t][e & 1], s[g][t][e]);
+          }
+      }
+      const float vs0 = ld_shared_f32(scales + stage * 16 + 8);
+      const float vs1 = box == kTile ? vs0 : ld_shared_f32(scales + stage * 16 + 12);
+      const float new_top = fmaxf(top, fmaxf(fabsf(vs0), fabsf(vs1)));
+      bool moved = new_top != top;
+      float m_new[NT][2];
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float total = l[t][e];
 #pragma unroll
-          for (int o = 4; o < 32; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-          const int row = t * 8 + 2 * q4 + e;
-          if (row >= rows || row0 + row / a.group >= a.rows) continue;
-          if (whole) {
-            const float by = total == 0.f ? 0.f : unit / total;
-            uint16_t* out = a.o + (row0 + row / a.group) * a.o_row + (at.g * a.group + row % a.group) * a.o_head + r * (D / 8);
+          for (int o = 4; o < 32; o <<= 1) high[t][e] = fmaxf(high[t][e], __shfl_xor_sync(0xffffffffu, high[t][e], o));
+          m_new[t][e] = fmaxf(m[t][e], high[t][e]);
+          moved |= m_new[t][e] != m[t][e];
+        }
+      if (__any_sync(0xffffffffu, moved)) {
+        const float shrink = top / new_top;
+        top = new_top;
+        from_top = 32768.0f / new_top;
 #pragma unroll
-            for (int c = 0; c < D / 64; ++c) {
-              uint32_t w[4];
+        for (int t = 0; t < NT; ++t) {
+          float corr[2];
 #pragma unroll
-              for (int x = 0; x < 4; ++x) {
-                const float y0 = acc[c * 4 + x][t][e] * by, y1 = acc[c * 4 + x][t][2 + e] * by;
-                w[x] = BF16 ? pack_bf16x2(y0, y1) : pack_f16x2(y0, y1);
-              }
-              *reinterpret_cast<uint4*>(out + c * 8) = make_uint4(w[0], w[1], w[2], w[3]);
-            }
+          for (int e = 0; e < 2; ++e) {
+            const float c = m[t][e] == -INFINITY ? 0.f : ex2_approx(m[t][e] - m_new[t][e]);
+            m[t][e] = m_new[t][e];
+            l[t][e] *= c;
+            corr[e] = c * shrink;
+          }
+#pragma unroll
+          for (int c = 0; c < kSteps; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[c][t][e] *= corr[e & 1];
+        }
+      }
+      uint32_t weight[2][NT][2];
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const float vs = (g == 0 ? vs0 : vs1) * from_top;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          float w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            w[e] = m[t][e & 1] == -INFINITY ? 0.f : ex2_approx(s[g][t][e] - m[t][e & 1]);
+            l[t][e & 1] += w[e];
+          }
+          weight[g][t][0] = transposed(pack_f16x2(w[0] * vs, w[1] * vs));
+          weight[g][t][1] = transposed(pack_f16x2(w[2] * vs, w[3] * vs));
+        }
+      }
+
+      // ---- output: a thread's columns of V are 16 (d = 64: 8) consecutive ones of tokens 2 * q4, + 1, + 8, + 9
+      const bool tail = token0 + kTile > context;  // what lies behind the context may be any bits
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        uint32_t v[4][D / 32];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int row = g * 16 + 2 * q4 + (e & 1) + (e >> 1) * 8;
+          if constexpr (D == 128) {
+            const uint4 x = ld_shared_16(values + row * 128 + ((r ^ (row & 7)) << 4));
+            v[e][0] = x.x, v[e][1] = x.y, v[e][2] = x.z, v[e][3] = x.w;
           } else {
-            float* out = p.partial + ((long long)slot * p.slot_rows + row) * (D + 4);
-            if (r == 0) *reinterpret_cast<float2*>(out) = make_float2(m[t][e], total);
+            const uint2 x = ld_shared_8(values + row * 64 + (((r >> 1) ^ ((row >> 1) & 3)) << 4) + (r & 1) * 8);
+            v[e][0] = x.x, v[e][1] = x.y;
+          }
+          if (tail && token0 + row >= context) {
 #pragma unroll
-            for (int c = 0; c < D / 32; ++c) {
-              *reinterpret_cast<float4*>(out + 4 + r * (D / 8) + c * 4) =
-                  make_float4(acc[c * 2][t][e] * unit, acc[c * 2][t][2 + e] * unit, acc[c * 2 + 1][t][e] * unit,
-                              acc[c * 2 + 1][t][2 + e] * unit);
-            }
+            for (int c = 0; c < D / 32; ++c) v[e][c] = 0;
           }
         }
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          const uint32_t x0 = __byte_perm(v[0][c], v[1][c], 0x5140), x1 = __byte_perm(v[0][c], v[1][c], 0x7362);
+          const uint32_t y0 = __byte_perm(v[2][c], v[3][c], 0x5140), y1 = __byte_perm(v[2][c], v[3][c], 0x7362);
+          const uint32_t a0 = halves_of(x0), a1 = halves_of(x0 >> 16), a2 = halves_of(y0), a3 = halves_of(y0 >> 16);
+          const uint32_t b0 = halves_of(x1), b1 = halves_of(x1 >> 16), b2 = halves_of(y1), b3 = halves_of(y1 >> 16);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            mma_f16(acc[2 * c][t], a0, a1, a2, a3, weight[g][t][0], weight[g][t][1]);
+            mma_f16(acc[2 * c + 1][t], b0, b1, b2, b3, weight[g][t][0], weight[g][t][1]);
+          }
+        }
+      }
+      __syncwarp();
+      if (i + kStages < count) issue(i + kStages);
+
+      // ---- the end of a piece
+      if (at.tile + 1 == at.tiles || i + 1 == count) {
+        const bool whole = piece == 0 && at.tile + 1 == at.tiles;
+        const int slot = 2 * unit + (i - (at.tile - piece) == 0 ? 0 : 1);
+        const float value = top * (1.0f / 32768.0f);
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float sum = l[t][e];
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            const int row = t * 8 + 2 * q4 + e;
+            if (row >= rows || row0 + row / a.group >= a.rows) continue;
+            if (whole) {
+              const float by = sum == 0.f ? 0.f : value / sum;
+              uint16_t* out = a.o + (row0 + row / a.group) * a.o_row + (g * a.group + row % a.group) * a.o_head + r * (D / 8);
+#pragma unroll
+              for (int c = 0; c < D / 64; ++c) {
+                uint32_t w[4];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                  const float y0 = acc[c * 4 + x][t][e] * by, y1 = acc[c * 4 + x][t][2 + e] * by;
+                  w[x] = BF16 ? pack_bf16x2(y0, y1) : pack_f16x2(y0, y1);
+                }
+                *reinterpret_cast<uint4*>(out + c * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+              }
+            } else {
+              float* out = p.partial + ((long long)slot * p.slot_rows + row) * (D + 4);
+              if (r == 0) *reinterpret_cast<float2*>(out) = make_float2(m[t][e], sum);
+#pragma unroll
+              for (int c = 0; c < D / 32; ++c) {
+                *reinterpret_cast<float4*>(out + 4 + r * (D / 8) + c * 4) =
+                    make_float4(acc[c * 2][t][e] * value, acc[c * 2][t][2 + e] * value, acc[c * 2 + 1][t][e] * value,
+                                acc[c * 2 + 1][t][2 + e] * value);
+              }
+            }
+          }
+      }
+      step(at, tiles, a.batch);
     }
-    step(at, tiles, a.batch, a.kv_heads);
+    done += count;
   }
   if (bad_page != 0) report_failure(status, kErrDeviceIndex, kSitePage, uint32_t(bad_page) & 0x7fffffffu);
   if (!ok) {  // let this warp's own copies land before the block's memory goes
@@ -507,63 +507,93 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   }
 }
 
-// Joins the pieces of split segments: a block per (segment, row), its warps take the pieces in turn,
-//   o = sum 2^(m_i - M) acc_i / sum 2^(m_i - M) l_i.
-// Launched as a programmatic dependent of the stream kernel, so that its launch overlaps that kernel's end.
-constexpr int kJoinWarps = 4;
+// Joins the pieces of split segments: a block per (request, kv head, row),
+//   o = sum 2^(m_i - M) acc_i / sum 2^(m_i - M) l_i,
+// first the pieces' factors, a thread each, then the sum, a column each; the warps share the pieces. Launched as a
+// programmatic dependent of the stream kernel, so that its launch overlaps that kernel's end.
+constexpr int kJoinThreads = 256;
+constexpr int kJoinPieces = 2 * kMaxBlocks;  // pieces at a time
 
 template <int D, bool BF16>
-__global__ void __launch_bounds__(kJoinWarps * 32) cache_join_kernel(StreamParams p, int warps_of_grid) {
-  constexpr int kCols = D / 32;
-  __shared__ float shared[kJoinWarps][D + 2];
+__global__ void __launch_bounds__(kJoinThreads) cache_join_kernel(StreamParams p, int grid_warps) {
+  constexpr int kLanes = D / 4;                       // threads per piece, four columns each
+  constexpr int kGroups = kJoinThreads / kLanes;      // pieces in work at once
+  __shared__ float factor[kJoinPieces];
+  __shared__ float4 shared[kJoinThreads];
+  __shared__ float red[2][kJoinThreads / 32];
   const CacheAttnParams& a = p.a;
   const int b = blockIdx.x / a.kv_heads, g = blockIdx.x % a.kv_heads, row = blockIdx.y;
-  const int warp = threadIdx.x >> 5, lane = int(lane_id());
+  const int tid = threadIdx.x, group = tid / kLanes, lane = tid % kLanes;
   const int row0 = a.row_start[b], n = a.row_start[b + 1] - row0;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int tiles = p.tiles[b + 1] - p.tiles[b], total = p.tiles[a.batch] * a.kv_heads;
+  const int first = p.tiles[b], tiles = p.tiles[b + 1] - first, total = p.tiles[a.batch];
   if (tiles == 0 || row >= n * a.group || row0 + row / a.group >= a.rows) return;
-  const int warps = warps_used(total, warps_of_grid);
-  const int first = p.tiles[b] * a.kv_heads + g * tiles, last = first + tiles - 1;
-  const int w0 = int(((long long)(first + 1) * warps - 1) / total), w1 = int(((long long)(last + 1) * warps - 1) / total);
-  if (w0 == w1) return;  // one warp had it all and has written it
-  float m = -INFINITY, l = 0.f, acc[kCols];
+  const int parts = stretches(total, grid_warps, a.kv_heads);
+  const int p0 = stretch_of(first, parts, total), p1 = stretch_of(first + tiles - 1, parts, total);
+  if (p0 == p1) return;  // one warp had it all and has written it
+  auto piece = [&](int part) {
+    const long long slot = 2ll * (part * a.kv_heads + g) + (first > first_tile(part, parts, total) ? 1 : 0);
+    return p.partial + (slot * p.slot_rows + row) * (D + 4);
+  };
+  float top = -INFINITY, den = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int base = p0; base <= p1; base += kJoinPieces) {
+    const int here = min(kJoinPieces, p1 + 1 - base);
+    float m[2], l[2], high = -INFINITY;
 #pragma unroll
-  for (int c = 0; c < kCols; ++c) acc[c] = 0.f;
-  for (int w = w0 + warp; w <= w1; w += kJoinWarps) {
-    const int slot = 2 * w + (first > first_tile(w, warps, total) ? 1 : 0);
-    const float* from = p.partial + ((long long)slot * p.slot_rows + row) * (D + 4);
-    const float2 ml = *reinterpret_cast<const float2*>(from);
-    float x[kCols];
+    for (int k = 0; k < 2; ++k) {
+      const int i = tid + k * kJoinThreads;
+      const float2 ml = i < here ? *reinterpret_cast<const float2*>(piece(base + i)) : make_float2(-INFINITY, 0.f);
+      m[k] = ml.x;
+      l[k] = ml.y;
+      high = fmaxf(high, ml.x);
+    }
 #pragma unroll
-    for (int c = 0; c < kCols; ++c) x[c] = from[4 + c * 32 + lane];
-    const float m_new = fmaxf(m, ml.x);
-    const float old = m == -INFINITY ? 0.f : exp2f(m - m_new), now = ml.x == -INFINITY ? 0.f : exp2f(ml.x - m_new);
-    m = m_new;
-    l = l * old + ml.y * now;
+    for (int o = 16; o > 0; o >>= 1) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
+    if ((tid & 31) == 0) red[0][tid >> 5] = high;
+    __syncthreads();
+    float top_new = top;
 #pragma unroll
-    for (int c = 0; c < kCols; ++c) acc[c] = acc[c] * old + x[c] * now;
+    for (int w = 0; w < kJoinThreads / 32; ++w) top_new = fmaxf(top_new, red[0][w]);
+    const float old = top == -INFINITY ? 0.f : exp2f(top - top_new);
+    top = top_new;
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int i = tid + k * kJoinThreads;
+      const float by = m[k] == -INFINITY ? 0.f : exp2f(m[k] - top);
+      if (i < here) factor[i] = by;
+      sum += by * l[k];
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if ((tid & 31) == 0) red[1][tid >> 5] = sum;
+    __syncthreads();
+    den *= old;
+#pragma unroll
+    for (int w = 0; w < kJoinThreads / 32; ++w) den += red[1][w];
+    acc.x *= old, acc.y *= old, acc.z *= old, acc.w *= old;
+#pragma unroll 8
+    for (int i = group; i < here; i += kGroups) {
+      const float by = factor[i];
+      const float4 x = *reinterpret_cast<const float4*>(piece(base + i) + 4 + lane * 4);
+      acc.x += by * x.x, acc.y += by * x.y, acc.z += by * x.z, acc.w += by * x.w;
+    }
+    __syncthreads();
   }
-  if (lane == 0) {
-    shared[warp][0] = m;
-    shared[warp][1] = l;
-  }
-#pragma unroll
-  for (int c = 0; c < kCols; ++c) shared[warp][2 + c * 32 + lane] = acc[c];
+  shared[tid] = acc;
   __syncthreads();
-  if (threadIdx.x >= D / 2) return;
-  float top = -INFINITY;
-  for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, shared[w][0]);
-  float den = 0.f, y0 = 0.f, y1 = 0.f;
-  for (int w = 0; w < kJoinWarps; ++w) {
-    const float by = shared[w][0] == -INFINITY ? 0.f : exp2f(shared[w][0] - top);
-    den += by * shared[w][1];
-    y0 += by * shared[w][2 + 2 * threadIdx.x];
-    y1 += by * shared[w][3 + 2 * threadIdx.x];
+  if (group > 0) return;
+#pragma unroll
+  for (int k = 1; k < kGroups; ++k) {
+    const float4 x = shared[k * kLanes + lane];
+    acc.x += x.x, acc.y += x.y, acc.z += x.z, acc.w += x.w;
   }
   const float by = den == 0.f ? 0.f : 1.0f / den;
-  uint32_t* out = reinterpret_cast<uint32_t*>(a.o + (row0 + row / a.group) * a.o_row + (g * a.group + row % a.group) * a.o_head);
-  out[threadIdx.x] = BF16 ? pack_bf16x2(y0 * by, y1 * by) : pack_f16x2(y0 * by, y1 * by);
+  uint2 w;
+  w.x = BF16 ? pack_bf16x2(acc.x * by, acc.y * by) : pack_f16x2(acc.x * by, acc.y * by);
+  w.y = BF16 ? pack_bf16x2(acc.z * by, acc.w * by) : pack_f16x2(acc.z * by, acc.w * by);
+  *reinterpret_cast<uint2*>(a.o + (long long)(row0 + row / a.group) * a.o_row + (g * a.group + row % a.group) * a.o_head + lane * 4) = w;
 }
 
 template <int D, bool BF16, int NT>
@@ -582,14 +612,15 @@ int launch_stream(const DeviceContext* ctx, const StreamParams& p, int64_t page_
       })) {
     return rc;
   }
-  const int64_t tiles = int64_t(a.batch) * a.kv_heads * ((a.max_context + kTile - 1) / kTile);
+  // no more blocks than the contexts could give warps work
+  const int64_t wanted = (int64_t(a.batch) * a.kv_heads * ((a.max_context + kTile - 1) / kTile) + kWarps - 1) / kWarps;
   const int most = ctx->sm_count < kMaxBlocks ? ctx->sm_count : kMaxBlocks;
-  const int blocks = int(tiles < most ? tiles : most);
+  const int blocks = int(wanted < most ? wanted : most);
   kernel<<<blocks, kWarps * 32, StreamLayout<D>::bytes(a.batch), stream>>>(map_k, map_v, p, ctx->status_dev);
   KRNB_CUDA(cudaGetLastError());
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(unsigned(a.batch) * unsigned(a.kv_heads), unsigned(p.slot_rows), 1);
-  config.blockDim = dim3(kJoinWarps * 32, 1, 1);
+  config.blockDim = dim3(kJoinThreads, 1, 1);
   config.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -609,8 +640,9 @@ int64_t slot_rows(int64_t max_new, int64_t group) {
 
 int64_t prefix_bytes(int64_t batch) { return (batch + 1 + 3) / 4 * 16; }
 
-int64_t stream_workspace(int64_t batch, int64_t d, int64_t rows) {
-  return prefix_bytes(batch) + 2 * int64_t(kMaxBlocks) * kWarps * rows * (d + 4) * 4;
+int64_t stream_workspace(int64_t batch, int64_t kv_heads, int64_t d, int64_t rows) {
+  const int64_t warps = int64_t(kMaxBlocks) * kWarps, units = warps > kv_heads ? warps : kv_heads;
+  return prefix_bytes(batch) + 2 * units * rows * (d + 4) * 4;
 }
 
 template <int D, bool BF16>
@@ -628,7 +660,7 @@ extern "C" int64_t krn_b200_cache_attn_workspace_bytes(int64_t batch, int64_t ro
   using namespace krnb;
   if (batch <= 0 || rows <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0 || d <= 0 || max_new <= 0) return 16;
   const int64_t few = slot_rows(max_new, q_heads / kv_heads);
-  return stream_workspace(batch, d, few) +
+  return stream_workspace(batch, kv_heads, d, few) +
          (max_new * (q_heads / kv_heads) <= few ? 0 : tile_workspace(batch, rows, q_heads, kv_heads, d, few, max_context));
 }
 
@@ -737,6 +769,6 @@ extern "C" int krn_b200_cache_attn(int type, const void* q, const void* k_pages,
     if (rc) return rc;
   }
   if (max_new * p.group <= p.few) return KRN_B200_OK;
-  float* partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + stream_workspace(batch, d, p.few));
+  float* partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + stream_workspace(batch, kv_heads, d, p.few));
   return launch_tiles(ctx, p, bf16, d, page_size, partial, stream);
 }
