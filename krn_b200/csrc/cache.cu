@@ -22,7 +22,7 @@ enum Site { kSitePlanPage = 41, kSiteAppendSlot = 42 };
 
 constexpr int kPlanThreads = 512;
 constexpr int kPlanWarps = kPlanThreads / 32;
-constexpr int kMaxBatch = 8192;             // three prefixes of the batch sit in shared memory
+constexpr int kMaxBatch = 8192;             // four prefixes of the batch sit in shared memory
 constexpr uint32_t kSaturated = 1u << 30;   // sums stop here: above every bound they are compared with
 
 struct PlanParams {
@@ -97,16 +97,29 @@ __device__ __forceinline__ void block_prefix(uint32_t (&v)[4], uint32_t (&carry)
   __syncthreads();  // scratch is free again
 }
 
+// The last request whose prefix is at or before `k`: of those that share a prefix only the last has anything.
+__device__ __forceinline__ int last_at_or_before(const uint32_t* prefix, int batch, int k) {
+  int low = 0, high = batch;
+  while (high - low > 1) {
+    const int mid = (low + high) >> 1;
+    if (prefix[mid] <= uint32_t(k)) low = mid; else high = mid;
+  }
+  return low;
+}
+
 // One launch, no communication between blocks: every block scans all request lengths by itself (a few loads per thread)
 // and then fills its own part of the slot map, the run list and the table. Bound by latency: launch, one pass over the
 // lengths, a binary search per row.
 __global__ void __launch_bounds__(kPlanThreads) cache_plan_kernel(PlanParams p, DeviceStatus* status) {
   extern __shared__ uint32_t plan_smem[];
   uint32_t* start = plan_smem;                 // [batch + 1] first row of each request
-  uint32_t* first = start + p.batch + 1;       // [batch] first page taken from (finished: given back to) the ring
+  uint32_t* first = start + p.batch + 1;       // [batch] first page taken from the ring
   uint32_t* run = first + p.batch;             // [batch] first entry of the run list
-  uint32_t* scratch = run + p.batch;           // [4 * kPlanWarps]
+  uint32_t* back = run + p.batch;              // [batch] first page given back to the ring
+  uint32_t* scratch = back + p.batch;          // [4 * kPlanWarps]
   const int page = 1 << p.page_shift;
+  launch_dependents();
+  wait_for_kernel_before();
 
   // totals first: a step that does not fit takes nothing
   uint32_t carry[4] = {0, 0, 0, 0};
@@ -122,12 +135,12 @@ __global__ void __launch_bounds__(kPlanThreads) cache_plan_kernel(PlanParams p, 
       v[2] = r.lead;
       v[3] = r.back;
     }
-    const bool gives = v[3] != 0;
     block_prefix(v, carry, scratch);
     if (i < p.batch) {
       start[i] = v[0];
-      first[i] = gives ? v[3] : v[1];
+      first[i] = v[1];
       run[i] = v[2];
+      back[i] = v[3];
     }
   }
   const long long taken = p.pool_state[0], given = p.pool_state[1];
@@ -164,11 +177,7 @@ __global__ void __launch_bounds__(kPlanThreads) cache_plan_kernel(PlanParams p, 
       p.slot_map[r] = -1;
       continue;
     }
-    int low = 0, high = p.batch;  // the last request that starts at or before r and is not empty
-    while (high - low > 1) {
-      const int mid = (low + high) >> 1;
-      if (start[mid] <= uint32_t(r)) low = mid; else high = mid;
-    }
+    const int low = last_at_or_before(start, p.batch, r);
     const long long most = (long long)p.max_pages << p.page_shift;
     const int context = int(min((long long)max(p.context_len[low], 0), most));
     const int have = (context + page - 1) >> p.page_shift;
@@ -193,21 +202,18 @@ __global__ void __launch_bounds__(kPlanThreads) cache_plan_kernel(PlanParams p, 
     p.slot_map[r] = good ? ((long long)id << p.page_shift) + (pos & (page - 1)) : -1;
   }
 
-  // pages of finished requests, a warp each: handed out from the next step on
+  // pages of finished requests: handed out from the next step on
   if (!overfull) {
-    for (int i = here >> 5; i < p.batch; i += stride >> 5) {
-      if (p.new_len[i] >= 0) continue;
-      const Request r = request_at(p, i);
-      for (int j = int(lane_id()); j < r.have; j += 32) {
-        long long spot = given_at + first[i] + j;
-        if (spot >= p.capacity) spot -= p.capacity;
-        p.free_pages[spot] = p.page_table[i * p.table_pitch + j];
-      }
+    for (int k = here; k < int(carry[3]); k += stride) {
+      const int low = last_at_or_before(back, p.batch, k);
+      long long spot = given_at + k;
+      if (spot >= p.capacity) spot -= p.capacity;
+      p.free_pages[spot] = p.page_table[low * p.table_pitch + (k - int(back[low]))];
     }
   }
 }
 
-size_t plan_smem_bytes(int64_t batch) { return size_t(3 * batch + 1 + 4 * kPlanWarps) * 4; }
+size_t plan_smem_bytes(int64_t batch) { return size_t(4 * batch + 1 + 4 * kPlanWarps) * 4; }
 
 // ---- append ----------------------------------------------------------------------------------------------------------
 
@@ -237,12 +243,6 @@ __device__ __forceinline__ float2 unpack(uint32_t w) {
   }
 }
 
-// |x|, or 0 where x is not finite: infinities and NaN have no say in a page's scale.
-__device__ __forceinline__ float finite_size(float x) {
-  const float a = fabsf(x);
-  return a <= 3.4028234663852886e38f ? a : 0.f;
-}
-
 // The least power of two 2^k, k >= kLeastExponent, with a <= 448 * 2^k, read off a's exponent: 448 = 1.75 * 2^8.
 __device__ __forceinline__ float scale_of(float a) {
   const uint32_t bits = __float_as_uint(a);
@@ -251,18 +251,11 @@ __device__ __forceinline__ float scale_of(float a) {
   return __uint_as_float(uint32_t(k + 127) << 23);
 }
 
-// Two values over `scale` to e4m3, nearest even, saturated; infinities become +-448, NaN stays NaN. Multiplying by the
-// reciprocal of a power of two is the division itself; a page that some other program filled may have any scale.
-struct Divisor {
-  float scale, inverse;
-  bool exact;
-  __device__ __forceinline__ uint32_t two(float2 v) const {
-    const float a = exact ? v.x * inverse : v.x / scale, b = exact ? v.y * inverse : v.y / scale;
-    uint16_t r;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(b), "f"(a));
-    return r;
-  }
-};
+__device__ __forceinline__ uint32_t codes_of(float2 v) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(v.y), "f"(v.x));
+  return r;
+}
 
 __device__ __forceinline__ uint32_t rescale_two(uint32_t codes, float ratio) {
   uint32_t h;
@@ -273,49 +266,18 @@ __device__ __forceinline__ uint32_t rescale_two(uint32_t codes, float ratio) {
   return r;
 }
 
-struct Run {
-  int row, count, offset, page;
-};
-
-// Entry `u` of the run list: rows [row, row + count) fill slots `offset`, ... of `page`. False where there is none.
-__device__ __forceinline__ bool run_at(const AppendParams& p, int u, Run& run, DeviceStatus* status) {
-  const int row = p.runs[u];
-  if (uint32_t(row) >= uint32_t(p.rows)) return false;
-  const long long slot = p.slot_map[row];
-  if (slot < 0) return false;
-  const long long page = slot >> p.page_shift;
-  if (page >= p.num_pages) {
-    report_failure(status, kErrDeviceIndex, kSiteAppendSlot, uint32_t(row));
-    return false;
-  }
-  run.row = row;
-  run.page = int(page);
-  run.offset = int(slot & ((1 << p.page_shift) - 1));
-  const int most = min((1 << p.page_shift) - run.offset, p.rows - row);
-  int count = 1;
-  for (int base = 0; base < most; base += 32) {
-    const int i = base + int(lane_id());
-    const bool same = i < most && p.slot_map[row + i] == slot + i;
-    const uint32_t mask = __ballot_sync(0xffffffffu, same);
-    if (mask != 0xffffffffu) {
-      count = base + __ffs(int(~mask)) - 1;
-      break;
-    }
-    count = base + 32;
-  }
-  run.count = min(count, most);
-  return true;
-}
-
 // A thread group of `Threads` owns one (run, kv head, K or V): no two groups share a page's scale, so the new scale, the
 // page's old codes and its new ones are settled without atomics, and the result does not depend on any order.
 //   1. the group reads its rows once (16 bytes a thread and pass; up to kHeld passes stay in registers) and takes the
-//      largest finite magnitude;
+//      largest finite magnitude: bit patterns of magnitudes are ordered as they are, two 16-bit ones at a time, and only a
+//      run that holds an infinity or a NaN is gone through value by value;
 //   2. scale = max(old, least power of two that fits); a run that begins a page ignores what the page held;
 //   3. where the scale grew, the codes already in the page are brought to it (a power-of-two ratio: only what falls below
 //      e4m3's normal range is rounded again);
-//   4. the rows go out as codes, 8 bytes a thread.
-// Bound by HBM for prompts (2 bytes in, 1 out per value) and by launch and load latency for single tokens.
+//   4. the rows go out as codes, 8 bytes a thread. Multiplying by the reciprocal of a power of two is the division itself;
+//      a page that some other program filled may have any scale, and is divided by.
+// The rows are under way before the slots that they go to are known. Bound by HBM for prompts (2 bytes in, 1 out per value)
+// and by launch and load latency for single tokens.
 constexpr int kHeld = 8;
 
 template <int D, bool BF16, int Threads>
@@ -323,53 +285,92 @@ __global__ void __launch_bounds__(128) cache_append_kernel(AppendParams p, Devic
   constexpr int kLanes = D / 8;                // threads per row
   constexpr int kRows = Threads / kLanes;      // rows per pass
   constexpr int kGroups = 128 / Threads;       // (run, head, side) items per block
-  __shared__ float peak[4];
+  constexpr uint32_t kInfinity = BF16 ? 0x7f80u : 0x7c00u;
+  __shared__ uint32_t peaks[4];
   const int tid = threadIdx.x % Threads;
-  const long long item = (long long)blockIdx.x * kGroups + threadIdx.x / Threads;
-  const int per_run = 2 * p.heads;
-  const int u = int(item / per_run), which = int(item % per_run);
+  const uint32_t item = blockIdx.x * kGroups + threadIdx.x / Threads, per_run = 2u * uint32_t(p.heads);
+  const int u = int(item / per_run), which = int(item - uint32_t(u) * per_run);
+  launch_dependents();
+  wait_for_kernel_before();
   if (u >= p.runs_len) return;
-  Run run;
-  if (!run_at(p, u, run, status)) return;
+  const int first = p.runs[u], next = u + 1 < p.runs_len ? p.runs[u + 1] : -1;
+  if (uint32_t(first) >= uint32_t(p.rows)) return;
+  const int page_size = 1 << p.page_shift;
+  int most = min(page_size, p.rows - first);
+  if (next > first) most = min(most, next - first);
   const AppendSide& side = p.side[which >= p.heads ? 1 : 0];
   const int head = which >= p.heads ? which - p.heads : which;
   const int lane = tid % kLanes, row0 = tid / kLanes;
-  const uint16_t* x = side.x + (long long)run.row * side.x_row + head * side.x_head + lane * 8;
-
+  const uint16_t* x = side.x + first * side.x_row + head * side.x_head + lane * 8;
   uint4 held[kHeld];
-  float a = 0.f;
-  auto take = [&](const uint4& w) {
-    const uint32_t words[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 v = unpack<BF16>(words[e]);
-      a = fmaxf(a, fmaxf(finite_size(v.x), finite_size(v.y)));
-    }
-  };
 #pragma unroll
   for (int i = 0; i < kHeld; ++i) {
     const int row = row0 + i * kRows;
-    held[i] = make_uint4(0, 0, 0, 0);
-    if (row < run.count) held[i] = *reinterpret_cast<const uint4*>(x + row * side.x_row);
-  }
-#pragma unroll
-  for (int i = 0; i < kHeld; ++i) take(held[i]);
-  for (int row = row0 + kHeld * kRows; row < run.count; row += kRows) take(*reinterpret_cast<const uint4*>(x + row * side.x_row));
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
-  if constexpr (Threads > 32) {
-    if (lane_id() == 0) peak[threadIdx.x >> 5] = a;
-    __syncthreads();
-    a = fmaxf(fmaxf(peak[0], peak[1]), fmaxf(peak[2], peak[3]));
+    held[i] = row < most ? *reinterpret_cast<const uint4*>(x + row * side.x_row) : make_uint4(0, 0, 0, 0);
   }
 
-  float* at = side.scale + (long long)run.page * p.heads + head;
-  const float old = run.offset > 0 ? *at : 0.f;
-  const float now = fmaxf(old, scale_of(a));
-  uint8_t* page = side.pages + run.page * side.page_pitch + head * side.head_pitch;
-  if (now != old && run.offset > 0) {
+  // where the rows go: slots that follow one another within the page
+  const long long slot = p.slot_map[first];
+  const long long page_id = slot >> p.page_shift;
+  if (slot < 0 || page_id >= p.num_pages) {
+    if (slot >= 0) report_failure(status, kErrDeviceIndex, kSiteAppendSlot, uint32_t(first));
+    return;
+  }
+  const int offset = int(slot) & (page_size - 1);
+  most = min(most, page_size - offset);
+  int count = 0;
+  for (int base = 0; base < most; base += 32) {
+    const int i = base + int(lane_id());
+    const uint32_t follows = __ballot_sync(0xffffffffu, i < most && p.slot_map[first + i] == slot + i);
+    count = base + (follows == 0xffffffffu ? 32 : __ffs(int(~follows)) - 1);
+    if (follows != 0xffffffffu) break;
+  }
+  float* scale_at = side.scale + page_id * p.heads + head;
+  const float old = offset > 0 ? *scale_at : 0.f;
+
+  // the largest magnitude
+  auto all_rows = [&](auto take) {
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      if (row0 + i * kRows < count) take(held[i], row0 + i * kRows);
+    }
+    for (int row = row0 + kHeld * kRows; row < count; row += kRows) take(*reinterpret_cast<const uint4*>(x + row * side.x_row), row);
+  };
+  auto group_max = [&](uint32_t v) {  // of both halves, over the group
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = __vmaxu2(v, __shfl_xor_sync(0xffffffffu, v, o));
+    if constexpr (Threads > 32) {
+      __syncthreads();
+      if (lane_id() == 0) peaks[threadIdx.x >> 5] = v;
+      __syncthreads();
+      v = __vmaxu2(__vmaxu2(peaks[0], peaks[1]), __vmaxu2(peaks[2], peaks[3]));
+    }
+    return max(v & 0xffffu, v >> 16);
+  };
+  uint32_t bits = 0;
+  all_rows([&](const uint4& w, int) {
+    constexpr uint32_t kSize = 0x7fff7fffu;
+    bits = __vmaxu2(__vmaxu2(bits, __vmaxu2(w.x & kSize, w.y & kSize)), __vmaxu2(w.z & kSize, w.w & kSize));
+  });
+  bits = group_max(bits);
+  if (bits >= kInfinity) {
+    bits = 0;
+    all_rows([&](const uint4& w, int) {
+      const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t size = (words[e >> 1] >> (16 * (e & 1))) & 0x7fffu;
+        if (size < kInfinity) bits = max(bits, size);
+      }
+    });
+    bits = group_max(bits);
+  }
+  const float now = fmaxf(old, scale_of(unpack<BF16>(bits).x));
+
+  uint8_t* page = side.pages + page_id * side.page_pitch + head * side.head_pitch;
+  if (now != old && offset > 0) {
     const float ratio = old / now;
-    for (int i = tid; i < run.offset * (D / 16); i += Threads) {
+    for (int i = tid; i < offset * (D / 16); i += Threads) {
       uint4* spot = reinterpret_cast<uint4*>(page + (i / (D / 16)) * side.token_pitch + (i % (D / 16)) * 16);
       uint4 w = *spot;
       w.x = rescale_two(w.x, ratio) | rescale_two(w.x >> 16, ratio) << 16;
@@ -379,31 +380,38 @@ __global__ void __launch_bounds__(128) cache_append_kernel(AppendParams p, Devic
       *spot = w;
     }
   }
-  const Divisor by = {now, 1.0f / now, (__float_as_uint(now) & 0x7fffffu) == 0};
-  auto put = [&](const uint4& w, int row) {
-    uint2 codes;
-    codes.x = by.two(unpack<BF16>(w.x)) | by.two(unpack<BF16>(w.y)) << 16;
-    codes.y = by.two(unpack<BF16>(w.z)) | by.two(unpack<BF16>(w.w)) << 16;
-    *reinterpret_cast<uint2*>(page + (run.offset + row) * side.token_pitch + lane * 8) = codes;
-  };
-#pragma unroll
-  for (int i = 0; i < kHeld; ++i) {
-    const int row = row0 + i * kRows;
-    if (row < run.count) put(held[i], row);
+  uint8_t* out = page + offset * side.token_pitch + lane * 8;
+  if ((__float_as_uint(now) & 0x7fffffu) == 0) {
+    const float by = 1.0f / now;
+    auto two = [&](uint32_t w) {
+      const float2 v = unpack<BF16>(w);
+      return codes_of(make_float2(v.x * by, v.y * by));
+    };
+    all_rows([&](const uint4& w, int row) {
+      *reinterpret_cast<uint2*>(out + row * side.token_pitch) = make_uint2(two(w.x) | two(w.y) << 16, two(w.z) | two(w.w) << 16);
+    });
+  } else {
+    all_rows([&](const uint4& w, int row) {
+      const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+      uint32_t codes[4];
+#pragma unroll 1
+      for (int e = 0; e < 4; ++e) {
+        const float2 v = unpack<BF16>(words[e]);
+        codes[e] = codes_of(make_float2(v.x / now, v.y / now));
+      }
+      *reinterpret_cast<uint2*>(out + row * side.token_pitch) = make_uint2(codes[0] | codes[1] << 16, codes[2] | codes[3] << 16);
+    });
   }
-  for (int row = row0 + kHeld * kRows; row < run.count; row += kRows) put(*reinterpret_cast<const uint4*>(x + row * side.x_row), row);
   // every thread has read the old scale before it is replaced
   if constexpr (Threads > 32) __syncthreads(); else __syncwarp();
-  if (tid == 0 && now != old) *at = now;
+  if (tid == 0 && now != old) *scale_at = now;
 }
 
 template <int D, bool BF16, int Threads>
 int launch_append(const AppendParams& p, DeviceStatus* status, cudaStream_t stream) {
   const long long items = (long long)p.runs_len * 2 * p.heads;
   const long long blocks = (items + 128 / Threads - 1) / (128 / Threads);
-  cache_append_kernel<D, BF16, Threads><<<unsigned(blocks), 128, 0, stream>>>(p, status);
-  KRNB_CUDA(cudaGetLastError());
-  return KRN_B200_OK;
+  return launch_dependent(cache_append_kernel<D, BF16, Threads>, dim3(unsigned(blocks)), 128, 0, stream, p, status);
 }
 
 bool page_size_ok(int64_t page_size) { return page_size >= 16 && page_size <= 256 && (page_size & (page_size - 1)) == 0; }
@@ -475,11 +483,11 @@ extern "C" int krn_b200_cache_plan(const int32_t* context_len, const int32_t* ne
       })) {
     return rc;
   }
-  const int64_t wanted = (rows + kPlanThreads - 1) / kPlanThreads;
+  // a thread per row, and blocks enough for the pages of a few finished requests
+  const int64_t wanted = (rows + batch * 8 + kPlanThreads - 1) / kPlanThreads;
   const int blocks = int(wanted < 1 ? 1 : wanted > ctx->sm_count ? ctx->sm_count : wanted);
-  cache_plan_kernel<<<blocks, kPlanThreads, smem, static_cast<cudaStream_t>(stream_handle)>>>(p, ctx->status_dev);
-  KRNB_CUDA(cudaGetLastError());
-  return KRN_B200_OK;
+  return launch_dependent(cache_plan_kernel, dim3(unsigned(blocks)), kPlanThreads, smem, static_cast<cudaStream_t>(stream_handle), p,
+                          ctx->status_dev);
 }
 
 extern "C" int krn_b200_cache_append(int type, const void* k, const void* v, const int64_t* slot_map, const int32_t* runs,

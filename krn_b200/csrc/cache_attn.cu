@@ -22,9 +22,10 @@ constexpr float kLeastScale = 7.70371977754894341e-34f;  // 2^-110: value scales
 // Partial results of the pieces of split segments, 2 + d floats (m, l, the unnormalised output) for each of `rows`.
 struct StreamParams {
   CacheAttnParams a;
-  int32_t* tiles;    // [batch + 1] exclusive prefix of the requests' tile counts, written for the join
+  int4* pieces;      // [batch] first and last stretch of each request, whether its first piece is a warp's second; for the join
   float* partial;
   int slot_rows;     // rows a partial slot holds
+  int beside;        // launched beside the tile kernel, which waited for what came before: wait for it at the end
 };
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -159,6 +160,8 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     prefetch_tensormap(&map_k);
     prefetch_tensormap(&map_v);
   }
+  launch_dependents();
+  if (!p.beside) wait_for_kernel_before();
   // ---- every block counts the batch's tiles for itself
   int carry = 0;
   for (int first = 0; first < a.batch; first += kWarps * 32) {
@@ -185,17 +188,21 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   }
   if (threadIdx.x == 0) tiles[a.batch] = carry;
   __syncthreads();
+  const int total = carry, grid_warps = int(gridDim.x) * kWarps;
+  const int parts = stretches(total, grid_warps, a.kv_heads);
   if (blockIdx.x == 0) {
-    for (int b = threadIdx.x; b <= a.batch; b += kWarps * 32) p.tiles[b] = tiles[b];
     for (int b = threadIdx.x; b < a.batch; b += kWarps * 32) {
+      const int first = tiles[b], last = tiles[b + 1] - 1;
+      const int p0 = last >= first ? stretch_of(first, parts, total) : 0, p1 = last >= first ? stretch_of(last, parts, total) : 0;
+      p.pieces[b] = make_int4(p0, p1, first > first_tile(p0, parts, total) ? 1 : 0, 0);
       const int n = a.row_start[b + 1] - a.row_start[b];
       if (n > a.max_new) report_failure(status, kErrDeviceIndex, kSiteRows, uint32_t(n));
     }
   }
-  const int total = carry, grid_warps = int(gridDim.x) * kWarps;
-  const int parts = stretches(total, grid_warps, a.kv_heads);
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (total == 0) return;
+  if (total == 0) {
+    wait_for_kernel_before();
+    return;
+  }
 
   const int page_mask = (1 << a.page_shift) - 1;
   const int box = min(kTile, page_mask + 1);  // tokens of one copy
@@ -505,95 +512,88 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   if (!ok) {  // let this warp's own copies land before the block's memory goes
     for (int i = 0; i < 1000; ++i) __nanosleep(1000);
   }
+  wait_for_kernel_before();
 }
 
-// Joins the pieces of split segments: a block per (request, kv head, row),
-//   o = sum 2^(m_i - M) acc_i / sum 2^(m_i - M) l_i,
-// first the pieces' factors, a thread each, then the sum, a column each; the warps share the pieces. Launched as a
-// programmatic dependent of the stream kernel, so that its launch overlaps that kernel's end.
+// Joins the pieces of split segments,
+//   o = sum 2^(m_i - M) acc_i / sum 2^(m_i - M) l_i.
+// A block takes `slots` rows of one (request, kv head); kGroups / slots groups of threads, four columns a thread, share a
+// row's pieces, eight of them in flight at a time, and meet in shared memory. Bound by latency: one load of what the stream
+// kernel says about the request, one round of pieces. Launched as a programmatic dependent of the stream kernel: its blocks
+// are resident when that ends.
 constexpr int kJoinThreads = 256;
-constexpr int kJoinPieces = 2 * kMaxBlocks;  // pieces at a time
 
 template <int D, bool BF16>
-__global__ void __launch_bounds__(kJoinThreads) cache_join_kernel(StreamParams p, int grid_warps) {
-  constexpr int kLanes = D / 4;                       // threads per piece, four columns each
-  constexpr int kGroups = kJoinThreads / kLanes;      // pieces in work at once
-  __shared__ float factor[kJoinPieces];
-  __shared__ float4 shared[kJoinThreads];
-  __shared__ float red[2][kJoinThreads / 32];
+__global__ void __launch_bounds__(kJoinThreads) cache_join_kernel(StreamParams p, int slots) {
+  constexpr int kLanes = D / 4, kGroups = kJoinThreads / kLanes;
+  __shared__ float4 shared_acc[kGroups][kLanes];
+  __shared__ float2 shared_ml[kGroups];
   const CacheAttnParams& a = p.a;
-  const int b = blockIdx.x / a.kv_heads, g = blockIdx.x % a.kv_heads, row = blockIdx.y;
-  const int tid = threadIdx.x, group = tid / kLanes, lane = tid % kLanes;
-  const int row0 = a.row_start[b], n = a.row_start[b + 1] - row0;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int first = p.tiles[b], tiles = p.tiles[b + 1] - first, total = p.tiles[a.batch];
-  if (tiles == 0 || row >= n * a.group || row0 + row / a.group >= a.rows) return;
-  const int parts = stretches(total, grid_warps, a.kv_heads);
-  const int p0 = stretch_of(first, parts, total), p1 = stretch_of(first + tiles - 1, parts, total);
-  if (p0 == p1) return;  // one warp had it all and has written it
-  auto piece = [&](int part) {
-    const long long slot = 2ll * (part * a.kv_heads + g) + (first > first_tile(part, parts, total) ? 1 : 0);
-    return p.partial + (slot * p.slot_rows + row) * (D + 4);
-  };
-  float top = -INFINITY, den = 0.f;
+  const int b = blockIdx.x / a.kv_heads, g = blockIdx.x % a.kv_heads;
+  const int group = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
+  const int row = blockIdx.y * slots + group % slots, share = group / slots, shares = kGroups / slots;
+  const int row0 = a.row_start[b], rows = (a.row_start[b + 1] - row0) * a.group;
+  const int at = row0 + row / a.group;
+  wait_for_kernel_before();
+  const int4 piece = p.pieces[b];
+  if (piece.x == piece.y) return;  // no split: the rows are written, or belong to the other path
+  const bool live = row < rows && at < a.rows;
+  float m = -INFINITY, l = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int base = p0; base <= p1; base += kJoinPieces) {
-    const int here = min(kJoinPieces, p1 + 1 - base);
-    float m[2], l[2], high = -INFINITY;
+  if (live) {
+    const long long pitch = (long long)p.slot_rows * (D + 4);  // of a slot; a stretch and kv head have two
+    const float* from = p.partial + 2 * g * pitch + (long long)row * (D + 4);
+#pragma unroll 1
+    for (int first = piece.x + share; first <= piece.y; first += 8 * shares) {
+      float2 ml[8];
+      float4 x[8];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int i = tid + k * kJoinThreads;
-      const float2 ml = i < here ? *reinterpret_cast<const float2*>(piece(base + i)) : make_float2(-INFINITY, 0.f);
-      m[k] = ml.x;
-      l[k] = ml.y;
-      high = fmaxf(high, ml.x);
+      for (int k = 0; k < 8; ++k) {
+        const int part = first + k * shares;
+        const bool there = part <= piece.y;
+        const float* at_piece = from + (2ll * (there ? part : piece.x) * a.kv_heads + (part == piece.x ? piece.z : 0)) * pitch;
+        ml[k] = there ? *reinterpret_cast<const float2*>(at_piece) : make_float2(-INFINITY, 0.f);
+        x[k] = there ? *reinterpret_cast<const float4*>(at_piece + 4 + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      float high = m;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) high = fmaxf(high, ml[k].x);
+      const float old = m == -INFINITY ? 0.f : ex2_approx(m - high);
+      m = high;
+      l *= old;
+      acc.x *= old, acc.y *= old, acc.z *= old, acc.w *= old;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float by = ml[k].x == -INFINITY ? 0.f : ex2_approx(ml[k].x - high);
+        l += by * ml[k].y;
+        acc.x += by * x[k].x, acc.y += by * x[k].y, acc.z += by * x[k].z, acc.w += by * x[k].w;
+      }
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
-    if ((tid & 31) == 0) red[0][tid >> 5] = high;
+  }
+  if (shares > 1) {
+    shared_acc[group][lane] = acc;
+    if (lane == 0) shared_ml[group] = make_float2(m, l);
     __syncthreads();
-    float top_new = top;
-#pragma unroll
-    for (int w = 0; w < kJoinThreads / 32; ++w) top_new = fmaxf(top_new, red[0][w]);
-    const float old = top == -INFINITY ? 0.f : exp2f(top - top_new);
-    top = top_new;
-    float sum = 0.f;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int i = tid + k * kJoinThreads;
-      const float by = m[k] == -INFINITY ? 0.f : exp2f(m[k] - top);
-      if (i < here) factor[i] = by;
-      sum += by * l[k];
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if ((tid & 31) == 0) red[1][tid >> 5] = sum;
-    __syncthreads();
-    den *= old;
-#pragma unroll
-    for (int w = 0; w < kJoinThreads / 32; ++w) den += red[1][w];
-    acc.x *= old, acc.y *= old, acc.z *= old, acc.w *= old;
-#pragma unroll 8
-    for (int i = group; i < here; i += kGroups) {
-      const float by = factor[i];
-      const float4 x = *reinterpret_cast<const float4*>(piece(base + i) + 4 + lane * 4);
+    if (share > 0) return;
+    float high = m;
+    for (int k = 1; k < shares; ++k) high = fmaxf(high, shared_ml[group + k * slots].x);
+    const float own = m == -INFINITY ? 0.f : ex2_approx(m - high);
+    l *= own;
+    acc.x *= own, acc.y *= own, acc.z *= own, acc.w *= own;
+    for (int k = 1; k < shares; ++k) {
+      const float2 ml = shared_ml[group + k * slots];
+      const float4 x = shared_acc[group + k * slots][lane];
+      const float by = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - high);
+      l += by * ml.y;
       acc.x += by * x.x, acc.y += by * x.y, acc.z += by * x.z, acc.w += by * x.w;
     }
-    __syncthreads();
   }
-  shared[tid] = acc;
-  __syncthreads();
-  if (group > 0) return;
-#pragma unroll
-  for (int k = 1; k < kGroups; ++k) {
-    const float4 x = shared[k * kLanes + lane];
-    acc.x += x.x, acc.y += x.y, acc.z += x.z, acc.w += x.w;
-  }
-  const float by = den == 0.f ? 0.f : 1.0f / den;
+  if (!live) return;
+  const float by = l == 0.f ? 0.f : 1.0f / l;
   uint2 w;
   w.x = BF16 ? pack_bf16x2(acc.x * by, acc.y * by) : pack_f16x2(acc.x * by, acc.y * by);
   w.y = BF16 ? pack_bf16x2(acc.z * by, acc.w * by) : pack_f16x2(acc.z * by, acc.w * by);
-  *reinterpret_cast<uint2*>(a.o + (long long)(row0 + row / a.group) * a.o_row + (g * a.group + row % a.group) * a.o_head + lane * 4) = w;
+  *reinterpret_cast<uint2*>(a.o + (long long)at * a.o_row + (long long)(g * a.group + row % a.group) * a.o_head + lane * 4) = w;
 }
 
 template <int D, bool BF16, int NT>
@@ -616,19 +616,17 @@ int launch_stream(const DeviceContext* ctx, const StreamParams& p, int64_t page_
   const int64_t wanted = (int64_t(a.batch) * a.kv_heads * ((a.max_context + kTile - 1) / kTile) + kWarps - 1) / kWarps;
   const int most = ctx->sm_count < kMaxBlocks ? ctx->sm_count : kMaxBlocks;
   const int blocks = int(wanted < most ? wanted : most);
-  kernel<<<blocks, kWarps * 32, StreamLayout<D>::bytes(a.batch), stream>>>(map_k, map_v, p, ctx->status_dev);
-  KRNB_CUDA(cudaGetLastError());
-  cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(unsigned(a.batch) * unsigned(a.kv_heads), unsigned(p.slot_rows), 1);
-  config.blockDim = dim3(kJoinThreads, 1, 1);
-  config.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = attr;
-  config.numAttrs = 1;
-  KRNB_CUDA(cudaLaunchKernelEx(&config, cache_join_kernel<D, BF16>, p, blocks * kWarps));
-  return KRN_B200_OK;
+  if (int rc = launch_dependent(kernel, dim3(unsigned(blocks)), kWarps * 32, StreamLayout<D>::bytes(a.batch), stream, map_k, map_v, p,
+                                ctx->status_dev)) {
+    return rc;
+  }
+  // rows of a block: as few as leave each group of threads no more than eight pieces, as the batch is split on average
+  constexpr int kGroups = kJoinThreads * 4 / D;
+  const int64_t pieces = int64_t(blocks) * kWarps / a.kv_heads / a.batch + 2;
+  int slots = kGroups;
+  while (slots > 1 && (slots / 2 >= p.slot_rows || pieces > 8 * (kGroups / slots))) slots /= 2;
+  const dim3 grid(unsigned(a.batch) * unsigned(a.kv_heads), unsigned((p.slot_rows + slots - 1) / slots));
+  return launch_dependent(cache_join_kernel<D, BF16>, grid, kJoinThreads, 0, stream, p, slots);
 }
 
 // Rows of a streamed request: all of them where every request has few; where some have many, those with one new token
@@ -638,11 +636,11 @@ int64_t slot_rows(int64_t max_new, int64_t group) {
   return group <= 8 ? 8 : group <= 16 ? 16 : group <= 32 ? 32 : 0;
 }
 
-int64_t prefix_bytes(int64_t batch) { return (batch + 1 + 3) / 4 * 16; }
+int64_t pieces_bytes(int64_t batch) { return batch * 16; }
 
 int64_t stream_workspace(int64_t batch, int64_t kv_heads, int64_t d, int64_t rows) {
   const int64_t warps = int64_t(kMaxBlocks) * kWarps, units = warps > kv_heads ? warps : kv_heads;
-  return prefix_bytes(batch) + 2 * units * rows * (d + 4) * 4;
+  return pieces_bytes(batch) + 2 * units * rows * (d + 4) * 4;
 }
 
 template <int D, bool BF16>
@@ -759,16 +757,22 @@ extern "C" int krn_b200_cache_attn(int type, const void* q, const void* k_pages,
   StreamParams sp;
   p.few = int(slot_rows(max_new, p.group));
   sp.a = p;
-  sp.tiles = static_cast<int32_t*>(workspace);
-  sp.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + prefix_bytes(batch));
+  sp.pieces = static_cast<int4*>(workspace);
+  sp.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + pieces_bytes(batch));
   sp.slot_rows = p.few;
+  // The two paths run side by side: the tile kernel first, whose blocks take longest, and the stream on the SMs that it
+  // leaves free.
+  const bool tiled = max_new * p.group > p.few && tile_blocks(batch, rows, p.group, p.few) > 0;
+  float* shares = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + stream_workspace(batch, kv_heads, d, p.few));
+  if (tiled) {
+    if (int rc = launch_tiles(ctx, p, bf16, d, page_size, shares, stream)) return rc;
+  }
   if (p.few > 0) {
+    sp.beside = tiled;
     int rc;
     if (d == 128) rc = bf16 ? launch_stream_rows<128, true>(ctx, sp, page_size, stream) : launch_stream_rows<128, false>(ctx, sp, page_size, stream);
     else rc = bf16 ? launch_stream_rows<64, true>(ctx, sp, page_size, stream) : launch_stream_rows<64, false>(ctx, sp, page_size, stream);
     if (rc) return rc;
   }
-  if (max_new * p.group <= p.few) return KRN_B200_OK;
-  float* partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + stream_workspace(batch, kv_heads, d, p.few));
-  return launch_tiles(ctx, p, bf16, d, page_size, partial, stream);
+  return tiled ? launch_tile_join(p, bf16, d, shares, stream) : KRN_B200_OK;
 }

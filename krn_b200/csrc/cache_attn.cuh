@@ -62,9 +62,13 @@ inline int encode_pool(CUtensorMap* map, const PoolSide& side, int64_t d, int64_
   return encode_tensor_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, side.pages, dims, strides, box, swizzle);
 }
 
-// Requests with many rows (cache_attn_tile.cu). `partial` holds tile_workspace() bytes.
+// Requests with many rows (cache_attn_tile.cu). `partial` holds tile_workspace() bytes. tile_blocks() bounds the blocks of
+// query rows that they can have: with none there is nothing to launch.
+int64_t tile_blocks(int64_t batch, int64_t rows, int64_t group, int64_t few);
 int64_t tile_workspace(int64_t batch, int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t d, int64_t few, int64_t max_context);
 int launch_tiles(const DeviceContext* ctx, const CacheAttnParams& a, bool bf16, int64_t d, int64_t page_size, float* partial,
                  cudaStream_t stream);
+// Joins what launch_tiles() split over the keys, behind the kernels that were launched since.
+int launch_tile_join(const CacheAttnParams& a, bool bf16, int64_t d, float* partial, cudaStream_t stream);
 
 }  // namespace krnb

@@ -152,6 +152,8 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   const int warp = threadIdx.x >> 5;
   const int lane = int(lane_id());
 
+  wait_for_kernel_before();
+  launch_dependents();  // what comes beside needs what came before
   // ---- which request: blocks of the batch's requests in order, the last (longest) block of a request first
   const int g = int(blockIdx.x) % a.kv_heads, wanted = int(blockIdx.x) / a.kv_heads;
   if (threadIdx.x == 0) {
@@ -658,6 +660,7 @@ __global__ void __launch_bounds__(128) cache_tile_join_kernel(TileParams p) {
   constexpr int kCols = D / 32;
   const CacheAttnParams& a = p.a;
   const int row = blockIdx.x, head = blockIdx.y * 4 + (threadIdx.x >> 5), lane = int(lane_id());
+  wait_for_kernel_before();
   if (head >= a.q_heads || row >= a.row_start[a.batch]) return;
   int low = 0, high = a.batch;  // the last request that starts at or before the row
   while (high - low > 1) {
@@ -687,13 +690,6 @@ __global__ void __launch_bounds__(128) cache_tile_join_kernel(TileParams p) {
     const float y = acc[c] * by;
     out[c * 32 + lane] = uint16_t((BF16 ? pack_bf16x2(y, 0.f) : pack_f16x2(y, 0.f)) & 0xffffu);
   }
-}
-
-// Blocks that the grid needs at most: every tiled request has more than `few` rows.
-int64_t blocks_bound(int64_t batch, int64_t rows, int64_t group, int64_t few) {
-  const int64_t least = few / group + 1, tokens = 2 * (kTileQ / group);
-  const int64_t requests = rows / least < batch ? rows / least : batch;
-  return rows / tokens + requests;
 }
 
 // Shares of the keys: as many as fill the GPU where there are few blocks, none shorter than four key tiles.
@@ -728,34 +724,43 @@ int launch(const DeviceContext* ctx, const TileParams& p, int64_t page_size, int
       })) {
     return rc;
   }
-  kernel<<<dim3(unsigned(blocks * a.kv_heads), unsigned(p.splits)), kThreads, L::kSmemBytes, stream>>>(map_k, map_v, p,
-                                                                                                    ctx->status_dev);
-  KRNB_CUDA(cudaGetLastError());
-  if (p.splits > 1) {
-    cache_tile_join_kernel<D, BF16><<<dim3(unsigned(a.rows), unsigned((a.q_heads + 3) / 4)), 128, 0, stream>>>(p);
-    KRNB_CUDA(cudaGetLastError());
-  }
-  return KRN_B200_OK;
+  return launch_dependent(kernel, dim3(unsigned(blocks * a.kv_heads), unsigned(p.splits)), kThreads, L::kSmemBytes, stream, map_k, map_v,
+                          p, ctx->status_dev);
+}
+
+TileParams tile_params(const CacheAttnParams& a, float* partial, int64_t blocks) {
+  return {a, partial, kTileQ / a.group, int(splits_of(blocks * a.kv_heads, a.max_context))};
 }
 
 }  // namespace
 
+// Every tiled request has more than `few` rows, so there are not many of them.
+int64_t tile_blocks(int64_t batch, int64_t rows, int64_t group, int64_t few) {
+  const int64_t least = few / group + 1, tokens = 2 * (kTileQ / group);
+  const int64_t requests = rows / least < batch ? rows / least : batch;
+  return requests > 0 ? rows / tokens + requests : 0;
+}
+
 int64_t tile_workspace(int64_t batch, int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t d, int64_t few, int64_t max_context) {
-  const int64_t splits = splits_of(blocks_bound(batch, rows, q_heads / kv_heads, few) * kv_heads, max_context);
+  const int64_t splits = splits_of(tile_blocks(batch, rows, q_heads / kv_heads, few) * kv_heads, max_context);
   return splits > 1 ? splits * rows * q_heads * (d + 4) * 4 : 0;
 }
 
 int launch_tiles(const DeviceContext* ctx, const CacheAttnParams& a, bool bf16, int64_t d, int64_t page_size, float* partial,
                  cudaStream_t stream) {
-  TileParams p;
-  p.a = a;
-  p.partial = partial;
-  p.tokens = kTileQ / a.group;
-  const int64_t blocks = blocks_bound(a.batch, a.rows, a.group, a.few);
-  if (blocks == 0) return KRN_B200_OK;
-  p.splits = int(splits_of(blocks * a.kv_heads, a.max_context));
+  const int64_t blocks = tile_blocks(a.batch, a.rows, a.group, a.few);
+  const TileParams p = tile_params(a, partial, blocks);
   if (d == 128) return bf16 ? launch<128, true>(ctx, p, page_size, blocks, stream) : launch<128, false>(ctx, p, page_size, blocks, stream);
   return bf16 ? launch<64, true>(ctx, p, page_size, blocks, stream) : launch<64, false>(ctx, p, page_size, blocks, stream);
+}
+
+int launch_tile_join(const CacheAttnParams& a, bool bf16, int64_t d, float* partial, cudaStream_t stream) {
+  const int64_t blocks = tile_blocks(a.batch, a.rows, a.group, a.few);
+  const TileParams p = tile_params(a, partial, blocks);
+  if (p.splits == 1) return KRN_B200_OK;
+  const dim3 grid(unsigned(a.rows), unsigned((a.q_heads + 3) / 4));
+  if (d == 128) return launch_dependent(bf16 ? cache_tile_join_kernel<128, true> : cache_tile_join_kernel<128, false>, grid, 128, 0, stream, p);
+  return launch_dependent(bf16 ? cache_tile_join_kernel<64, true> : cache_tile_join_kernel<64, false>, grid, 128, 0, stream, p);
 }
 
 }  // namespace krnb

@@ -71,6 +71,25 @@ class OncePerDevice {
   std::atomic<uint64_t> done_{0};
 };
 
+// Launches a kernel that begins with `griddepcontrol.wait`: its launch and what it does before that overlap the end of the
+// kernel before it in the stream, where that one lets dependents go (`griddepcontrol.launch_dependents`); behind any other
+// kernel this is an ordinary launch.
+template <class... Params, class... Args>
+int launch_dependent(void (*kernel)(Params...), dim3 grid, unsigned threads, size_t smem, cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = grid;
+  config.blockDim = dim3(threads, 1, 1);
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attr;
+  config.numAttrs = 1;
+  KRNB_CUDA(cudaLaunchKernelEx(&config, kernel, Params(args)...));
+  return KRN_B200_OK;
+}
+
 // ---- TMA descriptors -----------------------------------------------------------------------------------
 
 enum class Swizzle { kNone, k64B, k128B };

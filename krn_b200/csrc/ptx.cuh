@@ -83,6 +83,11 @@ __device__ __forceinline__ bool elect_one() {
   return chosen != 0;
 }
 
+// Programmatic dependent launch: let the next kernel of the stream begin / wait until the kernel before has completed and
+// its writes are visible. A kernel whose blocks all wait completes after everything before it in the stream.
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_kernel_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---- mbarrier ----------------------------------------------------------------------------------------
 
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
