@@ -305,19 +305,19 @@ int krn_b200_cache_plan(const int32_t* context_len, const int32_t* new_len, int3
                         int64_t page_size, int64_t num_pages, int64_t rows, int64_t runs_len, void* stream);
 
 /* Quantise the step's keys and values into the pool.
- *   k, v         bf16 or f16 (`type`) [rows, kv_heads, d]; *_strides: element strides of rows and heads, multiples of 8
+ *   k, v         bf16 or f16 (`type`) [rows, kv_heads, d]
  *   slot_map, runs  as krn_b200_cache_plan makes them: rows of one page are consecutive, in slot order, and no two runs
  *                share a page (two that do race on its scale). Rows with slot -1 and runs past the rows are skipped; a slot
  *                beyond the pool is skipped and reported (KRN_B200_ERR_DEVICE_INDEX)
- *   *_page_strides  element (= byte) strides of pages, tokens and heads of a pool
+ *   strides      HOST array of 10 element strides: rows and heads of k, rows and heads of v (multiples of 8), then pages,
+ *                tokens and heads of the K pool and of the V pool (multiples of 16)
  * For each run and head the page's scale becomes max(scale, least power of two 2^k, k >= -100, with all of the run's finite
  * magnitudes <= 448 * 2^k); a run that begins at a page's offset 0 ignores the scale the page had. Codes the page holds
  * already are rounded again to the new scale where it grew. Infinities become +-448 codes and NaN NaN codes; neither has a
  * say in the scale. */
 int krn_b200_cache_append(int type, const void* k, const void* v, const int64_t* slot_map, const int32_t* runs, void* k_pages,
                           void* v_pages, float* k_scale, float* v_scale, int64_t rows, int64_t runs_len, int64_t kv_heads,
-                          int64_t d, int64_t page_size, int64_t num_pages, const int64_t* k_strides, const int64_t* v_strides,
-                          const int64_t* k_page_strides, const int64_t* v_page_strides, void* stream);
+                          int64_t d, int64_t page_size, int64_t num_pages, const int64_t* strides, void* stream);
 
 /* Bytes of caller workspace krn_b200_cache_attn needs for these extents. */
 int64_t krn_b200_cache_attn_workspace_bytes(int64_t batch, int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t d,
@@ -325,14 +325,16 @@ int64_t krn_b200_cache_attn_workspace_bytes(int64_t batch, int64_t rows, int64_t
 
 /* Attention of packed query rows over the pool: row i of the n rows of a request with a context of c tokens (the new ones
  * included, already in the cache) stands at position c - n + i and sees keys 0 .. c - n + i.
- *   q, o         bf16 or f16 (`type`) [rows, q_heads, d]; *_strides: element strides of rows and heads, multiples of 8;
- *                q_heads % kv_heads == 0, at most 128 q heads per kv head
+ *   q, o         bf16 or f16 (`type`) [rows, q_heads, d]; q_heads % kv_heads == 0, at most 128 q heads per kv head
  *   row_start    int32 [batch + 1], context_len int32 [batch]: as krn_b200_cache_plan makes them. Contexts are clamped into
  *                [0, max_context]; rows of o behind row_start[batch] are left as they were; a row that sees no key gets zeros
  *   max_new      no request has more rows than this; one that has is not computed and reported
  *                (KRN_B200_ERR_DEVICE_INDEX). It chooses the kernels, as max_context does
  *   page ids outside [0, num_pages) are never fetched: their tokens read as zeros, and the status word reports
  *                KRN_B200_ERR_DEVICE_INDEX; entries past a request's context are never looked at
+ *   scales       are not negative
+ *   strides      HOST array of 10 element strides: rows and heads of q, rows and heads of o (multiples of 8), then pages,
+ *                tokens and heads of the K pool and of the V pool (multiples of 16)
  *   scale_log2   log2(e) * softmax scale
  *   workspace    at least krn_b200_cache_attn_workspace_bytes(...) bytes, 16-byte aligned; needs no preparation. Calls that
  *                may overlap on the GPU need one each */
@@ -340,8 +342,7 @@ int krn_b200_cache_attn(int type, const void* q, const void* k_pages, const void
                         const float* v_scale, const int32_t* page_table, const int32_t* context_len, const int32_t* row_start,
                         void* o, int64_t batch, int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t d, int64_t page_size,
                         int64_t num_pages, int64_t max_pages, int64_t table_pitch, int64_t max_new, int64_t max_context,
-                        const int64_t* q_strides, const int64_t* o_strides, const int64_t* k_page_strides,
-                        const int64_t* v_page_strides, float scale_log2, void* workspace, int64_t workspace_bytes, void* stream);
+                        const int64_t* strides, float scale_log2, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Copy this rank's column block C_local[M, n_local] into columns [col0, col0 + n_local) of the row-major
  * C_full[M, N] (ld in elements, elem_bytes 2 or 4). Used after the NCCL all-gather of GEMM output column

@@ -493,8 +493,7 @@ extern "C" int krn_b200_cache_plan(const int32_t* context_len, const int32_t* ne
 extern "C" int krn_b200_cache_append(int type, const void* k, const void* v, const int64_t* slot_map, const int32_t* runs,
                                      void* k_pages, void* v_pages, float* k_scale, float* v_scale, int64_t rows,
                                      int64_t runs_len, int64_t heads, int64_t d, int64_t page_size, int64_t num_pages,
-                                     const int64_t* k_strides, const int64_t* v_strides, const int64_t* k_page_strides,
-                                     const int64_t* v_page_strides, void* stream_handle) {
+                                     const int64_t* strides, void* stream_handle) {
   using namespace krnb;
   if (type != KRN_B200_BF16 && type != KRN_B200_F16) {
     return fail(KRN_B200_ERR_UNSUPPORTED, "cache append of element type %d is not available on sm_100a: keys and values come in "
@@ -517,10 +516,10 @@ extern "C" int krn_b200_cache_append(int type, const void* k, const void* v, con
     return fail(KRN_B200_ERR_UNSUPPORTED, "extents too large for this kernel's 32-bit indices");
   }
   if (k == nullptr || v == nullptr || slot_map == nullptr || runs == nullptr || k_pages == nullptr || v_pages == nullptr ||
-      k_scale == nullptr || v_scale == nullptr || k_strides == nullptr || v_strides == nullptr || k_page_strides == nullptr ||
-      v_page_strides == nullptr) {
+      k_scale == nullptr || v_scale == nullptr || strides == nullptr) {
     return fail(KRN_B200_ERR_INVALID_ARGUMENT, "null tensor address");
   }
+  const int64_t *k_strides = strides, *v_strides = strides + 2, *k_page_strides = strides + 4, *v_page_strides = strides + 7;
   if (!aligned16(k) || !aligned16(v) || !aligned16(k_pages) || !aligned16(v_pages) || k_strides[0] % 8 || k_strides[1] % 8 ||
       v_strides[0] % 8 || v_strides[1] % 8) {
     return fail(KRN_B200_ERR_INVALID_ARGUMENT, "rows are read 16 bytes at a time: addresses and strides must be multiples of 16 bytes");

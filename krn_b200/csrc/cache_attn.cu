@@ -666,8 +666,7 @@ extern "C" int krn_b200_cache_attn(int type, const void* q, const void* k_pages,
                                    const float* v_scale, const int32_t* page_table, const int32_t* context_len,
                                    const int32_t* row_start, void* o, int64_t batch, int64_t rows, int64_t q_heads,
                                    int64_t kv_heads, int64_t d, int64_t page_size, int64_t num_pages, int64_t max_pages,
-                                   int64_t table_pitch, int64_t max_new, int64_t max_context, const int64_t* q_strides,
-                                   const int64_t* o_strides, const int64_t* k_page_strides, const int64_t* v_page_strides,
+                                   int64_t table_pitch, int64_t max_new, int64_t max_context, const int64_t* strides,
                                    float scale_log2, void* workspace, int64_t workspace_bytes, void* stream_handle) {
   using namespace krnb;
   if (type != KRN_B200_BF16 && type != KRN_B200_F16) {
@@ -706,10 +705,10 @@ extern "C" int krn_b200_cache_attn(int type, const void* q, const void* k_pages,
     return fail(KRN_B200_ERR_UNSUPPORTED, "extents too large for this kernel's 32-bit indices");
   }
   if (q == nullptr || k_pages == nullptr || v_pages == nullptr || k_scale == nullptr || v_scale == nullptr ||
-      page_table == nullptr || context_len == nullptr || row_start == nullptr || o == nullptr || q_strides == nullptr ||
-      o_strides == nullptr || k_page_strides == nullptr || v_page_strides == nullptr) {
+      page_table == nullptr || context_len == nullptr || row_start == nullptr || o == nullptr || strides == nullptr) {
     return fail(KRN_B200_ERR_INVALID_ARGUMENT, "null tensor address");
   }
+  const int64_t *q_strides = strides, *o_strides = strides + 2, *k_page_strides = strides + 4, *v_page_strides = strides + 7;
   if (!aligned16(q) || !aligned16(o) || !aligned16(k_pages) || !aligned16(v_pages) || q_strides[0] % 8 || q_strides[1] % 8 ||
       o_strides[0] % 8 || o_strides[1] % 8) {
     return fail(KRN_B200_ERR_INVALID_ARGUMENT, "addresses and the strides of q and o must be multiples of 16 bytes");

@@ -6,7 +6,7 @@ from __future__ import annotations
 
 import math
 from dataclasses import dataclass
-from typing import Any
+from typing import Any, NamedTuple
 
 import numpy as np
 
@@ -18,6 +18,13 @@ from krn_b200.runtime.device import DeviceTensor, _raw, default_device
 
 def _stream(stream: Any):
     return getattr(stream, "raw", stream)
+
+
+_LOG2_E = math.log2(math.e)
+
+
+def _all_raw(*values: Any) -> list[Any]:
+    return [value.data if isinstance(value, DeviceTensor) else value for value in values]
 
 
 def matmul_nt(a: Any, b: Any, out: Any, stream: Any = None) -> Any:
@@ -223,8 +230,7 @@ def decode_attention(q: Any, k_pages: Any, v_pages: Any, page_table: Any, contex
     return out
 
 
-@dataclass(frozen=True)
-class PagedCache:
+class PagedCache(NamedTuple):
     """A paged 8-bit key/value cache on the device: e4m3 codes [pages, page size, kv heads, d] and one f32 scale per
     (page, kv head), for keys and for values; a value is code * scale. Pages are 16, 32, 64, 128 or 256 tokens, d is 64 or
     128. The d axis is contiguous; the other strides are free (multiples of 16 bytes), so the two pools may be halves of one
@@ -254,8 +260,7 @@ def paged_cache(num_pages: int, page_size: int, kv_heads: int, d: int, device: A
     return PagedCache(*codes, *scales)
 
 
-@dataclass(frozen=True)
-class CachePlan:
+class CachePlan(NamedTuple):
     """What `plan_cache` says of a step: the requests' new contexts (int32 [batch]), the first row of each request in the
     step's packed rows (int32 [batch + 1]), the slot of every row (int64 [rows], page * page size + offset; -1 behind the
     last request), the rows where a page's run of new tokens begins (int32, -1 behind the last) and the pool's state
@@ -291,9 +296,7 @@ def plan_cache(context_len: Any, new_len: Any, page_table: Any, free_pages: Any,
     Fills `plan`, whose `context_len` and `pool_state` are the next step's inputs (with another plan: outputs never share
     memory with inputs). A step that does not fit is refused whole: `plan.pool_state[2]` is then not 0 and no row has a
     slot."""
-    calls.cache_plan(_raw(context_len), _raw(new_len), _raw(page_table), _raw(free_pages), _raw(pool_state),
-                     _raw(plan.context_len), _raw(plan.row_start), _raw(plan.slot_map), _raw(plan.runs), _raw(plan.pool_state),
-                     page_size, num_pages, _stream(stream))
+    calls.cache_plan(*_all_raw(context_len, new_len, page_table, free_pages, pool_state, *plan), page_size, num_pages, _stream(stream))
     return plan
 
 
@@ -303,8 +306,7 @@ def append_cache(k: Any, v: Any, slot_map: Any, runs: Any, cache: PagedCache, st
     grows while the page fills: the codes the page holds already are then rounded again to the new scale, which a power of
     two leaves exact but for values below e4m3's normal range. Rows of one page must be consecutive and in slot order, as
     `plan_cache` lays them out."""
-    calls.cache_append(_raw(k), _raw(v), _raw(slot_map), _raw(runs), _raw(cache.k_pages), _raw(cache.v_pages),
-                       _raw(cache.k_scale), _raw(cache.v_scale), _stream(stream))
+    calls.cache_append(*_all_raw(k, v, slot_map, runs, *cache), _stream(stream))
     return cache
 
 
@@ -322,11 +324,9 @@ def cache_attention(q: Any, cache: PagedCache, page_table: Any, context_len: Any
     in one call. `scale` defaults to 1/sqrt(d). `max_new` is the most rows any request has (one with more is not computed
     and reported), contexts are clamped to `max_context`. Rows that see no key get zeros; rows behind the last request are
     left as they were."""
-    d = q.shape[-1]
-    scale = (1.0 / math.sqrt(d)) if scale is None else scale
-    calls.cache_attention(_raw(q), _raw(cache.k_pages), _raw(cache.v_pages), _raw(cache.k_scale), _raw(cache.v_scale),
-                          _raw(page_table), _raw(context_len), _raw(row_start), _raw(out), scale * math.log2(math.e), max_new,
-                          max_context, _raw(workspace), _stream(stream))
+    scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
+    calls.cache_attention(*_all_raw(q, *cache, page_table, context_len, row_start, out), scale * _LOG2_E, max_new, max_context,
+                          _raw(workspace), _stream(stream))
     return out
 
 

@@ -5,6 +5,7 @@ missing kernel library raises `LibraryNotFound`."""
 from __future__ import annotations
 
 import ctypes
+import struct
 import sys
 from typing import Any
 
@@ -270,13 +271,13 @@ def attention_decode_fp8_paged_noalloc(q: Any, k_pages: Any, v_pages: Any, page_
     native.check(status, "paged FP8 decode attention (built-in scratch)")
 
 
-_Strides2, _Strides3 = ctypes.c_int64 * 2, ctypes.c_int64 * 3
+_pack_strides = struct.Struct("10q").pack  # what the paged cache's entry points take: one array, filled in one go
 
 
 class _Place:
     """Checks of one call's tensors and their addresses. Every tensor lives on the current CUDA device: an address of host
     memory or of another GPU never reaches a kernel. These run before every launch of kernels of a few microseconds, so
-    they ask a tensor for as little as they can."""
+    they ask a tensor for as little as they can and say what was wrong apart."""
 
     __slots__ = ("feature", "torch", "device")
 
@@ -286,25 +287,34 @@ class _Place:
         self.feature, self.torch, self.device = feature, torch, -2
 
     def address(self, name: str, tensor: Any) -> int:
-        place = tensor.get_device() if hasattr(tensor, "get_device") else -1
+        try:
+            place = tensor.get_device()
+        except AttributeError:
+            place = -1
         if place != self.device:
-            if place < 0:
-                raise ValueError(f"{self.feature}: `{name}` must be a CUDA tensor")
-            self.device = self.torch.cuda.current_device()
-            if place != self.device:
-                raise ValueError(f"{self.feature}: `{name}` is on cuda:{place}, the current device is cuda:{self.device}")
+            self._settle(name, place)
         return tensor.data_ptr()
+
+    def _settle(self, name: str, place: int) -> None:
+        if place < 0:
+            raise ValueError(f"{self.feature}: `{name}` must be a CUDA tensor")
+        self.device = self.torch.cuda.current_device()
+        if place != self.device:
+            raise ValueError(f"{self.feature}: `{name}` is on cuda:{place}, the current device is cuda:{self.device}")
 
     def vector(self, name: str, tensor: Any, dtype: Any, length: int = -1) -> int:
         """A contiguous rank-1 tensor of `dtype` (and of `length` elements)."""
         address = self.address(name, tensor)
+        if tensor.dtype is not dtype or tensor.dim() != 1 or not tensor.is_contiguous() or -1 < length != tensor.numel():
+            self._refuse_vector(name, tensor, dtype, length)
+        return address
+
+    def _refuse_vector(self, name: str, tensor: Any, dtype: Any, length: int) -> None:
         if tensor.dtype is not dtype:
             raise TypeError(f"{self.feature}: `{name}` must be {str(dtype)[6:]}, got {tensor.dtype}")
         if tensor.dim() != 1 or not tensor.is_contiguous():
             raise ValueError(f"{self.feature}: `{name}` must be a contiguous vector, got shape {tuple(tensor.shape)}")
-        if length >= 0 and tensor.numel() != length:
-            raise ValueError(f"{self.feature}: `{name}` has {tensor.numel()} elements, {length} expected")
-        return address
+        raise ValueError(f"{self.feature}: `{name}` has {tensor.numel()} elements, {length} expected")
 
     def table(self, name: str, tensor: Any, batch: int) -> tuple[int, int, int]:
         """(address, entries per row, row pitch) of an int32 page table [batch, entries]."""
@@ -325,7 +335,7 @@ class _Place:
             return native.F16
         return _type_of(tensor)
 
-    def pool(self, cache: tuple[Any, Any, Any, Any], written: bool) -> tuple[tuple[int, ...], Any, Any]:
+    def pool(self, cache: tuple[Any, Any, Any, Any], written: bool) -> tuple[tuple[int, ...], tuple[int, ...]]:
         """Checks of a paged cache: codes [pages, page size, kv heads, d], scales [pages, kv heads]; the four addresses and
         the pools' byte strides."""
         torch, feature = self.torch, self.feature
@@ -343,16 +353,15 @@ class _Place:
                 raise TypeError(f"{feature}: `{name}` must be float32, got {scale.dtype}")
             if scale.shape != (shape[0], shape[2]) or not scale.is_contiguous():
                 raise ValueError(f"{feature}: `{name}` must be contiguous [{shape[0]}, {shape[2]}], got {tuple(scale.shape)}")
-        return addresses, self.strides("k_pages", k_pages, written), self.strides("v_pages", v_pages, written)
+        return addresses, self.strides("k_pages", k_pages, written) + self.strides("v_pages", v_pages, written)
 
-    def strides(self, name: str, tensor: Any, written: bool) -> Any:
+    def strides(self, name: str, tensor: Any, written: bool) -> tuple[int, ...]:
         """Element strides of the outer axes of a tensor whose last axis is contiguous; an axis of one element counts as
         packed. A tensor that is written must not overlap itself."""
         shape, strides = tensor.shape, tensor.stride()
         outer = len(shape) - 1
-        of = _Strides2 if outer == 2 else _Strides3
         if tensor.is_contiguous() and 1 not in shape:
-            return of(*strides[:outer])
+            return strides[:outer]
         if shape[outer] > 1 and strides[outer] != 1:
             raise ValueError(f"{self.feature}: the last axis of `{name}` must be contiguous")
         strides = [strides[i] if shape[i] > 1 else shape[outer] for i in range(outer)]
@@ -363,7 +372,7 @@ class _Place:
                     raise ValueError(f"{self.feature}: `{name}` is written and must not overlap itself (shape {tuple(shape)}, "
                                      f"strides {tuple(tensor.stride())})")
                 room = stride * (size - 1) + room
-        return of(*strides)
+        return tuple(strides)
 
     def stream(self, stream: Any) -> Any:
         """As `_stream`, without the objects that torch makes around its current stream."""
@@ -398,7 +407,7 @@ def cache_append(k: Any, v: Any, slot_map: Any, runs: Any, k_pages: Any, v_pages
     """Quantise rows of keys and values [rows, kv heads, d] into the pool (see krn_b200_cache_append)."""
     at = _Place("cache append")
     keys, values = at.address("k", k), at.address("v", v)
-    pool, k_page_strides, v_page_strides = at.pool((k_pages, v_pages, k_scale, v_scale), True)
+    pool, page_strides = at.pool((k_pages, v_pages, k_scale, v_scale), True)
     num_pages, page_size, heads, d = k_pages.shape
     shape = k.shape
     if len(shape) != 3 or v.shape != shape or shape[1] != heads or shape[2] != d:
@@ -408,7 +417,7 @@ def cache_append(k: Any, v: Any, slot_map: Any, runs: Any, k_pages: Any, v_pages
     slots, starts = at.vector("slot_map", slot_map, at.torch.int64), at.vector("runs", runs, at.torch.int32)
     status = native.library().krn_b200_cache_append(
         at.element("k", k), keys, values, slots, starts, *pool, min(shape[0], slot_map.shape[0]), runs.shape[0], heads, d, page_size,
-        num_pages, at.strides("k", k, False), at.strides("v", v, False), k_page_strides, v_page_strides, at.stream(stream))
+        num_pages, _pack_strides(*at.strides("k", k, False), *at.strides("v", v, False), *page_strides), at.stream(stream))
     native.check(status, at.feature)
 
 
@@ -423,7 +432,7 @@ def cache_attention(q: Any, k_pages: Any, v_pages: Any, k_scale: Any, v_scale: A
     """Attention of packed query rows [rows, q heads, d] over the pool (see krn_b200_cache_attn)."""
     at = _Place("cache attention")
     queries, out, scratch = at.address("q", q), at.address("out", o), at.address("workspace", workspace)
-    pool, k_page_strides, v_page_strides = at.pool((k_pages, v_pages, k_scale, v_scale), False)
+    pool, page_strides = at.pool((k_pages, v_pages, k_scale, v_scale), False)
     num_pages, page_size, heads, d = k_pages.shape
     shape = q.shape
     if len(shape) != 3 or shape[2] != d or o.shape != shape:
@@ -437,7 +446,7 @@ def cache_attention(q: Any, k_pages: Any, v_pages: Any, k_scale: Any, v_scale: A
     status = native.library().krn_b200_cache_attn(
         at.element("q", q), queries, k_at, v_at, k_scale_at, v_scale_at, table, context,
         at.vector("row_start", row_start, at.torch.int32, batch + 1), out, batch, shape[0], shape[1], heads, d, page_size, num_pages,
-        entries, pitch, max_new, max_context, at.strides("q", q, False), at.strides("out", o, True), k_page_strides, v_page_strides,
+        entries, pitch, max_new, max_context, _pack_strides(*at.strides("q", q, False), *at.strides("out", o, True), *page_strides),
         scale_log2, scratch, workspace.nbytes, at.stream(stream))
     native.check(status, at.feature)
 

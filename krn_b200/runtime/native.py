@@ -54,9 +54,9 @@ PROTOTYPES: dict[str, tuple[type, list[type]]] = {
                _ptr]),
     "krn_b200_cache_runs": (_i64, [_i64, _i64, _i64]),
     "krn_b200_cache_plan": (_int, [_ptr] * 10 + [_i64] * 8 + [_ptr]),
-    "krn_b200_cache_append": (_int, [_int] + [_ptr] * 8 + [_i64] * 6 + [ctypes.POINTER(_i64)] * 4 + [_ptr]),
+    "krn_b200_cache_append": (_int, [_int] + [_ptr] * 8 + [_i64] * 6 + [_ptr] * 2),
     "krn_b200_cache_attn_workspace_bytes": (_i64, [_i64] * 7),
-    "krn_b200_cache_attn": (_int, [_int] + [_ptr] * 9 + [_i64] * 11 + [ctypes.POINTER(_i64)] * 4 + [_f32, _ptr, _i64, _ptr]),
+    "krn_b200_cache_attn": (_int, [_int] + [_ptr] * 9 + [_i64] * 11 + [_ptr, _f32, _ptr, _i64, _ptr]),
     "krn_b200_scatter_columns": (_int, [_ptr, _ptr, _i64, _i64, _i64, _i64, _int, _ptr]),
 }
 

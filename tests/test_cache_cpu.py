@@ -80,8 +80,7 @@ def test_plan_refusals(change, status, text) -> None:
 
 def append_status(**change) -> int:
     a = dict(type=native.BF16, k=16, v=16, slot=16, runs=16, kp=16, vp=16, ks=16, vs=16, rows=8, runs_len=8, heads=2, d=128, page=64,
-             pages=4, k_strides=_strides(256, 128), v_strides=_strides(256, 128), kps=_strides(16384, 256, 128),
-             vps=_strides(16384, 256, 128), stream=None)
+             pages=4, strides=_strides(256, 128, 256, 128, 16384, 256, 128, 16384, 256, 128), stream=None)
     a.update(change)
     return native.library().krn_b200_cache_append(*a.values())
 
@@ -91,9 +90,9 @@ def append_status(**change) -> int:
     (dict(d=96), native.ERR_UNSUPPORTED, "head dimension 96"),
     (dict(page=20), native.ERR_UNSUPPORTED, "page size 20"),
     (dict(k=24), native.ERR_INVALID_ARGUMENT, "16 bytes"),
-    (dict(v_strides=_strides(256, 132)), native.ERR_INVALID_ARGUMENT, "16 bytes"),
-    (dict(kps=_strides(16384, 264, 128)), native.ERR_INVALID_ARGUMENT, "strides of a page pool"),
-    (dict(vps=_strides(0, 256, 128)), native.ERR_INVALID_ARGUMENT, "strides of a page pool"),
+    (dict(strides=_strides(256, 128, 256, 132, 16384, 256, 128, 16384, 256, 128)), native.ERR_INVALID_ARGUMENT, "16 bytes"),
+    (dict(strides=_strides(256, 128, 256, 128, 16384, 264, 128, 16384, 256, 128)), native.ERR_INVALID_ARGUMENT, "strides of a page pool"),
+    (dict(strides=_strides(256, 128, 256, 128, 16384, 256, 128, 0, 256, 128)), native.ERR_INVALID_ARGUMENT, "strides of a page pool"),
     (dict(ks=None), native.ERR_INVALID_ARGUMENT, "null"),
     (dict(pages=0), native.ERR_INVALID_ARGUMENT, "bad extents"),
     (dict(heads=65536), native.ERR_UNSUPPORTED, "32-bit"),
@@ -105,8 +104,8 @@ def test_append_refusals(change, status, text) -> None:
 
 def attention_status(**change) -> int:
     a = dict(type=native.BF16, q=16, kp=16, vp=16, ks=16, vs=16, table=16, context=16, start=16, o=16, batch=2, rows=2, q_heads=8,
-             kv_heads=2, d=128, page=64, pages=4, width=2, pitch=2, max_new=1, max_context=128, q_strides=_strides(1024, 128),
-             o_strides=_strides(1024, 128), kps=_strides(16384, 256, 128), vps=_strides(16384, 256, 128), scale=1.0, workspace=16,
+             kv_heads=2, d=128, page=64, pages=4, width=2, pitch=2, max_new=1, max_context=128,
+             strides=_strides(1024, 128, 1024, 128, 16384, 256, 128, 16384, 256, 128), scale=1.0, workspace=16,
              size=1 << 40, stream=None)
     a.update(change)
     return native.library().krn_b200_cache_attn(*a.values())
@@ -124,8 +123,8 @@ def attention_status(**change) -> int:
     (dict(batch=8192, width=1 << 24, pitch=1 << 24, max_context=1 << 30), native.ERR_UNSUPPORTED, "32-bit"),
     (dict(o=None), native.ERR_INVALID_ARGUMENT, "null"),
     (dict(q=8), native.ERR_INVALID_ARGUMENT, "16 bytes"),
-    (dict(q_strides=_strides(1028, 128)), native.ERR_INVALID_ARGUMENT, "16 bytes"),
-    (dict(kps=_strides(16384, 256, 100)), native.ERR_INVALID_ARGUMENT, "strides of a page pool"),
+    (dict(strides=_strides(1028, 128, 1024, 128, 16384, 256, 128, 16384, 256, 128)), native.ERR_INVALID_ARGUMENT, "16 bytes"),
+    (dict(strides=_strides(1024, 128, 1024, 128, 16384, 256, 100, 16384, 256, 128)), native.ERR_INVALID_ARGUMENT, "strides of a page pool"),
     (dict(size=8), native.ERR_WORKSPACE, "too small"),
     (dict(workspace=None), native.ERR_WORKSPACE, "too small"),
 ])
@@ -175,7 +174,7 @@ def test_layout_checks(monkeypatch) -> None:
     with pytest.raises(ValueError, match="last axis"):
         at.strides("x", torch.zeros(6, 4, 256)[..., ::2], False)
     codes, scale = torch.zeros(3, 16, 2, 64, dtype=torch.uint8), torch.zeros(3, 2)
-    assert list(at.pool((codes, codes, scale, scale), True)[1]) == [2048, 128, 64]
+    assert list(at.pool((codes, codes, scale, scale), True)[1]) == [2048, 128, 64] * 2
     with pytest.raises(TypeError, match="e4m3"):
         at.pool((codes.to(torch.int8), codes, scale, scale), True)
     with pytest.raises(TypeError, match="float32"):
