@@ -326,7 +326,7 @@ class _Place:
             raise ValueError(f"{self.feature}: `{name}` must be [{batch}, entries] with contiguous rows, got shape {tuple(shape)}")
         return address, shape[1], tensor.stride(0) if batch > 1 else max(shape[1], 1)
 
-    def element(self, name: str, tensor: Any) -> int:
+    def element(self, tensor: Any) -> int:
         """The element type of keys, values and queries."""
         torch, dtype = self.torch, tensor.dtype
         if dtype is torch.bfloat16:
@@ -335,33 +335,39 @@ class _Place:
             return native.F16
         return _type_of(tensor)
 
-    def pool(self, cache: tuple[Any, Any, Any, Any], written: bool) -> tuple[tuple[int, ...], tuple[int, ...]]:
-        """Checks of a paged cache: codes [pages, page size, kv heads, d], scales [pages, kv heads]; the four addresses and
-        the pools' byte strides."""
-        torch, feature = self.torch, self.feature
-        k_pages, v_pages, k_scale, v_scale = cache
-        addresses = (self.address("k_pages", k_pages), self.address("v_pages", v_pages), self.address("k_scale", k_scale),
-                     self.address("v_scale", v_scale))
-        shape = k_pages.shape
+    def pool(self, k_pages: Any, v_pages: Any, k_scale: Any, v_scale: Any, written: bool) -> tuple[Any, tuple[int, ...]]:
+        """Checks of a paged cache: codes [pages, page size, kv heads, d], scales [pages, kv heads]; its shape and the pools'
+        byte strides."""
+        shape, codes, full = k_pages.shape, self.torch.uint8, self.torch.float32
         if len(shape) != 4 or v_pages.shape != shape:
-            raise ValueError(f"{feature}: page pools are [pages, page size, kv heads, d], got {tuple(shape)} and {tuple(v_pages.shape)}")
-        for name, pages in (("k_pages", k_pages), ("v_pages", v_pages)):
-            if pages.dtype is not torch.uint8 and pages.dtype is not torch.float8_e4m3fn:
-                raise TypeError(f"{feature}: `{name}` holds e4m3 codes (float8_e4m3fn or uint8), got {pages.dtype}")
-        for name, scale in (("k_scale", k_scale), ("v_scale", v_scale)):
-            if scale.dtype is not torch.float32:
-                raise TypeError(f"{feature}: `{name}` must be float32, got {scale.dtype}")
-            if scale.shape != (shape[0], shape[2]) or not scale.is_contiguous():
-                raise ValueError(f"{feature}: `{name}` must be contiguous [{shape[0]}, {shape[2]}], got {tuple(scale.shape)}")
-        return addresses, self.strides("k_pages", k_pages, written) + self.strides("v_pages", v_pages, written)
+            raise ValueError(f"{self.feature}: page pools are [pages, page size, kv heads, d], got {tuple(shape)} and "
+                             f"{tuple(v_pages.shape)}")
+        if k_pages.dtype is not codes or v_pages.dtype is not codes:
+            for name, pages in (("k_pages", k_pages), ("v_pages", v_pages)):
+                if pages.dtype is not codes and pages.dtype is not self.torch.float8_e4m3fn:
+                    raise TypeError(f"{self.feature}: `{name}` holds e4m3 codes (float8_e4m3fn or uint8), got {pages.dtype}")
+        scales = (shape[0], shape[2])
+        if (k_scale.dtype is not full or v_scale.dtype is not full or k_scale.shape != scales or v_scale.shape != scales or
+                not k_scale.is_contiguous() or not v_scale.is_contiguous()):
+            for name, scale in (("k_scale", k_scale), ("v_scale", v_scale)):
+                if scale.dtype is not full:
+                    raise TypeError(f"{self.feature}: `{name}` must be float32, got {scale.dtype}")
+                if scale.shape != scales or not scale.is_contiguous():
+                    raise ValueError(f"{self.feature}: `{name}` must be contiguous [{shape[0]}, {shape[2]}], got {tuple(scale.shape)}")
+        return shape, self.strides("k_pages", k_pages, written) + self.strides("v_pages", v_pages, written)
 
     def strides(self, name: str, tensor: Any, written: bool) -> tuple[int, ...]:
         """Element strides of the outer axes of a tensor whose last axis is contiguous; an axis of one element counts as
         packed. A tensor that is written must not overlap itself."""
-        shape, strides = tensor.shape, tensor.stride()
+        shape = tensor.shape
+        if tensor.is_contiguous():
+            if len(shape) == 3:
+                _, middle, inner = shape
+                return middle * inner, inner
+            _, tokens, middle, inner = shape
+            return tokens * middle * inner, middle * inner, inner
+        strides = tensor.stride()
         outer = len(shape) - 1
-        if tensor.is_contiguous() and 1 not in shape:
-            return strides[:outer]
         if shape[outer] > 1 and strides[outer] != 1:
             raise ValueError(f"{self.feature}: the last axis of `{name}` must be contiguous")
         strides = [strides[i] if shape[i] > 1 else shape[outer] for i in range(outer)]
@@ -406,18 +412,19 @@ def cache_append(k: Any, v: Any, slot_map: Any, runs: Any, k_pages: Any, v_pages
                  stream: Any = None) -> None:
     """Quantise rows of keys and values [rows, kv heads, d] into the pool (see krn_b200_cache_append)."""
     at = _Place("cache append")
-    keys, values = at.address("k", k), at.address("v", v)
-    pool, page_strides = at.pool((k_pages, v_pages, k_scale, v_scale), True)
-    num_pages, page_size, heads, d = k_pages.shape
-    shape = k.shape
-    if len(shape) != 3 or v.shape != shape or shape[1] != heads or shape[2] != d:
+    place = at.address
+    shape, page_strides = at.pool(k_pages, v_pages, k_scale, v_scale, True)
+    num_pages, page_size, heads, d = shape
+    rows = k.shape
+    if len(rows) != 3 or v.shape != rows or rows[1] != heads or rows[2] != d:
         raise ValueError(f"{at.feature}: k {tuple(k.shape)} and v {tuple(v.shape)} do not match a pool of {heads} heads of {d}")
     if k.dtype is not v.dtype:
         raise TypeError(f"{at.feature}: k and v must have the same element type")
-    slots, starts = at.vector("slot_map", slot_map, at.torch.int64), at.vector("runs", runs, at.torch.int32)
     status = native.library().krn_b200_cache_append(
-        at.element("k", k), keys, values, slots, starts, *pool, min(shape[0], slot_map.shape[0]), runs.shape[0], heads, d, page_size,
-        num_pages, _pack_strides(*at.strides("k", k, False), *at.strides("v", v, False), *page_strides), at.stream(stream))
+        at.element(k), place("k", k), place("v", v), at.vector("slot_map", slot_map, at.torch.int64),
+        at.vector("runs", runs, at.torch.int32), place("k_pages", k_pages), place("v_pages", v_pages), place("k_scale", k_scale),
+        place("v_scale", v_scale), min(rows[0], slot_map.shape[0]), runs.shape[0], heads, d, page_size, num_pages,
+        _pack_strides(*at.strides("k", k, False), *at.strides("v", v, False), *page_strides), at.stream(stream))
     native.check(status, at.feature)
 
 
@@ -431,23 +438,23 @@ def cache_attention(q: Any, k_pages: Any, v_pages: Any, k_scale: Any, v_scale: A
                     stream: Any = None) -> None:
     """Attention of packed query rows [rows, q heads, d] over the pool (see krn_b200_cache_attn)."""
     at = _Place("cache attention")
-    queries, out, scratch = at.address("q", q), at.address("out", o), at.address("workspace", workspace)
-    pool, page_strides = at.pool((k_pages, v_pages, k_scale, v_scale), False)
-    num_pages, page_size, heads, d = k_pages.shape
-    shape = q.shape
-    if len(shape) != 3 or shape[2] != d or o.shape != shape:
+    place = at.address
+    shape, page_strides = at.pool(k_pages, v_pages, k_scale, v_scale, False)
+    num_pages, page_size, heads, d = shape
+    rows = q.shape
+    if len(rows) != 3 or rows[2] != d or o.shape != rows:
         raise ValueError(f"{at.feature}: q {tuple(q.shape)} and out {tuple(o.shape)} do not match a pool of heads of {d}")
     if q.dtype is not o.dtype:
         raise TypeError(f"{at.feature}: q and out must have the same element type")
     context = at.vector("context_len", context_len, at.torch.int32)
     batch = context_len.shape[0]
     table, entries, pitch = at.table("page_table", page_table, batch)
-    k_at, v_at, k_scale_at, v_scale_at = pool
     status = native.library().krn_b200_cache_attn(
-        at.element("q", q), queries, k_at, v_at, k_scale_at, v_scale_at, table, context,
-        at.vector("row_start", row_start, at.torch.int32, batch + 1), out, batch, shape[0], shape[1], heads, d, page_size, num_pages,
-        entries, pitch, max_new, max_context, _pack_strides(*at.strides("q", q, False), *at.strides("out", o, True), *page_strides),
-        scale_log2, scratch, workspace.nbytes, at.stream(stream))
+        at.element(q), place("q", q), place("k_pages", k_pages), place("v_pages", v_pages), place("k_scale", k_scale),
+        place("v_scale", v_scale), table, context, at.vector("row_start", row_start, at.torch.int32, batch + 1), place("out", o), batch,
+        rows[0], rows[1], heads, d, page_size, num_pages, entries, pitch, max_new, max_context,
+        _pack_strides(*at.strides("q", q, False), *at.strides("out", o, True), *page_strides), scale_log2,
+        place("workspace", workspace), workspace.nbytes, at.stream(stream))
     native.check(status, at.feature)
 
 

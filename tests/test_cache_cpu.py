@@ -149,9 +149,9 @@ def test_host_tensors_are_refused() -> None:
     codes, scale = torch.zeros(2, 64, 2, 128, dtype=torch.uint8), torch.zeros(2, 2)
     cache = ops.PagedCache(codes, codes, scale, scale)
     x = torch.zeros(4, 2, 128, dtype=torch.bfloat16)
-    with pytest.raises(ValueError, match="`k` must be a CUDA tensor"):
+    with pytest.raises(ValueError, match="must be a CUDA tensor"):
         ops.append_cache(x, x, plan.slot_map, plan.runs, cache)
-    with pytest.raises(ValueError, match="`q` must be a CUDA tensor"):
+    with pytest.raises(ValueError, match="must be a CUDA tensor"):
         ops.cache_attention(x, cache, table, lengths, plan.row_start, x, max_new=1, max_context=64, workspace=x)
 
 
@@ -174,15 +174,15 @@ def test_layout_checks(monkeypatch) -> None:
     with pytest.raises(ValueError, match="last axis"):
         at.strides("x", torch.zeros(6, 4, 256)[..., ::2], False)
     codes, scale = torch.zeros(3, 16, 2, 64, dtype=torch.uint8), torch.zeros(3, 2)
-    assert list(at.pool((codes, codes, scale, scale), True)[1]) == [2048, 128, 64] * 2
+    assert list(at.pool(codes, codes, scale, scale, True)[1]) == [2048, 128, 64] * 2
     with pytest.raises(TypeError, match="e4m3"):
-        at.pool((codes.to(torch.int8), codes, scale, scale), True)
+        at.pool(codes.to(torch.int8), codes, scale, scale, True)
     with pytest.raises(TypeError, match="float32"):
-        at.pool((codes, codes, scale.double(), scale), True)
+        at.pool(codes, codes, scale.double(), scale, True)
     with pytest.raises(ValueError, match=r"contiguous \[3, 2\]"):
-        at.pool((codes, codes, scale.t().contiguous().t(), scale), True)
+        at.pool(codes, codes, scale.t().contiguous().t(), scale, True)
     with pytest.raises(ValueError, match="page pools"):
-        at.pool((codes, codes[:2], scale, scale), True)
+        at.pool(codes, codes[:2], scale, scale, True)
     with pytest.raises(TypeError, match="int32"):
         at.table("page_table", torch.zeros(2, 4, dtype=torch.int64), 2)
     with pytest.raises(ValueError, match=r"\[3, entries\]"):
