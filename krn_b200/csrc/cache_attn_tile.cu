@@ -3,10 +3,11 @@
 // A block owns two tiles of 128 query rows of one (request, kv head): 128 / group consecutive tokens of each q head that
 // shares the kv head, so K and V are fetched once for the whole group. It runs over the keys in tiles of 128:
 //
-//   warp 0        TMA producer: K codes into a ring of kKStages tiles, V codes into a ring of two;
-//   warp 1        MMA issuer: S_t = Q_t K^T (kind::f8f6f4) on the cache's bytes as they are, O_t += P_t V (kind::f16);
-//   warps 2, 3    turn a V tile into f16, times its pages' scales: 16-bit P needs a 16-bit V;
-//   warps 4..11   softmax of the two query tiles, a thread per row; then the output.
+//   warp 0        issues S = Q_t K^T (kind::f8f6f4) on the cache's bytes as they are;
+//   warp 1        issues O_t += P_t V (kind::f16);
+//   warp 2        issues the copies (TMA): K codes into a ring of kKStages tiles, V codes into a ring of two;
+//   warps 4..7    turn a V tile into f16, times its pages' scales: a 16-bit P needs a 16-bit V;
+//   warps 8..15   softmax of the two query tiles, a thread per row; then the output.
 //
 // Q is split into e4m3 parts, each the rounded remainder of the ones before (a power-of-two factor puts the row's largest
 // magnitude into [128, 256)): two parts hold bf16's 8 significant bits exactly, three hold f16's 11, but for elements below
@@ -17,7 +18,11 @@
 // largest one that this block meets and times 2^7 (448 * 2^7 is within f16): for scales that are powers of two V stays
 // exact down to 2^-22 of the largest; any other scale costs two roundings of 2^-12.
 //
-// Tensor memory (512 columns): S0 | S1 | O0 | O1, 128 columns each; P_t (f16) lies over the first 64 columns of S_t.
+// Tensor memory (512 columns): S (128) | P0 (64) | P1 (64) | O0 (128) | O1 (128). The two query tiles take turns in one S:
+// a softmax warp reads its scores into registers at once, so S is free for the other tile's scores long before the
+// exponentials are done, and each tile finds its next scores ready when it has handed over its weights. Two warps issue,
+// because one sets the pace: it spends over a hundred cycles on each wait and about 80 on each product, 2030 cycles a query
+// and key tile in a trace, of which the tensor cores work 1024.
 #include "cache_attn.cuh"
 
 #include <cmath>
@@ -27,7 +32,8 @@ namespace {
 
 constexpr int kTileQ = 128;
 constexpr int kTileKV = 128;
-constexpr int kThreads = 384;
+constexpr int kThreads = 512;
+constexpr int kRegsFew = 56, kRegsMany = 200;  // warps 0..7 / 8..15, of the 128 that each thread is launched with
 constexpr int kSMs = 148;                 // blocks that run at once: fewer are split over the keys
 constexpr float kRescaleThreshold = 8.0f;
 constexpr float kNone = -3.0e38f;         // reference maximum of a row that has seen no key
@@ -97,8 +103,8 @@ __device__ __forceinline__ int blocks_of(const TileParams& p, int b) {
   return (n + 2 * p.tokens - 1) / (2 * p.tokens);
 }
 
-// Page ids of the 16-token groups of key tiles, one group per lane of 8, two tiles ahead, and the groups' scales one ahead:
-// a loader that hides both loads behind the tile in work. Groups without a page in the pool have the scale `none`.
+// The scales of the 16-token groups of key tiles, one group per lane of 8. Page ids are fetched two tiles ahead and scales
+// one, by a call placed where a tile's long work follows. Groups without a page in the pool have the scale `none`.
 struct ScaleAhead {
   const int32_t* table;
   const float* scale;
@@ -117,20 +123,18 @@ struct ScaleAhead {
     next = scale_at(id_at(tile));
     id = id_at(tile + 1);
   }
-  // The scale of group lane & 7 of `tile`; afterwards those of tile + 1 are under way.
-  __device__ __forceinline__ float take(int tile) {
-    const float now = next;
+  // `next` is the scale of `tile` before the call and that of tile + 1, on its way, after it.
+  __device__ __forceinline__ void fetch(int tile) {
     next = scale_at(id);
     id = id_at(tile + 2);
-    return now;
   }
 };
 
-template <int D, bool BF16>
+template <int D, bool BF16, int Groups>
 __global__ void __launch_bounds__(kThreads, 1)
 cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, TileParams p,
                   DeviceStatus* status) {
-  constexpr int Parts = BF16 ? 2 : 3;
+  constexpr int Parts = BF16 ? 2 : 3, kGroup = kTileKV / Groups;  // keys of a scale
   using L = Layout<D, Parts>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
@@ -143,11 +147,12 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   const uint32_t bars = smem_u32(tail);
   const uint32_t q_full = bars, k_full = bars + 8, k_empty = bars + 32, raw_full = bars + 56, raw_empty = bars + 72;
   const uint32_t v_full = bars + 88, v_empty = bars + 104, s_full = bars + 120, p_full = bars + 136, o_full = bars + 152;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail + 168);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + 172);
-  int32_t* found = reinterpret_cast<int32_t*>(tail + 176);  // request, block of it, blocks of it
-  int32_t* sums = reinterpret_cast<int32_t*>(tail + 192);   // [12]
-  float* tops = reinterpret_cast<float*>(tail + 256);       // [12]
+  const uint32_t s_read = bars + 168;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail + 176);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + 180);
+  int32_t* found = reinterpret_cast<int32_t*>(tail + 184);  // request, block of it, blocks of it
+  int32_t* sums = reinterpret_cast<int32_t*>(tail + 200);   // [kThreads / 32]
+  float* tops = reinterpret_cast<float*>(tail + 272);       // [kThreads / 32]
 
   const int warp = threadIdx.x >> 5;
   const int lane = int(lane_id());
@@ -232,14 +237,15 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   }
   if (threadIdx.x == 0) {
     mbar_init(q_full, 8);
+    mbar_init(s_read, 4);
     for (int i = 0; i < 3; ++i) {
       mbar_init(k_full + 8 * i, 1);
       mbar_init(k_empty + 8 * i, 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(raw_full + 8 * i, 1);
-      mbar_init(raw_empty + 8 * i, 2);
-      mbar_init(v_full + 8 * i, 2);
+      mbar_init(raw_empty + 8 * i, 4);
+      mbar_init(v_full + 8 * i, 4);
       mbar_init(v_empty + 8 * i, 1);
       mbar_init(s_full + 8 * i, 1);
       mbar_init(p_full + 8 * i, 4);
@@ -261,9 +267,88 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
 #pragma unroll
   for (int w = 0; w < kThreads / 32; ++w) top = fmaxf(top, tops[w]);
 
-  if (warp < 4) reg_dealloc<56>();
-  if (warp == 0) {
-    // ---------------------------------------------------------------- TMA producer
+  if (warp < 8) reg_dealloc<kRegsFew>();
+  if (warp < 2) {
+    // ---------------------------------------------------------------- MMA issuers: warp 0 the scores, warp 1 P V
+    const bool leader = elect_one();
+    const int nt[2] = {n0, n1};
+    auto wait = [&](uint32_t bar, uint32_t parity, int site) {
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, site)) != 0;
+    };
+    bool ok = true;
+    if (warp == 0) {
+      const uint32_t idesc = umma_idesc(kFmtE4M3, kFmtE4M3, kTileQ, kTileKV, 0, 0);
+      const uint64_t q_desc = umma_desc_kmajor_sw128(0);
+      const uint64_t k_desc = D == 128 ? umma_desc_kmajor_sw128(0) : desc_kmajor_sw64(0);
+      const uint32_t q_hi = uint32_t(q_desc >> 32), k_hi = uint32_t(k_desc >> 32);
+      const uint32_t q_lo = uint32_t(q_desc) + (q_addr >> 4), k_lo = uint32_t(k_desc) + (k_addr >> 4);
+      int stage = 0;
+      uint32_t phase = 0, reads = 0;  // reads: score tiles issued so far, each of which a softmax reads once
+      if (count > 0) ok = wait(q_full, 0, kSiteQuery);
+      for (int j = 0; j < count && ok; ++j) {
+        ok = wait(k_full + 8 * stage, phase, kSiteKeys);
+        for (int t = 0; t < 2 && ok; ++t) {
+          if (j >= nt[t]) continue;
+          if (reads > 0 && !wait(s_read, (reads - 1) & 1, kSiteRead)) {
+            ok = false;
+            break;
+          }
+          ++reads;
+          tc_fence_after();
+          // S = sum over Q's parts: D / 32 instructions of K = 32 columns each
+          const uint32_t qa = q_lo + t * (L::kQBytes >> 4), ka = k_lo + stage * (L::kRawBytes >> 4);
+          if (leader) {
+#pragma unroll
+            for (int part = 0; part < Parts; ++part) {
+#pragma unroll
+              for (int ks = 0; ks < D / 32; ++ks) {
+                const uint32_t off = ((part / L::kPerRow) * L::kBlockBytes + (part % L::kPerRow) * D + ks * 32) >> 4;
+                umma_ss_halves<1, true>(tmem_base, qa + off, q_hi, ka + ks * 2, k_hi, idesc, part + ks > 0 ? 1u : 0u);
+              }
+            }
+            umma_commit(s_full + 8 * t);
+          }
+          __syncwarp();
+        }
+        if (ok && leader) umma_commit(k_empty + 8 * stage);
+        __syncwarp();
+        if (++stage == L::kKStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    } else {
+      const uint32_t idesc = umma_idesc(kFmtF16, kFmtF16, kTileQ, D, 0, 1);
+      const uint64_t v_desc = umma_desc_mnmajor_sw128(0, L::kBlockBytes, 1024);
+      const uint32_t v_hi = uint32_t(v_desc >> 32), v_lo = uint32_t(v_desc) + (half_addr >> 4);
+      for (int j = 0; j < count && ok; ++j) {
+        const int stage = j & 1;
+        ok = wait(v_full + 8 * stage, (j >> 1) & 1, kSiteValues);
+        for (int t = 0; t < 2 && ok; ++t) {
+          if (j >= nt[t]) continue;
+          if (!wait(p_full + 8 * t, j & 1, kSiteWeights)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          // O_t += P_t V: 8 instructions of K = 16 keys; P_t from tensor memory, V with d contiguous in 64-column blocks
+          const uint32_t va = v_lo + stage * (L::kHalfBytes >> 4);
+          if (leader) {
+#pragma unroll
+            for (int ks = 0; ks < kTileKV / 16; ++ks) {
+              umma_ts_f16_halves(tmem_base + 256 + t * 128, tmem_base + 128 + t * 64 + ks * 8, va + ks * (2048 >> 4), v_hi, idesc,
+                                 (j > 0 || ks > 0) ? 1u : 0u);
+            }
+            umma_commit(o_full + 8 * t);
+          }
+          __syncwarp();
+        }
+        if (ok && leader) umma_commit(v_empty + 8 * stage);
+        __syncwarp();
+      }
+    }
+  } else if (warp == 2) {
+    // ---------------------------------------------------------------- copies, a lane each
     const int box = min(kTileKV, 1 << a.page_shift), copies = kTileKV / box;
     int ids = 0, ids_first = -64;
     for (int j = 0; j < count; ++j) {
@@ -295,137 +380,40 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
                     raw_full + 8 * v_stage);
       }
     }
-  } else if (warp == 1) {
-    // ---------------------------------------------------------------- MMA issuer
-    if (count > 0) {
-      const bool leader = elect_one();
-      const uint32_t idesc_s = umma_idesc(kFmtE4M3, kFmtE4M3, kTileQ, kTileKV, 0, 0);
-      const uint32_t idesc_pv = umma_idesc(kFmtF16, kFmtF16, kTileQ, D, 0, 1);
-      const int nt[2] = {n0, n1};
-      const uint64_t q_desc = umma_desc_kmajor_sw128(0);
-      const uint64_t k_desc = D == 128 ? umma_desc_kmajor_sw128(0) : desc_kmajor_sw64(0);
-      const uint64_t v_desc = umma_desc_mnmajor_sw128(0, L::kBlockBytes, 1024);
-      const uint32_t q_hi = uint32_t(q_desc >> 32), k_hi = uint32_t(k_desc >> 32), v_hi = uint32_t(v_desc >> 32);
-      const uint32_t q_lo = uint32_t(q_desc) + (q_addr >> 4), k_lo = uint32_t(k_desc) + (k_addr >> 4);
-      const uint32_t v_lo = uint32_t(v_desc) + (half_addr >> 4);
-
-      // S_t = sum over Q's parts: D / 32 instructions of K = 32 columns each
-      auto issue_s = [&](int t, int stage) {
-        const uint32_t qa = q_lo + t * (L::kQBytes >> 4);
-        const uint32_t ka = k_lo + stage * (L::kRawBytes >> 4);
-        if (leader) {
-#pragma unroll
-          for (int part = 0; part < Parts; ++part) {
-#pragma unroll
-            for (int ks = 0; ks < D / 32; ++ks) {
-              const uint32_t off = ((part / L::kPerRow) * L::kBlockBytes + (part % L::kPerRow) * D + ks * 32) >> 4;
-              umma_ss_halves<1, true>(tmem_base + t * 128, qa + off, q_hi, ka + ks * 2, k_hi, idesc_s, part + ks > 0 ? 1u : 0u);
-            }
-          }
-          umma_commit(s_full + 8 * t);
-        }
-        __syncwarp();
-      };
-      // O_t += P_t V: 8 instructions of K = 16 keys; P_t from tensor memory, V with d contiguous in 64-column blocks
-      auto issue_pv = [&](int t, int stage, bool accumulate) {
-        const uint32_t va = v_lo + stage * (L::kHalfBytes >> 4);
-        if (leader) {
-#pragma unroll
-          for (int ks = 0; ks < kTileKV / 16; ++ks) {
-            umma_ts_f16_halves(tmem_base + 256 + t * 128, tmem_base + t * 128 + ks * 8, va + ks * (2048 >> 4), v_hi, idesc_pv,
-                               (accumulate || ks > 0) ? 1u : 0u);
-          }
-        }
-        __syncwarp();
-      };
-      auto wait = [&](uint32_t bar, uint32_t parity, int site) {
-        return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, site)) != 0;
-      };
-      bool ok = wait(q_full, 0, kSiteQuery) && wait(k_full, 0, kSiteScores);
-      if (ok) {
-        tc_fence_after();
-        for (int t = 0; t < 2; ++t)
-          if (nt[t] > 0) issue_s(t, 0);
-        if (leader) umma_commit(k_empty);
-      }
-      int k_stage = 0;          // stage and phase of the K tile behind the one in work
-      uint32_t k_phase = 0;
-      for (int j = 0; j < count && ok; ++j) {
-        const int stage = j & 1;
-        if (++k_stage == L::kKStages) {
-          k_stage = 0;
-          k_phase ^= 1u;
-        }
-        if (!wait(v_full + 8 * stage, (j >> 1) & 1, kSiteScores)) break;
-        bool next_k_ready = false;
-        for (int t = 0; t < 2 && ok; ++t) {
-          if (j >= nt[t]) continue;
-          if (!wait(p_full + 8 * t, j & 1, kSiteWeights)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          issue_pv(t, stage, j > 0);
-          if (j + 1 < nt[t]) {
-            if (!next_k_ready) {
-              if (!wait(k_full + 8 * k_stage, k_phase, kSiteScores)) {
-                ok = false;
-                break;
-              }
-              tc_fence_after();
-              next_k_ready = true;
-            }
-            issue_s(t, k_stage);
-          } else {
-            if (leader) umma_commit(o_full + 8 * t);
-          }
-        }
-        if (!ok) break;
-        if (leader) {
-          umma_commit(v_empty + 8 * stage);
-          if (j + 1 < count) umma_commit(k_empty + 8 * k_stage);
-        }
-        __syncwarp();
-      }
-    }
-  } else if (warp < 4) {
+  } else if (warp >= 4 && warp < 8) {
     // ---------------------------------------------------------------- V to f16
     constexpr int kLanes = D / 16;               // threads per row, 16 codes each
-    constexpr int kRows = 64 / kLanes;           // rows per pass of the two warps
-    const int tid = int(threadIdx.x) - 64;
-    const int row0_of = tid / kLanes, c = tid % kLanes;
+    constexpr int kRows = 128 / kLanes;          // rows per pass of the four warps
+    const int tid = int(threadIdx.x) - 128;
+    const int row_of = tid / kLanes, c = tid % kLanes;
     ScaleAhead scales = {table, a.v.scale, a.page_shift, pages, a.num_pages, a.kv_heads, g, lane, 0.f, 0, 0.f};
     if (count > 0) scales.start(j0);
     const float unit = 128.0f / top;
-    // the two 16-byte halves of a thread's 16 columns, in an order that spreads a row over all banks
-    const int turn = (c >> 2) & 1;
+    // a thread's two stores, in an order that spreads a row over all banks
+    const uint32_t turn = uint32_t(c >> 2) & 1u, even = uint32_t(2 * c) & 7u;
     for (int j = 0; j < count; ++j) {
       const int stage = j & 1;
-      const float factor = scales.take(j0 + j) * unit;
+      const float factor = scales.next * unit;
+      scales.fetch(j0 + j);
       const uint32_t mine = pack_f16x2(factor, factor);
-      bool ok = mbar_wait(raw_full + 8 * stage, (j >> 1) & 1, abort_flag, status, kSiteValues) &&
-                mbar_wait(v_empty + 8 * stage, ((j >> 1) & 1) ^ 1u, abort_flag, status, kSiteRoom);
+      const bool ok = mbar_wait(raw_full + 8 * stage, (j >> 1) & 1, abort_flag, status, kSiteValues) &&
+                      mbar_wait(v_empty + 8 * stage, ((j >> 1) & 1) ^ 1u, abort_flag, status, kSiteRoom);
       if (!__all_sync(0xffffffffu, ok)) break;
       const int valid = context - (j0 + j) * kTileKV;  // rows behind the context may hold any bits
-      const uint32_t from = raw_addr + stage * L::kRawBytes, to = half_addr + stage * L::kHalfBytes;
+      const uint32_t from = raw_addr + stage * L::kRawBytes + c * 16;
+      const uint32_t to = half_addr + stage * L::kHalfBytes + (c >> 2) * L::kBlockBytes;
 #pragma unroll 4
       for (int i = 0; i < kTileKV / kRows; ++i) {
-        const int row = i * kRows + row0_of;
-        uint4 w = ld_shared_16(from + row * D + c * 16);
+        const int row = i * kRows + row_of;
+        uint4 w = ld_shared_16(from + row * D);
         if (row >= valid) w = make_uint4(0, 0, 0, 0);
-        const uint32_t by = __shfl_sync(0xffffffffu, mine, (i * kRows) >> 4);
-        const uint32_t x[8] = {times(halves_of(w.x), by), times(halves_of(w.x >> 16), by), times(halves_of(w.y), by),
-                               times(halves_of(w.y >> 16), by), times(halves_of(w.z), by), times(halves_of(w.z >> 16), by),
-                               times(halves_of(w.w), by), times(halves_of(w.w >> 16), by)};
-        const uint32_t at = to + (c >> 2) * L::kBlockBytes + row * 128;
-        const uint32_t even = uint32_t((2 * c) & 7), x7 = uint32_t(row & 7);
-        if (turn == 0) {
-          st_shared_16(at + ((even ^ x7) << 4), x[0], x[1], x[2], x[3]);
-          st_shared_16(at + (((even + 1) ^ x7) << 4), x[4], x[5], x[6], x[7]);
-        } else {
-          st_shared_16(at + (((even + 1) ^ x7) << 4), x[4], x[5], x[6], x[7]);
-          st_shared_16(at + ((even ^ x7) << 4), x[0], x[1], x[2], x[3]);
-        }
+        const uint32_t by = __shfl_sync(0xffffffffu, mine, row >> 4);
+        if (turn) w = make_uint4(w.z, w.w, w.x, w.y);
+        const uint32_t at = to + row * 128, x7 = uint32_t(row & 7);
+        st_shared_16(at + (((even + turn) ^ x7) << 4), times(halves_of(w.x), by), times(halves_of(w.x >> 16), by),
+                     times(halves_of(w.y), by), times(halves_of(w.y >> 16), by));
+        st_shared_16(at + (((even + 1 - turn) ^ x7) << 4), times(halves_of(w.z), by), times(halves_of(w.z >> 16), by),
+                     times(halves_of(w.w), by), times(halves_of(w.w >> 16), by));
       }
       fence_async_smem();
       __syncwarp();
@@ -434,10 +422,10 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         mbar_arrive(raw_empty + 8 * stage);
       }
     }
-  } else {
+  } else if (warp >= 8) {
     // ---------------------------------------------------------------- Q, softmax, output
-    reg_alloc<224>();
-    const int t = (warp - 4) >> 2;
+    reg_alloc<kRegsMany>();
+    const int t = (warp - 8) >> 2;
     const int quarter = warp & 3;
     const int nt = t == 0 ? n0 : n1;
     const int row_in_tile = quarter * 32 + lane;
@@ -445,7 +433,7 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     const bool live = row_in_tile < p.tokens * a.group && token < n && row0 + token < a.rows;
     const int head = g * a.group + row_in_tile % a.group;
     const uint32_t lane_base = tmem_base + (uint32_t(quarter * 32) << 16);
-    const uint32_t s_tmem = lane_base + t * 128;
+    const uint32_t s_tmem = lane_base, p_tmem = lane_base + 128 + t * 64;
     const uint32_t o_tmem = lane_base + 256 + t * 128;
     float row_scale;
 
@@ -510,11 +498,10 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     bool ok = true;
 
     for (int j = 0; j < nt; ++j) {
-      const float scale_lane = scales.take(j0 + j);
-      float scale[8];
+      float scale[Groups];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float x = __shfl_sync(0xffffffffu, scale_lane, i) * row_scale;
+      for (int i = 0; i < Groups; ++i) {
+        const float x = __shfl_sync(0xffffffffu, scales.next, i * (8 / Groups)) * row_scale;
         scale[i] = x < 0x1p-126f ? 0x1p-126f : x;  // never 0: a masked score is -inf times this
       }
       if (!__all_sync(0xffffffffu, mbar_wait(s_full + 8 * t, j & 1, abort_flag, status, kSiteScores))) {
@@ -529,6 +516,10 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       tie(s[1]);
       tie(s[2]);
       tie(s[3]);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(s_read);
+      scales.fetch(j0 + j);
 
       const int visible = sees - (j0 + j) * kTileKV;
       if (visible < kTileKV) {
@@ -539,21 +530,30 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           if (64 + i >= visible) s[2][i] = 0xff800000u;
           if (96 + i >= visible) s[3][i] = 0xff800000u;
         }
+#pragma unroll
+        for (int c = 0; c < Groups; ++c) {
+          if (c * kGroup >= visible) scale[c] = 1.f;  // whatever the page holds, nothing of it is seen
+        }
       }
       float m_new = m_ref;
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        float mx = __uint_as_float(s[c >> 1][(c & 1) * 16]);
+      for (int c = 0; c < Groups; ++c) {
+        float mx = __uint_as_float(s[c * kGroup / 32][c * kGroup % 32]);
 #pragma unroll
-        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, __uint_as_float(s[c >> 1][(c & 1) * 16 + i]));
-        if (c * 16 < visible) m_new = fmaxf(m_new, mx * scale[c]);  // a group out of sight has no scale
+        for (int i = 1; i < kGroup; ++i) mx = fmaxf(mx, __uint_as_float(s[(c * kGroup + i) / 32][(c * kGroup + i) % 32]));
+        m_new = fmaxf(m_new, mx * scale[c]);
       }
       if (j == 0) {
         m_ref = m_new;
       } else {
         const bool moved = m_new - m_ref > kRescaleThreshold;
         if (__any_sync(0xffffffffu, moved)) {
-          // S_t(j) was issued after P_t(j-1) V(j-1), so O_t is complete and idle until p_full is signalled
+          // O_t is idle from the end of P_t(j - 1) V(j - 1) until p_full is signalled
+          if (!__all_sync(0xffffffffu, mbar_wait(o_full + 8 * t, (j - 1) & 1, abort_flag, status, kSiteOutput))) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
           const float corr = moved ? ex2_approx(m_ref - m_new) : 1.0f;
           l *= corr;
           if (moved) m_ref = m_new;
@@ -578,7 +578,7 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       for (int i = 0; i < 16; ++i) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          const float by = scale[2 * c + (i >> 3)];
+          const float by = scale[(c * 32 + 2 * i) / kGroup];
           const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[c][2 * i]), __uint_as_float(s[c][2 * i + 1])),
                                       make_float2(by, by), shift2);
           const float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
@@ -588,8 +588,14 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       }
       const float2 all = __fadd2_rn(__fadd2_rn(sum[0], sum[1]), __fadd2_rn(sum[2], sum[3]));
       l += all.x + all.y;
-      tmem_st_32x32(s_tmem, packed[0]);       // keys 0..63  -> columns 0..31
-      tmem_st_32x32(s_tmem + 32, packed[1]);  // keys 64..127 -> columns 32..63
+      // P_t is free when P_t(j - 1) V(j - 1) has read it
+      if (j > 0 && !__all_sync(0xffffffffu, mbar_wait(o_full + 8 * t, (j - 1) & 1, abort_flag, status, kSiteOutput))) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      tmem_st_32x32(p_tmem, packed[0]);       // keys 0..63  -> columns 0..31
+      tmem_st_32x32(p_tmem + 32, packed[1]);  // keys 64..127 -> columns 32..63
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
@@ -597,7 +603,7 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     }
 
     // ---- O_t over l, or a split's share of it
-    if (nt > 0 && ok) ok = __all_sync(0xffffffffu, mbar_wait(o_full + 8 * t, 0, abort_flag, status, kSiteOutput));
+    if (nt > 0 && ok) ok = __all_sync(0xffffffffu, mbar_wait(o_full + 8 * t, (nt - 1) & 1, abort_flag, status, kSiteOutput));
     if (ok) {
       tc_fence_after();
       const bool split = p.splits > 1;
@@ -700,7 +706,7 @@ int64_t splits_of(int64_t blocks, int64_t max_context) {
   return splits < 1 ? 1 : splits;
 }
 
-template <int D, bool BF16>
+template <int D, bool BF16, int Groups>
 int launch(const DeviceContext* ctx, const TileParams& p, int64_t page_size, int64_t blocks, cudaStream_t stream) {
   const CacheAttnParams& a = p.a;
   using L = Layout<D, BF16 ? 2 : 3>;
@@ -709,16 +715,16 @@ int launch(const DeviceContext* ctx, const TileParams& p, int64_t page_size, int
   const Swizzle swizzle = D == 128 ? Swizzle::k128B : Swizzle::k64B;
   if (int rc = encode_pool(&map_k, a.k, D, a.kv_heads, page_size, a.num_pages, box, swizzle)) return rc;
   if (int rc = encode_pool(&map_v, a.v, D, a.kv_heads, page_size, a.num_pages, box, Swizzle::kNone)) return rc;
-  auto kernel = cache_tile_kernel<D, BF16>;
+  auto kernel = cache_tile_kernel<D, BF16, Groups>;
   static OncePerDevice ready;
   if (int rc = ready(ctx->device, [&] {
         KRNB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmemBytes));
-        // setmaxnreg.inc blocks until the CTA's register pool can cover it: 128 x (R - 56) must reach 256 x (224 - R)
+        // setmaxnreg.inc blocks until the registers that the other warps let go cover it
         cudaFuncAttributes attributes;
         KRNB_CUDA(cudaFuncGetAttributes(&attributes, kernel));
-        if ((attributes.numRegs - 56) * 128 < (224 - attributes.numRegs) * 256) {
+        if (2 * attributes.numRegs < kRegsFew + kRegsMany || attributes.numRegs < kRegsFew) {
           return fail(KRN_B200_ERR_UNSUPPORTED, "cache attention kernel was built with %d registers per thread; the register "
-                      "re-partitioning needs at least 168", attributes.numRegs);
+                      "re-partitioning needs %d", attributes.numRegs, (kRegsFew + kRegsMany) / 2);
         }
         return KRN_B200_OK;
       })) {
@@ -726,6 +732,12 @@ int launch(const DeviceContext* ctx, const TileParams& p, int64_t page_size, int
   }
   return launch_dependent(kernel, dim3(unsigned(blocks * a.kv_heads), unsigned(p.splits)), kThreads, L::kSmemBytes, stream, map_k, map_v,
                           p, ctx->status_dev);
+}
+
+// A key tile has two scales at most where pages are 64 tokens or more, up to eight where they are smaller.
+template <int D, bool BF16>
+int launch_pages(const DeviceContext* ctx, const TileParams& p, int64_t page_size, int64_t blocks, cudaStream_t stream) {
+  return page_size >= 64 ? launch<D, BF16, 2>(ctx, p, page_size, blocks, stream) : launch<D, BF16, 8>(ctx, p, page_size, blocks, stream);
 }
 
 TileParams tile_params(const CacheAttnParams& a, float* partial, int64_t blocks) {
@@ -750,8 +762,8 @@ int launch_tiles(const DeviceContext* ctx, const CacheAttnParams& a, bool bf16, 
                  cudaStream_t stream) {
   const int64_t blocks = tile_blocks(a.batch, a.rows, a.group, a.few);
   const TileParams p = tile_params(a, partial, blocks);
-  if (d == 128) return bf16 ? launch<128, true>(ctx, p, page_size, blocks, stream) : launch<128, false>(ctx, p, page_size, blocks, stream);
-  return bf16 ? launch<64, true>(ctx, p, page_size, blocks, stream) : launch<64, false>(ctx, p, page_size, blocks, stream);
+  if (d == 128) return bf16 ? launch_pages<128, true>(ctx, p, page_size, blocks, stream) : launch_pages<128, false>(ctx, p, page_size, blocks, stream);
+  return bf16 ? launch_pages<64, true>(ctx, p, page_size, blocks, stream) : launch_pages<64, false>(ctx, p, page_size, blocks, stream);
 }
 
 int launch_tile_join(const CacheAttnParams& a, bool bf16, int64_t d, float* partial, cudaStream_t stream) {
