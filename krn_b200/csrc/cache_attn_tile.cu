@@ -33,7 +33,7 @@ namespace {
 constexpr int kTileQ = 128;
 constexpr int kTileKV = 128;
 constexpr int kThreads = 512;
-constexpr int kRegsFew = 56, kRegsMany = 200;  // warps 0..7 / 8..15, of the 128 that each thread is launched with
+constexpr int kRegsFew = 40, kRegsMany = 216;  // warps 0..7 / 8..15, of the 128 that each thread is launched with
 constexpr int kSMs = 148;                 // blocks that run at once: fewer are split over the keys
 constexpr float kRescaleThreshold = 8.0f;
 constexpr float kNone = -3.0e38f;         // reference maximum of a row that has seen no key
@@ -538,10 +538,21 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       float m_new = m_ref;
 #pragma unroll
       for (int c = 0; c < Groups; ++c) {
-        float mx = __uint_as_float(s[c * kGroup / 32][c * kGroup % 32]);
+        // sixteen short chains over the tile: one long one waits for itself
+        constexpr int kChains = 16 / Groups, kLength = kGroup / kChains;
+        float mx[kChains];
 #pragma unroll
-        for (int i = 1; i < kGroup; ++i) mx = fmaxf(mx, __uint_as_float(s[(c * kGroup + i) / 32][(c * kGroup + i) % 32]));
-        m_new = fmaxf(m_new, mx * scale[c]);
+        for (int i = 0; i < kLength; i += 2) {
+#pragma unroll
+          for (int x = 0; x < kChains; ++x) {
+            const int at = c * kGroup + x * kLength + i;
+            const float pair = fmaxf(__uint_as_float(s[at / 32][at % 32]), __uint_as_float(s[at / 32][at % 32 + 1]));
+            mx[x] = i == 0 ? pair : fmaxf(mx[x], pair);
+          }
+        }
+#pragma unroll
+        for (int x = 1; x < kChains; ++x) mx[0] = fmaxf(mx[0], mx[x]);
+        m_new = fmaxf(m_new, mx[0] * scale[c]);
       }
       if (j == 0) {
         m_ref = m_new;
