@@ -17,7 +17,8 @@ constexpr int kWarps = 8;
 constexpr int kStages = 3;         // tiles a warp has in flight or in work
 constexpr int kMaxBlocks = 160;    // bounds the workspace; a B200 has 148 SMs
 constexpr int kMaxBatch = 8192;    // tile counts of the batch sit in shared memory
-constexpr float kLeastScale = 7.70371977754894341e-34f;  // 2^-110: value scales below it are held against it
+constexpr float kLeastScale = 0x1p-110f;  // value scales below it are held against it
+constexpr float kNone = -3.0e38f;         // reference maximum of a row that has seen no key
 
 // Partial results of the pieces of split segments, 2 + d floats (m, l, the unnormalised output) for each of `rows`.
 struct StreamParams {
@@ -255,7 +256,8 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     for (int i = 0; i < min(count, kStages); ++i) issue(i);
 
     Spot at = spot_at(tiles, a.batch, begin);
-    float acc[kSteps][NT][4], m[NT][2], l[NT][2], row_scale[NT][2];
+    float acc[kSteps][NT][4], m[NT][2];
+    float2 l[NT], row_scale[NT];
     uint32_t query[NT][kSteps][2];
     int limit[NT][2], context = 0, rows = 0, row0 = 0, nearest = 0;
     float top = kLeastScale, from_top = 0.f;
@@ -275,8 +277,9 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           const int mine = t * 8 + r;
           uint4 w[D / 32];
           float size = 0.f;
-          const bool live = mine < rows && row0 + mine / a.group < a.rows;
-          const uint16_t* src = a.q + (row0 + mine / a.group) * a.q_row + (g * a.group + mine % a.group) * a.q_head + q4 * (D / 4);
+          const RowAt row = row_at(a, mine);
+          const bool live = mine < rows && row0 + row.token < a.rows;
+          const uint16_t* src = a.q + (long long)(row0 + row.token) * a.q_row + (long long)(g * a.group + row.head) * a.q_head + q4 * (D / 4);
 #pragma unroll
           for (int c = 0; c < D / 32; ++c) {
             w[c] = live ? *reinterpret_cast<const uint4*>(src + c * 8) : make_uint4(0, 0, 0, 0);
@@ -291,7 +294,7 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           size = fmaxf(size, __shfl_xor_sync(0xffffffffu, size, 2));
           // the row's largest magnitude comes to lie in [2^14, 2^15)
           const int up = max(-113, min(126, 14 - (int(__float_as_uint(size) >> 23) - 127)));
-          const float by = __uint_as_float(uint32_t(up + 127) << 23);
+          const float by = copysignf(__uint_as_float(uint32_t(up + 127) << 23), a.scale_log2);
 #pragma unroll
           for (int c = 0; c < D / 32; ++c) {
             const uint32_t words[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
@@ -301,14 +304,15 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
               query[t][c * 2 + e / 2][e & 1] = pack_f16x2(v.x * by, v.y * by);
             }
           }
-          const float back = __uint_as_float(uint32_t(127 - up) << 23) * a.scale_log2;
+          const float back = __uint_as_float(uint32_t(127 - up) << 23) * fabsf(a.scale_log2);
+          // of the rows whose scores this thread holds
+          row_scale[t] = make_float2(__shfl_sync(0xffffffffu, back, q4 * 8), __shfl_sync(0xffffffffu, back, q4 * 8 + 4));
+          l[t] = make_float2(0.f, 0.f);
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const int row = t * 8 + 2 * q4 + e;  // the rows whose scores this thread holds
-            row_scale[t][e] = __shfl_sync(0xffffffffu, back, (2 * q4 + e) * 4);
-            limit[t][e] = row < rows ? nearest + row / a.group : context;
-            m[t][e] = -INFINITY;
-            l[t][e] = 0.f;
+            const int at_row = t * 8 + 2 * q4 + e;
+            limit[t][e] = at_row < rows ? nearest + row_at(a, at_row).token : context;
+            m[t][e] = kNone;
           }
         }
 #pragma unroll
@@ -332,11 +336,11 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       // ---- scores: a thread's words of K are 32 (d = 64: 16) consecutive bytes of rows r and r + 8; q holds the same columns
       float s[2][NT][4];
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
+      for (int u = 0; u < 2; ++u) {
         uint32_t ka[kWords], kb[kWords];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          const int row = g * 16 + half * 8 + r;
+          const int row = u * 16 + half * 8 + r;
           uint32_t(&k)[kWords] = half == 0 ? ka : kb;
           if constexpr (D == 128) {
 #pragma unroll
@@ -352,91 +356,100 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[g][t][e] = 0.f;
+          for (int e = 0; e < 4; ++e) s[u][t][e] = 0.f;
 #pragma unroll
         for (int c = 0; c < kSteps; ++c) {
           const uint32_t a0 = halves_of(ka[c]), a2 = halves_of(ka[c] >> 16), a1 = halves_of(kb[c]), a3 = halves_of(kb[c] >> 16);
 #pragma unroll
-          for (int t = 0; t < NT; ++t) mma_f16(s[g][t], a0, a1, a2, a3, query[t][c][0], query[t][c][1]);
+          for (int t = 0; t < NT; ++t) mma_f16(s[u][t], a0, a1, a2, a3, query[t][c][0], query[t][c][1]);
         }
       }
 
-      // ---- softmax: the thread's tokens are g * 16 + r and + 8, its rows 2 * q4 and + 1 of each eight
-      const bool edge = token0 + kTile > nearest;  // some row does not see all of the tile
-      float high[NT][2];
+      // ---- softmax: the thread's tokens are u * 16 + r and + 8, its rows 2 * q4 and + 1 of each eight. Arithmetic goes two
+      // rows at a time; the maximum is taken of the raw scores, whose factors are positive
+      if (token0 + kTile > nearest) {  // some row does not see all of the tile
 #pragma unroll
-      for (int t = 0; t < NT; ++t) high[t][0] = high[t][1] = -INFINITY;
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        const float ks = ld_shared_f32(scales + stage * 16 + (box == kTile ? 0 : g) * 4);
+          for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            s[g][t][e] *= ks * row_scale[t][e & 1];
-            if (edge && token0 + g * 16 + r + (e >> 1) * 8 >= limit[t][e & 1]) s[g][t][e] = -INFINITY;
-            high[t][e & 1] = fmaxf(high[t][e & 1], s[g][t][e]);
-          }
+            for (int e = 0; e < 4; ++e) {
+              if (token0 + u * 16 + r + (e >> 1) * 8 >= limit[t][e & 1]) s[u][t][e] = -INFINITY;
+            }
       }
-      const float vs0 = ld_shared_f32(scales + stage * 16 + 8);
+      const float ks0 = ld_shared_f32(scales + stage * 16), vs0 = ld_shared_f32(scales + stage * 16 + 8);
+      const float ks1 = box == kTile ? ks0 : ld_shared_f32(scales + stage * 16 + 4);
       const float vs1 = box == kTile ? vs0 : ld_shared_f32(scales + stage * 16 + 12);
+      auto factor = [&](int u, int t) {  // never 0: a masked score is -inf times it
+        const float ks = u == 0 ? ks0 : ks1;
+        const float2 f = __fmul2_rn(row_scale[t], make_float2(ks, ks));
+        return make_float2(f.x < 0x1p-126f ? 0x1p-126f : f.x, f.y < 0x1p-126f ? 0x1p-126f : f.y);
+      };
       const float new_top = fmaxf(top, fmaxf(fabsf(vs0), fabsf(vs1)));
       bool moved = new_top != top;
       float m_new[NT][2];
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
+      for (int t = 0; t < NT; ++t) {
+        const float2 f0 = factor(0, t), f1 = factor(1, t);
+        float high[2] = {fmaxf(fmaxf(s[0][t][0], s[0][t][2]) * f0.x, fmaxf(s[1][t][0], s[1][t][2]) * f1.x),
+                         fmaxf(fmaxf(s[0][t][1], s[0][t][3]) * f0.y, fmaxf(s[1][t][1], s[1][t][3]) * f1.y)};
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
 #pragma unroll
-          for (int o = 4; o < 32; o <<= 1) high[t][e] = fmaxf(high[t][e], __shfl_xor_sync(0xffffffffu, high[t][e], o));
-          m_new[t][e] = fmaxf(m[t][e], high[t][e]);
+          for (int o = 4; o < 32; o <<= 1) high[e] = fmaxf(high[e], __shfl_xor_sync(0xffffffffu, high[e], o));
+          m_new[t][e] = fmaxf(m[t][e], high[e]);
           moved |= m_new[t][e] != m[t][e];
         }
+      }
       if (__any_sync(0xffffffffu, moved)) {
         const float shrink = top / new_top;
         top = new_top;
         from_top = 32768.0f / new_top;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          float corr[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float c = m[t][e] == -INFINITY ? 0.f : ex2_approx(m[t][e] - m_new[t][e]);
-            m[t][e] = m_new[t][e];
-            l[t][e] *= c;
-            corr[e] = c * shrink;
-          }
+          float2 corr;
+          corr.x = ex2_approx(m[t][0] - m_new[t][0]);
+          corr.y = ex2_approx(m[t][1] - m_new[t][1]);
+          m[t][0] = m_new[t][0];
+          m[t][1] = m_new[t][1];
+          l[t] = __fmul2_rn(l[t], corr);
+          corr = __fmul2_rn(corr, make_float2(shrink, shrink));
 #pragma unroll
           for (int c = 0; c < kSteps; ++c)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[c][t][e] *= corr[e & 1];
+            for (int e = 0; e < 4; e += 2) {
+              const float2 x = __fmul2_rn(make_float2(acc[c][t][e], acc[c][t][e + 1]), corr);
+              acc[c][t][e] = x.x;
+              acc[c][t][e + 1] = x.y;
+            }
         }
       }
       uint32_t weight[2][NT][2];
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        const float vs = (g == 0 ? vs0 : vs1) * from_top;
+      for (int u = 0; u < 2; ++u) {
+        const float vs = (u == 0 ? vs0 : vs1) * from_top;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          float w[4];
+          const float2 f = factor(u, t), shift = make_float2(-m[t][0], -m[t][1]);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            w[e] = m[t][e & 1] == -INFINITY ? 0.f : ex2_approx(s[g][t][e] - m[t][e & 1]);
-            l[t][e & 1] += w[e];
+          for (int e = 0; e < 2; ++e) {
+            const float2 x = __ffma2_rn(make_float2(s[u][t][2 * e], s[u][t][2 * e + 1]), f, shift);
+            const float2 w = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+            l[t] = __fadd2_rn(l[t], w);
+            const float2 y = __fmul2_rn(w, make_float2(vs, vs));
+            weight[u][t][e] = transposed(pack_f16x2(y.x, y.y));
           }
-          weight[g][t][0] = transposed(pack_f16x2(w[0] * vs, w[1] * vs));
-          weight[g][t][1] = transposed(pack_f16x2(w[2] * vs, w[3] * vs));
         }
       }
 
       // ---- output: a thread's columns of V are 16 (d = 64: 8) consecutive ones of tokens 2 * q4, + 1, + 8, + 9
       const bool tail = token0 + kTile > context;  // what lies behind the context may be any bits
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
+      for (int u = 0; u < 2; ++u) {
         uint32_t v[4][D / 32];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int row = g * 16 + 2 * q4 + (e & 1) + (e >> 1) * 8;
+          const int row = u * 16 + 2 * q4 + (e & 1) + (e >> 1) * 8;
           if constexpr (D == 128) {
             const uint4 x = ld_shared_16(values + row * 128 + ((r ^ (row & 7)) << 4));
             v[e][0] = x.x, v[e][1] = x.y, v[e][2] = x.z, v[e][3] = x.w;
@@ -457,8 +470,8 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           const uint32_t b0 = halves_of(x1), b1 = halves_of(x1 >> 16), b2 = halves_of(y1), b3 = halves_of(y1 >> 16);
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
-            mma_f16(acc[2 * c][t], a0, a1, a2, a3, weight[g][t][0], weight[g][t][1]);
-            mma_f16(acc[2 * c + 1][t], b0, b1, b2, b3, weight[g][t][0], weight[g][t][1]);
+            mma_f16(acc[2 * c][t], a0, a1, a2, a3, weight[u][t][0], weight[u][t][1]);
+            mma_f16(acc[2 * c + 1][t], b0, b1, b2, b3, weight[u][t][0], weight[u][t][1]);
           }
         }
       }
@@ -474,14 +487,15 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float sum = l[t][e];
+            float sum = e == 0 ? l[t].x : l[t].y;
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
             const int row = t * 8 + 2 * q4 + e;
-            if (row >= rows || row0 + row / a.group >= a.rows) continue;
+            const RowAt at_row = row_at(a, row);
+            if (row >= rows || row0 + at_row.token >= a.rows) continue;
             if (whole) {
               const float by = sum == 0.f ? 0.f : value / sum;
-              uint16_t* out = a.o + (row0 + row / a.group) * a.o_row + (g * a.group + row % a.group) * a.o_head + r * (D / 8);
+              uint16_t* out = a.o + (long long)(row0 + at_row.token) * a.o_row + (long long)(g * a.group + at_row.head) * a.o_head + r * (D / 8);
 #pragma unroll
               for (int c = 0; c < D / 64; ++c) {
                 uint32_t w[4];
@@ -533,12 +547,13 @@ __global__ void __launch_bounds__(kJoinThreads) cache_join_kernel(StreamParams p
   const int group = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
   const int row = blockIdx.y * slots + group % slots, share = group / slots, shares = kGroups / slots;
   const int row0 = a.row_start[b], rows = (a.row_start[b + 1] - row0) * a.group;
-  const int at = row0 + row / a.group;
+  const RowAt where = row_at(a, row);
+  const int at = row0 + where.token;
   wait_for_kernel_before();
   const int4 piece = p.pieces[b];
   if (piece.x == piece.y) return;  // no split: the rows are written, or belong to the other path
   const bool live = row < rows && at < a.rows;
-  float m = -INFINITY, l = 0.f;
+  float m = kNone, l = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   if (live) {
     const long long pitch = (long long)p.slot_rows * (D + 4);  // of a slot; a stretch and kv head have two
@@ -552,19 +567,19 @@ __global__ void __launch_bounds__(kJoinThreads) cache_join_kernel(StreamParams p
         const int part = first + k * shares;
         const bool there = part <= piece.y;
         const float* at_piece = from + (2ll * (there ? part : piece.x) * a.kv_heads + (part == piece.x ? piece.z : 0)) * pitch;
-        ml[k] = there ? *reinterpret_cast<const float2*>(at_piece) : make_float2(-INFINITY, 0.f);
+        ml[k] = there ? *reinterpret_cast<const float2*>(at_piece) : make_float2(kNone, 0.f);
         x[k] = there ? *reinterpret_cast<const float4*>(at_piece + 4 + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
       float high = m;
 #pragma unroll
       for (int k = 0; k < 8; ++k) high = fmaxf(high, ml[k].x);
-      const float old = m == -INFINITY ? 0.f : ex2_approx(m - high);
+      const float old = ex2_approx(m - high);
       m = high;
       l *= old;
       acc.x *= old, acc.y *= old, acc.z *= old, acc.w *= old;
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const float by = ml[k].x == -INFINITY ? 0.f : ex2_approx(ml[k].x - high);
+        const float by = ex2_approx(ml[k].x - high);
         l += by * ml[k].y;
         acc.x += by * x[k].x, acc.y += by * x[k].y, acc.z += by * x[k].z, acc.w += by * x[k].w;
       }
@@ -577,13 +592,13 @@ __global__ void __launch_bounds__(kJoinThreads) cache_join_kernel(StreamParams p
     if (share > 0) return;
     float high = m;
     for (int k = 1; k < shares; ++k) high = fmaxf(high, shared_ml[group + k * slots].x);
-    const float own = m == -INFINITY ? 0.f : ex2_approx(m - high);
+    const float own = ex2_approx(m - high);
     l *= own;
     acc.x *= own, acc.y *= own, acc.z *= own, acc.w *= own;
     for (int k = 1; k < shares; ++k) {
       const float2 ml = shared_ml[group + k * slots];
       const float4 x = shared_acc[group + k * slots][lane];
-      const float by = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - high);
+      const float by = ex2_approx(ml.x - high);
       l += by * ml.y;
       acc.x += by * x.x, acc.y += by * x.y, acc.z += by * x.z, acc.w += by * x.w;
     }
@@ -593,7 +608,7 @@ __global__ void __launch_bounds__(kJoinThreads) cache_join_kernel(StreamParams p
   uint2 w;
   w.x = BF16 ? pack_bf16x2(acc.x * by, acc.y * by) : pack_f16x2(acc.x * by, acc.y * by);
   w.y = BF16 ? pack_bf16x2(acc.z * by, acc.w * by) : pack_f16x2(acc.z * by, acc.w * by);
-  *reinterpret_cast<uint2*>(a.o + (long long)at * a.o_row + (long long)(g * a.group + row % a.group) * a.o_head + lane * 4) = w;
+  *reinterpret_cast<uint2*>(a.o + (long long)at * a.o_row + (long long)(g * a.group + where.head) * a.o_head + lane * 4) = w;
 }
 
 template <int D, bool BF16, int NT>
@@ -745,6 +760,7 @@ extern "C" int krn_b200_cache_attn(int type, const void* q, const void* k_pages,
   p.q_heads = int(q_heads);
   p.kv_heads = int(kv_heads);
   p.group = int(q_heads / kv_heads);
+  p.group_inverse = uint32_t((65536 + p.group - 1) / p.group);
   p.page_shift = 0;
   while ((int64_t(1) << p.page_shift) < page_size) ++p.page_shift;
   p.num_pages = int(num_pages);

@@ -28,9 +28,21 @@ struct CacheAttnParams {
   const int32_t* context_len;
   const int32_t* row_start;
   int batch, rows, q_heads, kv_heads, group, page_shift, num_pages, max_new, max_context;
+  uint32_t group_inverse;  // ceil(2^16 / group)
   int few;  // a request with at most this many rows (new tokens x q heads of a kv head) is streamed, one with more is tiled
   float scale_log2;
 };
+
+// Row `row` of a (request, kv head) is new token row / group, q head row % group of the kv head; for rows below 2^9 and
+// groups up to 2^7, (row * ceil(2^16 / group)) >> 16 is that quotient.
+struct RowAt {
+  int token, head;
+};
+
+__device__ __forceinline__ RowAt row_at(const CacheAttnParams& a, int row) {
+  const int token = int(uint32_t(row) * a.group_inverse >> 16);
+  return {token, row - token * a.group};
+}
 
 // Whether request b's n rows can be computed: some, no more than announced, and beginning within q.
 __device__ __forceinline__ bool rows_ok(const CacheAttnParams& a, int b, int n) {
