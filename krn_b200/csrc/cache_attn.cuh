@@ -10,7 +10,7 @@ namespace krnb {
 
 constexpr int kErrDeviceIndex = 6;  // mirrors KRN_B200_ERR_DEVICE_INDEX in include/krn_b200.h
 
-enum CacheAttnSite { kSitePage = 51, kSiteRows = 52, kSiteTile = 53, kSiteKeys = 54, kSiteValues = 55, kSiteQuery = 56,
+enum CacheAttnSite { kSitePage = 51, kSiteRows = 52, kSiteTile = 53, kSiteKeys = 54, kSiteValues = 55,
                      kSiteScores = 57, kSiteWeights = 58, kSiteOutput = 59, kSiteRoom = 60, kSiteRead = 61 };
 
 struct PoolSide {

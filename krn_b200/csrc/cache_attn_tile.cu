@@ -58,7 +58,7 @@ struct Layout {
   static constexpr int kOffRaw = kOffK + kKStages * kRawBytes;
   static constexpr int kOffHalf = kOffRaw + 2 * kRawBytes;
   static constexpr int kOffTail = kOffHalf + 2 * kHalfBytes;
-  static constexpr int kSmemBytes = kOffTail + 512 + 1024;
+  static constexpr int kSmemBytes = kOffTail + 512 + 2 * kTileQ * 4 + 1024;
 };
 
 __device__ __forceinline__ void tie(uint32_t (&r)[32]) {
@@ -88,6 +88,14 @@ __device__ __forceinline__ uint4 ld_shared_16(uint32_t addr) {
   uint4 v;
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
   return v;
+}
+
+// One lane polls, the warp follows. (For a warp that has others of its kind to wait with, polling with every lane is faster:
+// 3170 against 3450 cycles a key tile for the softmax warps.)
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, DeviceStatus* status, int site) {
+  bool ok = true;
+  if (lane_id() == 0) ok = mbar_wait(bar, parity, abort_flag, status, site);
+  return __all_sync(0xffffffffu, ok);
 }
 
 __device__ __forceinline__ uint32_t times(uint32_t a, uint32_t b) {  // f16x2
@@ -145,7 +153,7 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   const uint32_t q_addr = base, k_addr = base + L::kOffK, raw_addr = base + L::kOffRaw, half_addr = base + L::kOffHalf;
   uint8_t* tail = smem + L::kOffTail;
   const uint32_t bars = smem_u32(tail);
-  const uint32_t q_full = bars, k_full = bars + 8, k_empty = bars + 32, raw_full = bars + 56, raw_empty = bars + 72;
+  const uint32_t k_full = bars + 8, k_empty = bars + 32, raw_full = bars + 56, raw_empty = bars + 72;
   const uint32_t v_full = bars + 88, v_empty = bars + 104, s_full = bars + 120, p_full = bars + 136, o_full = bars + 152;
   const uint32_t s_read = bars + 168;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail + 176);
@@ -153,6 +161,7 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   int32_t* found = reinterpret_cast<int32_t*>(tail + 184);  // request, block of it, blocks of it
   int32_t* sums = reinterpret_cast<int32_t*>(tail + 200);   // [kThreads / 32]
   float* tops = reinterpret_cast<float*>(tail + 272);       // [kThreads / 32]
+  float* row_scales = reinterpret_cast<float*>(tail + 512); // [2 * kTileQ]
 
   const int warp = threadIdx.x >> 5;
   const int lane = int(lane_id());
@@ -219,6 +228,20 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   const int n0 = max(0, min(counts[0], j1) - j0), n1 = max(0, min(counts[1], j1) - j0);
   const int count = max(n0, n1);
 
+  // ---- Q: every thread takes 16 bytes of some rows; what it loads arrives while the rest is set up
+  constexpr int kQLanes = D / 8, kQRows = kThreads / kQLanes, kQPasses = 2 * kTileQ / kQRows;
+  const int q_lane = int(threadIdx.x) % kQLanes, q_row = int(threadIdx.x) / kQLanes;
+  uint4 q_words[kQPasses];
+#pragma unroll
+  for (int i = 0; i < kQPasses; ++i) {
+    const int row = i * kQRows + q_row, in_tile = row % kTileQ;
+    const RowAt at = row_at(a, in_tile);
+    const int token = token0 + (row / kTileQ) * p.tokens + at.token;
+    const bool live = at.token < p.tokens && token < n && row0 + token < a.rows;
+    const uint16_t* src = a.q + (long long)(row0 + token) * a.q_row + (long long)(g * a.group + at.head) * a.q_head + q_lane * 8;
+    q_words[i] = live ? *reinterpret_cast<const uint4*>(src) : make_uint4(0, 0, 0, 0);
+  }
+
   // ---- the largest value scale of these keys; ids outside the pool are reported
   {
     float top = 0.f;
@@ -235,30 +258,96 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (lane == 0) tops[warp] = top;
   }
-  if (threadIdx.x == 0) {
-    mbar_init(q_full, 8);
-    mbar_init(s_read, 4);
-    for (int i = 0; i < 3; ++i) {
-      mbar_init(k_full + 8 * i, 1);
-      mbar_init(k_empty + 8 * i, 1);
+  // Copies of K and V tile j, a lane each, by warp 2; page ids come 32 at a time.
+  const int box = min(kTileKV, 1 << a.page_shift), copies = kTileKV / box;
+  int ids = 0, ids_first = -64;
+  auto copy = [&](const CUtensorMap* map, int j, uint32_t dst, uint32_t bar) {
+    const int token = (j0 + j) * kTileKV, first_page = token >> a.page_shift;
+    if (first_page < ids_first || first_page + copies > ids_first + 32) {
+      ids_first = first_page;
+      ids = first_page + lane < pages ? table[first_page + lane] : 0;
     }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(raw_full + 8 * i, 1);
-      mbar_init(raw_empty + 8 * i, 4);
-      mbar_init(v_full + 8 * i, 4);
-      mbar_init(v_empty + 8 * i, 1);
-      mbar_init(s_full + 8 * i, 1);
-      mbar_init(p_full + 8 * i, 4);
-      mbar_init(o_full + 8 * i, 1);
+    int page = __shfl_sync(0xffffffffu, ids, (first_page + lane - ids_first) & 31);
+    if (uint32_t(page) >= uint32_t(a.num_pages)) page = a.num_pages;  // one past the pool: TMA fills zeros
+    const int there = min(copies, pages - first_page);
+    if (lane == 0) mbar_arrive_expect_tx(bar, uint32_t(there) * uint32_t(box) * D);
+    __syncwarp();
+    if (lane < there) tma_load_4d(dst + lane * box * D, map, 0, g, token & ((1 << a.page_shift) - 1), page, bar);
+  };
+  auto copy_k = [&](int j) { copy(&map_k, j, k_addr + (j % L::kKStages) * L::kRawBytes, k_full + 8 * (j % L::kKStages)); };
+  auto copy_v = [&](int j) { copy(&map_v, j, raw_addr + (j & 1) * L::kRawBytes, raw_full + 8 * (j & 1)); };
+  if (warp == 2) {
+    if (lane == 0) {
+      mbar_init(s_read, 4);
+      for (int i = 0; i < 3; ++i) {
+        mbar_init(k_full + 8 * i, 1);
+        mbar_init(k_empty + 8 * i, 1);
+      }
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(raw_full + 8 * i, 1);
+        mbar_init(raw_empty + 8 * i, 4);
+        mbar_init(v_full + 8 * i, 4);
+        mbar_init(v_empty + 8 * i, 1);
+        mbar_init(s_full + 8 * i, 1);
+        mbar_init(p_full + 8 * i, 4);
+        mbar_init(o_full + 8 * i, 1);
+      }
+      fence_mbar_init();
     }
-    fence_mbar_init();
-    prefetch_tensormap(&map_k);
-    prefetch_tensormap(&map_v);
+    __syncwarp();
+    for (int j = 0; j < min(count, 2); ++j) {  // both rings have room for two
+      copy_k(j);
+      copy_v(j);
+    }
   }
   if (warp == 1) {
     tmem_alloc<1>(smem_u32(tmem_slot), 512);
     tmem_relinquish<1>();
   }
+  // ---- Q as e4m3 parts
+#pragma unroll
+  for (int i = 0; i < kQPasses; ++i) {
+    const int row = i * kQRows + q_row, in_tile = row % kTileQ;
+    const uint32_t words[4] = {q_words[i].x, q_words[i].y, q_words[i].z, q_words[i].w};
+    float2 v[4];
+    float size = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[e] = unpack<BF16>(words[e]);
+      size = fmaxf(size, fmaxf(fabsf(v[e].x), fabsf(v[e].y)));
+    }
+#pragma unroll
+    for (int o = 1; o < kQLanes; o <<= 1) size = fmaxf(size, __shfl_xor_sync(0xffffffffu, size, o));
+    const int up = max(-120, min(126, 7 - (int(__float_as_uint(size) >> 23) - 127)));
+    const float by = copysignf(__uint_as_float(uint32_t(up + 127) << 23), a.scale_log2);
+    if (q_lane == 0) {
+      const float back = __uint_as_float(uint32_t(127 - up) << 23) * fabsf(a.scale_log2);
+      row_scales[row] = size > 3.4028234663852886e38f ? __int_as_float(0x7fffffff) : back;  // no factor brings an infinity back
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = __fmul2_rn(v[e], make_float2(by, by));
+    const uint32_t row_addr = q_addr + (row / kTileQ) * L::kQBytes + in_tile * 128 + (q_lane & 1) * 8;
+#pragma unroll
+    for (int part = 0; part < Parts; ++part) {
+      uint32_t code[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        uint16_t two;
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(two) : "f"(v[e].y), "f"(v[e].x));
+        code[e] = two;
+        if (part + 1 < Parts) {
+          const uint32_t h = halves_of(two);
+          const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&h));
+          v[e].x -= back.x;
+          v[e].y -= back.y;
+        }
+      }
+      const uint32_t chunk = uint32_t((part % L::kPerRow) * (D / 16) + (q_lane >> 1));
+      const uint32_t at = row_addr + (part / L::kPerRow) * L::kBlockBytes + ((chunk ^ (uint32_t(in_tile) & 7u)) << 4);
+      asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at), "r"(code[0] | code[1] << 16), "r"(code[2] | code[3] << 16) : "memory");
+    }
+  }
+  fence_async_smem();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -284,7 +373,6 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       const uint32_t q_lo = uint32_t(q_desc) + (q_addr >> 4), k_lo = uint32_t(k_desc) + (k_addr >> 4);
       int stage = 0;
       uint32_t phase = 0, reads = 0;  // reads: score tiles issued so far, each of which a softmax reads once
-      if (count > 0) ok = wait(q_full, 0, kSiteQuery);
       for (int j = 0; j < count && ok; ++j) {
         ok = wait(k_full + 8 * stage, phase, kSiteKeys);
         for (int t = 0; t < 2 && ok; ++t) {
@@ -348,37 +436,13 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       }
     }
   } else if (warp == 2) {
-    // ---------------------------------------------------------------- copies, a lane each
-    const int box = min(kTileKV, 1 << a.page_shift), copies = kTileKV / box;
-    int ids = 0, ids_first = -64;
-    for (int j = 0; j < count; ++j) {
-      const int token = (j0 + j) * kTileKV, first_page = token >> a.page_shift;
-      if (first_page + copies > ids_first + 32) {
-        ids_first = first_page;
-        ids = first_page + lane < pages ? table[first_page + lane] : 0;
-      }
-      int page = __shfl_sync(0xffffffffu, ids, (first_page + lane - ids_first) & 31);
-      if (uint32_t(page) >= uint32_t(a.num_pages)) page = a.num_pages;  // one past the pool: TMA fills zeros
-      const int there = min(copies, pages - first_page);
-      const uint32_t bytes = uint32_t(there) * uint32_t(box) * D;
-      const int stage = j % L::kKStages, v_stage = j & 1;
-      bool ok = true;
-      if (lane == 0) ok = mbar_wait(k_empty + 8 * stage, ((j / L::kKStages) & 1) ^ 1u, abort_flag, status, kSiteKeys);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      if (lane == 0) mbar_arrive_expect_tx(k_full + 8 * stage, bytes);
-      __syncwarp();
-      if (lane < there) {
-        tma_load_4d(k_addr + stage * L::kRawBytes + lane * box * D, &map_k, 0, g, token & ((1 << a.page_shift) - 1), page,
-                    k_full + 8 * stage);
-      }
-      if (lane == 0) ok = mbar_wait(raw_empty + 8 * v_stage, ((j >> 1) & 1) ^ 1u, abort_flag, status, kSiteValues);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      if (lane == 0) mbar_arrive_expect_tx(raw_full + 8 * v_stage, bytes);
-      __syncwarp();
-      if (lane < there) {
-        tma_load_4d(raw_addr + v_stage * L::kRawBytes + lane * box * D, &map_v, 0, g, token & ((1 << a.page_shift) - 1), page,
-                    raw_full + 8 * v_stage);
-      }
+    // ---------------------------------------------------------------- copies behind the first two
+    for (int j = 2; j < count; ++j) {
+      const int stage = j % L::kKStages;
+      if (!warp_wait(k_empty + 8 * stage, ((j / L::kKStages) & 1) ^ 1u, abort_flag, status, kSiteKeys)) break;
+      copy_k(j);
+      if (!warp_wait(raw_empty + 8 * (j & 1), ((j >> 1) & 1) ^ 1u, abort_flag, status, kSiteValues)) break;
+      copy_v(j);
     }
   } else if (warp >= 4 && warp < 8) {
     // ---------------------------------------------------------------- V to f16
@@ -429,68 +493,13 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     const int quarter = warp & 3;
     const int nt = t == 0 ? n0 : n1;
     const int row_in_tile = quarter * 32 + lane;
-    const int token = token0 + t * p.tokens + row_in_tile / a.group;
-    const bool live = row_in_tile < p.tokens * a.group && token < n && row0 + token < a.rows;
-    const int head = g * a.group + row_in_tile % a.group;
+    const RowAt where = row_at(a, row_in_tile);
+    const int token = token0 + t * p.tokens + where.token, head = g * a.group + where.head;
+    const bool live = where.token < p.tokens && token < n && row0 + token < a.rows;
+    const float row_scale = row_scales[t * kTileQ + row_in_tile];
     const uint32_t lane_base = tmem_base + (uint32_t(quarter * 32) << 16);
     const uint32_t s_tmem = lane_base, p_tmem = lane_base + 128 + t * 64;
     const uint32_t o_tmem = lane_base + 256 + t * 128;
-    float row_scale;
-
-    // ---- this thread's row of Q as e4m3 parts
-    {
-      const uint16_t* src = a.q + (long long)(row0 + token) * a.q_row + (long long)head * a.q_head;
-      uint4 w[D / 8];
-      float size = 0.f;
-#pragma unroll
-      for (int c = 0; c < D / 8; ++c) w[c] = live ? *reinterpret_cast<const uint4*>(src + c * 8) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-      for (int c = 0; c < D / 8; ++c) {
-        const uint32_t words[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 v = unpack<BF16>(words[e]);
-          size = fmaxf(size, fmaxf(fabsf(v.x), fabsf(v.y)));
-        }
-      }
-      const int up = max(-120, min(126, 7 - (int(__float_as_uint(size) >> 23) - 127)));
-      const float by = copysignf(__uint_as_float(uint32_t(up + 127) << 23), a.scale_log2);
-      row_scale = __uint_as_float(uint32_t(127 - up) << 23) * fabsf(a.scale_log2);
-      if (size > 3.4028234663852886e38f) row_scale = __int_as_float(0x7fffffff);  // no factor brings an infinity back
-      const uint32_t row_addr = q_addr + t * L::kQBytes + row_in_tile * 128;
-#pragma unroll
-      for (int c = 0; c < D / 16; ++c) {
-        float v[16];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint4& x = w[2 * c + (e >> 2)];
-          const float2 y = unpack<BF16>((e & 3) == 0 ? x.x : (e & 3) == 1 ? x.y : (e & 3) == 2 ? x.z : x.w);
-          v[2 * e] = y.x * by;
-          v[2 * e + 1] = y.y * by;
-        }
-#pragma unroll
-        for (int part = 0; part < Parts; ++part) {
-          uint32_t code[4];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            uint16_t two;
-            asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(two) : "f"(v[2 * e + 1]), "f"(v[2 * e]));
-            const uint32_t h = halves_of(two);
-            const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&h));
-            v[2 * e] -= back.x;
-            v[2 * e + 1] -= back.y;
-            code[e >> 1] = (e & 1) ? code[e >> 1] | uint32_t(two) << 16 : uint32_t(two);
-          }
-          const uint32_t chunk = uint32_t((part % L::kPerRow) * (D / 16) + c);
-          st_shared_16(row_addr + (part / L::kPerRow) * L::kBlockBytes + ((chunk ^ (uint32_t(row_in_tile) & 7u)) << 4), code[0],
-                       code[1], code[2], code[3]);
-        }
-      }
-      fence_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(q_full);
-    }
-
     const int sees = live ? max(0, min(context, context - n + token + 1)) : 0;  // keys of this row
     ScaleAhead scales = {table, a.k.scale, a.page_shift, pages, a.num_pages, a.kv_heads, g, lane, 1.f, 0, 0.f};
     if (nt > 0) scales.start(j0);
@@ -617,31 +626,43 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     if (nt > 0 && ok) ok = __all_sync(0xffffffffu, mbar_wait(o_full + 8 * t, (nt - 1) & 1, abort_flag, status, kSiteOutput));
     if (ok) {
       tc_fence_after();
-      const bool split = p.splits > 1;
-      float* share = p.partial + (((long long)blockIdx.y * a.rows + row0 + token) * a.q_heads + head) * (D + 4);
-      uint16_t* out = a.o + (long long)(row0 + token) * a.o_row + (long long)head * a.o_head;
       const float unit = top * (1.0f / 128.0f);
-      const float by = split ? unit : l == 0.f ? 0.f : unit / l;
-      if (split && live) *reinterpret_cast<float2*>(share) = make_float2(nt > 0 ? m_ref : kNone, l);
+      if (p.splits > 1) {
+        float* share = p.partial + (((long long)blockIdx.y * a.rows + row0 + token) * a.q_heads + head) * (D + 4);
+        if (live) *reinterpret_cast<float2*>(share) = make_float2(nt > 0 ? m_ref : kNone, l);
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t o[32];
-        __syncwarp();
-        if (nt > 0) {
-          tmem_ld_32x32(o_tmem + c * 32, o);
-          tmem_ld_wait(o);
-        } else {
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          __syncwarp();
+          if (nt > 0) {
+            tmem_ld_32x32(o_tmem + c * 32, o);
+            tmem_ld_wait(o);
+          } else {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = 0;
-        }
-        if (live && split) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            *reinterpret_cast<float4*>(share + 4 + c * 32 + i * 4) =
-                make_float4(__uint_as_float(o[4 * i]) * by, __uint_as_float(o[4 * i + 1]) * by,
-                            __uint_as_float(o[4 * i + 2]) * by, __uint_as_float(o[4 * i + 3]) * by);
+            for (int i = 0; i < 32; ++i) o[i] = 0;
           }
-        } else if (live) {
+          if (live) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              *reinterpret_cast<float4*>(share + 4 + c * 32 + i * 4) =
+                  make_float4(__uint_as_float(o[4 * i]) * unit, __uint_as_float(o[4 * i + 1]) * unit,
+                              __uint_as_float(o[4 * i + 2]) * unit, __uint_as_float(o[4 * i + 3]) * unit);
+            }
+          }
+        }
+      } else {
+        // through this tile's Q, which no product reads any more, so that a row's bytes go out side by side
+        constexpr int kLanes = D / 8;  // threads per row, 16 bytes each
+        const float by = l == 0.f ? 0.f : unit / l;
+        const uint32_t stage = q_addr + t * L::kQBytes + quarter * 32 * D * 2;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          __syncwarp();
+          if (nt > 0) {
+            tmem_ld_32x32(o_tmem + c * 32, o);
+            tmem_ld_wait(o);
+          }
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             uint32_t w[4];
@@ -651,8 +672,18 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
               const float y = l == 0.f ? 0.f : __uint_as_float(o[8 * i + 2 * e + 1]) * by;
               w[e] = BF16 ? pack_bf16x2(x, y) : pack_f16x2(x, y);
             }
-            *reinterpret_cast<uint4*>(out + c * 32 + i * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+            const uint32_t chunk = uint32_t(c * 4 + i);
+            st_shared_16(stage + lane * D * 2 + ((chunk ^ (uint32_t(lane) & 7u)) << 4), w[0], w[1], w[2], w[3]);
           }
+        }
+        __syncwarp();
+        const long long mine = live ? (long long)(row0 + token) * a.o_row + (long long)head * a.o_head : -1;
+#pragma unroll 4
+        for (int i = 0; i < kLanes; ++i) {  // 32 / kLanes rows at a time
+          const int row = i * (32 / kLanes) + lane / kLanes;
+          const long long at = __shfl_sync(0xffffffffu, mine, row);
+          const uint4 w = ld_shared_16(stage + row * D * 2 + ((uint32_t(lane % kLanes) ^ (uint32_t(row) & 7u)) << 4));
+          if (at >= 0) *reinterpret_cast<uint4*>(a.o + at + (lane % kLanes) * 8) = w;
         }
       }
     }
