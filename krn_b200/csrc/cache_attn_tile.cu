@@ -228,6 +228,16 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   const int n0 = max(0, min(counts[0], j1) - j0), n1 = max(0, min(counts[1], j1) - j0);
   const int count = max(n0, n1);
 
+  // ---- the pages of these keys, one a thread, and behind them the largest value scale: their loads come around the others'
+  const int first_page = (j0 * kTileKV) >> a.page_shift, end_page = min(pages, (((j0 + count) * kTileKV - 1) >> a.page_shift) + 1);
+  int scan_page = first_page + int(threadIdx.x) < end_page ? table[first_page + int(threadIdx.x)] : 0;
+  auto scan = [&](int at, int page) -> float {  // ids outside the pool are reported
+    if (at >= end_page) return 0.f;
+    if (uint32_t(page) < uint32_t(a.num_pages)) return fabsf(a.v.scale[(long long)page * a.kv_heads + g]);
+    report_failure(status, kErrDeviceIndex, kSitePage, uint32_t(page) & 0x7fffffffu);
+    return 0.f;
+  };
+
   // ---- Q: every thread takes 16 bytes of some rows; what it loads arrives while the rest is set up
   constexpr int kQLanes = D / 8, kQRows = kThreads / kQLanes, kQPasses = 2 * kTileQ / kQRows;
   const int q_lane = int(threadIdx.x) % kQLanes, q_row = int(threadIdx.x) / kQLanes;
@@ -242,22 +252,6 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     q_words[i] = live ? *reinterpret_cast<const uint4*>(src) : make_uint4(0, 0, 0, 0);
   }
 
-  // ---- the largest value scale of these keys; ids outside the pool are reported
-  {
-    float top = 0.f;
-    const int first = (j0 * kTileKV) >> a.page_shift, last = min(pages, (((j0 + count) * kTileKV - 1) >> a.page_shift) + 1);
-    for (int at = first + int(threadIdx.x); at < last; at += kThreads) {
-      const int page = table[at];
-      if (uint32_t(page) < uint32_t(a.num_pages)) {
-        top = fmaxf(top, fabsf(a.v.scale[(long long)page * a.kv_heads + g]));
-      } else {
-        report_failure(status, kErrDeviceIndex, kSitePage, uint32_t(page) & 0x7fffffffu);
-      }
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (lane == 0) tops[warp] = top;
-  }
   // Copies of K and V tile j, a lane each, by warp 2; page ids come 32 at a time.
   const int box = min(kTileKV, 1 << a.page_shift), copies = kTileKV / box;
   int ids = 0, ids_first = -64;
@@ -304,6 +298,8 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     tmem_alloc<1>(smem_u32(tmem_slot), 512);
     tmem_relinquish<1>();
   }
+  float top = scan(first_page + int(threadIdx.x), scan_page);
+
   // ---- Q as e4m3 parts
 #pragma unroll
   for (int i = 0; i < kQPasses; ++i) {
@@ -347,12 +343,16 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at), "r"(code[0] | code[1] << 16), "r"(code[2] | code[3] << 16) : "memory");
     }
   }
+  for (int at = first_page + int(threadIdx.x) + kThreads; at < end_page; at += kThreads) top = fmaxf(top, scan(at, table[at]));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (lane == 0) tops[warp] = top;
   fence_async_smem();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  float top = 0x1p-110f;
+  top = 0x1p-110f;  // smaller value scales are held against it
 #pragma unroll
   for (int w = 0; w < kThreads / 32; ++w) top = fmaxf(top, tops[w]);
 
