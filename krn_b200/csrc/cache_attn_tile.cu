@@ -16,7 +16,8 @@
 //
 // A page's key scale multiplies its columns of S in f32, before the maximum. Its value scale multiplies V, relative to the
 // largest one that this block meets and times 2^7 (448 * 2^7 is within f16): for scales that are powers of two V stays
-// exact down to 2^-22 of the largest; any other scale costs two roundings of 2^-12.
+// exact down to 2^-22 of the largest; any other scale costs two roundings of at most 2^-11, small beside bf16's 2^-8. f16
+// outputs would show them: there only the power of two in the scale goes to V, and the rest of it to P before its rounding.
 //
 // Tensor memory (512 columns): S (128) | P0 (64) | P1 (64) | O0 (128) | O1 (128). The two query tiles take turns in one S:
 // a softmax warp reads its scores into registers at once, so S is free for the other tile's scores long before the
@@ -111,7 +112,7 @@ __device__ __forceinline__ int blocks_of(const TileParams& p, int b) {
   return (n + 2 * p.tokens - 1) / (2 * p.tokens);
 }
 
-// The scales of the 16-token groups of key tiles, one group per lane of 8. Page ids are fetched two tiles ahead and scales
+// The scales of the 16-token groups of key tiles, one group per lane of 8 (a warp may have two of them). Page ids are fetched two tiles ahead and scales
 // one, by a call placed where a tile's long work follows. Groups without a page in the pool have the scale `none`.
 struct ScaleAhead {
   const int32_t* table;
@@ -457,7 +458,8 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     const uint32_t turn = uint32_t(c >> 2) & 1u, even = uint32_t(2 * c) & 7u;
     for (int j = 0; j < count; ++j) {
       const int stage = j & 1;
-      const float factor = scales.next * unit;
+      float factor = scales.next * unit;
+      if (!BF16) factor = __uint_as_float(__float_as_uint(factor) & 0x7f800000u);
       scales.fetch(j0 + j);
       const uint32_t mine = pack_f16x2(factor, factor);
       const bool ok = mbar_wait(raw_full + 8 * stage, (j >> 1) & 1, abort_flag, status, kSiteValues) &&
@@ -501,13 +503,21 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     const uint32_t s_tmem = lane_base, p_tmem = lane_base + 128 + t * 64;
     const uint32_t o_tmem = lane_base + 256 + t * 128;
     const int sees = live ? max(0, min(context, context - n + token + 1)) : 0;  // keys of this row
-    ScaleAhead scales = {table, a.k.scale, a.page_shift, pages, a.num_pages, a.kv_heads, g, lane, 1.f, 0, 0.f};
+    // lanes 0..7 hold K's scales; f16: lanes 8..15 V's
+    const bool for_v = !BF16 && (lane & 8) != 0;
+    ScaleAhead scales = {table, for_v ? a.v.scale : a.k.scale, a.page_shift, pages, a.num_pages, a.kv_heads, g, lane, 1.f, 0, 0.f};
+    const float unit_v = 128.0f / top;
     if (nt > 0) scales.start(j0);
     float m_ref = kNone, l = 0.f;
     bool ok = true;
 
     for (int j = 0; j < nt; ++j) {
-      float scale[Groups];
+      float scale[Groups], rest[Groups];  // rest: V's scale without its power of two
+      if (!BF16) {
+        const float mine = __uint_as_float((__float_as_uint(scales.next * unit_v) & 0x7fffffu) | 0x3f800000u);
+#pragma unroll
+        for (int i = 0; i < Groups; ++i) rest[i] = __shfl_sync(0xffffffffu, mine, 8 + i * (8 / Groups));
+      }
 #pragma unroll
       for (int i = 0; i < Groups; ++i) {
         const float x = __shfl_sync(0xffffffffu, scales.next, i * (8 / Groups)) * row_scale;
@@ -603,7 +613,8 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
                                       make_float2(by, by), shift2);
           const float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
           sum[c] = __fadd2_rn(sum[c], e);
-          packed[c >> 1][(c & 1) * 16 + i] = pack_f16x2(e.x, e.y);
+          const float2 w = BF16 ? e : __fmul2_rn(e, make_float2(rest[(c * 32 + 2 * i) / kGroup], rest[(c * 32 + 2 * i) / kGroup]));
+          packed[c >> 1][(c & 1) * 16 + i] = pack_f16x2(w.x, w.y);
         }
       }
       const float2 all = __fadd2_rn(__fadd2_rn(sum[0], sum[1]), __fadd2_rn(sum[2], sum[3]));
