@@ -118,8 +118,8 @@ __global__ void __launch_bounds__(kPlanThreads) cache_plan_kernel(PlanParams p, 
   uint32_t* back = run + p.batch;              // [batch] first page given back to the ring
   uint32_t* scratch = back + p.batch;          // [4 * kPlanWarps]
   const int page = 1 << p.page_shift;
-  launch_dependents();
   wait_for_kernel_before();
+  launch_dependents();
 
   // totals first: a step that does not fit takes nothing
   uint32_t carry[4] = {0, 0, 0, 0};
@@ -290,8 +290,8 @@ __global__ void __launch_bounds__(128) cache_append_kernel(AppendParams p, Devic
   const int tid = threadIdx.x % Threads;
   const uint32_t item = blockIdx.x * kGroups + threadIdx.x / Threads, per_run = 2u * uint32_t(p.heads);
   const int u = int(item / per_run), which = int(item - uint32_t(u) * per_run);
-  launch_dependents();
   wait_for_kernel_before();
+  launch_dependents();
   if (u >= p.runs_len) return;
   const int first = p.runs[u], next = u + 1 < p.runs_len ? p.runs[u + 1] : -1;
   if (uint32_t(first) >= uint32_t(p.rows)) return;

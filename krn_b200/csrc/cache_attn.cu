@@ -161,8 +161,8 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     prefetch_tensormap(&map_k);
     prefetch_tensormap(&map_v);
   }
-  launch_dependents();
   if (!p.beside) wait_for_kernel_before();
+  launch_dependents();
   // ---- every block counts the batch's tiles for itself
   int carry = 0;
   for (int first = 0; first < a.batch; first += kWarps * 32) {
@@ -546,10 +546,10 @@ __global__ void __launch_bounds__(kJoinThreads) cache_join_kernel(StreamParams p
   const int b = blockIdx.x / a.kv_heads, g = blockIdx.x % a.kv_heads;
   const int group = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
   const int row = blockIdx.y * slots + group % slots, share = group / slots, shares = kGroups / slots;
+  wait_for_kernel_before();
   const int row0 = a.row_start[b], rows = (a.row_start[b + 1] - row0) * a.group;
   const RowAt where = row_at(a, row);
   const int at = row0 + where.token;
-  wait_for_kernel_before();
   const int4 piece = p.pieces[b];
   if (piece.x == piece.y) return;  // no split: the rows are written, or belong to the other path
   const bool live = row < rows && at < a.rows;
@@ -715,7 +715,7 @@ extern "C" int krn_b200_cache_attn(int type, const void* q, const void* k_pages,
     return fail(KRN_B200_ERR_UNSUPPORTED, "a batch of %lld requests is not available: their tile counts sit in shared memory, at "
                 "most %d fit. Instead: split the batch", (long long)batch, kMaxBatch);
   }
-  if (batch * kv_heads * ((max_context + kTile - 1) / kTile) > INT32_MAX / 2 || kv_heads > 65535 || rows > INT32_MAX / 256 || rows * q_heads > INT32_MAX / 2 ||
+  if (batch * kv_heads * ((max_context + kTile - 1) / kTile) > INT32_MAX / 2 || q_heads > 65535 || rows > INT32_MAX / 256 || rows * q_heads > INT32_MAX / 2 ||
       max_context > INT32_MAX / 2 || num_pages >= INT32_MAX) {
     return fail(KRN_B200_ERR_UNSUPPORTED, "extents too large for this kernel's 32-bit indices");
   }

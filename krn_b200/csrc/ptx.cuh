@@ -83,8 +83,9 @@ __device__ __forceinline__ bool elect_one() {
   return chosen != 0;
 }
 
-// Programmatic dependent launch: let the next kernel of the stream begin / wait until the kernel before has completed and
-// its writes are visible. A kernel whose blocks all wait completes after everything before it in the stream.
+// Programmatic dependent launch: wait until the kernel before this one in the stream has completed and its writes are
+// visible / let the kernel behind this one begin. Kernels here wait first: whatever begins behind one of them then finds
+// everything before that one complete, and a kernel all of whose blocks wait completes after everything before it.
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_kernel_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 

@@ -455,6 +455,56 @@ def test_attention_of_large_and_small_queries(cuda, new) -> None:
         check_attention(cuda, dict(case, q=q * 2.0 ** power), scale=2.0 ** -power / math.sqrt(128))
 
 
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("new", [2, 70])
+def test_attention_of_rows_with_nan_and_infinities(cuda, dtype, new) -> None:
+    """A query row that holds a NaN or an infinity is NaN, and no other row is touched by it."""
+    rng = np.random.default_rng(45)
+    case = attention_case(cuda, rng, dtype, [150, 80], [new, 1], 16, 1, 4, 128)
+    clean = run_attention(cuda, case)
+    q = case["q"].clone()
+    q[0, 1, 5], q[1, 3, 0], q[new, 2, 127] = math.nan, math.inf, -math.inf
+    got = run_attention(cuda, dict(case, q=q))
+    for row, head in ((0, 1), (1, 3), (new, 2)):
+        assert bool(got[row, head].isnan().all())
+        got[row, head] = clean[row, head]
+    assert cuda.equal(got, clean)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_attention_with_a_negative_scale(cuda, new) -> None:
+    rng = np.random.default_rng(46)
+    check_attention(cuda, attention_case(cuda, rng, "bfloat16", [150, 80], [new, 1], 32, 1, 4, 64), scale=-0.2)
+
+
+def test_pools_beyond_four_gigabytes(cuda) -> None:
+    """Pages whose byte offsets do not fit 32 bits: the same bits as in a small pool."""
+    torch, rng = cuda, np.random.default_rng(47)
+    page, heads, d, far = 64, 8, 128, 70000
+    context, new = np.array([100, 0, 77]), np.array([1, 130, 1])
+    rows = int(new.sum())
+    table, start, slot, runs, total = lay_out(rng, context, new, page, rows)
+    (kc, ks), (vc, vs) = pool(rng, total, page, heads, d), pool(rng, total, page, heads, d)
+    k, v, q = (torch.randn(rows, h, d, device="cuda").to(torch.bfloat16) for h in (heads, heads, 4 * heads))
+    results = []
+    for base, pages in ((0, total), (far, far + total)):
+        cache = ops.PagedCache(*(torch.empty((pages, page, heads, d), dtype=torch.uint8, device="cuda") for _ in range(2)),
+                               *(torch.empty((pages, heads), device="cuda") for _ in range(2)))
+        for held, values in zip(cache, (kc, vc, ks, vs)):
+            held[base:].copy_(torch.from_numpy(values))
+        ids = torch.from_numpy(np.where(table >= 0, table + base, -1).astype(np.int32)).cuda()
+        ops.append_cache(k, v, torch.from_numpy(slot + base * page).cuda(), torch.from_numpy(runs).cuda(), cache)
+        out = torch.zeros_like(q)
+        longest = table.shape[1] * page
+        workspace = torch.empty(ops.cache_attention_workspace(3, rows, 4 * heads, heads, d, max_new=130, max_context=longest),
+                                dtype=torch.uint8, device="cuda")
+        ops.cache_attention(q, cache, ids, torch.from_numpy((context + new).astype(np.int32)).cuda(), torch.from_numpy(start).cuda(),
+                            out, max_new=130, max_context=longest, workspace=workspace)
+        results.append([x[base:].clone() for x in cache] + [out])
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+
+
 def test_attention_of_strided_tensors(cuda) -> None:
     """q cut from a fused projection, out head by head, pools as halves of one head-major allocation, a table with a pitch."""
     torch, rng = cuda, np.random.default_rng(39)
