@@ -274,57 +274,57 @@ def attention_decode_fp8_paged_noalloc(q: Any, k_pages: Any, v_pages: Any, page_
 _pack_strides = struct.Struct("10q").pack  # what the paged cache's entry points take: one array, filled in one go
 
 
-class _Place:
-    """Checks of one call's tensors and their addresses. Every tensor lives on the current CUDA device: an address of host
-    memory or of another GPU never reaches a kernel. These run before every launch of kernels of a few microseconds, so
-    they ask a tensor for as little as they can and say what was wrong apart."""
+class _Checks:
+    """Checks of one call's tensors. They run before every launch of kernels of a few microseconds, so they ask a tensor for
+    as little as they can and say what was wrong apart."""
 
     __slots__ = ("feature", "torch", "device")
 
     def __init__(self, feature: str) -> None:
         import torch
 
-        self.feature, self.torch, self.device = feature, torch, -2
+        self.feature, self.torch = feature, torch
 
-    def address(self, name: str, tensor: Any) -> int:
+    def addresses(self, names: str, tensors: tuple[Any, ...]) -> list[int]:
+        """The tensors' addresses. Every one lives on the current CUDA device: an address of host memory or of another GPU
+        never reaches a kernel."""
         try:
-            place = tensor.get_device()
+            places = [tensor.get_device() for tensor in tensors]
         except AttributeError:
-            place = -1
-        if place != self.device:
-            self._settle(name, place)
-        return tensor.data_ptr()
+            places = [tensor.get_device() if hasattr(tensor, "get_device") else -1 for tensor in tensors]
+        device = self.device = places[0]
+        if places.count(device) != len(places) or device < 0 or device != self.torch.cuda.current_device():
+            for name, place in zip(names.split(), places):
+                if place < 0:
+                    raise ValueError(f"{self.feature}: `{name}` must be a CUDA tensor")
+                if place != self.torch.cuda.current_device():
+                    raise ValueError(f"{self.feature}: `{name}` is on cuda:{place}, the current device is "
+                                     f"cuda:{self.torch.cuda.current_device()}")
+        return [tensor.data_ptr() for tensor in tensors]
 
-    def _settle(self, name: str, place: int) -> None:
-        if place < 0:
-            raise ValueError(f"{self.feature}: `{name}` must be a CUDA tensor")
-        self.device = self.torch.cuda.current_device()
-        if place != self.device:
-            raise ValueError(f"{self.feature}: `{name}` is on cuda:{place}, the current device is cuda:{self.device}")
+    def vector(self, name: str, tensor: Any, dtype: Any, length: int) -> int:
+        """The length of a contiguous rank-1 tensor of `dtype` (and of `length` elements, where that is not negative)."""
+        elements = tensor.numel()
+        if tensor.dtype is not dtype or not tensor.is_contiguous() or tensor.dim() != 1 or -1 < length != elements:
+            if tensor.dtype is not dtype:
+                raise TypeError(f"{self.feature}: `{name}` must be {str(dtype)[6:]}, got {tensor.dtype}")
+            if tensor.dim() != 1 or not tensor.is_contiguous():
+                raise ValueError(f"{self.feature}: `{name}` must be a contiguous vector, got shape {tuple(tensor.shape)}")
+            raise ValueError(f"{self.feature}: `{name}` has {elements} elements, {length} expected")
+        return elements
 
-    def vector(self, name: str, tensor: Any, dtype: Any, length: int = -1) -> int:
-        """A contiguous rank-1 tensor of `dtype` (and of `length` elements)."""
-        address = self.address(name, tensor)
-        if tensor.dtype is not dtype or tensor.dim() != 1 or not tensor.is_contiguous() or -1 < length != tensor.numel():
-            self._refuse_vector(name, tensor, dtype, length)
-        return address
-
-    def _refuse_vector(self, name: str, tensor: Any, dtype: Any, length: int) -> None:
-        if tensor.dtype is not dtype:
-            raise TypeError(f"{self.feature}: `{name}` must be {str(dtype)[6:]}, got {tensor.dtype}")
-        if tensor.dim() != 1 or not tensor.is_contiguous():
-            raise ValueError(f"{self.feature}: `{name}` must be a contiguous vector, got shape {tuple(tensor.shape)}")
-        raise ValueError(f"{self.feature}: `{name}` has {tensor.numel()} elements, {length} expected")
-
-    def table(self, name: str, tensor: Any, batch: int) -> tuple[int, int, int]:
-        """(address, entries per row, row pitch) of an int32 page table [batch, entries]."""
-        address = self.address(name, tensor)
+    def table(self, name: str, tensor: Any, batch: int) -> tuple[int, int]:
+        """(entries per row, row pitch) of an int32 page table [batch, entries]."""
+        shape = tensor.shape
         if tensor.dtype is not self.torch.int32:
             raise TypeError(f"{self.feature}: `{name}` must be int32, got {tensor.dtype}")
-        shape = tensor.shape
-        if len(shape) != 2 or shape[0] != batch or (shape[1] > 1 and tensor.stride(1) != 1):
-            raise ValueError(f"{self.feature}: `{name}` must be [{batch}, entries] with contiguous rows, got shape {tuple(shape)}")
-        return address, shape[1], tensor.stride(0) if batch > 1 else max(shape[1], 1)
+        if len(shape) == 2 and shape[0] == batch:
+            entries = shape[1]
+            if tensor.is_contiguous():
+                return entries, entries
+            if entries <= 1 or tensor.stride(1) == 1:
+                return entries, tensor.stride(0) if batch > 1 else entries
+        raise ValueError(f"{self.feature}: `{name}` must be [{batch}, entries] with contiguous rows, got shape {tuple(shape)}")
 
     def element(self, tensor: Any) -> int:
         """The element type of keys, values and queries."""
@@ -354,18 +354,19 @@ class _Place:
                     raise TypeError(f"{self.feature}: `{name}` must be float32, got {scale.dtype}")
                 if scale.shape != scales or not scale.is_contiguous():
                     raise ValueError(f"{self.feature}: `{name}` must be contiguous [{shape[0]}, {shape[2]}], got {tuple(scale.shape)}")
+        if k_pages.is_contiguous() and v_pages.is_contiguous():
+            _, tokens, heads, d = shape
+            strides = (tokens * heads * d, heads * d, d)
+            return shape, strides + strides
         return shape, self.strides("k_pages", k_pages, written) + self.strides("v_pages", v_pages, written)
 
     def strides(self, name: str, tensor: Any, written: bool) -> tuple[int, ...]:
         """Element strides of the outer axes of a tensor whose last axis is contiguous; an axis of one element counts as
         packed. A tensor that is written must not overlap itself."""
         shape = tensor.shape
-        if tensor.is_contiguous():
-            if len(shape) == 3:
-                _, middle, inner = shape
-                return middle * inner, inner
-            _, tokens, middle, inner = shape
-            return tokens * middle * inner, middle * inner, inner
+        if tensor.is_contiguous() and len(shape) == 3:
+            _, middle, inner = shape
+            return middle * inner, inner
         strides = tensor.stride()
         outer = len(shape) - 1
         if shape[outer] > 1 and strides[outer] != 1:
@@ -394,25 +395,31 @@ def cache_plan(context_len: Any, new_len: Any, page_table: Any, free_pages: Any,
                row_start: Any, slot_map: Any, runs: Any, state_out: Any, page_size: int, num_pages: int,
                stream: Any = None) -> None:
     """Pages, slots and page runs of a step's new tokens from request lengths (see krn_b200_cache_plan)."""
-    at = _Place("cache plan")
-    int32, int64 = at.torch.int32, at.torch.int64
-    context = at.vector("context_len", context_len, int32)
-    batch = context_len.shape[0]
-    brings = at.vector("new_len", new_len, int32, batch)
-    table, entries, pitch = at.table("page_table", page_table, batch)
-    status = native.library().krn_b200_cache_plan(
-        context, brings, table, at.vector("free_pages", free_pages, int32), at.vector("pool_state", pool_state, int64, 3),
-        at.vector("context_out", context_out, int32, batch), at.vector("row_start", row_start, int32, batch + 1),
-        at.vector("slot_map", slot_map, int64), at.vector("runs", runs, int32), at.vector("state_out", state_out, int64, 3), batch,
-        entries, pitch, free_pages.shape[0], page_size, num_pages, slot_map.shape[0], runs.shape[0], at.stream(stream))
+    at = _Checks("cache plan")
+    addresses = at.addresses("context_len new_len page_table free_pages pool_state context_out row_start slot_map runs state_out",
+                             (context_len, new_len, page_table, free_pages, pool_state, context_out, row_start, slot_map, runs,
+                              state_out))
+    vector, int32, int64 = at.vector, at.torch.int32, at.torch.int64
+    batch = vector("context_len", context_len, int32, -1)
+    vector("new_len", new_len, int32, batch)
+    entries, pitch = at.table("page_table", page_table, batch)
+    capacity = vector("free_pages", free_pages, int32, -1)
+    vector("pool_state", pool_state, int64, 3)
+    vector("context_out", context_out, int32, batch)
+    vector("row_start", row_start, int32, batch + 1)
+    rows, runs_len = vector("slot_map", slot_map, int64, -1), vector("runs", runs, int32, -1)
+    vector("state_out", state_out, int64, 3)
+    status = native.library().krn_b200_cache_plan(*addresses, batch, entries, pitch, capacity, page_size, num_pages, rows, runs_len,
+                                                  at.stream(stream))
     native.check(status, at.feature)
 
 
 def cache_append(k: Any, v: Any, slot_map: Any, runs: Any, k_pages: Any, v_pages: Any, k_scale: Any, v_scale: Any,
                  stream: Any = None) -> None:
     """Quantise rows of keys and values [rows, kv heads, d] into the pool (see krn_b200_cache_append)."""
-    at = _Place("cache append")
-    place = at.address
+    at = _Checks("cache append")
+    addresses = at.addresses("k v slot_map runs k_pages v_pages k_scale v_scale",
+                             (k, v, slot_map, runs, k_pages, v_pages, k_scale, v_scale))
     shape, page_strides = at.pool(k_pages, v_pages, k_scale, v_scale, True)
     num_pages, page_size, heads, d = shape
     rows = k.shape
@@ -420,10 +427,9 @@ def cache_append(k: Any, v: Any, slot_map: Any, runs: Any, k_pages: Any, v_pages
         raise ValueError(f"{at.feature}: k {tuple(k.shape)} and v {tuple(v.shape)} do not match a pool of {heads} heads of {d}")
     if k.dtype is not v.dtype:
         raise TypeError(f"{at.feature}: k and v must have the same element type")
+    slots, runs_len = at.vector("slot_map", slot_map, at.torch.int64, -1), at.vector("runs", runs, at.torch.int32, -1)
     status = native.library().krn_b200_cache_append(
-        at.element(k), place("k", k), place("v", v), at.vector("slot_map", slot_map, at.torch.int64),
-        at.vector("runs", runs, at.torch.int32), place("k_pages", k_pages), place("v_pages", v_pages), place("k_scale", k_scale),
-        place("v_scale", v_scale), min(rows[0], slot_map.shape[0]), runs.shape[0], heads, d, page_size, num_pages,
+        at.element(k), *addresses, min(rows[0], slots), runs_len, heads, d, page_size, num_pages,
         _pack_strides(*at.strides("k", k, False), *at.strides("v", v, False), *page_strides), at.stream(stream))
     native.check(status, at.feature)
 
@@ -437,8 +443,9 @@ def cache_attention(q: Any, k_pages: Any, v_pages: Any, k_scale: Any, v_scale: A
                     row_start: Any, o: Any, scale_log2: float, max_new: int, max_context: int, workspace: Any,
                     stream: Any = None) -> None:
     """Attention of packed query rows [rows, q heads, d] over the pool (see krn_b200_cache_attn)."""
-    at = _Place("cache attention")
-    place = at.address
+    at = _Checks("cache attention")
+    *addresses, scratch = at.addresses("q k_pages v_pages k_scale v_scale page_table context_len row_start out workspace",
+                                       (q, k_pages, v_pages, k_scale, v_scale, page_table, context_len, row_start, o, workspace))
     shape, page_strides = at.pool(k_pages, v_pages, k_scale, v_scale, False)
     num_pages, page_size, heads, d = shape
     rows = q.shape
@@ -446,15 +453,13 @@ def cache_attention(q: Any, k_pages: Any, v_pages: Any, k_scale: Any, v_scale: A
         raise ValueError(f"{at.feature}: q {tuple(q.shape)} and out {tuple(o.shape)} do not match a pool of heads of {d}")
     if q.dtype is not o.dtype:
         raise TypeError(f"{at.feature}: q and out must have the same element type")
-    context = at.vector("context_len", context_len, at.torch.int32)
-    batch = context_len.shape[0]
-    table, entries, pitch = at.table("page_table", page_table, batch)
+    batch = at.vector("context_len", context_len, at.torch.int32, -1)
+    at.vector("row_start", row_start, at.torch.int32, batch + 1)
+    entries, pitch = at.table("page_table", page_table, batch)
     status = native.library().krn_b200_cache_attn(
-        at.element(q), place("q", q), place("k_pages", k_pages), place("v_pages", v_pages), place("k_scale", k_scale),
-        place("v_scale", v_scale), table, context, at.vector("row_start", row_start, at.torch.int32, batch + 1), place("out", o), batch,
-        rows[0], rows[1], heads, d, page_size, num_pages, entries, pitch, max_new, max_context,
-        _pack_strides(*at.strides("q", q, False), *at.strides("out", o, True), *page_strides), scale_log2,
-        place("workspace", workspace), workspace.nbytes, at.stream(stream))
+        at.element(q), *addresses, batch, rows[0], rows[1], heads, d, page_size, num_pages, entries, pitch, max_new, max_context,
+        _pack_strides(*at.strides("q", q, False), *at.strides("out", o, True), *page_strides), scale_log2, scratch,
+        workspace.nbytes, at.stream(stream))
     native.check(status, at.feature)
 
 

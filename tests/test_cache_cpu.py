@@ -155,12 +155,11 @@ def test_host_tensors_are_refused() -> None:
         ops.cache_attention(x, cache, table, lengths, plan.row_start, x, max_new=1, max_context=64, workspace=x)
 
 
-def test_layout_checks(monkeypatch) -> None:
-    """The checks behind the calls, on host tensors that pass for the device's."""
+def test_layout_checks() -> None:
+    """The checks behind the calls, on host tensors."""
     import torch
 
-    at = calls._Place("t")
-    monkeypatch.setattr(calls._Place, "address", lambda self, name, tensor: tensor.data_ptr())
+    at = calls._Checks("t")
     x = torch.zeros(6, 4, 128)
     assert list(at.strides("x", x, True)) == [512, 128]
     assert list(at.strides("x", x.transpose(0, 1), True)) == [128, 512]
@@ -190,6 +189,8 @@ def test_layout_checks(monkeypatch) -> None:
     with pytest.raises(ValueError, match="5 expected"):
         at.vector("x", torch.zeros(4, dtype=torch.int32), torch.int32, 5)
     with pytest.raises(ValueError, match="contiguous vector"):
-        at.vector("x", torch.zeros(8, dtype=torch.int32)[::2], torch.int32)
+        at.vector("x", torch.zeros(8, dtype=torch.int32)[::2], torch.int32, -1)
     with pytest.raises(TypeError, match="must be int32, got torch.int64"):
-        at.vector("x", torch.zeros(8, dtype=torch.int64), torch.int32)
+        at.vector("x", torch.zeros(8, dtype=torch.int64), torch.int32, -1)
+    with pytest.raises(ValueError, match="must be a CUDA tensor"):
+        at.addresses("a b", (torch.zeros(2, device="meta"), object()))
