@@ -20,12 +20,12 @@ constexpr int kMaxBatch = 8192;    // tile counts of the batch sit in shared mem
 constexpr float kLeastScale = 0x1p-110f;  // value scales below it are held against it
 constexpr float kNone = -3.0e38f;         // reference maximum of a row that has seen no key
 
-// Partial results of the pieces of split segments, 2 + d floats (m, l, the unnormalised output) for each of `rows`.
+// Partial results of the pieces of split segments, d + 4 floats (m, l, two unused, the unnormalised output) for each row.
 struct StreamParams {
   CacheAttnParams a;
   int4* pieces;      // [batch] first and last stretch of each request, whether its first piece is a warp's second; for the join
   float* partial;
-  int slot_rows;     // rows a partial slot holds
+  int row_blocks;    // warps that share a stretch and kv head, each with its own NT * 8 rows of every request
   int beside;        // launched beside the tile kernel, which waited for what came before: wait for it at the end
 };
 
@@ -82,8 +82,8 @@ __device__ __forceinline__ int first_tile(int part, int parts, int total) { retu
 // The stretch that holds tile `at`.
 __device__ __forceinline__ int stretch_of(int at, int parts, int total) { return int(((long long)(at + 1) * parts - 1) / total); }
 
-// Stretches: one warp for each and kv head, one tile at least.
-__device__ __forceinline__ int stretches(int total, int warps, int kv_heads) { return max(1, min(warps / kv_heads, total)); }
+// Stretches: one warp for each, kv head and block of rows, one tile at least.
+__device__ __forceinline__ int stretches(int total, int warps, int sharers) { return max(1, min(warps / sharers, total)); }
 
 // Where a warp stands in the line.
 struct Spot {
@@ -137,6 +137,7 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   using L = StreamLayout<D>;
   constexpr int kSteps = D / 16;       // MMA steps over d
   constexpr int kWords = D / 16;       // 32-bit words of a K row that a thread holds
+  constexpr int kSlotRows = NT * 8;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
@@ -190,7 +191,7 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   if (threadIdx.x == 0) tiles[a.batch] = carry;
   __syncthreads();
   const int total = carry, grid_warps = int(gridDim.x) * kWarps;
-  const int parts = stretches(total, grid_warps, a.kv_heads);
+  const int sharers = a.kv_heads * p.row_blocks, parts = stretches(total, grid_warps, sharers);
   if (blockIdx.x == 0) {
     for (int b = threadIdx.x; b < a.batch; b += kWarps * 32) {
       const int first = tiles[b], last = tiles[b + 1] - 1;
@@ -211,8 +212,9 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 
   bool ok = true;
   int done = 0;  // tiles of earlier units: the ring goes on
-  for (int unit = int(blockIdx.x) * kWarps + warp; unit < parts * a.kv_heads && ok; unit += grid_warps) {
-    const int part = unit / a.kv_heads, g = unit - part * a.kv_heads;
+  for (int unit = int(blockIdx.x) * kWarps + warp; unit < parts * sharers && ok; unit += grid_warps) {
+    const int part = unit / sharers, g = (unit - part * sharers) / p.row_blocks;
+    const int row_base = (unit % p.row_blocks) * kSlotRows;  // first row of each request that is this warp's
     const int begin = first_tile(part, parts, total), count = first_tile(part + 1, parts, total) - begin;
 
     // ---- the stretch's tiles in order: page ids come 32 at a time, one per lane
@@ -227,7 +229,8 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         ids_b = ahead.b;
         ids_first = first_page;
         const int context = max(0, min(a.context_len[ahead.b], a.max_context));
-        ahead_pages = (context + page_mask) >> a.page_shift;
+        const bool mine = (a.row_start[ahead.b + 1] - a.row_start[ahead.b]) * a.group > row_base;  // else nothing is fetched
+        ahead_pages = mine ? (context + page_mask) >> a.page_shift : 0;
         ids = first_page + lane < ahead_pages ? a.page_table[ahead.b * a.table_pitch + first_page + lane] : 0;
       }
       // sub-tile 0 / 1: tokens 0..15 / 16..31 for 16-token pages; else one copy of 32 tokens
@@ -274,7 +277,7 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         nearest = context - n + 1;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          const int mine = t * 8 + r;
+          const int mine = row_base + t * 8 + r;
           uint4 w[D / 32];
           float size = 0.f;
           const RowAt row = row_at(a, mine);
@@ -310,7 +313,7 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           l[t] = make_float2(0.f, 0.f);
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const int at_row = t * 8 + 2 * q4 + e;
+            const int at_row = row_base + t * 8 + 2 * q4 + e;
             limit[t][e] = at_row < rows ? nearest + row_at(a, at_row).token : context;
             m[t][e] = kNone;
           }
@@ -330,6 +333,11 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       if (!__all_sync(0xffffffffu, mbar_wait(bars + 8 * stage, ((done + i) / kStages) & 1, abort_flag, status, kSiteTile))) {
         ok = false;
         break;
+      }
+      if (rows <= row_base) {  // a request with fewer rows than others
+        if (i + kStages < count) issue(i + kStages);
+        step(at, tiles, a.batch);
+        continue;
       }
       const int token0 = at.tile * kTile;
 
@@ -490,7 +498,7 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             float sum = e == 0 ? l[t].x : l[t].y;
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            const int row = t * 8 + 2 * q4 + e;
+            const int in_slot = t * 8 + 2 * q4 + e, row = row_base + in_slot;
             const RowAt at_row = row_at(a, row);
             if (row >= rows || row0 + at_row.token >= a.rows) continue;
             if (whole) {
@@ -507,7 +515,7 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                 *reinterpret_cast<uint4*>(out + c * 8) = make_uint4(w[0], w[1], w[2], w[3]);
               }
             } else {
-              float* out = p.partial + ((long long)slot * p.slot_rows + row) * (D + 4);
+              float* out = p.partial + ((long long)slot * kSlotRows + in_slot) * (D + 4);
               if (r == 0) *reinterpret_cast<float2*>(out) = make_float2(m[t][e], sum);
 #pragma unroll
               for (int c = 0; c < D / 32; ++c) {
@@ -538,7 +546,7 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 constexpr int kJoinThreads = 256;
 
 template <int D, bool BF16>
-__global__ void __launch_bounds__(kJoinThreads) cache_join_kernel(StreamParams p, int slots) {
+__global__ void __launch_bounds__(kJoinThreads) cache_join_kernel(StreamParams p, int slot_rows, int slots) {
   constexpr int kLanes = D / 4, kGroups = kJoinThreads / kLanes;
   __shared__ float4 shared_acc[kGroups][kLanes];
   __shared__ float2 shared_ml[kGroups];
@@ -556,8 +564,9 @@ __global__ void __launch_bounds__(kJoinThreads) cache_join_kernel(StreamParams p
   float m = kNone, l = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   if (live) {
-    const long long pitch = (long long)p.slot_rows * (D + 4);  // of a slot; a stretch and kv head have two
-    const float* from = p.partial + 2 * g * pitch + (long long)row * (D + 4);
+    const long long pitch = (long long)slot_rows * (D + 4);  // of a slot; every warp of a stretch has two
+    const int sharers = a.kv_heads * p.row_blocks, block = row / slot_rows;
+    const float* from = p.partial + 2 * (g * p.row_blocks + block) * pitch + (long long)(row - block * slot_rows) * (D + 4);
 #pragma unroll 1
     for (int first = piece.x + share; first <= piece.y; first += 8 * shares) {
       float2 ml[8];
@@ -566,7 +575,7 @@ __global__ void __launch_bounds__(kJoinThreads) cache_join_kernel(StreamParams p
       for (int k = 0; k < 8; ++k) {
         const int part = first + k * shares;
         const bool there = part <= piece.y;
-        const float* at_piece = from + (2ll * (there ? part : piece.x) * a.kv_heads + (part == piece.x ? piece.z : 0)) * pitch;
+        const float* at_piece = from + (2ll * (there ? part : piece.x) * sharers + (part == piece.x ? piece.z : 0)) * pitch;
         ml[k] = there ? *reinterpret_cast<const float2*>(at_piece) : make_float2(kNone, 0.f);
         x[k] = there ? *reinterpret_cast<const float4*>(at_piece + 4 + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
@@ -628,7 +637,8 @@ int launch_stream(const DeviceContext* ctx, const StreamParams& p, int64_t page_
     return rc;
   }
   // no more blocks than the contexts could give warps work
-  const int64_t wanted = (int64_t(a.batch) * a.kv_heads * ((a.max_context + kTile - 1) / kTile) + kWarps - 1) / kWarps;
+  const int64_t sharers = int64_t(a.kv_heads) * p.row_blocks;
+  const int64_t wanted = (int64_t(a.batch) * sharers * ((a.max_context + kTile - 1) / kTile) + kWarps - 1) / kWarps;
   const int most = ctx->sm_count < kMaxBlocks ? ctx->sm_count : kMaxBlocks;
   const int blocks = int(wanted < most ? wanted : most);
   if (int rc = launch_dependent(kernel, dim3(unsigned(blocks)), kWarps * 32, StreamLayout<D>::bytes(a.batch), stream, map_k, map_v, p,
@@ -637,32 +647,42 @@ int launch_stream(const DeviceContext* ctx, const StreamParams& p, int64_t page_
   }
   // rows of a block: as few as leave each group of threads no more than eight pieces, as the batch is split on average
   constexpr int kGroups = kJoinThreads * 4 / D;
-  const int64_t pieces = int64_t(blocks) * kWarps / a.kv_heads / a.batch + 2;
+  const int64_t pieces = int64_t(blocks) * kWarps / sharers / a.batch + 2;
   int slots = kGroups;
-  while (slots > 1 && (slots / 2 >= p.slot_rows || pieces > 8 * (kGroups / slots))) slots /= 2;
-  const dim3 grid(unsigned(a.batch) * unsigned(a.kv_heads), unsigned((p.slot_rows + slots - 1) / slots));
-  return launch_dependent(cache_join_kernel<D, BF16>, grid, kJoinThreads, 0, stream, p, slots);
+  while (slots > 1 && (slots / 2 >= a.few || pieces > 8 * (kGroups / slots))) slots /= 2;
+  const dim3 grid(unsigned(a.batch) * unsigned(a.kv_heads), unsigned((a.few + slots - 1) / slots));
+  return launch_dependent(cache_join_kernel<D, BF16>, grid, kJoinThreads, 0, stream, p, NT * 8, slots);
 }
 
 // Rows of a streamed request: all of them where every request has few; where some have many, those with one new token
 // (or the few that fit beside it) are streamed and the rest is tiled.
-int64_t slot_rows(int64_t max_new, int64_t group) {
+int64_t few_rows(int64_t max_new, int64_t group) {
   if (max_new * group <= 32) return max_new * group;
   return group <= 8 ? 8 : group <= 16 ? 16 : group <= 32 ? 32 : 0;
 }
 
 int64_t pieces_bytes(int64_t batch) { return batch * 16; }
 
-int64_t stream_workspace(int64_t batch, int64_t kv_heads, int64_t d, int64_t rows) {
-  const int64_t warps = int64_t(kMaxBlocks) * kWarps, units = warps > kv_heads ? warps : kv_heads;
-  return pieces_bytes(batch) + 2 * units * rows * (d + 4) * 4;
+// Rows of a warp: 8, 16 or, with rows of 64 columns, 32, as registers hold them (32 rows of 128 columns spilled: 58 us
+// against 44 for two warps of 16 rows each, 24 requests of 8 x 4 rows over 4096 tokens). Where a request may have more,
+// several warps share a stretch.
+int64_t warp_rows(int64_t d, int64_t few) { return few <= 8 ? 8 : few <= 16 || d == 128 ? 16 : 32; }
+
+int64_t row_blocks(int64_t d, int64_t few) { return (few + warp_rows(d, few) - 1) / warp_rows(d, few); }
+
+int64_t stream_workspace(int64_t batch, int64_t kv_heads, int64_t d, int64_t few) {
+  const int64_t warps = int64_t(kMaxBlocks) * kWarps, sharers = kv_heads * row_blocks(d, few);
+  const int64_t units = warps > sharers ? warps : sharers;
+  return pieces_bytes(batch) + 2 * units * warp_rows(d, few) * (d + 4) * 4;
 }
 
 template <int D, bool BF16>
 int launch_stream_rows(const DeviceContext* ctx, const StreamParams& p, int64_t page_size, cudaStream_t stream) {
-  if (p.slot_rows <= 8) return launch_stream<D, BF16, 1>(ctx, p, page_size, stream);
-  if (p.slot_rows <= 16) return launch_stream<D, BF16, 2>(ctx, p, page_size, stream);
-  return launch_stream<D, BF16, 4>(ctx, p, page_size, stream);
+  const int64_t rows = warp_rows(D, p.a.few);
+  if constexpr (D == 64) {
+    if (rows == 32) return launch_stream<D, BF16, 4>(ctx, p, page_size, stream);
+  }
+  return rows == 8 ? launch_stream<D, BF16, 1>(ctx, p, page_size, stream) : launch_stream<D, BF16, 2>(ctx, p, page_size, stream);
 }
 
 }  // namespace
@@ -672,7 +692,7 @@ extern "C" int64_t krn_b200_cache_attn_workspace_bytes(int64_t batch, int64_t ro
                                                        int64_t max_new, int64_t max_context) {
   using namespace krnb;
   if (batch <= 0 || rows <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0 || d <= 0 || max_new <= 0) return 16;
-  const int64_t few = slot_rows(max_new, q_heads / kv_heads);
+  const int64_t few = few_rows(max_new, q_heads / kv_heads);
   return stream_workspace(batch, kv_heads, d, few) +
          (max_new * (q_heads / kv_heads) <= few ? 0 : tile_workspace(batch, rows, q_heads, kv_heads, d, few, max_context));
 }
@@ -770,11 +790,11 @@ extern "C" int krn_b200_cache_attn(int type, const void* q, const void* k_pages,
   cudaStream_t stream = static_cast<cudaStream_t>(stream_handle);
   const bool bf16 = type == KRN_B200_BF16;
   StreamParams sp;
-  p.few = int(slot_rows(max_new, p.group));
+  p.few = int(few_rows(max_new, p.group));
   sp.a = p;
   sp.pieces = static_cast<int4*>(workspace);
   sp.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + pieces_bytes(batch));
-  sp.slot_rows = p.few;
+  sp.row_blocks = int(row_blocks(d, p.few));
   // The two paths run side by side: the tile kernel first, whose blocks take longest, and the stream on the SMs that it
   // leaves free.
   const bool tiled = max_new * p.group > p.few && tile_blocks(batch, rows, p.group, p.few) > 0;
