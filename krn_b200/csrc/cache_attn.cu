@@ -13,8 +13,7 @@ namespace {
 // ---- few rows: a stream of keys per warp ---------------------------------------------------------------------------------
 
 constexpr int kTile = 32;          // tokens a warp takes at a time
-constexpr int kWarps = 8;
-constexpr int kStages = 3;         // tiles a warp has in flight or in work
+constexpr int kMaxWarps = 12;      // of a block
 constexpr int kMaxBlocks = 160;    // bounds the workspace; a B200 has 148 SMs
 constexpr int kMaxBatch = 8192;    // tile counts of the batch sit in shared memory
 constexpr float kLeastScale = 0x1p-110f;  // value scales below it are held against it
@@ -108,8 +107,14 @@ __device__ __forceinline__ void step(Spot& s, const int32_t* tiles, int batch) {
   if (s.b < batch) s.tiles = tiles[s.b + 1] - tiles[s.b];
 }
 
-template <int D>
+// Warps of a block and their rings. Rows of 128 columns: 8 warps with 3 tiles of 8 KB each, 105 us on the 64-sequence mix of
+// 1024 to 8192 tokens (10 warps with 2: 105.4, 12 with 2: 109, 9 with 2: 111). Rows of 64: tiles of 4 KB leave room for 12
+// warps, 30.5 us against 34.5 with 8 (64 sequences of 2048 to 4096 tokens, 4 kv heads; 16 with 3: 29.8, but 19.5 against
+// 17.6 us for one sequence of 60000).
+template <int D, int NT>
 struct StreamLayout {
+  static constexpr int kWarps = D == 64 && NT == 1 ? 12 : 8;
+  static constexpr int kStages = 3;                       // tiles a warp has in flight or in work
   static constexpr int kSide = kTile * D;                 // one of K and V, bytes
   static constexpr int kStage = 2 * kSide;
   static constexpr int kRing = kWarps * kStages * kStage;
@@ -131,10 +136,11 @@ struct StreamLayout {
 // 2^-29 of the largest one. A warp whose stretch covers a whole segment writes its output; pieces of split segments go to
 // the workspace and cache_join_kernel joins them.
 template <int D, bool BF16, int NT>
-__global__ void __launch_bounds__(kWarps * 32, 1)
+__global__ void __launch_bounds__(StreamLayout<D, NT>::kWarps * 32, 1)
 cache_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, StreamParams p,
                     DeviceStatus* status) {
-  using L = StreamLayout<D>;
+  using L = StreamLayout<D, NT>;
+  constexpr int kWarps = L::kWarps, kStages = L::kStages;
   constexpr int kSteps = D / 16;       // MMA steps over d
   constexpr int kWords = D / 16;       // 32-bit words of a K row that a thread holds
   constexpr int kSlotRows = NT * 8;
@@ -631,17 +637,18 @@ int launch_stream(const DeviceContext* ctx, const StreamParams& p, int64_t page_
   auto kernel = cache_stream_kernel<D, BF16, NT>;
   static OncePerDevice ready;
   if (int rc = ready(ctx->device, [&] {
-        KRNB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, StreamLayout<D>::bytes(kMaxBatch)));
+        KRNB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, StreamLayout<D, NT>::bytes(kMaxBatch)));
         return KRN_B200_OK;
       })) {
     return rc;
   }
+  constexpr int kWarps = StreamLayout<D, NT>::kWarps;
   // no more blocks than the contexts could give warps work
   const int64_t sharers = int64_t(a.kv_heads) * p.row_blocks;
   const int64_t wanted = (int64_t(a.batch) * sharers * ((a.max_context + kTile - 1) / kTile) + kWarps - 1) / kWarps;
   const int most = ctx->sm_count < kMaxBlocks ? ctx->sm_count : kMaxBlocks;
   const int blocks = int(wanted < most ? wanted : most);
-  if (int rc = launch_dependent(kernel, dim3(unsigned(blocks)), kWarps * 32, StreamLayout<D>::bytes(a.batch), stream, map_k, map_v, p,
+  if (int rc = launch_dependent(kernel, dim3(unsigned(blocks)), kWarps * 32, StreamLayout<D, NT>::bytes(a.batch), stream, map_k, map_v, p,
                                 ctx->status_dev)) {
     return rc;
   }
@@ -671,7 +678,7 @@ int64_t warp_rows(int64_t d, int64_t few) { return few <= 8 ? 8 : few <= 16 || d
 int64_t row_blocks(int64_t d, int64_t few) { return (few + warp_rows(d, few) - 1) / warp_rows(d, few); }
 
 int64_t stream_workspace(int64_t batch, int64_t kv_heads, int64_t d, int64_t few) {
-  const int64_t warps = int64_t(kMaxBlocks) * kWarps, sharers = kv_heads * row_blocks(d, few);
+  const int64_t warps = int64_t(kMaxBlocks) * kMaxWarps, sharers = kv_heads * row_blocks(d, few);
   const int64_t units = warps > sharers ? warps : sharers;
   return pieces_bytes(batch) + 2 * units * warp_rows(d, few) * (d + 4) * 4;
 }
