@@ -791,7 +791,7 @@ extern "C" int krn_b200_cache_attn(int type, const void* q, const void* k_pages,
   p.page_shift = 0;
   while ((int64_t(1) << p.page_shift) < page_size) ++p.page_shift;
   p.num_pages = int(num_pages);
-  p.max_new = int(max_new);
+  p.max_new = int(max_new < rows ? max_new : rows);  // no request has more rows than there are
   p.max_context = int(max_context);
   p.scale_log2 = scale_log2;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_handle);

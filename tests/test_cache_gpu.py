@@ -505,6 +505,53 @@ def test_pools_beyond_four_gigabytes(cuda) -> None:
         assert torch.equal(a, b)
 
 
+def test_attention_of_more_heads_than_warps(cuda) -> None:
+    """More kv heads than the grid has warps: each takes several in turn."""
+    rng = np.random.default_rng(48)
+    check_attention(cuda, attention_case(cuda, rng, "bfloat16", [40], [1], 16, 1300, 1, 64))
+    check_attention(cuda, attention_case(cuda, rng, "float16", [33, 5], [2, 1], 32, 1200, 2, 64))
+
+
+@pytest.mark.parametrize("batch,new,group", [(1500, 1, 2), (700, 12, 4)])
+def test_attention_of_many_requests(cuda, batch, new, group) -> None:
+    """More requests than a block has threads, some without rows, some without keys."""
+    rng = np.random.default_rng(49)
+    rows = rng.integers(0, new + 1, batch)
+    context = np.where(rng.random(batch) < 0.1, 0, rng.integers(0, 70, batch))
+    check_attention(cuda, attention_case(cuda, rng, "bfloat16", context, rows, 16, 1, group, 64), max_new=new)
+
+
+def test_attention_announced_larger_than_it_is(cuda) -> None:
+    """`max_new` and `max_context` only bound: any that hold give the same numbers within the kernels' roundings."""
+    rng = np.random.default_rng(50)
+    case = attention_case(cuda, rng, "bfloat16", [100, 37, 260], [2, 1, 5], 32, 2, 4, 128)
+    for max_new in (5, 8, 9, 1000, 2 ** 40):
+        check_attention(cuda, case, max_new=max_new)
+    check_attention(cuda, case, max_context=260)
+
+
+def test_device_tensors_and_streams_of_the_package(cuda) -> None:
+    """The package's own tensors and streams in place of torch's."""
+    import krn_b200
+    from krn_b200.runtime.device import DeviceTensor
+
+    torch, rng = cuda, np.random.default_rng(51)
+    case = attention_case(torch, rng, "bfloat16", [100, 37], [1, 3], 32, 2, 4, 128)
+    want = run_attention(torch, case)
+    cache = ops.PagedCache(*(DeviceTensor(torch.from_numpy(x).cuda()) for x in (*case["codes"], *case["scales"])))
+    table, context, start = (DeviceTensor(torch.from_numpy(case[x]).cuda()) for x in ("table", "context", "start"))
+    out = DeviceTensor(torch.full_like(case["q"], 7.0))
+    longest = case["table"].shape[1] * 32
+    workspace = DeviceTensor(torch.empty(ops.cache_attention_workspace(2, case["q"].shape[0], 8, 2, 128, max_new=3, max_context=longest),
+                                         dtype=torch.uint8, device="cuda"))
+    stream = krn_b200.host.Device.current().default_stream
+    torch.cuda.synchronize()
+    assert ops.cache_attention(DeviceTensor(case["q"]), cache, table, context, start, out, max_new=3, max_context=longest,
+                               workspace=workspace, stream=stream) is out
+    stream.record().wait(60)
+    assert torch.equal(out.data, want)
+
+
 def test_attention_of_strided_tensors(cuda) -> None:
     """q cut from a fused projection, out head by head, pools as halves of one head-major allocation, a table with a pitch."""
     torch, rng = cuda, np.random.default_rng(39)
