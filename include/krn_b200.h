@@ -331,7 +331,9 @@ int64_t krn_b200_cache_attn_workspace_bytes(int64_t batch, int64_t rows, int64_t
  *   max_new      no request has more rows than this; one that has is not computed and reported
  *                (KRN_B200_ERR_DEVICE_INDEX). It chooses the kernels, as max_context does
  *   page ids outside [0, num_pages) are never fetched: their tokens read as zeros, and the status word reports
- *                KRN_B200_ERR_DEVICE_INDEX; entries past a request's context are never looked at
+ *                KRN_B200_ERR_DEVICE_INDEX; entries past a request's context are never looked at, and what pages hold
+ *                behind it (NaN codes, infinite scales) reaches nothing. A NaN code among a request's own values may reach
+ *                rows of the request that do not see it yet, as a weight of 0 times it does
  *   scales       are not negative
  *   strides      HOST array of 10 element strides: rows and heads of q, rows and heads of o (multiples of 8), then pages,
  *                tokens and heads of the K pool and of the V pool (multiples of 16)
