@@ -319,7 +319,8 @@ int krn_b200_cache_append(int type, const void* k, const void* v, const int64_t*
                           void* v_pages, float* k_scale, float* v_scale, int64_t rows, int64_t runs_len, int64_t kv_heads,
                           int64_t d, int64_t page_size, int64_t num_pages, const int64_t* strides, void* stream);
 
-/* Bytes of caller workspace krn_b200_cache_attn needs for these extents. */
+/* Bytes of caller workspace krn_b200_cache_attn needs for these extents, and for all calls with fewer requests, rows, new
+ * tokens or context and the same heads. */
 int64_t krn_b200_cache_attn_workspace_bytes(int64_t batch, int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t d,
                                             int64_t max_new, int64_t max_context);
 
@@ -328,7 +329,8 @@ int64_t krn_b200_cache_attn_workspace_bytes(int64_t batch, int64_t rows, int64_t
  *   q, o         bf16 or f16 (`type`) [rows, q_heads, d]; q_heads % kv_heads == 0, at most 128 q heads per kv head
  *   row_start    int32 [batch + 1], context_len int32 [batch]: as krn_b200_cache_plan makes them. Contexts are clamped into
  *                [0, max_context]; rows of o behind row_start[batch] are left as they were; a row that sees no key gets zeros
- *   max_new      no request has more rows than this; one that has is not computed and reported
+ *   max_new      no request has more rows than this; one that has, or whose rows are not all among q's, is not computed
+ *                and reported
  *                (KRN_B200_ERR_DEVICE_INDEX). It chooses the kernels, as max_context does
  *   page ids outside [0, num_pages) are never fetched: their tokens read as zeros, and the status word reports
  *                KRN_B200_ERR_DEVICE_INDEX; entries past a request's context are never looked at, and what pages hold

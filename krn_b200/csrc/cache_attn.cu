@@ -203,8 +203,7 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       const int first = tiles[b], last = tiles[b + 1] - 1;
       const int p0 = last >= first ? stretch_of(first, parts, total) : 0, p1 = last >= first ? stretch_of(last, parts, total) : 0;
       p.pieces[b] = make_int4(p0, p1, first > first_tile(p0, parts, total) ? 1 : 0, 0);
-      const int n = a.row_start[b + 1] - a.row_start[b];
-      if (n > a.max_new) report_failure(status, kErrDeviceIndex, kSiteRows, uint32_t(n));
+      report_rows(a, b, status);
     }
   }
   if (total == 0) {
@@ -677,7 +676,9 @@ int64_t warp_rows(int64_t d, int64_t few) { return few <= 8 ? 8 : few <= 16 || d
 
 int64_t row_blocks(int64_t d, int64_t few) { return (few + warp_rows(d, few) - 1) / warp_rows(d, few); }
 
-int64_t stream_workspace(int64_t batch, int64_t kv_heads, int64_t d, int64_t few) {
+// Of any smaller call too: `few` is the most rows that a call with up to max_new rows a request streams.
+int64_t stream_workspace(int64_t batch, int64_t kv_heads, int64_t d, int64_t max_new, int64_t group) {
+  const int64_t few = group > 32 ? 0 : max_new * group < 32 ? max_new * group : 32;
   const int64_t warps = int64_t(kMaxBlocks) * kMaxWarps, sharers = kv_heads * row_blocks(d, few);
   const int64_t units = warps > sharers ? warps : sharers;
   return pieces_bytes(batch) + 2 * units * warp_rows(d, few) * (d + 4) * 4;
@@ -699,9 +700,8 @@ extern "C" int64_t krn_b200_cache_attn_workspace_bytes(int64_t batch, int64_t ro
                                                        int64_t max_new, int64_t max_context) {
   using namespace krnb;
   if (batch <= 0 || rows <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0 || d <= 0 || max_new <= 0) return 16;
-  const int64_t few = few_rows(max_new, q_heads / kv_heads);
-  return stream_workspace(batch, kv_heads, d, few) +
-         (max_new * (q_heads / kv_heads) <= few ? 0 : tile_workspace(batch, rows, q_heads, kv_heads, d, few, max_context));
+  const int64_t group = q_heads / kv_heads, most = max_new < rows ? max_new : rows;  // no request has more rows than there are
+  return stream_workspace(batch, kv_heads, d, most, group) + (most * group <= 32 ? 0 : tile_workspace(rows, q_heads, d, max_context));
 }
 
 extern "C" int krn_b200_cache_attn(int type, const void* q, const void* k_pages, const void* v_pages, const float* k_scale,
@@ -791,21 +791,21 @@ extern "C" int krn_b200_cache_attn(int type, const void* q, const void* k_pages,
   p.page_shift = 0;
   while ((int64_t(1) << p.page_shift) < page_size) ++p.page_shift;
   p.num_pages = int(num_pages);
-  p.max_new = int(max_new < rows ? max_new : rows);  // no request has more rows than there are
+  p.max_new = int(max_new < rows ? max_new : rows);
   p.max_context = int(max_context);
   p.scale_log2 = scale_log2;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_handle);
   const bool bf16 = type == KRN_B200_BF16;
   StreamParams sp;
-  p.few = int(few_rows(max_new, p.group));
+  p.few = int(few_rows(p.max_new, p.group));
   sp.a = p;
   sp.pieces = static_cast<int4*>(workspace);
   sp.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + pieces_bytes(batch));
   sp.row_blocks = int(row_blocks(d, p.few));
   // The two paths run side by side: the tile kernel first, whose blocks take longest, and the stream on the SMs that it
   // leaves free.
-  const bool tiled = max_new * p.group > p.few && tile_blocks(batch, rows, p.group, p.few) > 0;
-  float* shares = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + stream_workspace(batch, kv_heads, d, p.few));
+  const bool tiled = int64_t(p.max_new) * p.group > p.few && tile_blocks(batch, rows, p.group, p.few) > 0;
+  float* shares = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + stream_workspace(batch, kv_heads, d, p.max_new, p.group));
   if (tiled) {
     if (int rc = launch_tiles(ctx, p, bf16, d, page_size, shares, stream)) return rc;
   }

@@ -44,9 +44,16 @@ __device__ __forceinline__ RowAt row_at(const CacheAttnParams& a, int row) {
   return {token, row - token * a.group};
 }
 
-// Whether request b's n rows can be computed: some, no more than announced, and beginning within q.
+// Whether request b's n rows can be computed: some, no more than announced, and all of them rows of q.
 __device__ __forceinline__ bool rows_ok(const CacheAttnParams& a, int b, int n) {
-  return n > 0 && n <= a.max_new && uint32_t(a.row_start[b]) <= uint32_t(a.rows);
+  const int first = a.row_start[b];
+  return n > 0 && n <= a.max_new && first >= 0 && first <= a.rows - n;
+}
+
+// Requests that have rows and cannot be computed are left out and reported.
+__device__ __forceinline__ void report_rows(const CacheAttnParams& a, int b, DeviceStatus* status) {
+  const int n = a.row_start[b + 1] - a.row_start[b];
+  if (n > 0 && !rows_ok(a, b, n)) report_failure(status, kErrDeviceIndex, kSiteRows, uint32_t(n));
 }
 
 template <bool BF16>
@@ -77,7 +84,7 @@ inline int encode_pool(CUtensorMap* map, const PoolSide& side, int64_t d, int64_
 // Requests with many rows (cache_attn_tile.cu). `partial` holds tile_workspace() bytes. tile_blocks() bounds the blocks of
 // query rows that they can have: with none there is nothing to launch.
 int64_t tile_blocks(int64_t batch, int64_t rows, int64_t group, int64_t few);
-int64_t tile_workspace(int64_t batch, int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t d, int64_t few, int64_t max_context);
+int64_t tile_workspace(int64_t rows, int64_t q_heads, int64_t d, int64_t max_context);
 int launch_tiles(const DeviceContext* ctx, const CacheAttnParams& a, bool bf16, int64_t d, int64_t page_size, float* partial,
                  cudaStream_t stream);
 // Joins what launch_tiles() split over the keys, behind the kernels that were launched since.

@@ -179,9 +179,7 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   for (int first = 0; first < a.batch; first += kThreads) {
     const int b = first + int(threadIdx.x);
     const int own = b < a.batch ? blocks_of(p, b) : 0;
-    if (blockIdx.x == 0 && blockIdx.y == 0 && b < a.batch && a.row_start[b + 1] - a.row_start[b] > a.max_new) {
-      report_failure(status, kErrDeviceIndex, kSiteRows, uint32_t(a.row_start[b + 1] - a.row_start[b]));
-    }
+    if (blockIdx.x == 0 && blockIdx.y == 0 && b < a.batch) report_rows(a, b, status);
     int v = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -204,7 +202,7 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       found[1] = own - 1 - (wanted - start);
     }
     carry = total;
-    if (carry > wanted) break;
+    if (carry > wanted && blockIdx.x + blockIdx.y > 0) break;  // the first block looks at every request
   }
   __syncthreads();
   const int b = found[0];
@@ -752,10 +750,12 @@ __global__ void __launch_bounds__(128) cache_tile_join_kernel(TileParams p) {
 }
 
 // Shares of the keys: as many as fill the GPU where there are few blocks, none shorter than four key tiles.
+int64_t most_splits(int64_t max_context) { return (max_context + 4 * kTileKV - 1) / (4 * kTileKV); }
+
 int64_t splits_of(int64_t blocks, int64_t max_context) {
   if (blocks <= 0) return 1;
-  const int64_t room = kSMs / blocks, tiles = (max_context + 4 * kTileKV - 1) / (4 * kTileKV);
-  const int64_t splits = room < tiles ? room : tiles;
+  const int64_t room = kSMs / blocks, most = most_splits(max_context);
+  const int64_t splits = room < most ? room : most;
   return splits < 1 ? 1 : splits;
 }
 
@@ -806,9 +806,12 @@ int64_t tile_blocks(int64_t batch, int64_t rows, int64_t group, int64_t few) {
   return requests > 0 ? rows / tokens + requests : 0;
 }
 
-int64_t tile_workspace(int64_t batch, int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t d, int64_t few, int64_t max_context) {
-  const int64_t splits = splits_of(tile_blocks(batch, rows, q_heads / kv_heads, few) * kv_heads, max_context);
-  return splits > 1 ? splits * rows * q_heads * (d + 4) * 4 : 0;
+// Of any smaller call too: splits * blocks * kv_heads is at most kSMs, and a block has 2 * kTileQ rows at most.
+int64_t tile_workspace(int64_t rows, int64_t q_heads, int64_t d, int64_t max_context) {
+  const int64_t most = most_splits(max_context);
+  if (most <= 1) return 0;
+  const int64_t shares = (most < kSMs ? most : kSMs) * rows * q_heads, bound = int64_t(kSMs) * 2 * kTileQ;
+  return (shares < bound ? shares : bound) * (d + 4) * 4;
 }
 
 int launch_tiles(const DeviceContext* ctx, const CacheAttnParams& a, bool bf16, int64_t d, int64_t page_size, float* partial,

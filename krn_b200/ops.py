@@ -312,7 +312,8 @@ def append_cache(k: Any, v: Any, slot_map: Any, runs: Any, cache: PagedCache, st
 
 def cache_attention_workspace(batch: int, rows: int, q_heads: int, kv_heads: int, d: int, *, max_new: int,
                               max_context: int) -> int:
-    """Bytes of workspace that `cache_attention` needs for these extents."""
+    """Bytes of workspace that `cache_attention` needs for these extents, and for every call with fewer requests, rows, new
+    tokens or context: one workspace of a server's largest step serves all of them, one after the other."""
     return calls.cache_attention_workspace_bytes(batch, rows, q_heads, kv_heads, d, max_new, max_context)
 
 
@@ -321,8 +322,8 @@ def cache_attention(q: Any, cache: PagedCache, page_table: Any, context_len: Any
     """Attention of packed query rows [rows, q heads, d] (bf16 or f16) over the cache: row i of the n rows of request b
     (rows `row_start[b]` to `row_start[b + 1]`) stands at position `context_len[b]` - n + i and sees the keys up to it, its
     own included: one row a request for plain decoding, a few for drafted tokens, many for a prompt or a chunk of one, mixed
-    in one call. `scale` defaults to 1/sqrt(d). `max_new` is the most rows any request has (one with more is not computed
-    and reported), contexts are clamped to `max_context`. Rows that see no key get zeros; rows behind the last request are
+    in one call. `scale` defaults to 1/sqrt(d). `max_new` is the most rows any request has (one with more, or with rows
+    beyond q's, is not computed and reported), contexts are clamped to `max_context`. Rows that see no key get zeros; rows behind the last request are
     left as they were."""
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
     calls.cache_attention(*_all_raw(q, *cache, page_table, context_len, row_start, out), scale * _LOG2_E, max_new, max_context,

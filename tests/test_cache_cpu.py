@@ -194,3 +194,14 @@ def test_layout_checks() -> None:
         at.vector("x", torch.zeros(8, dtype=torch.int64), torch.int32, -1)
     with pytest.raises(ValueError, match="must be a CUDA tensor"):
         at.addresses("a b", (torch.zeros(2, device="meta"), object()))
+
+
+def test_workspace_of_the_largest_step_serves_all() -> None:
+    rng = np.random.default_rng(52)
+    for _ in range(2000):
+        heads, group, d = (int(rng.choice(x)) for x in ((1, 2, 8, 500), (1, 2, 4, 7, 8, 12, 33, 128), (64, 128)))
+        largest = [int(2 ** rng.uniform(0, top)) for top in (9, 15, 14, 18)]  # requests, rows, new tokens, context
+        smaller = [int(rng.integers(1, x + 1)) if rng.random() < 0.7 else x for x in largest]
+        sizes = [ops.cache_attention_workspace(batch, rows, heads * group, heads, d, max_new=new, max_context=context)
+                 for batch, rows, new, context in (largest, smaller)]
+        assert sizes[0] >= sizes[1], (heads, group, d, largest, smaller)

@@ -432,6 +432,31 @@ def test_attention_reports_more_rows_than_announced(cuda) -> None:
         assert bool((out[: announced + 1] == 7).all()) and not bool((out[announced + 1] == 7).any())
 
 
+@pytest.mark.parametrize("new,group", [(3, 4), (40, 4), (40, 1), (5, 40)])
+def test_attention_refuses_rows_that_q_does_not_have(cuda, new, group) -> None:
+    """A request whose rows reach behind q's last one is left out whole and reported; the others are computed."""
+    rng = np.random.default_rng(53)
+    case = attention_case(cuda, rng, "bfloat16", [100, 90], [2, new], 16, 1, group, 128)
+    whole = run_attention(cuda, case, max_new=new)
+    for missing in (1, new - 1):
+        out = run_attention(cuda, dict(case, q=case["q"][: 2 + new - missing].contiguous()), max_new=new)
+        assert native.device_status()[:2] == (native.ERR_DEVICE_INDEX, 52)
+        assert bool((out[2:] == 7).all()) and not bool((out[:2] == 7).all(-1).any())
+        # fewer rows may choose other kernels: each rounds its result by 2^-8 of it, and weights, values and scales to f16 (four
+        # times 2^-11 of the largest value)
+        assert cuda.allclose(out[:2].float(), whole[:2].float(), rtol=2 ** -7, atol=2 ** -8 * 448 * float(case["scales"][1].max()))
+
+
+def test_bad_rows_of_late_requests_are_reported(cuda) -> None:
+    """Requests behind those that the first block of a grid belongs to."""
+    rng = np.random.default_rng(54)
+    case = attention_case(cuda, rng, "bfloat16", [20] * 1200, [1] * 1199 + [2], 16, 1, 40, 64)
+    out = run_attention(cuda, case, max_new=1)
+    assert native.device_status()[:2] == (native.ERR_DEVICE_INDEX, 52)
+    # whole rows: one of three million results may well round to 7
+    assert bool((out[1199:] == 7).all()) and not bool((out[:1199] == 7).all(-1).any())
+
+
 @pytest.mark.parametrize("new", [1, 64])
 def test_attention_with_scales_far_apart(cuda, new) -> None:
     """Page scales from 2^-12 to 2^12 for both pools, and sharp softmaxes that settle on single keys."""
