@@ -109,7 +109,7 @@ __device__ __forceinline__ int last_at_or_before(const uint32_t* prefix, int bat
 
 // One launch, no communication between blocks: every block scans all request lengths by itself (a few loads per thread)
 // and then fills its own part of the slot map, the run list and the table. Bound by latency: launch, one pass over the
-// lengths, a binary search per row.
+// lengths, a binary search per row: 3.8 us for 16 requests, 6.7 us for 1000 with 41 000 new rows and 40 finished ones.
 __global__ void __launch_bounds__(kPlanThreads) cache_plan_kernel(PlanParams p, DeviceStatus* status) {
   extern __shared__ uint32_t plan_smem[];
   uint32_t* start = plan_smem;                 // [batch + 1] first row of each request
@@ -276,8 +276,9 @@ __device__ __forceinline__ uint32_t rescale_two(uint32_t codes, float ratio) {
 //      e4m3's normal range is rounded again);
 //   4. the rows go out as codes, 8 bytes a thread. Multiplying by the reciprocal of a power of two is the division itself;
 //      a page that some other program filled may have any scale, and is divided by.
-// The rows are under way before the slots that they go to are known. Bound by HBM for prompts (2 bytes in, 1 out per value)
-// and by launch and load latency for single tokens.
+// The rows are under way before the slots that they go to are known. Bound by HBM for prompts (2 bytes in, 1 out per value):
+// 16384 rows of 8 heads of 128, K and V, in pages of 64: 101 MB in 21.6 us = 4.7 TB/s; by launch and load latency for single
+// tokens (64 of them: 2.4 us).
 constexpr int kHeld = 8;
 
 template <int D, bool BF16, int Threads>
@@ -546,8 +547,15 @@ extern "C" int krn_b200_cache_append(int type, const void* k, const void* v, con
   p.num_pages = int(num_pages);
   cudaStream_t stream = static_cast<cudaStream_t>(stream_handle);
   const bool bf16 = type == KRN_B200_BF16;
-  // a warp per (run, head) where runs hold a few rows, a block where they are whole pages
-  if (rows < 4 * runs_len) {
+  // A warp per (run, head, side) or a block? The run list is padded, and a block costs as much for an empty entry as for a
+  // full one; a warp is slow at runs that its registers (16 rows of 128) do not hold. Where all blocks are resident at once
+  // a block pays from 6 rows an entry: 20 requests of 16 / 24 / 64 rows, 8 heads of 128, pages of 64: warp 2.6 / 3.5 / 7.0 us,
+  // block 2.6 / 2.7 / 3.0. Where they are not, from 16 rows an entry in pages that hold more than 32: 200 requests of
+  // 16 / 40 / 64 rows: warp 5.3 / 16.3 / 22.3, block 12.0 / 18.1 / 22.1; 8 of 2048 in pages of 16 / 32 / 64: warp
+  // 19.9 / 25.1 / 34.8, block 40.5 / 25.3 / 21.6.
+  const bool resident = runs_len * 2 * heads <= 8 * int64_t(ctx->sm_count);
+  const bool block = resident ? page_size > 16 && rows > 6 * runs_len : page_size > 32 && rows > 16 * runs_len;
+  if (!block) {
     if (d == 128) return bf16 ? launch_append<128, true, 32>(p, ctx->status_dev, stream) : launch_append<128, false, 32>(p, ctx->status_dev, stream);
     return bf16 ? launch_append<64, true, 32>(p, ctx->status_dev, stream) : launch_append<64, false, 32>(p, ctx->status_dev, stream);
   }

@@ -24,9 +24,11 @@
 // exponentials are done, and each tile finds its next scores ready when it has handed over its weights. Two warps issue,
 // because one sets the pace: it spends over a hundred cycles on each wait and about 80 on each product, 2030 cycles a query
 // and key tile in a trace, of which the tensor cores work 1024.
+//
+// Bound by the exponentials (128 a row and key tile: 2048 cycles for both query tiles) and by what surrounds them in the chain
+// of a query tile, 3170 cycles a step; a prompt of 8192 tokens, 8 kv heads of 128, group 4: 500 to 530 us = 1040 TFLOP/s under
+// the power limit. Two threads a query row (16 softmax warps of 104 registers): the same time.
 #include "cache_attn.cuh"
-
-#include <cmath>
 
 namespace krnb {
 namespace {
@@ -749,7 +751,9 @@ __global__ void __launch_bounds__(128) cache_tile_join_kernel(TileParams p) {
   }
 }
 
-// Shares of the keys: as many as fill the GPU where there are few blocks, none shorter than four key tiles.
+// Shares of the keys: as many as fill the GPU where there are few blocks, none shorter than four key tiles. One request of 40
+// new tokens, 4 kv heads of 128, over 2000 / 8000 / 60000 tokens: 24.7 / 34 / 81 us, 42 / 138 / 968 with one share; 512 new
+// tokens over 8000 / 60000: 50 / 221, 110 / 765 with one.
 int64_t most_splits(int64_t max_context) { return (max_context + 4 * kTileKV - 1) / (4 * kTileKV); }
 
 int64_t splits_of(int64_t blocks, int64_t max_context) {
@@ -787,7 +791,8 @@ int launch(const DeviceContext* ctx, const TileParams& p, int64_t page_size, int
                           p, ctx->status_dev);
 }
 
-// A key tile has two scales at most where pages are 64 tokens or more, up to eight where they are smaller.
+// A key tile has two scales at most where pages are 64 tokens or more, up to eight where they are smaller. Eight would do for
+// both: 178 us against 174 for four prompts of 2048 tokens, 8 kv heads of 128, group 4, within 2 % elsewhere.
 template <int D, bool BF16>
 int launch_pages(const DeviceContext* ctx, const TileParams& p, int64_t page_size, int64_t blocks, cudaStream_t stream) {
   return page_size >= 64 ? launch<D, BF16, 2>(ctx, p, page_size, blocks, stream) : launch<D, BF16, 8>(ctx, p, page_size, blocks, stream);
