@@ -25,7 +25,7 @@ struct StreamParams {
   int4* pieces;      // [batch] first and last stretch of each request, whether its first piece is a warp's second; for the join
   float* partial;
   int row_blocks;    // warps that share a stretch and kv head, each with its own NT * 8 rows of every request
-  int beside;        // launched beside the tile kernel, which waited for what came before: wait for it at the end
+  int beside;        // launched beside the tile kernel, which waited for what came before
 };
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -207,8 +207,12 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       report_rows(a, b, status);
     }
   }
+  // Beside the tile kernel this grid must not end before it, which one block sees to: the others leave their SMs to the next.
+  const auto leave = [&] {
+    if (blockIdx.x + 1 == gridDim.x) wait_for_kernel_before();
+  };
   if (total == 0) {
-    wait_for_kernel_before();
+    leave();
     return;
   }
 
@@ -540,7 +544,7 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   if (!ok) {  // let this warp's own copies land before the block's memory goes
     for (int i = 0; i < 1000; ++i) __nanosleep(1000);
   }
-  wait_for_kernel_before();
+  leave();
 }
 
 // Joins the pieces of split segments,
