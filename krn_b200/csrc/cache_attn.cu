@@ -17,7 +17,6 @@ constexpr int kMaxWarps = 12;      // of a block
 constexpr int kMaxBlocks = 160;    // bounds the workspace; a B200 has 148 SMs
 constexpr int kMaxBatch = 8192;    // tile counts of the batch sit in shared memory
 constexpr float kLeastScale = 0x1p-110f;  // value scales below it are held against it
-constexpr float kNone = -3.0e38f;         // reference maximum of a row that has seen no key
 
 // Partial results of the pieces of split segments, d + 4 floats (m, l, two unused, the unnormalised output) for each row.
 struct StreamParams {
@@ -26,6 +25,7 @@ struct StreamParams {
   float* partial;
   int row_blocks;    // warps that share a stretch and kv head, each with its own NT * 8 rows of every request
   int beside;        // launched beside the tile kernel, which waited for what came before
+  TileShares tiles;  // what the tile kernel may have split, for the join
 };
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -556,7 +556,7 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 constexpr int kJoinThreads = 256;
 
 template <int D, bool BF16>
-__global__ void __launch_bounds__(kJoinThreads) cache_join_kernel(StreamParams p, int slot_rows, int slots) {
+__device__ __forceinline__ void join_pieces(const StreamParams& p, int slot_rows, int slots) {
   constexpr int kLanes = D / 4, kGroups = kJoinThreads / kLanes;
   __shared__ float4 shared_acc[kGroups][kLanes];
   __shared__ float2 shared_ml[kGroups];
@@ -564,7 +564,6 @@ __global__ void __launch_bounds__(kJoinThreads) cache_join_kernel(StreamParams p
   const int b = blockIdx.x / a.kv_heads, g = blockIdx.x % a.kv_heads;
   const int group = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
   const int row = blockIdx.y * slots + group % slots, share = group / slots, shares = kGroups / slots;
-  wait_for_kernel_before();
   const int row0 = a.row_start[b], rows = (a.row_start[b + 1] - row0) * a.group;
   const RowAt where = row_at(a, row);
   const int at = row0 + where.token;
@@ -630,6 +629,14 @@ __global__ void __launch_bounds__(kJoinThreads) cache_join_kernel(StreamParams p
   *reinterpret_cast<uint2*>(a.o + (long long)at * a.o_row + (long long)(g * a.group + where.head) * a.o_head + lane * 4) = w;
 }
 
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kJoinThreads) cache_join_kernel(StreamParams p, int slot_rows, int slots) {
+  wait_for_kernel_before();
+  const int2 split = p.tiles.header != nullptr ? p.tiles.header->split : make_int2(1, 0);
+  if (int(blockIdx.y) * slots < p.a.few) join_pieces<D, BF16>(p, slot_rows, slots);
+  join_shares<D, BF16>(p.a, p.tiles, split, blockIdx.y * gridDim.x + blockIdx.x, gridDim.x * gridDim.y);
+}
+
 template <int D, bool BF16, int NT>
 int launch_stream(const DeviceContext* ctx, const StreamParams& p, int64_t page_size, cudaStream_t stream) {
   const CacheAttnParams& a = p.a;
@@ -663,8 +670,10 @@ int launch_stream(const DeviceContext* ctx, const StreamParams& p, int64_t page_
   const int64_t pieces = int64_t(blocks) * kWarps / sharers / a.batch + 2;
   int slots = kGroups;
   while (slots > 1 && (slots / 2 >= a.few || pieces > 8 * (kGroups / slots))) slots /= 2;
-  const dim3 grid(unsigned(a.batch) * unsigned(a.kv_heads), unsigned((a.few + slots - 1) / slots));
-  return launch_dependent(cache_join_kernel<D, BF16>, grid, kJoinThreads, 0, stream, p, NT * 8, slots);
+  unsigned depth = unsigned((a.few + slots - 1) / slots);
+  const unsigned width = unsigned(a.batch) * unsigned(a.kv_heads);
+  if (p.tiles.header != nullptr && width * depth < 3 * kSMs) depth = (3 * kSMs + width - 1) / width;  // blocks for what was split
+  return launch_dependent(cache_join_kernel<D, BF16>, dim3(width, depth), kJoinThreads, 0, stream, p, NT * 8, slots);
 }
 
 // Rows of a streamed request: all of them where every request has few; where some have many, those with one new token
@@ -710,7 +719,8 @@ extern "C" int64_t krn_b200_cache_attn_workspace_bytes(int64_t batch, int64_t ro
   using namespace krnb;
   if (batch <= 0 || rows <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0 || d <= 0 || max_new <= 0) return 16;
   const int64_t group = q_heads / kv_heads, most = max_new < rows ? max_new : rows;  // no request has more rows than there are
-  return stream_workspace(batch, kv_heads, d, most, group) + (most * group <= 32 ? 0 : tile_workspace(rows, q_heads, d, max_context));
+  return stream_workspace(batch, kv_heads, d, most, group) +
+         (most * group <= 32 ? 0 : tile_workspace(batch, rows, q_heads, kv_heads, d, few_rows(most, group), max_context));
 }
 
 extern "C" int krn_b200_cache_attn(int type, const void* q, const void* k_pages, const void* v_pages, const float* k_scale,
@@ -814,16 +824,15 @@ extern "C" int krn_b200_cache_attn(int type, const void* q, const void* k_pages,
   // The two paths run side by side: the tile kernel first, whose blocks take longest, and the stream on the SMs that it
   // leaves free.
   const bool tiled = int64_t(p.max_new) * p.group > p.few && tile_blocks(batch, rows, p.group, p.few) > 0;
-  float* shares = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + stream_workspace(batch, kv_heads, d, p.max_new, p.group));
+  void* split = static_cast<uint8_t*>(workspace) + stream_workspace(batch, kv_heads, d, p.max_new, p.group);
+  sp.tiles = tiled ? tile_shares(p, split) : TileShares{nullptr, nullptr, 0};
   if (tiled) {
-    if (int rc = launch_tiles(ctx, p, bf16, d, page_size, shares, stream)) return rc;
+    if (int rc = launch_tiles(ctx, p, sp.tiles, bf16, d, page_size, stream)) return rc;
   }
   if (p.few > 0) {
     sp.beside = tiled;
-    int rc;
-    if (d == 128) rc = bf16 ? launch_stream_rows<128, true>(ctx, sp, page_size, stream) : launch_stream_rows<128, false>(ctx, sp, page_size, stream);
-    else rc = bf16 ? launch_stream_rows<64, true>(ctx, sp, page_size, stream) : launch_stream_rows<64, false>(ctx, sp, page_size, stream);
-    if (rc) return rc;
+    if (d == 128) return bf16 ? launch_stream_rows<128, true>(ctx, sp, page_size, stream) : launch_stream_rows<128, false>(ctx, sp, page_size, stream);
+    return bf16 ? launch_stream_rows<64, true>(ctx, sp, page_size, stream) : launch_stream_rows<64, false>(ctx, sp, page_size, stream);
   }
-  return tiled ? launch_tile_join(p, bf16, d, shares, stream) : KRN_B200_OK;
+  return tiled ? launch_tile_join(p, sp.tiles, bf16, d, stream) : KRN_B200_OK;
 }

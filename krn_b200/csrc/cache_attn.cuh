@@ -81,13 +81,107 @@ inline int encode_pool(CUtensorMap* map, const PoolSide& side, int64_t d, int64_
   return encode_tensor_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, side.pages, dims, strides, box, swizzle);
 }
 
-// Requests with many rows (cache_attn_tile.cu). `partial` holds tile_workspace() bytes. tile_blocks() bounds the blocks of
-// query rows that they can have: with none there is nothing to launch.
+// ---- requests with many rows (cache_attn_tile.cu)
+
+constexpr int kTileQ = 128;        // rows of a query tile; a block has two
+constexpr int kSMs = 148;          // blocks that run at once: fewer may be split over the keys
+constexpr float kNone = -3.0e38f;  // reference maximum of a row that has seen no key
+
+// What the join has to know of the split blocks.
+struct SplitHeader {
+  int2 split;            // shares of each block's keys, blocks x kv heads
+  int2 block[kSMs / 2];  // request and first token of each
+};
+constexpr int kHeaderBytes = (sizeof(SplitHeader) + 15) / 16 * 16;
+
+struct TileShares {
+  SplitHeader* header;  // null: nothing is split
+  float* partial;       // [shares, blocks, 2 * kTileQ rows, d + 4]: m, l, two unused, the unnormalised output
+  int tokens;           // tokens of a query tile: 128 / group
+};
+
+// kRows rows a warp at a time: their loads hide each other's latency.
+template <int D, bool BF16, int kRows>
+__device__ __forceinline__ void join_rows(const CacheAttnParams& a, const TileShares& p, int shares, int units, int part, int parts) {
+  constexpr int kCols = D / 32, kLanes = 32 / kRows;  // a lane's columns; lanes that look for a row's maximum
+  const int lane = int(lane_id());
+  const long long stride = (long long)units * 2 * kTileQ * (D + 4);
+  for (int i = (part * 8 + int(threadIdx.x >> 5)) * kRows; i < units * 2 * kTileQ; i += parts * 8 * kRows) {
+    const int unit = i / (2 * kTileQ), first = i % (2 * kTileQ);
+    const int2 block = p.header->block[unit];
+    const float* from = p.partial + (long long)i * (D + 4);
+    float high = kNone;
+    for (int s = lane % kLanes; s < shares; s += kLanes) high = fmaxf(high, from[s * stride + lane / kLanes * (D + 4)]);
+#pragma unroll
+    for (int o = 1; o < kLanes; o <<= 1) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
+    float m[kRows], l[kRows], acc[kRows][kCols];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      m[r] = __shfl_sync(0xffffffffu, high, r * kLanes);
+      l[r] = 0.f;
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) acc[r][c] = 0.f;
+    }
+#pragma unroll(8 / kRows)
+    for (int s = 0; s < shares; ++s) {
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        const float* at = from + s * stride + r * (D + 4);
+        const float2 ml = *reinterpret_cast<const float2*>(at);
+        float x[kCols];
+        if constexpr (D == 128) {
+          const float4 v = *reinterpret_cast<const float4*>(at + 4 + lane * 4);
+          x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+        } else {
+          const float2 v = *reinterpret_cast<const float2*>(at + 4 + lane * 2);
+          x[0] = v.x, x[1] = v.y;
+        }
+        const bool seen = ml.y != 0.f;  // some key of this share
+        const float by = ex2_approx(ml.x - m[r]);
+        l[r] += seen ? ml.y * by : 0.f;
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) acc[r][c] += seen ? x[c] * by : 0.f;
+      }
+    }
+    const int row0 = a.row_start[block.x], n = a.row_start[block.x + 1] - row0;
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const RowAt where = row_at(a, (first + r) % kTileQ);
+      const int token = block.y + (first + r) / kTileQ * p.tokens + where.token;
+      if (where.token >= p.tokens || token >= n) continue;  // no row: nothing was written of it
+      const float by = l[r] == 0.f ? 0.f : 1.0f / l[r];
+      uint32_t w[kCols / 2];
+#pragma unroll
+      for (int c = 0; c < kCols / 2; ++c) {
+        const float x = acc[r][2 * c] * by, y = acc[r][2 * c + 1] * by;
+        w[c] = BF16 ? pack_bf16x2(x, y) : pack_f16x2(x, y);
+      }
+      uint16_t* out = a.o + (long long)(row0 + token) * a.o_row + (long long)(unit % a.kv_heads * a.group + where.head) * a.o_head + lane * kCols;
+      if constexpr (D == 128) *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
+      else *reinterpret_cast<uint32_t*>(out) = w[0];
+    }
+  }
+}
+
+// Joins the shares of split blocks, by part `part` of `parts` blocks of 256 threads, `split` being the
+// first two words of the header: a row a warp where there are warps enough
+// (few blocks have many shares), else four. What was not split, and rows behind the last request, are not touched.
+template <int D, bool BF16>
+__device__ __forceinline__ void join_shares(const CacheAttnParams& a, const TileShares& p, int2 split, int part, int parts) {
+  const int shares = split.x, units = split.y;
+  if (shares == 1) return;
+  if (units * 2 * kTileQ <= parts * 8) join_rows<D, BF16, 1>(a, p, shares, units, part, parts);
+  else join_rows<D, BF16, 4>(a, p, shares, units, part, parts);
+}
+
+// tile_blocks() bounds the blocks of query rows: with none there is nothing to launch. `workspace` holds tile_workspace()
+// bytes. The shares of what was split are joined behind the kernels that were launched since, by launch_tile_join() or a
+// kernel that calls join_shares().
 int64_t tile_blocks(int64_t batch, int64_t rows, int64_t group, int64_t few);
-int64_t tile_workspace(int64_t rows, int64_t q_heads, int64_t d, int64_t max_context);
-int launch_tiles(const DeviceContext* ctx, const CacheAttnParams& a, bool bf16, int64_t d, int64_t page_size, float* partial,
+int64_t tile_workspace(int64_t batch, int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t d, int64_t few, int64_t max_context);
+TileShares tile_shares(const CacheAttnParams& a, void* workspace);
+int launch_tiles(const DeviceContext* ctx, const CacheAttnParams& a, const TileShares& shares, bool bf16, int64_t d, int64_t page_size,
                  cudaStream_t stream);
-// Joins what launch_tiles() split over the keys, behind the kernels that were launched since.
-int launch_tile_join(const CacheAttnParams& a, bool bf16, int64_t d, float* partial, cudaStream_t stream);
+int launch_tile_join(const CacheAttnParams& a, const TileShares& shares, bool bf16, int64_t d, cudaStream_t stream);
 
 }  // namespace krnb

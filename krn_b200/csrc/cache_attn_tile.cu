@@ -33,19 +33,18 @@
 namespace krnb {
 namespace {
 
-constexpr int kTileQ = 128;
 constexpr int kTileKV = 128;
 constexpr int kThreads = 512;
 constexpr int kRegsFew = 40, kRegsMany = 216;  // warps 0..7 / 8..15, of the 128 that each thread is launched with
-constexpr int kSMs = 148;                 // blocks that run at once: fewer are split over the keys
+constexpr int kShortest = 4;              // key tiles of a share, at least
+constexpr float kStreamWork = 0.5f;       // a streamed request's 128 keys, in steps of a block: 25 us on all SMs for 36 requests
+                                          // of 4096 tokens and 4 kv heads of 128, at 1.7 us a step
 constexpr float kRescaleThreshold = 8.0f;
-constexpr float kNone = -3.0e38f;         // reference maximum of a row that has seen no key
 
 struct TileParams {
   CacheAttnParams a;
-  float* partial;  // [splits, rows, q_heads, d + 4]: m, l, the unnormalised output
-  int tokens;      // tokens of a query tile: 128 / group
-  int splits;
+  TileShares shares;
+  int room;  // shares that the workspace holds
 };
 
 template <int D, int Parts>
@@ -61,7 +60,7 @@ struct Layout {
   static constexpr int kOffRaw = kOffK + kKStages * kRawBytes;
   static constexpr int kOffHalf = kOffRaw + 2 * kRawBytes;
   static constexpr int kOffTail = kOffHalf + 2 * kHalfBytes;
-  static constexpr int kSmemBytes = kOffTail + 512 + 2 * kTileQ * 4 + 1024;
+  static constexpr int kSmemBytes = kOffTail + 528 + 2 * kTileQ * 4 + 1024;
 };
 
 __device__ __forceinline__ void tie(uint32_t (&r)[32]) {
@@ -111,7 +110,7 @@ __device__ __forceinline__ uint32_t times(uint32_t a, uint32_t b) {  // f16x2
 __device__ __forceinline__ int blocks_of(const TileParams& p, int b) {
   const int n = p.a.row_start[b + 1] - p.a.row_start[b];
   if (!rows_ok(p.a, b, n) || (long long)n * p.a.group <= p.a.few) return 0;
-  return (n + 2 * p.tokens - 1) / (2 * p.tokens);
+  return (n + 2 * p.shares.tokens - 1) / (2 * p.shares.tokens);
 }
 
 // The scales of the 16-token groups of key tiles, one group per lane of 8 (a warp may have two of them). Page ids are fetched two tiles ahead and scales
@@ -162,56 +161,85 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail + 176);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + 180);
   int32_t* found = reinterpret_cast<int32_t*>(tail + 184);  // request, block of it, blocks of it
-  int32_t* sums = reinterpret_cast<int32_t*>(tail + 200);   // [kThreads / 32]
-  float* tops = reinterpret_cast<float*>(tail + 272);       // [kThreads / 32]
-  float* row_scales = reinterpret_cast<float*>(tail + 512); // [2 * kTileQ]
+  int4* sums = reinterpret_cast<int4*>(tail + 208);         // [kThreads / 32]
+  float* tops = reinterpret_cast<float*>(tail + 464);       // [kThreads / 32]
+  float* row_scales = reinterpret_cast<float*>(tail + 528); // [2 * kTileQ]
 
   const int warp = threadIdx.x >> 5;
   const int lane = int(lane_id());
 
   wait_for_kernel_before();
   launch_dependents();  // what comes beside needs what came before
-  // ---- which request: blocks of the batch's requests in order, the last (longest) block of a request first
-  const int g = int(blockIdx.x) % a.kv_heads, wanted = int(blockIdx.x) / a.kv_heads;
+  // ---- the batch's blocks and their work
   if (threadIdx.x == 0) {
     found[0] = -1;
     *abort_flag = 0;
   }
-  int carry = 0;
-  for (int first = 0; first < a.batch; first += kThreads) {
+  int blocks = 0, start = 0, own = 0, longest = 0;
+  float work = 0.f;  // key tiles of this path's blocks, and what the stream has to do in that measure
+  const auto count_blocks = [&](int first) {  // requests first, ..., one a thread: `blocks` goes on, `start` is the request's own
     const int b = first + int(threadIdx.x);
-    const int own = b < a.batch ? blocks_of(p, b) : 0;
-    if (blockIdx.x == 0 && blockIdx.y == 0 && b < a.batch) report_rows(a, b, status);
+    own = b < a.batch ? blocks_of(p, b) : 0;
     int v = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int below = __shfl_up_sync(0xffffffffu, v, o);
       if (lane >= o) v += below;
     }
+    const int steps = b < a.batch ? (max(0, min(a.context_len[b], a.max_context)) + kTileKV - 1) / kTileKV : 0;
+    float mine = own > 0 ? float(own) * float(steps) : kStreamWork * float(steps);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    const int high = __reduce_max_sync(0xffffffffu, own > 0 ? steps : 0);
     __syncthreads();
-    if (lane == 31) sums[warp] = v;
+    if (lane == 31) sums[warp] = make_int4(v, high, __float_as_int(mine), 0);
     __syncthreads();
-    int before = carry, total = carry;
+    start = blocks + v - own;
 #pragma unroll
     for (int w = 0; w < kThreads / 32; ++w) {
-      const int s = sums[w];
-      if (w < warp) before += s;
-      total += s;
+      const int4 s = sums[w];
+      if (w < warp) start += s.x;
+      blocks += s.x;
+      longest = max(longest, s.y);
+      work += __int_as_float(s.z);
     }
-    const int start = before + v - own;
+  };
+  for (int first = 0; first < a.batch; first += kThreads) {
+    count_blocks(first);
+    if (blockIdx.x == 0 && first + int(threadIdx.x) < a.batch) report_rows(a, first + int(threadIdx.x), status);
+  }
+  // ---- shares of the keys: so many that the longest block takes little longer than all work spread over the GPU. The kernel
+  // decides, which knows the lengths: the host's bounds are loose where rows are padded or decode requests are among them.
+  // One request of 40 new tokens, 4 kv heads of 128, over 2000 / 8000 / 60000 tokens: 23 / 26 / 55 us, 42 / 138 / 968 with
+  // one share; 512 new tokens over 8000 / 60000: 51 / 237, 110 / 765 with one; 64 new tokens in 4096 padded rows over 8192
+  // tokens, 8 kv heads: 31, 114 with one; beside 36 decode requests, all over 32768 tokens, 4 kv heads: 351, 452 with one.
+  // With more shares than this, 2 x 512 new tokens beside 36 decode requests over 4096: 73 -> 89 us (nothing runs beside).
+  const int units = blocks * a.kv_heads;
+  const float even = fmaxf(work * float(a.kv_heads) * (1.0f / kSMs), float(kShortest));
+  const int splits = units == 0 ? 1 : max(1, min(p.room / units, int(float(longest) / even + 0.75f)));
+  if (blockIdx.x == 0 && threadIdx.x == 0 && p.shares.header != nullptr) {
+    p.shares.header->split = make_int2(splits, units);
+  }
+  // ---- whose block this is: requests in order, the last (longest) block of a request first
+  if (int(blockIdx.x) >= units * splits) return;  // the whole block: the grid is sized by a bound
+  const int split = int(blockIdx.x) / units, unit = int(blockIdx.x) - split * units;
+  const int g = unit % a.kv_heads, wanted = unit / a.kv_heads;
+  if (a.batch > kThreads) blocks = 0;
+  for (int first = 0; first < a.batch; first += kThreads) {
+    if (a.batch > kThreads) count_blocks(first);
     if (wanted >= start && wanted < start + own) {
-      found[0] = b;
+      found[0] = first + int(threadIdx.x);
       found[1] = own - 1 - (wanted - start);
     }
-    carry = total;
-    if (carry > wanted && blockIdx.x + blockIdx.y > 0) break;  // the first block looks at every request
+    if (blocks > wanted) break;
   }
   __syncthreads();
   const int b = found[0];
-  if (b < 0) return;  // the whole block: the grid is sized by a bound
+  if (b < 0) return;
   const int row0 = a.row_start[b], n = a.row_start[b + 1] - row0;
   const int context = max(0, min(a.context_len[b], a.max_context));
-  const int token0 = found[1] * 2 * p.tokens;  // first token of query tile 0
+  const int token0 = found[1] * 2 * p.shares.tokens;  // first token of query tile 0
+  if (splits > 1 && split == 0 && threadIdx.x == 0) p.shares.header->block[unit] = make_int2(b, token0);
   const int32_t* table = a.page_table + b * a.table_pitch;
   const int pages = (context + (1 << a.page_shift) - 1) >> a.page_shift;
 
@@ -220,12 +248,12 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   int most = 0;
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
-    const int last = min(n, token0 + (t + 1) * p.tokens) - 1;  // last token of the tile
-    const int keys = token0 + t * p.tokens < n ? max(0, min(context, context - n + last + 1)) : 0;
+    const int last = min(n, token0 + (t + 1) * p.shares.tokens) - 1;  // last token of the tile
+    const int keys = token0 + t * p.shares.tokens < n ? max(0, min(context, context - n + last + 1)) : 0;
     counts[t] = (keys + kTileKV - 1) / kTileKV;
     most = max(most, counts[t]);
   }
-  const int j0 = int((long long)most * blockIdx.y / p.splits), j1 = int((long long)most * (blockIdx.y + 1) / p.splits);
+  const int j0 = int((long long)most * split / splits), j1 = int((long long)most * (split + 1) / splits);
   const int n0 = max(0, min(counts[0], j1) - j0), n1 = max(0, min(counts[1], j1) - j0);
   const int count = max(n0, n1);
 
@@ -247,8 +275,8 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   for (int i = 0; i < kQPasses; ++i) {
     const int row = i * kQRows + q_row, in_tile = row % kTileQ;
     const RowAt at = row_at(a, in_tile);
-    const int token = token0 + (row / kTileQ) * p.tokens + at.token;
-    const bool live = at.token < p.tokens && token < n && row0 + token < a.rows;
+    const int token = token0 + (row / kTileQ) * p.shares.tokens + at.token;
+    const bool live = at.token < p.shares.tokens && token < n && row0 + token < a.rows;
     const uint16_t* src = a.q + (long long)(row0 + token) * a.q_row + (long long)(g * a.group + at.head) * a.q_head + q_lane * 8;
     q_words[i] = live ? *reinterpret_cast<const uint4*>(src) : make_uint4(0, 0, 0, 0);
   }
@@ -496,8 +524,8 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     const int nt = t == 0 ? n0 : n1;
     const int row_in_tile = quarter * 32 + lane;
     const RowAt where = row_at(a, row_in_tile);
-    const int token = token0 + t * p.tokens + where.token, head = g * a.group + where.head;
-    const bool live = where.token < p.tokens && token < n && row0 + token < a.rows;
+    const int token = token0 + t * p.shares.tokens + where.token, head = g * a.group + where.head;
+    const bool live = where.token < p.shares.tokens && token < n && row0 + token < a.rows;
     const float row_scale = row_scales[t * kTileQ + row_in_tile];
     const uint32_t lane_base = tmem_base + (uint32_t(quarter * 32) << 16);
     const uint32_t s_tmem = lane_base, p_tmem = lane_base + 128 + t * 64;
@@ -638,8 +666,8 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     if (ok) {
       tc_fence_after();
       const float unit = top * (1.0f / 128.0f);
-      if (p.splits > 1) {
-        float* share = p.partial + (((long long)blockIdx.y * a.rows + row0 + token) * a.q_heads + head) * (D + 4);
+      if (splits > 1) {
+        float* share = p.shares.partial + ((long long)blockIdx.x * 2 * kTileQ + t * kTileQ + row_in_tile) * (D + 4);
         if (live) *reinterpret_cast<float2*>(share) = make_float2(nt > 0 ? m_ref : kNone, l);
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
@@ -712,55 +740,11 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   }
 }
 
-// Joins the splits, a warp per (row, q head). Rows of requests that were streamed, and rows behind the last request, are
-// not touched.
+// Where no stream kernel and no join of its pieces follow.
 template <int D, bool BF16>
-__global__ void __launch_bounds__(128) cache_tile_join_kernel(TileParams p) {
-  constexpr int kCols = D / 32;
-  const CacheAttnParams& a = p.a;
-  const int row = blockIdx.x, head = blockIdx.y * 4 + (threadIdx.x >> 5), lane = int(lane_id());
+__global__ void __launch_bounds__(256) cache_tile_join_kernel(TileParams p) {
   wait_for_kernel_before();
-  if (head >= a.q_heads || row >= a.row_start[a.batch]) return;
-  int low = 0, high = a.batch;  // the last request that starts at or before the row
-  while (high - low > 1) {
-    const int mid = (low + high) >> 1;
-    if (a.row_start[mid] <= row) low = mid; else high = mid;
-  }
-  if (blocks_of(p, low) == 0) return;
-  const float* from = p.partial + ((long long)row * a.q_heads + head) * (D + 4);
-  const long long stride = (long long)a.rows * a.q_heads * (D + 4);
-  float m = kNone, l = 0.f, acc[kCols];
-#pragma unroll
-  for (int c = 0; c < kCols; ++c) acc[c] = 0.f;
-  for (int s = 0; s < p.splits; ++s) {
-    const float2 ml = *reinterpret_cast<const float2*>(from + s * stride);
-    if (ml.y == 0.f) continue;  // no key of this split was seen
-    const float m_new = fmaxf(m, ml.x);
-    const float old = exp2f(m - m_new), now = exp2f(ml.x - m_new);
-    m = m_new;
-    l = l * old + ml.y * now;
-#pragma unroll
-    for (int c = 0; c < kCols; ++c) acc[c] = acc[c] * old + from[s * stride + 4 + c * 32 + lane] * now;
-  }
-  const float by = l == 0.f ? 0.f : 1.0f / l;
-  uint16_t* out = a.o + (long long)row * a.o_row + (long long)head * a.o_head;
-#pragma unroll
-  for (int c = 0; c < kCols; ++c) {
-    const float y = acc[c] * by;
-    out[c * 32 + lane] = uint16_t((BF16 ? pack_bf16x2(y, 0.f) : pack_f16x2(y, 0.f)) & 0xffffu);
-  }
-}
-
-// Shares of the keys: as many as fill the GPU where there are few blocks, none shorter than four key tiles. One request of 40
-// new tokens, 4 kv heads of 128, over 2000 / 8000 / 60000 tokens: 24.7 / 34 / 81 us, 42 / 138 / 968 with one share; 512 new
-// tokens over 8000 / 60000: 50 / 221, 110 / 765 with one.
-int64_t most_splits(int64_t max_context) { return (max_context + 4 * kTileKV - 1) / (4 * kTileKV); }
-
-int64_t splits_of(int64_t blocks, int64_t max_context) {
-  if (blocks <= 0) return 1;
-  const int64_t room = kSMs / blocks, most = most_splits(max_context);
-  const int64_t splits = room < most ? room : most;
-  return splits < 1 ? 1 : splits;
+  join_shares<D, BF16>(p.a, p.shares, p.shares.header->split, blockIdx.x, gridDim.x);
 }
 
 template <int D, bool BF16, int Groups>
@@ -787,7 +771,7 @@ int launch(const DeviceContext* ctx, const TileParams& p, int64_t page_size, int
       })) {
     return rc;
   }
-  return launch_dependent(kernel, dim3(unsigned(blocks * a.kv_heads), unsigned(p.splits)), kThreads, L::kSmemBytes, stream, map_k, map_v,
+  return launch_dependent(kernel, dim3(unsigned(blocks)), kThreads, L::kSmemBytes, stream, map_k, map_v,
                           p, ctx->status_dev);
 }
 
@@ -798,9 +782,8 @@ int launch_pages(const DeviceContext* ctx, const TileParams& p, int64_t page_siz
   return page_size >= 64 ? launch<D, BF16, 2>(ctx, p, page_size, blocks, stream) : launch<D, BF16, 8>(ctx, p, page_size, blocks, stream);
 }
 
-TileParams tile_params(const CacheAttnParams& a, float* partial, int64_t blocks) {
-  return {a, partial, kTileQ / a.group, int(splits_of(blocks * a.kv_heads, a.max_context))};
-}
+// Shares of a block's keys, at most: none is shorter than kShortest key tiles.
+int64_t most_shares(int64_t max_context) { return (max_context + kShortest * kTileKV - 1) / (kShortest * kTileKV); }
 
 }  // namespace
 
@@ -811,29 +794,45 @@ int64_t tile_blocks(int64_t batch, int64_t rows, int64_t group, int64_t few) {
   return requests > 0 ? rows / tokens + requests : 0;
 }
 
-// Of any smaller call too: splits * blocks * kv_heads is at most kSMs, and a block has 2 * kTileQ rows at most.
-int64_t tile_workspace(int64_t rows, int64_t q_heads, int64_t d, int64_t max_context) {
-  const int64_t most = most_splits(max_context);
-  if (most <= 1) return 0;
-  const int64_t shares = (most < kSMs ? most : kSMs) * rows * q_heads, bound = int64_t(kSMs) * 2 * kTileQ;
-  return (shares < bound ? shares : bound) * (d + 4) * 4;
+bool tiles_split(int64_t max_context) { return most_shares(max_context) > 1; }
+
+namespace {
+
+// As many as run at once, at most.
+int64_t share_room(int64_t blocks, int64_t max_context) {
+  const int64_t most = most_shares(max_context);
+  return most <= 1 ? 0 : blocks >= kSMs || most >= kSMs || blocks * most >= kSMs ? kSMs : blocks * most;
 }
 
-int launch_tiles(const DeviceContext* ctx, const CacheAttnParams& a, bool bf16, int64_t d, int64_t page_size, float* partial,
+}  // namespace
+
+TileShares tile_shares(const CacheAttnParams& a, void* workspace) {
+  uint8_t* at = static_cast<uint8_t*>(workspace);
+  return {tiles_split(a.max_context) ? reinterpret_cast<SplitHeader*>(at) : nullptr, reinterpret_cast<float*>(at + kHeaderBytes),
+          kTileQ / a.group};
+}
+
+int64_t tile_workspace(int64_t batch, int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t d, int64_t few, int64_t max_context) {
+  if (!tiles_split(max_context)) return 0;
+  const int64_t blocks = tile_blocks(batch, rows, q_heads / kv_heads, few) * kv_heads;
+  return kHeaderBytes + share_room(blocks, max_context) * 2 * kTileQ * (d + 4) * 4;
+}
+
+int launch_tiles(const DeviceContext* ctx, const CacheAttnParams& a, const TileShares& shares, bool bf16, int64_t d, int64_t page_size,
                  cudaStream_t stream) {
-  const int64_t blocks = tile_blocks(a.batch, a.rows, a.group, a.few);
-  const TileParams p = tile_params(a, partial, blocks);
+  const int64_t bound = tile_blocks(a.batch, a.rows, a.group, a.few) * a.kv_heads, room = share_room(bound, a.max_context);
+  const TileParams p = {a, shares, int(room)};
+  const int64_t blocks = bound < room ? room : bound;
   if (d == 128) return bf16 ? launch_pages<128, true>(ctx, p, page_size, blocks, stream) : launch_pages<128, false>(ctx, p, page_size, blocks, stream);
   return bf16 ? launch_pages<64, true>(ctx, p, page_size, blocks, stream) : launch_pages<64, false>(ctx, p, page_size, blocks, stream);
 }
 
-int launch_tile_join(const CacheAttnParams& a, bool bf16, int64_t d, float* partial, cudaStream_t stream) {
-  const int64_t blocks = tile_blocks(a.batch, a.rows, a.group, a.few);
-  const TileParams p = tile_params(a, partial, blocks);
-  if (p.splits == 1) return KRN_B200_OK;
-  const dim3 grid(unsigned(a.rows), unsigned((a.q_heads + 3) / 4));
-  if (d == 128) return launch_dependent(bf16 ? cache_tile_join_kernel<128, true> : cache_tile_join_kernel<128, false>, grid, 128, 0, stream, p);
-  return launch_dependent(bf16 ? cache_tile_join_kernel<64, true> : cache_tile_join_kernel<64, false>, grid, 128, 0, stream, p);
+int launch_tile_join(const CacheAttnParams& a, const TileShares& shares, bool bf16, int64_t d, cudaStream_t stream) {
+  if (shares.header == nullptr) return KRN_B200_OK;
+  const TileParams p = {a, shares, 0};
+  const dim3 grid(3 * kSMs);
+  if (d == 128) return launch_dependent(bf16 ? cache_tile_join_kernel<128, true> : cache_tile_join_kernel<128, false>, grid, 256, 0, stream, p);
+  return launch_dependent(bf16 ? cache_tile_join_kernel<64, true> : cache_tile_join_kernel<64, false>, grid, 256, 0, stream, p);
 }
 
 }  // namespace krnb

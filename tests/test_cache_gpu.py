@@ -546,6 +546,18 @@ def test_attention_of_many_requests(cuda, batch, new, group) -> None:
     check_attention(cuda, attention_case(cuda, rng, "bfloat16", context, rows, 16, 1, group, 64), max_new=new)
 
 
+@pytest.mark.parametrize("batch,at,dtype,d,page", [(21, 20, "bfloat16", 128, 32), (4, 0, "float16", 128, 64), (700, 600, "bfloat16", 64, 16)])
+def test_attention_of_a_chunk_among_decode_requests(cuda, batch, at, dtype, d, page) -> None:
+    """One long request's keys are split over the blocks that the others leave, whatever the rows and requests would allow."""
+    rng = np.random.default_rng(55)
+    context, rows = rng.integers(1, 100, batch), np.ones(batch, int)
+    context[at], rows[at] = 2900, 150
+    rows[(at + 1) % batch], context[(at + 1) % batch] = 20, 700
+    case = attention_case(cuda, rng, dtype, context, rows, page, 2, 4, d, padding=400)
+    check_attention(cuda, case, max_new=200)
+    check_attention(cuda, case, max_new=200, max_context=case["table"].shape[1] * page - 3)
+
+
 def test_attention_announced_larger_than_it_is(cuda) -> None:
     """`max_new` and `max_context` only bound: any that hold give the same numbers within the kernels' roundings."""
     rng = np.random.default_rng(50)
