@@ -215,6 +215,14 @@ def test_append_against_reference(cuda, dtype, d, page, heads, context, new) -> 
     check_append(cuda, rng, dtype, np.array(context), np.array(new), page, heads, d, padding=len(new) - 1)
 
 
+@pytest.mark.parametrize("dtype,d", [("bfloat16", 128), ("float16", 64)])
+@pytest.mark.parametrize("batch,most,page", [(40, 64, 64), (25, 300, 64), (30, 200, 32), (12, 700, 256)])
+def test_append_of_many_runs_of_all_lengths(cuda, dtype, d, batch, most, page) -> None:
+    """More runs than the GPU holds blocks, short and longer than a warp or a block keeps in registers."""
+    rng = np.random.default_rng(56)
+    check_append(cuda, rng, dtype, rng.integers(0, 3 * page, batch), rng.integers(0, most + 1, batch), page, 9, d, padding=33)
+
+
 def test_append_of_many_single_tokens(cuda) -> None:
     rng = np.random.default_rng(20)
     check_append(cuda, rng, "bfloat16", rng.integers(0, 500, 130), np.ones(130, np.int64), 64, 4, 128)
