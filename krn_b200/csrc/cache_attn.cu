@@ -553,11 +553,9 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 // row's pieces, eight of them in flight at a time, and meet in shared memory. Bound by latency: one load of what the stream
 // kernel says about the request, one round of pieces: 4 us after the stream kernel, as whose programmatic dependent it is
 // launched: its blocks are resident when that ends.
-constexpr int kJoinThreads = 256;
-
-template <int D, bool BF16>
+template <int D, bool BF16, int Threads>
 __device__ __forceinline__ void join_pieces(const StreamParams& p, int slot_rows, int slots) {
-  constexpr int kLanes = D / 4, kGroups = kJoinThreads / kLanes;
+  constexpr int kLanes = D / 4, kGroups = Threads / kLanes;
   __shared__ float4 shared_acc[kGroups][kLanes];
   __shared__ float2 shared_ml[kGroups];
   const CacheAttnParams& a = p.a;
@@ -629,11 +627,11 @@ __device__ __forceinline__ void join_pieces(const StreamParams& p, int slot_rows
   *reinterpret_cast<uint2*>(a.o + (long long)at * a.o_row + (long long)(g * a.group + where.head) * a.o_head + lane * 4) = w;
 }
 
-template <int D, bool BF16>
-__global__ void __launch_bounds__(kJoinThreads) cache_join_kernel(StreamParams p, int slot_rows, int slots) {
+template <int D, bool BF16, int Threads>
+__global__ void __launch_bounds__(Threads) cache_join_kernel(StreamParams p, int slot_rows, int slots) {
   wait_for_kernel_before();
   const int2 split = p.tiles.header != nullptr ? p.tiles.header->split : make_int2(1, 0);
-  if (int(blockIdx.y) * slots < p.a.few) join_pieces<D, BF16>(p, slot_rows, slots);
+  if (int(blockIdx.y) * slots < p.a.few) join_pieces<D, BF16, Threads>(p, slot_rows, slots);
   join_shares<D, BF16>(p.a, p.tiles, split, blockIdx.y * gridDim.x + blockIdx.x, gridDim.x * gridDim.y);
 }
 
@@ -666,22 +664,31 @@ int launch_stream(const DeviceContext* ctx, const StreamParams& p, int64_t page_
   // Rows of a block: as many as leave each group of threads no more than eight pieces, as the batch is split on average. One
   // sequence of 60000 tokens: 25.1 us (stream and join) with one row a block, 48.5 with eight; 64 sequences of up to 4 rows
   // over 1024 to 8192 tokens: 83 us with one, 69.6 with eight.
-  constexpr int kGroups = kJoinThreads * 4 / D;
+  constexpr int kGroups = 256 * 4 / D;
   const int64_t pieces = int64_t(blocks) * kWarps / sharers / a.batch + 2;
   int slots = kGroups;
   while (slots > 1 && (slots / 2 >= a.few || pieces > 8 * (kGroups / slots))) slots /= 2;
   unsigned depth = unsigned((a.few + slots - 1) / slots);
   const unsigned width = unsigned(a.batch) * unsigned(a.kv_heads);
   if (p.tiles.header != nullptr && width * depth < 3 * kSMs) depth = (3 * kSMs + width - 1) / width;  // blocks for what was split
-  return launch_dependent(cache_join_kernel<D, BF16>, dim3(width, depth), kJoinThreads, 0, stream, p, NT * 8, slots);
+  const dim3 grid(width, depth);
+  // Many pieces, which takes few sequences, are worth twice the groups: one sequence of 60000 tokens 25.2 -> 20.5 us, eight of
+  // 4096 13.5 -> 12.7; 64 of 8192 would go from 60 to 62. Not where the blocks, one to an SM, come in several waves (four
+  // sequences of 4096 with 32 rows each: 20.7 -> 25.6), nor beside the tile kernel, where the batch is not what these are of.
+  if (!p.beside && pieces > 4 * kGroups && width * depth <= unsigned(ctx->sm_count)) return launch_dependent(cache_join_kernel<D, BF16, 512>, grid, 512, 0, stream, p, NT * 8, slots);
+  return launch_dependent(cache_join_kernel<D, BF16, 256>, grid, 256, 0, stream, p, NT * 8, slots);
 }
 
+// Rows that count as few: 32 of 128 columns, 64 of 64. With 4 kv heads and a group of 4, streamed and tiled: 32 rows of 128
+// columns 12.4 and 21.3 us (1 request of up to 4096 tokens), 44 and 70 (24 of them), 91 and 118 (64), 31 and 44 (1 of 60000);
+// 64 rows: 16.1 and 21.6, 70 and 71, 163 and 119, 49 and 45. 64 rows of 64 columns: 15.2 and 19.4, 45 and 64, 95 and 110, 34
+// and 36.
+int64_t few_limit(int64_t d) { return d == 128 ? 32 : 64; }
+
 // Rows of a streamed request: all of them where every request has few; where some have many, those with one new token
-// (or the few that fit beside it) are streamed and the rest is tiled. Few is 32, with 4 kv heads of 128: 32 rows, streamed and
-// tiled, 14.0 and 24.2 us (1 request of up to 4096 tokens), 44 and 66 (24 of them), 90 and 117 (64), 34 and 69 (1 of 60000);
-// 64 rows: 15.7 and 25.0, 70 and 66, 163 and 117, 48 and 70: the many requests that fill the GPU decide.
-int64_t few_rows(int64_t max_new, int64_t group) {
-  if (max_new * group <= 32) return max_new * group;
+// (or the few that fit beside it) are streamed and the rest is tiled.
+int64_t few_rows(int64_t d, int64_t max_new, int64_t group) {
+  if (max_new * group <= few_limit(d)) return max_new * group;
   return group <= 8 ? 8 : group <= 16 ? 16 : group <= 32 ? 32 : 0;
 }
 
@@ -696,7 +703,7 @@ int64_t row_blocks(int64_t d, int64_t few) { return (few + warp_rows(d, few) - 1
 
 // Of any smaller call too: `few` is the most rows that a call with up to max_new rows a request streams.
 int64_t stream_workspace(int64_t batch, int64_t kv_heads, int64_t d, int64_t max_new, int64_t group) {
-  const int64_t few = group > 32 ? 0 : max_new * group < 32 ? max_new * group : 32;
+  const int64_t limit = few_limit(d), few = group > limit ? 0 : max_new * group < limit ? max_new * group : limit;
   const int64_t warps = int64_t(kMaxBlocks) * kMaxWarps, sharers = kv_heads * row_blocks(d, few);
   const int64_t units = warps > sharers ? warps : sharers;
   return pieces_bytes(batch) + 2 * units * warp_rows(d, few) * (d + 4) * 4;
@@ -720,7 +727,7 @@ extern "C" int64_t krn_b200_cache_attn_workspace_bytes(int64_t batch, int64_t ro
   if (batch <= 0 || rows <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0 || d <= 0 || max_new <= 0) return 16;
   const int64_t group = q_heads / kv_heads, most = max_new < rows ? max_new : rows;  // no request has more rows than there are
   return stream_workspace(batch, kv_heads, d, most, group) +
-         (most * group <= 32 ? 0 : tile_workspace(batch, rows, q_heads, kv_heads, d, few_rows(most, group), max_context));
+         (most * group <= few_limit(d) ? 0 : tile_workspace(batch, rows, q_heads, kv_heads, d, few_rows(d, most, group), max_context));
 }
 
 extern "C" int krn_b200_cache_attn(int type, const void* q, const void* k_pages, const void* v_pages, const float* k_scale,
@@ -816,7 +823,7 @@ extern "C" int krn_b200_cache_attn(int type, const void* q, const void* k_pages,
   cudaStream_t stream = static_cast<cudaStream_t>(stream_handle);
   const bool bf16 = type == KRN_B200_BF16;
   StreamParams sp;
-  p.few = int(few_rows(p.max_new, p.group));
+  p.few = int(few_rows(d, p.max_new, p.group));
   sp.a = p;
   sp.pieces = static_cast<int4*>(workspace);
   sp.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + pieces_bytes(batch));

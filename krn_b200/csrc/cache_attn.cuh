@@ -102,11 +102,11 @@ struct TileShares {
 
 // kRows rows a warp at a time: their loads hide each other's latency.
 template <int D, bool BF16, int kRows>
-__device__ __forceinline__ void join_rows(const CacheAttnParams& a, const TileShares& p, int shares, int units, int part, int parts) {
+__device__ __forceinline__ void join_rows(const CacheAttnParams& a, const TileShares& p, int shares, int units, int warp, int warps) {
   constexpr int kCols = D / 32, kLanes = 32 / kRows;  // a lane's columns; lanes that look for a row's maximum
   const int lane = int(lane_id());
   const long long stride = (long long)units * 2 * kTileQ * (D + 4);
-  for (int i = (part * 8 + int(threadIdx.x >> 5)) * kRows; i < units * 2 * kTileQ; i += parts * 8 * kRows) {
+  for (int i = warp * kRows; i < units * 2 * kTileQ; i += warps * kRows) {
     const int unit = i / (2 * kTileQ), first = i % (2 * kTileQ);
     const int2 block = p.header->block[unit];
     const float* from = p.partial + (long long)i * (D + 4);
@@ -163,15 +163,15 @@ __device__ __forceinline__ void join_rows(const CacheAttnParams& a, const TileSh
   }
 }
 
-// Joins the shares of split blocks, by part `part` of `parts` blocks of 256 threads, `split` being the
-// first two words of the header: a row a warp where there are warps enough
-// (few blocks have many shares), else four. What was not split, and rows behind the last request, are not touched.
+// Joins the shares of split blocks, by block `part` of `parts`, `split` being the first two words of the header: a row a warp
+// where there are warps enough (few blocks have many shares), else four. What was not split, and rows behind the last request, are not touched.
 template <int D, bool BF16>
 __device__ __forceinline__ void join_shares(const CacheAttnParams& a, const TileShares& p, int2 split, int part, int parts) {
   const int shares = split.x, units = split.y;
   if (shares == 1) return;
-  if (units * 2 * kTileQ <= parts * 8) join_rows<D, BF16, 1>(a, p, shares, units, part, parts);
-  else join_rows<D, BF16, 4>(a, p, shares, units, part, parts);
+  const int each = int(blockDim.x) >> 5, warp = part * each + int(threadIdx.x >> 5), warps = parts * each;
+  if (units * 2 * kTileQ <= warps) join_rows<D, BF16, 1>(a, p, shares, units, warp, warps);
+  else join_rows<D, BF16, 4>(a, p, shares, units, warp, warps);
 }
 
 // tile_blocks() bounds the blocks of query rows: with none there is nothing to launch. `workspace` holds tile_workspace()

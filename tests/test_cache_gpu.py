@@ -369,6 +369,15 @@ def test_attention_of_head_groups(cuda, group, new) -> None:
     check_attention(cuda, attention_case(cuda, rng, "bfloat16", [77, 200], [new, 1], 16, 1, group, 128))
 
 
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("new,group,d", [(8, 4, 128), (9, 4, 128), (5, 6, 128), (1, 33, 128), (16, 4, 64), (17, 4, 64), (5, 12, 64),
+                                         (9, 7, 64), (1, 64, 64), (1, 65, 64), (2, 33, 64)])
+def test_attention_at_the_border_of_the_paths(cuda, dtype, new, group, d) -> None:
+    """As many rows a request as are streamed, and the next more."""
+    rng = np.random.default_rng(57)
+    check_attention(cuda, attention_case(cuda, rng, dtype, [new, 300, 0, 1500], [new, new, 1, max(1, new - 1)], 32, 2, group, d), max_new=new)
+
+
 def test_attention_of_a_long_context(cuda) -> None:
     """One request over thousands of keys: the work is split over the keys and joined."""
     rng = np.random.default_rng(31)
