@@ -110,10 +110,10 @@ __device__ __forceinline__ void step(Spot& s, const int32_t* tiles, int batch) {
 // Warps of a block and their rings. Rows of 128 columns: 8 warps with 3 tiles of 8 KB each, 105 us on the 64-sequence mix of
 // 1024 to 8192 tokens (10 warps with 2: 105.4, 12 with 2: 109, 9 with 2: 111). Rows of 64: tiles of 4 KB leave room for 12
 // warps, 30.5 us against 34.5 with 8 (64 sequences of 2048 to 4096 tokens, 4 kv heads; 16 with 3: 29.8, but 19.5 against
-// 17.6 us for one sequence of 60000).
-template <int D, int NT>
+// 17.6 us for one sequence of 60000), with 16 rows a warp 38.9 against 40.6 (11.1 against 9.8 for one request of 4096).
+template <int D>
 struct StreamLayout {
-  static constexpr int kWarps = D == 64 && NT == 1 ? 12 : 8;
+  static constexpr int kWarps = D == 64 ? 12 : 8;
   static constexpr int kStages = 3;                       // tiles a warp has in flight or in work
   static constexpr int kSide = kTile * D;                 // one of K and V, bytes
   static constexpr int kStage = 2 * kSide;
@@ -137,10 +137,10 @@ struct StreamLayout {
 // the workspace and cache_join_kernel joins them. 64 sequences of 1024 to 8192 tokens, 8 kv heads of 128, one new token each:
 // 605 MB in 100 us = 6.06 TB/s.
 template <int D, bool BF16, int NT>
-__global__ void __launch_bounds__(StreamLayout<D, NT>::kWarps * 32, 1)
+__global__ void __launch_bounds__(StreamLayout<D>::kWarps * 32, 1)
 cache_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, StreamParams p,
                     DeviceStatus* status) {
-  using L = StreamLayout<D, NT>;
+  using L = StreamLayout<D>;
   constexpr int kWarps = L::kWarps, kStages = L::kStages;
   constexpr int kSteps = D / 16;       // MMA steps over d
   constexpr int kWords = D / 16;       // 32-bit words of a K row that a thread holds
@@ -646,18 +646,18 @@ int launch_stream(const DeviceContext* ctx, const StreamParams& p, int64_t page_
   auto kernel = cache_stream_kernel<D, BF16, NT>;
   static OncePerDevice ready;
   if (int rc = ready(ctx->device, [&] {
-        KRNB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, StreamLayout<D, NT>::bytes(kMaxBatch)));
+        KRNB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, StreamLayout<D>::bytes(kMaxBatch)));
         return KRN_B200_OK;
       })) {
     return rc;
   }
-  constexpr int kWarps = StreamLayout<D, NT>::kWarps;
+  constexpr int kWarps = StreamLayout<D>::kWarps;
   // no more blocks than the contexts could give warps work
   const int64_t sharers = int64_t(a.kv_heads) * p.row_blocks;
   const int64_t wanted = (int64_t(a.batch) * sharers * ((a.max_context + kTile - 1) / kTile) + kWarps - 1) / kWarps;
   const int most = ctx->sm_count < kMaxBlocks ? ctx->sm_count : kMaxBlocks;
   const int blocks = int(wanted < most ? wanted : most);
-  if (int rc = launch_dependent(kernel, dim3(unsigned(blocks)), kWarps * 32, StreamLayout<D, NT>::bytes(a.batch), stream, map_k, map_v, p,
+  if (int rc = launch_dependent(kernel, dim3(unsigned(blocks)), kWarps * 32, StreamLayout<D>::bytes(a.batch), stream, map_k, map_v, p,
                                 ctx->status_dev)) {
     return rc;
   }
@@ -681,7 +681,7 @@ int launch_stream(const DeviceContext* ctx, const StreamParams& p, int64_t page_
 
 // Rows that count as few: 32 of 128 columns, 64 of 64. With 4 kv heads and a group of 4, streamed and tiled: 32 rows of 128
 // columns 12.4 and 21.3 us (1 request of up to 4096 tokens), 44 and 70 (24 of them), 91 and 118 (64), 31 and 44 (1 of 60000);
-// 64 rows: 16.1 and 21.6, 70 and 71, 163 and 119, 49 and 45. 64 rows of 64 columns: 15.2 and 19.4, 45 and 64, 95 and 110, 34
+// 64 rows: 16.1 and 21.6, 70 and 71, 163 and 119, 49 and 45. 64 rows of 64 columns: 12.1 and 19.4, 47 and 64, 106 and 110, 33
 // and 36.
 int64_t few_limit(int64_t d) { return d == 128 ? 32 : 64; }
 
@@ -694,28 +694,24 @@ int64_t few_rows(int64_t d, int64_t max_new, int64_t group) {
 
 int64_t pieces_bytes(int64_t batch) { return batch * 16; }
 
-// Rows of a warp: 8, 16 or, with rows of 64 columns, 32, as registers hold them (32 rows of 128 columns spilled: 58 us
-// against 44 for two warps of 16 rows each, 24 requests of 8 x 4 rows over 4096 tokens). Where a request may have more,
-// several warps share a stretch.
-int64_t warp_rows(int64_t d, int64_t few) { return few <= 8 ? 8 : few <= 16 || d == 128 ? 16 : 32; }
+// Rows of a warp: 8 or 16, as registers hold them (32 rows of 128 columns spilled: 58 us against 44 for two warps of 16 rows
+// each, 24 requests of 8 x 4 rows over 4096 tokens; 32 of 64 columns leave room for 8 warps a block, not 12: 31.4 us against
+// 30.0, 18.4 against 14.8 with 4 requests, 55 against 60 with 64). Where a request may have more, several warps share a stretch.
+int64_t warp_rows(int64_t few) { return few <= 8 ? 8 : 16; }
 
-int64_t row_blocks(int64_t d, int64_t few) { return (few + warp_rows(d, few) - 1) / warp_rows(d, few); }
+int64_t row_blocks(int64_t few) { return (few + warp_rows(few) - 1) / warp_rows(few); }
 
 // Of any smaller call too: `few` is the most rows that a call with up to max_new rows a request streams.
 int64_t stream_workspace(int64_t batch, int64_t kv_heads, int64_t d, int64_t max_new, int64_t group) {
   const int64_t limit = few_limit(d), few = group > limit ? 0 : max_new * group < limit ? max_new * group : limit;
-  const int64_t warps = int64_t(kMaxBlocks) * kMaxWarps, sharers = kv_heads * row_blocks(d, few);
+  const int64_t warps = int64_t(kMaxBlocks) * kMaxWarps, sharers = kv_heads * row_blocks(few);
   const int64_t units = warps > sharers ? warps : sharers;
-  return pieces_bytes(batch) + 2 * units * warp_rows(d, few) * (d + 4) * 4;
+  return pieces_bytes(batch) + 2 * units * warp_rows(few) * (d + 4) * 4;
 }
 
 template <int D, bool BF16>
 int launch_stream_rows(const DeviceContext* ctx, const StreamParams& p, int64_t page_size, cudaStream_t stream) {
-  const int64_t rows = warp_rows(D, p.a.few);
-  if constexpr (D == 64) {
-    if (rows == 32) return launch_stream<D, BF16, 4>(ctx, p, page_size, stream);
-  }
-  return rows == 8 ? launch_stream<D, BF16, 1>(ctx, p, page_size, stream) : launch_stream<D, BF16, 2>(ctx, p, page_size, stream);
+  return warp_rows(p.a.few) == 8 ? launch_stream<D, BF16, 1>(ctx, p, page_size, stream) : launch_stream<D, BF16, 2>(ctx, p, page_size, stream);
 }
 
 }  // namespace
@@ -827,7 +823,7 @@ extern "C" int krn_b200_cache_attn(int type, const void* q, const void* k_pages,
   sp.a = p;
   sp.pieces = static_cast<int4*>(workspace);
   sp.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + pieces_bytes(batch));
-  sp.row_blocks = int(row_blocks(d, p.few));
+  sp.row_blocks = int(row_blocks(p.few));
   // The two paths run side by side: the tile kernel first, whose blocks take longest, and the stream on the SMs that it
   // leaves free.
   const bool tiled = int64_t(p.max_new) * p.group > p.few && tile_blocks(batch, rows, p.group, p.few) > 0;
