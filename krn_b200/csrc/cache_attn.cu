@@ -16,6 +16,7 @@ constexpr int kTile = 32;          // tokens a warp takes at a time
 constexpr int kMaxWarps = 12;      // of a block
 constexpr int kMaxBlocks = 160;    // bounds the workspace; a B200 has 148 SMs
 constexpr int kMaxBatch = 8192;    // tile counts of the batch sit in shared memory
+constexpr int kMaxGroup = kTileQ;  // q heads of a kv head: a query tile holds a token's rows whole
 constexpr float kLeastScale = 0x1p-110f;  // value scales below it are held against it
 
 // Partial results of the pieces of split segments, d + 4 floats (m, l, two unused, the unnormalised output) for each row.
@@ -722,6 +723,7 @@ extern "C" int64_t krn_b200_cache_attn_workspace_bytes(int64_t batch, int64_t ro
   using namespace krnb;
   if (batch <= 0 || rows <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0 || d <= 0 || max_new <= 0) return 16;
   const int64_t group = q_heads / kv_heads, most = max_new < rows ? max_new : rows;  // no request has more rows than there are
+  if (group > kMaxGroup) return 16;  // refused by the call
   return stream_workspace(batch, kv_heads, d, most, group) +
          (most * group <= few_limit(d) ? 0 : tile_workspace(batch, rows, q_heads, kv_heads, d, few_rows(d, most, group), max_context));
 }
@@ -751,9 +753,9 @@ extern "C" int krn_b200_cache_attn(int type, const void* q, const void* k_pages,
                 "max_new %lld, max_context %lld)", (long long)batch, (long long)rows, (long long)q_heads, (long long)kv_heads,
                 (long long)num_pages, (long long)max_pages, (long long)max_new, (long long)max_context);
   }
-  if (q_heads / kv_heads > 128) {
-    return fail(KRN_B200_ERR_UNSUPPORTED, "%lld q heads per kv head is not available: a tile holds 128 rows. Instead: repeat the "
-                "kv heads", (long long)(q_heads / kv_heads));
+  if (q_heads / kv_heads > kMaxGroup) {
+    return fail(KRN_B200_ERR_UNSUPPORTED, "%lld q heads per kv head is not available: a tile holds %d rows. Instead: repeat the "
+                "kv heads", (long long)(q_heads / kv_heads), kMaxGroup);
   }
   if (max_context > max_pages * page_size) {
     return fail(KRN_B200_ERR_INVALID_ARGUMENT, "max_context %lld does not fit %lld pages per sequence", (long long)max_context,
