@@ -301,8 +301,8 @@ def plan_cache(context_len: Any, new_len: Any, page_table: Any, free_pages: Any,
 
 
 def append_cache(k: Any, v: Any, slot_map: Any, runs: Any, cache: PagedCache, stream: Any = None) -> PagedCache:
-    """Quantise the step's keys and values [rows, kv heads, d] (bf16 or f16) into the cache at the plan's `slot_map` and
-    `runs`. A page's scale is a power of two, the least that holds its largest finite magnitude within e4m3's 448, and only
+    """Quantise the step's keys and values [rows, kv heads, d] (bf16 or f16) into the cache at the plan's `slot_map`, one slot
+    a row, and `runs`. A page's scale is a power of two, the least that holds its largest finite magnitude within e4m3's 448, and only
     grows while the page fills: the codes the page holds already are then rounded again to the new scale, which a power of
     two leaves exact but for values below e4m3's normal range. Rows of one page must be consecutive and in slot order, as
     `plan_cache` lays them out."""

@@ -427,9 +427,10 @@ def cache_append(k: Any, v: Any, slot_map: Any, runs: Any, k_pages: Any, v_pages
         raise ValueError(f"{at.feature}: k {tuple(k.shape)} and v {tuple(v.shape)} do not match a pool of {heads} heads of {d}")
     if k.dtype is not v.dtype:
         raise TypeError(f"{at.feature}: k and v must have the same element type")
-    slots, runs_len = at.vector("slot_map", slot_map, at.torch.int64, -1), at.vector("runs", runs, at.torch.int32, -1)
+    at.vector("slot_map", slot_map, at.torch.int64, rows[0])  # a row without a slot, or a slot without its row, would go unseen
+    runs_len = at.vector("runs", runs, at.torch.int32, -1)
     status = native.library().krn_b200_cache_append(
-        at.element(k), *addresses, min(rows[0], slots), runs_len, heads, d, page_size, num_pages,
+        at.element(k), *addresses, rows[0], runs_len, heads, d, page_size, num_pages,
         _pack_strides(*at.strides("k", k, False), *at.strides("v", v, False), *page_strides), at.stream(stream))
     native.check(status, at.feature)
 

@@ -5,7 +5,7 @@ from __future__ import annotations
 import pytest
 
 from krn_b200 import ops
-from krn_b200.runtime import native
+from krn_b200.runtime import calls, native
 from tests.test_cache_cpu import attention_status
 
 
@@ -23,3 +23,22 @@ def test_workspace_of_groups_that_the_call_refuses(group, max_new, max_context, 
 @pytest.mark.parametrize("group", [1, 64, 127, 128])
 def test_workspace_of_the_largest_groups(group) -> None:
     assert ops.cache_attention_workspace(3, 40, group, 1, 128, max_new=40, max_context=100000) > 1 << 20
+
+
+@pytest.fixture
+def host_tensors(monkeypatch):
+    """Lets the checks behind the calls see host tensors. For refusals only: a call that passes them would launch on them."""
+    monkeypatch.setattr(calls._Checks, "addresses", lambda self, names, tensors: [t.data_ptr() for t in tensors])
+    import torch
+
+    return torch
+
+
+@pytest.mark.parametrize("slots", [0, 3, 5, 80])
+def test_append_refuses_slots_and_rows_of_other_numbers(host_tensors, slots) -> None:
+    """Rows without a slot would not be written, slots without a row would keep what their page held."""
+    torch = host_tensors
+    cache = ops.PagedCache(*(torch.zeros(2, 16, 2, 64, dtype=torch.uint8) for _ in range(2)), *(torch.zeros(2, 2) for _ in range(2)))
+    x = torch.zeros(4, 2, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match=f"`slot_map` has {slots} elements, 4 expected"):
+        ops.append_cache(x, x, torch.zeros(slots, dtype=torch.int64), torch.zeros(4, dtype=torch.int32), cache)
