@@ -457,6 +457,8 @@ def cache_attention(q: Any, k_pages: Any, v_pages: Any, k_scale: Any, v_scale: A
     batch = at.vector("context_len", context_len, at.torch.int32, -1)
     at.vector("row_start", row_start, at.torch.int32, batch + 1)
     entries, pitch = at.table("page_table", page_table, batch)
+    if not workspace.is_contiguous():  # its size in bytes would not be the memory it has
+        raise ValueError(f"{at.feature}: `workspace` must be contiguous, got strides {tuple(workspace.stride())}")
     status = native.library().krn_b200_cache_attn(
         at.element(q), *addresses, batch, rows[0], rows[1], heads, d, page_size, num_pages, entries, pitch, max_new, max_context,
         _pack_strides(*at.strides("q", q, False), *at.strides("out", o, True), *page_strides), scale_log2, scratch,

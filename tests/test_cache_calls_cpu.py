@@ -42,3 +42,15 @@ def test_append_refuses_slots_and_rows_of_other_numbers(host_tensors, slots) -> 
     x = torch.zeros(4, 2, 64, dtype=torch.bfloat16)
     with pytest.raises(ValueError, match=f"`slot_map` has {slots} elements, 4 expected"):
         ops.append_cache(x, x, torch.zeros(slots, dtype=torch.int64), torch.zeros(4, dtype=torch.int32), cache)
+
+
+def test_attention_refuses_a_workspace_that_is_not_one_piece_of_memory(host_tensors) -> None:
+    """An expanded tensor counts more bytes than there are behind it, a strided one shares its bytes with another."""
+    torch = host_tensors
+    cache = ops.PagedCache(*(torch.zeros(2, 16, 2, 64, dtype=torch.uint8) for _ in range(2)), *(torch.zeros(2, 2) for _ in range(2)))
+    q = torch.zeros(4, 2, 64, dtype=torch.bfloat16)
+    table, lengths = torch.zeros(1, 2, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    for workspace in (torch.zeros(1, dtype=torch.uint8).expand(1 << 26), torch.zeros(64, 2, dtype=torch.uint8)[:, 0]):
+        with pytest.raises(ValueError, match="`workspace` must be contiguous"):
+            ops.cache_attention(q, cache, table, lengths, torch.zeros(2, dtype=torch.int32), torch.zeros_like(q), max_new=4,
+                                max_context=32, workspace=workspace)
