@@ -297,7 +297,7 @@ int64_t krn_b200_cache_runs(int64_t rows, int64_t batch, int64_t page_size);
  * holds is refused whole: state_out[2] has bit 0 set, nothing is taken, row_start and the contexts are those of a step
  * without new tokens; finished requests still give their pages back. Bit 1: more pages came back than the ring has room
  * for (a page was given back twice): none was accepted. A page id outside [0, num_pages) gets slot -1, and the status word
- * reports KRN_B200_ERR_DEVICE_INDEX. Outputs must not share memory with inputs (page_table and free_pages are both).
+ * reports KRN_B200_ERR_DEVICE_INDEX. What is written (page_table and free_pages too) must not share memory with anything else.
  * batch is at most 8192. */
 int krn_b200_cache_plan(const int32_t* context_len, const int32_t* new_len, int32_t* page_table, int32_t* free_pages,
                         const int64_t* pool_state, int32_t* context_out, int32_t* row_start, int64_t* slot_map, int32_t* runs,

@@ -415,6 +415,27 @@ int launch_append(const AppendParams& p, DeviceStatus* status, cudaStream_t stre
   return launch_dependent(cache_append_kernel<D, BF16, Threads>, dim3(unsigned(blocks)), 128, 0, stream, p, status);
 }
 
+struct Span {
+  const void* at;
+  int64_t bytes;
+};
+
+bool overlap(const Span& a, const Span& b) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(b.at);
+  return a.bytes > 0 && b.bytes > 0 && (x < y ? y - x < uint64_t(a.bytes) : x - y < uint64_t(b.bytes));
+}
+
+// Whether `a` meets one of `count` rows of `bytes` bytes, `pitch` bytes apart: the row that begins at or before it, or the
+// next one.
+bool overlaps_table(const Span& a, const void* table, int64_t count, int64_t bytes, int64_t pitch) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(table);
+  const int64_t row = x < y ? 0 : int64_t((x - y) / uint64_t(pitch));
+  for (int64_t i = row; i <= row + 1 && i < count; ++i) {
+    if (overlap(a, {static_cast<const char*>(table) + i * pitch, bytes})) return true;
+  }
+  return false;
+}
+
 bool page_size_ok(int64_t page_size) { return page_size >= 16 && page_size <= 256 && (page_size & (page_size - 1)) == 0; }
 
 int shift_of(int64_t page_size) {
@@ -466,9 +487,19 @@ extern "C" int krn_b200_cache_plan(const int32_t* context_len, const int32_t* ne
       (runs_len > 0 && runs == nullptr)) {
     return fail(KRN_B200_ERR_INVALID_ARGUMENT, "null tensor address");
   }
-  if (context_out == context_len || context_out == new_len || state_out == pool_state) {
-    return fail(KRN_B200_ERR_INVALID_ARGUMENT, "the plan's outputs must not share memory with its inputs: blocks read the "
-                "lengths while others write");
+  // what is written comes first: it shares no memory with anything before or behind it in the list
+  const Span spans[] = {{context_out, batch * 4}, {row_start, (batch + 1) * 4}, {slot_map, rows * 8}, {runs, runs_len * 4},
+                        {state_out, 24}, {free_pages, capacity * 4}, {context_len, batch * 4}, {new_len, batch * 4},
+                        {pool_state, 24}};
+  constexpr int kWritten = 6, kSpans = int(sizeof(spans) / sizeof(spans[0]));
+  bool shared = false;
+  for (int i = 0; i < kSpans; ++i) {
+    for (int j = i + 1; j < kSpans && i < kWritten; ++j) shared |= overlap(spans[i], spans[j]);
+    shared |= overlaps_table(spans[i], page_table, batch, max_pages * 4, table_pitch * 4);
+  }
+  if (shared) {
+    return fail(KRN_B200_ERR_INVALID_ARGUMENT, "the plan's outputs must not share memory with its inputs or with one another: "
+                "blocks read the lengths while others write");
   }
   DeviceContext* ctx = current_context();
   if (ctx == nullptr) return KRN_B200_ERR_CUDA;

@@ -294,7 +294,7 @@ def plan_cache(context_len: Any, new_len: Any, page_table: Any, free_pages: Any,
     live entries are positions `pool_state[0]` to `pool_state[1]` (modulo its length), and written into `page_table`
     [batch, entries]; the pages of finished requests go back to the ring's end and are handed out from the next step on.
     Fills `plan`, whose `context_len` and `pool_state` are the next step's inputs (with another plan: outputs never share
-    memory with inputs). A step that does not fit is refused whole: `plan.pool_state[2]` is then not 0 and no row has a
+    memory with inputs or with one another). A step that does not fit is refused whole: `plan.pool_state[2]` is then not 0 and no row has a
     slot."""
     calls.cache_plan(*_all_raw(context_len, new_len, page_table, free_pages, pool_state, *plan), page_size, num_pages, _stream(stream))
     return plan

@@ -6,7 +6,7 @@ import pytest
 
 from krn_b200 import ops
 from krn_b200.runtime import calls, native
-from tests.test_cache_cpu import attention_status
+from tests.test_cache_cpu import attention_status, plan_status
 
 
 @pytest.mark.parametrize("group", [129, 256, 1000])
@@ -54,3 +54,19 @@ def test_attention_refuses_a_workspace_that_is_not_one_piece_of_memory(host_tens
         with pytest.raises(ValueError, match="`workspace` must be contiguous"):
             ops.cache_attention(q, cache, table, lengths, torch.zeros(2, dtype=torch.int32), torch.zeros_like(q), max_new=4,
                                 max_context=32, workspace=workspace)
+
+
+# addresses that share nothing: 4 requests, 8 table entries at a pitch of 20, ring of 32, 16 rows, 9 runs
+APART = dict(context=0x1000, new=0x1010, table=0x2000, pitch=20, ring=0x3000, state=0x4000, context_out=0x5000, start=0x5010, slot=0x6000,
+             runs=0x6080, out=0x7000)
+
+
+@pytest.mark.parametrize("change", [
+    dict(context_out=0x100c), dict(context_out=0x0ff4), dict(start=0x101c), dict(out=0x4010), dict(out=0x3ff0),  # inputs
+    dict(slot=0x1008), dict(runs=0x0fe0), dict(ring=0x0f84), dict(ring=0x3f90),
+    dict(start=0x500c), dict(slot=0x6004), dict(runs=0x607c), dict(out=0x5008), dict(ring=0x6f90),                  # other outputs
+    dict(context_out=0x201c), dict(start=0x1ff0), dict(runs=0x204c), dict(out=0x2108), dict(context=0x20fc),      # rows of the table
+])
+def test_plan_refuses_memory_that_outputs_share(change) -> None:
+    assert plan_status(**(APART | change)) == native.ERR_INVALID_ARGUMENT
+    assert "share memory" in native.last_error()
