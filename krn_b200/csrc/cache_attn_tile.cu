@@ -9,10 +9,12 @@
 //   warps 4..7    turn a V tile into f16, times its pages' scales: a 16-bit P needs a 16-bit V;
 //   warps 8..15   softmax of the two query tiles, a thread per row; then the output.
 //
-// Q is split into e4m3 parts, each the rounded remainder of the ones before (a power-of-two factor puts the row's largest
-// magnitude into [128, 256)): two parts hold bf16's 8 significant bits exactly, three hold f16's 11, but for elements below
-// 2^-9 of the row's largest, where the remainder is under 2^-17 of it. S is the sum over the parts, and two e4m3 products
-// take the tensor cores as long as one of 16 bits, so K needs no conversion at all.
+// Q is split into 8-bit parts, each the rounded remainder of the ones before (a power-of-two factor puts the row's largest
+// magnitude into [128, 256)): e4m3, the last one e5m2, whose three significant bits are what is left of a value by then and whose
+// range goes seven octaves further down. Two parts hold bf16's 8 significant bits exactly down to 2^-13 of the row's largest
+// magnitude, three hold f16's 11 down to 2^-10; below, the remainder is at most 2^-21 of it (2^-17 with an e4m3 part in the last
+// place). S is the sum over the parts, and two 8-bit products take the tensor cores as long as one of 16 bits, so K needs no
+// conversion at all.
 //
 // A page's key scale multiplies its columns of S in f32, before the maximum. Its value scale multiplies V, relative to the
 // largest one that this block meets and times 2^7 (448 * 2^7 is within f16): for scales that are powers of two V stays
@@ -330,7 +332,7 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   }
   float top = scan(first_page + int(threadIdx.x), scan_page);
 
-  // ---- Q as e4m3 parts
+  // ---- Q as 8-bit parts
 #pragma unroll
   for (int i = 0; i < kQPasses; ++i) {
     const int row = i * kQRows + q_row, in_tile = row % kTileQ;
@@ -359,9 +361,12 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         uint16_t two;
-        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(two) : "f"(v[e].y), "f"(v[e].x));
-        code[e] = two;
-        if (part + 1 < Parts) {
+        if (part + 1 == Parts) {
+          asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(two) : "f"(v[e].y), "f"(v[e].x));
+          code[e] = two;
+        } else {
+          asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(two) : "f"(v[e].y), "f"(v[e].x));
+          code[e] = two;
           const uint32_t h = halves_of(two);
           const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&h));
           v[e].x -= back.x;
@@ -396,7 +401,8 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     };
     bool ok = true;
     if (warp == 0) {
-      const uint32_t idesc = umma_idesc(kFmtE4M3, kFmtE4M3, kTileQ, kTileKV, 0, 0);
+      constexpr uint32_t kIdesc = umma_idesc(kFmtE4M3, kFmtE4M3, kTileQ, kTileKV, 0, 0);
+      constexpr uint32_t kIdescLast = umma_idesc(kFmtE5M2, kFmtE4M3, kTileQ, kTileKV, 0, 0);  // Q's last part
       const uint64_t q_desc = umma_desc_kmajor_sw128(0);
       const uint64_t k_desc = D == 128 ? umma_desc_kmajor_sw128(0) : desc_kmajor_sw64(0);
       const uint32_t q_hi = uint32_t(q_desc >> 32), k_hi = uint32_t(k_desc >> 32);
@@ -421,7 +427,8 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
 #pragma unroll
               for (int ks = 0; ks < D / 32; ++ks) {
                 const uint32_t off = ((part / L::kPerRow) * L::kBlockBytes + (part % L::kPerRow) * D + ks * 32) >> 4;
-                umma_ss_halves<1, true>(tmem_base, qa + off, q_hi, ka + ks * 2, k_hi, idesc, part + ks > 0 ? 1u : 0u);
+                umma_ss_halves<1, true>(tmem_base, qa + off, q_hi, ka + ks * 2, k_hi, part + 1 == Parts ? kIdescLast : kIdesc,
+                                        part + ks > 0 ? 1u : 0u);
               }
             }
             umma_commit(s_full + 8 * t);

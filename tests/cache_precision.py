@@ -9,9 +9,9 @@ With u_j = exp(s_j - max s), L = sum u_j, w_j = u_j / L and o = sum w_j v_j, wha
 
 * eps_j: a weight is rounded to f16, whose half step is 2^-11 of it, and 2^-25 below f16's normal range, the largest being 1 at
   least: max(2^-11 u_j, 2^-25) / L. A page's value scale is rounded to f16 and so is its product with a value: 2^-11 w_j each;
-* delta_j: the score's error. The query is held to 2^-17 of its row's largest magnitude (e4m3 parts, see `query_parts`; the
-  streamed kernel's f16 copy is finer), which meets the key's d values with signs of their own; sums of 256 products in f32 are
-  taken as 2^-20 of sum |q_i k_i|;
+* delta_j: the score's error. The query is held to 2^-21 of its row's largest magnitude (e4m3 parts, the last of them e5m2:
+  see `query_parts`; the streamed kernel's f16 copy is finer), which meets the key's d values with signs of their own; sums of
+  256 products in f32 are taken as 2^-20 of sum |q_i k_i|;
 * rho: the result's own rounding, half a step of its type.
 
 A rounding within half a step h has a variance of h^2 / 3 at most. Adding variances gives E |e|^2 <= T^2 with
@@ -68,7 +68,7 @@ def expected(dtype, q, *cache, page, scale):
         v2 = (v * v).sum(axis=1)
         weight = np.where(seen, np.maximum(2.0 ** -11 * u, 2.0 ** -25), 0.0) / total
         squares = (weight ** 2 + 2 * (2.0 ** -11 * w) ** 2) @ v2 / 3
-        query = 2.0 ** -17 * np.abs(x).max(axis=1, keepdims=True) * np.sqrt((k * k).sum(axis=1))[None, :] / np.sqrt(3.0)
+        query = 2.0 ** -21 * np.abs(x).max(axis=1, keepdims=True) * np.sqrt((k * k).sum(axis=1))[None, :] / np.sqrt(3.0)
         delta = scale * (query + 2.0 ** -20 * (np.abs(x) @ np.abs(k).T))
         away = v2[None, :] - 2 * o @ v.T + (o * o).sum(axis=1, keepdims=True)  # |v_j - o|^2
         squares += ((w * delta) ** 2 * np.maximum(away, 0.0)).sum(axis=1)
@@ -91,24 +91,32 @@ def holds(worst, together) -> bool:
 # ---- a model of the tiled kernel's roundings, for the checks themselves -------------------------------------------------
 
 
-def query_parts(x, parts):
-    """The query as the sum of `parts` e4m3 parts, each the rounded remainder of those before."""
+def e5m2(x):
+    """x rounded to the nearest e5m2 value."""
+    _, e = np.frexp(x)
+    step = np.exp2(np.maximum(e - 1, -14) - 2.0)
+    return np.round(x / step) * step
+
+
+def query_parts(x, parts, last=e5m2):
+    """The query as the sum of `parts` 8-bit parts, each the rounded remainder of those before: e4m3, the last one e5m2."""
     size = np.abs(x).max(axis=-1, keepdims=True)
     factor = np.exp2(7 - np.floor(np.log2(np.where(size > 0, size, 1.0))))
     held = np.zeros_like(x)
     for part in range(parts):
-        held = held + DECODE[encode(x * factor - held)]
+        rest = x * factor - held
+        held = held + (last(rest) if part + 1 == parts else DECODE[encode(rest)])
     return held / factor
 
 
-def modelled(dtype, q, *cache, page, scale, parts=None, by=1.0):
-    """Attention with the tiled kernel's roundings (two of them together for the values); `parts` and `by` plant mistakes."""
+def modelled(dtype, q, *cache, page, scale, parts=None, last=e5m2, by=1.0):
+    """Attention with the tiled kernel's roundings (two of them together for the values); `parts`, `last` and `by` plant mistakes."""
     import torch
 
     parts = parts or (2 if dtype == "bfloat16" else 3)
     out = np.zeros(q.shape)
     for rows, h, x, k, v, seen in requests(q, *cache, page=page):
-        u, total = softmax(query_parts(x, parts) @ k.T * scale, seen)
+        u, total = softmax(query_parts(x, parts, last) @ k.T * scale, seen)
         weight = u.astype(np.float16).astype(np.float64)
         size = np.exp2(np.floor(np.log2(np.abs(v).max())) - 14)
         out[rows, h] = weight / total @ ((v / size).astype(np.float16).astype(np.float64) * size) * by

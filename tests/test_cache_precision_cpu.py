@@ -7,12 +7,13 @@ import math
 import numpy as np
 import pytest
 
+from krn_b200 import formats
 from tests import cache_precision as precision
 from tests import cache_reference as ref
 
 
-def case(rng, dtype, context, new, page, heads, group, d):
-    """Normally distributed queries, keys and values."""
+def case(rng, dtype, context, new, page, heads, group, d, outlier=0.0):
+    """Normally distributed queries, keys and values. outlier: octaves that a query's first element lies above the others, which the keys do not have."""
     import torch
 
     context, new = np.array(context), np.array(new)
@@ -23,6 +24,8 @@ def case(rng, dtype, context, new, page, heads, group, d):
     q = rng.standard_normal((int(new.sum()), heads * group, d))
     codes, scales = [], []
     x, y = (rng.standard_normal((len(order), page, heads, d)) for _ in range(2))
+    if outlier:
+        x[..., 0], q[..., 0] = 0.0, 2.0 ** outlier
     for z in (x, y):
         s = np.abs(z).max(axis=(1, 3)) / 448.0
         codes.append(ref.encode(z / s[:, None, :, None]))
@@ -32,8 +35,8 @@ def case(rng, dtype, context, new, page, heads, group, d):
     return q, (*codes, *scales, table, context.astype(np.int32), start)
 
 
-def judged(rng, dtype, shape, scale=1.0, **mistake):
-    q, cache = case(rng, dtype, *shape)
+def judged(rng, dtype, shape, scale=1.0, outlier=0.0, **mistake):
+    q, cache = case(rng, dtype, *shape, outlier=outlier)
     given = dict(page=shape[2], scale=scale / math.sqrt(shape[5]))
     return precision.judge(precision.modelled(dtype, q, *cache, **given, **mistake), *precision.expected(dtype, q, *cache, **given))
 
@@ -42,19 +45,29 @@ SHAPES = [([300], [20], 16, 1, 4, 128), ([1000, 90], [9, 30], 64, 2, 2, 64), ([4
 BOTH = pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
 
 
+def test_model_rounds_to_e5m2() -> None:
+    import torch
+
+    x = np.concatenate([np.random.default_rng(0).standard_normal(4000) * np.exp2(np.random.default_rng(1).integers(-18, 15, 4000)), [0.0]])
+    x = x.astype(np.float32).astype(np.float64)
+    np.testing.assert_array_equal(precision.e5m2(x), torch.from_numpy(x).float().to(torch.float8_e5m2).double().numpy())
+    table = [c for c in formats.E5M2.table if math.isfinite(c)]
+    np.testing.assert_array_equal(precision.e5m2(np.array(table)), table)
+
+
 @BOTH
 def test_query_parts(dtype) -> None:
-    """Exact down to 2^-9 of the row's largest magnitude, off by 2^-17 of it at most below."""
+    """Exact down to 2^-13 (bf16) and 2^-10 (f16) of the row's largest magnitude, off by 2^-21 of it at most below."""
     import torch
 
     rng = np.random.default_rng(2)
-    parts, exact = (2, 9) if dtype == "bfloat16" else (3, 6)
+    parts, exact = (2, 13) if dtype == "bfloat16" else (3, 10)
     x = rng.standard_normal((3000, 64)) * np.exp2(-rng.uniform(0, 22, (3000, 64)))
     x = torch.from_numpy(x).to(getattr(torch, dtype)).double().numpy()
     largest = np.abs(x).max(axis=1, keepdims=True)
     off = np.abs(precision.query_parts(x, parts) - x)
     assert not off[np.abs(x) >= largest * 2.0 ** -exact].any()
-    assert (off <= largest * 2.0 ** -17).all()
+    assert (off <= largest * 2.0 ** -21).all()
 
 
 @BOTH
@@ -62,6 +75,12 @@ def test_query_parts(dtype) -> None:
 @pytest.mark.parametrize("scale", [1.0, 3.0])
 def test_roundings_pass(dtype, shape, scale) -> None:
     assert precision.holds(*judged(np.random.default_rng(3), dtype, shape, scale))
+
+
+@BOTH
+@pytest.mark.parametrize("outlier", [4.0, 8.0, 10.0, 12.0])
+def test_roundings_pass_with_a_large_element(dtype, outlier) -> None:
+    assert precision.holds(*judged(np.random.default_rng(6), dtype, SHAPES[0], outlier=outlier))
 
 
 @BOTH
@@ -76,3 +95,10 @@ def test_a_lost_part_of_the_query_does_not_pass(dtype, shape) -> None:
 @pytest.mark.parametrize("shape", SHAPES)
 def test_a_fiftieth_does_not_pass(dtype, shape, by) -> None:
     assert not precision.holds(*judged(np.random.default_rng(8), dtype, shape, by=by))
+
+
+@BOTH
+@pytest.mark.parametrize("outlier", [10.0, 12.0])
+def test_parts_of_e4m3_alone_do_not_pass_with_a_large_element(dtype, outlier) -> None:
+    e4m3 = lambda x: ref.DECODE[ref.encode(x)]  # noqa: E731
+    assert not precision.holds(*judged(np.random.default_rng(11), dtype, SHAPES[0], outlier=outlier, last=e4m3, scale=4.0))

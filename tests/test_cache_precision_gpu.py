@@ -1,5 +1,5 @@
 """Attention over the paged 8-bit cache against its definition, held to what its roundings add up to (tests/cache_precision.py):
-keys streamed and tiled, split and joined."""
+queries kept whole, keys streamed and tiled, split and joined."""
 
 from __future__ import annotations
 
@@ -15,9 +15,9 @@ from tests.test_cache_precision_cpu import case
 pytestmark = pytest.mark.gpu
 
 
-def check(torch, rng, dtype, shape, scale=1.0):
+def check(torch, rng, dtype, shape, scale=1.0, **what):
     context, new, page, heads, group, d = shape
-    q, cache = case(rng, dtype, *shape)
+    q, cache = case(rng, dtype, *shape, **what)
     *pools, table, lengths, start = (torch.from_numpy(x).cuda() for x in cache)
     dq = torch.from_numpy(q).to(getattr(torch, dtype)).cuda()
     out = torch.full_like(dq, 7.0)
@@ -42,3 +42,11 @@ TILED = [([300], [20], 16, 1, 4, 128), ([1000, 90], [9, 40], 64, 2, 2, 64), ([50
 @pytest.mark.parametrize("scale", [1.0, 3.0])
 def test_attention_is_held_to_its_roundings(cuda, dtype, shape, scale) -> None:
     check(cuda, np.random.default_rng(70), dtype, shape, scale)
+
+
+@BOTH
+@pytest.mark.parametrize("shape", STREAMED + TILED)
+@pytest.mark.parametrize("outlier", [6.0, 10.0, 12.0])
+def test_attention_of_queries_with_a_large_element(cuda, dtype, shape, outlier) -> None:
+    """An element of the query far above the others, where the keys are zero: the scores are made of the others."""
+    check(cuda, np.random.default_rng(72), dtype, shape, 4.0, outlier=outlier)
