@@ -21,6 +21,12 @@
 // exact down to 2^-22 of the largest; any other scale costs two roundings of at most 2^-11, small beside bf16's 2^-8. f16
 // outputs would show them: there only the power of two in the scale goes to V, and the rest of it to P before its rounding.
 //
+// Weights are f16 in P, relative to a reference that the row's maximum may pass by 8 octaves before O is rescaled, and lifted by
+// 2^7 (f16 outputs 2^6), which l carries too, so that it leaves with the division: a weight has eleven bits down to 2^-21 (2^-20)
+// of the row's largest and vanishes at 2^-32 (2^-31). Without the lift, outputs made of small weights lost them: 2 % of a result
+// where one key of 8192 lies 21.7 octaves above the others and has a value of zero, 7 % with 131072 keys and 23.2 octaves. A
+// rescale at 7 / 6 / 5 octaves with a lift of 8 / 9 / 10 takes 1 / 2 / 4 % more time for a prompt of 8192 tokens.
+//
 // Tensor memory (512 columns): S (128) | P0 (64) | P1 (64) | O0 (128) | O1 (128). The two query tiles take turns in one S:
 // a softmax warp reads its scores into registers at once, so S is free for the other tile's scores long before the
 // exponentials are done, and each tile finds its next scores ready when it has handed over its weights. Two warps issue,
@@ -42,7 +48,8 @@ constexpr int kRegsFew = 40, kRegsMany = 216;  // warps 0..7 / 8..15, of the 128
 constexpr int kShortest = 4;              // key tiles of a share, at least
 constexpr float kStreamWork = 0.5f;       // a streamed request's 128 keys, in steps of a block: 25 us on all SMs for 36 requests
                                           // of 4096 tokens and 4 kv heads of 128, at 1.7 us a step
-constexpr float kRescaleThreshold = 8.0f;
+constexpr float kRescaleThreshold = 8.0f;           // octaves by which a row's maximum may pass its reference
+constexpr float kLift = 15.0f - kRescaleThreshold;  // octaves that weights are lifted by: the largest stay below f16's 2^16
 
 struct TileParams {
   CacheAttnParams a;
@@ -634,8 +641,9 @@ cache_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           }
         }
       }
-      // p = exp2(s * scale - m_ref), summed in f32 before the rounding to f16
-      const float2 shift2 = make_float2(-m_ref, -m_ref);
+      // p = 2^lift exp2(s * scale - m_ref), summed in f32 before the rounding to f16
+      constexpr float kOwnLift = BF16 ? kLift : kLift - 1.0f;  // f16: `rest` doubles a weight at most
+      const float2 shift2 = make_float2(kOwnLift - m_ref, kOwnLift - m_ref);
       float2 sum[4];
       uint32_t packed[2][32];
 #pragma unroll

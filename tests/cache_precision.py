@@ -7,8 +7,9 @@ With u_j = exp(s_j - max s), L = sum u_j, w_j = u_j / L and o = sum w_j v_j, wha
 
     e = sum_j eps_j v_j + sum_j w_j delta_j (v_j - o) + rho,
 
-* eps_j: a weight is rounded to f16, whose half step is 2^-11 of it, and 2^-25 below f16's normal range, the largest being 1 at
-  least: max(2^-11 u_j, 2^-25) / L. A page's value scale is rounded to f16 and so is its product with a value: 2^-11 w_j each;
+* eps_j: a weight is rounded to f16, whose half step is 2^-11 of it, and 2^-25 below f16's normal range. Weights are lifted by
+  `lift` octaves before that, the largest being 2^lift at least, so the error is max(2^-11 u_j, 2^-25 - lift) / L. A page's value
+  scale is rounded to f16 and so is its product with a value: 2^-11 w_j each;
 * delta_j: the score's error. The query is held to 2^-21 of its row's largest magnitude (e4m3 parts, the last of them e5m2:
   see `query_parts`; the streamed kernel's f16 copy is finer), which meets the key's d values with signs of their own; sums of
   256 products in f32 are taken as 2^-20 of sum |q_i k_i|;
@@ -16,7 +17,7 @@ With u_j = exp(s_j - max s), L = sum u_j, w_j = u_j / L and o = sum w_j v_j, wha
 
 A rounding within half a step h has a variance of h^2 / 3 at most. Adding variances gives E |e|^2 <= T^2 with
 
-    T^2 = sum_j |v_j|^2 (max(2^-11 u_j, 2^-25)^2 / L^2 + 2 (2^-11 w_j)^2) / 3 + sum_j w_j^2 delta_j^2 |v_j - o|^2 + sum h^2 / 3.
+    T^2 = sum_j |v_j|^2 (max(2^-11 u_j, 2^-25 - lift)^2 / L^2 + 2 (2^-11 w_j)^2) / 3 + sum_j w_j^2 delta_j^2 |v_j - o|^2 + sum h^2 / 3.
 
 A row where one key has all the weight has a single eps, which may reach sqrt(3) of its deviation; where many have, |e| lies close
 to T. So |e| <= 3 T for each row. Summed over the rows of a case, hundreds of errors, |e| <= 1.25 T."""
@@ -28,6 +29,7 @@ import numpy as np
 from tests.cache_reference import DECODE, encode
 
 ROW, ALL = 3.0, 1.25
+LIFT = {"bfloat16": 7, "float16": 6}       # of the tiled kernel; the streamed one lifts by 15
 HALF_STEP = {"bfloat16": 2.0 ** -8, "float16": 2.0 ** -11}
 LEAST_HALF_STEP = {"bfloat16": 0.0, "float16": 2.0 ** -25}
 
@@ -66,7 +68,7 @@ def expected(dtype, q, *cache, page, scale):
         w = u / total
         o = w @ v
         v2 = (v * v).sum(axis=1)
-        weight = np.where(seen, np.maximum(2.0 ** -11 * u, 2.0 ** -25), 0.0) / total
+        weight = np.where(seen, np.maximum(2.0 ** -11 * u, 2.0 ** (-25 - LIFT[dtype])), 0.0) / total
         squares = (weight ** 2 + 2 * (2.0 ** -11 * w) ** 2) @ v2 / 3
         query = 2.0 ** -21 * np.abs(x).max(axis=1, keepdims=True) * np.sqrt((k * k).sum(axis=1))[None, :] / np.sqrt(3.0)
         delta = scale * (query + 2.0 ** -20 * (np.abs(x) @ np.abs(k).T))
@@ -109,15 +111,17 @@ def query_parts(x, parts, last=e5m2):
     return held / factor
 
 
-def modelled(dtype, q, *cache, page, scale, parts=None, last=e5m2, by=1.0):
-    """Attention with the tiled kernel's roundings (two of them together for the values); `parts`, `last` and `by` plant mistakes."""
+def modelled(dtype, q, *cache, page, scale, parts=None, last=e5m2, lift=None, by=1.0):
+    """Attention with the tiled kernel's roundings (two of them together for the values); `parts`, `last`, `lift` and `by` plant
+    mistakes."""
     import torch
 
     parts = parts or (2 if dtype == "bfloat16" else 3)
+    lift = LIFT[dtype] if lift is None else lift
     out = np.zeros(q.shape)
     for rows, h, x, k, v, seen in requests(q, *cache, page=page):
         u, total = softmax(query_parts(x, parts, last) @ k.T * scale, seen)
-        weight = u.astype(np.float16).astype(np.float64)
+        weight = (u * 2.0 ** lift).astype(np.float16).astype(np.float64) / 2.0 ** lift
         size = np.exp2(np.floor(np.log2(np.abs(v).max())) - 14)
         out[rows, h] = weight / total @ ((v / size).astype(np.float16).astype(np.float64) * size) * by
     return torch.from_numpy(out).to(getattr(torch, dtype)).double().numpy()

@@ -1,5 +1,5 @@
 """Attention over the paged 8-bit cache against its definition, held to what its roundings add up to (tests/cache_precision.py):
-queries kept whole, keys streamed and tiled, split and joined."""
+queries kept whole, weights far below the largest, keys split and joined."""
 
 from __future__ import annotations
 
@@ -42,6 +42,14 @@ TILED = [([300], [20], 16, 1, 4, 128), ([1000, 90], [9, 40], 64, 2, 2, 64), ([50
 @pytest.mark.parametrize("scale", [1.0, 3.0])
 def test_attention_is_held_to_its_roundings(cuda, dtype, shape, scale) -> None:
     check(cuda, np.random.default_rng(70), dtype, shape, scale)
+
+
+@BOTH
+@pytest.mark.parametrize("shape", STREAMED + TILED)
+@pytest.mark.parametrize("sink", [12.0, 18.0, 22.0, 24.0])
+def test_attention_beside_a_sink(cuda, dtype, shape, sink) -> None:
+    """One key has nearly all the weight and a value of zero: the output is made of the small weights."""
+    check(cuda, np.random.default_rng(71), dtype, shape, sink=sink)
 
 
 @BOTH
