@@ -297,7 +297,9 @@ int64_t krn_b200_cache_runs(int64_t rows, int64_t batch, int64_t page_size);
  * holds is refused whole: state_out[2] has bit 0 set, nothing is taken, row_start and the contexts are those of a step
  * without new tokens; finished requests still give their pages back. Bit 1: more pages came back than the ring has room
  * for (a page was given back twice): none was accepted. A page id outside [0, num_pages) gets slot -1, and the status word
- * reports KRN_B200_ERR_DEVICE_INDEX. What is written (page_table and free_pages too) must not share memory with anything else.
+ * reports KRN_B200_ERR_DEVICE_INDEX. A request holds ceil(context_len / page_size) pages: a caller that cuts a context (drafted
+ * tokens that were not kept) puts the pages that it no longer reaches into the ring itself, at position `given`, and adds their
+ * number to it. What is written (page_table and free_pages too) must not share memory with anything else.
  * batch is at most 8192. */
 int krn_b200_cache_plan(const int32_t* context_len, const int32_t* new_len, int32_t* page_table, int32_t* free_pages,
                         const int64_t* pool_state, int32_t* context_out, int32_t* row_start, int64_t* slot_map, int32_t* runs,
@@ -327,8 +329,10 @@ int64_t krn_b200_cache_attn_workspace_bytes(int64_t batch, int64_t rows, int64_t
 /* Attention of packed query rows over the pool: row i of the n rows of a request with a context of c tokens (the new ones
  * included, already in the cache) stands at position c - n + i and sees keys 0 .. c - n + i.
  *   q, o         bf16 or f16 (`type`) [rows, q_heads, d]; q_heads % kv_heads == 0, at most 128 q heads per kv head
+ *                o may be q itself, else the two must not overlap
  *   row_start    int32 [batch + 1], context_len int32 [batch]: as krn_b200_cache_plan makes them. Contexts are clamped into
- *                [0, max_context]; rows of o behind row_start[batch] are left as they were; a row that sees no key gets zeros
+ *                [0, max_context] without a report: a request that outgrew the bound is answered as if it ended there. Rows of o
+ *                behind row_start[batch] are left as they were; a row that sees no key gets zeros
  *   max_new      no request has more rows than this; one that has, or whose rows are not all among q's, is not computed
  *                and reported
  *                (KRN_B200_ERR_DEVICE_INDEX). It chooses the kernels, as max_context does
@@ -340,6 +344,10 @@ int64_t krn_b200_cache_attn_workspace_bytes(int64_t batch, int64_t rows, int64_t
  *   strides      HOST array of 10 element strides: rows and heads of q, rows and heads of o (multiples of 8), then pages,
  *                tokens and heads of the K pool and of the V pool (multiples of 16)
  *   scale_log2   log2(e) * softmax scale
+ * What is rounded to fewer than 32 bits: a row of q is held whole, but for elements below 2^-10 of its largest, which may be off by
+ * 2^-21 of it; weights are f16, with eleven bits down to 2^-20 of the row's largest; for requests with many rows the product of a
+ * value and its page's scale is f16 too (scales 2^-22 below the request's largest lose bits). Scores, maxima, sums and outputs
+ * before their last rounding are f32.
  *   workspace    at least krn_b200_cache_attn_workspace_bytes(...) bytes, 16-byte aligned; needs no preparation. Calls that
  *                may overlap on the GPU need one each */
 int krn_b200_cache_attn(int type, const void* q, const void* k_pages, const void* v_pages, const float* k_scale,

@@ -294,8 +294,12 @@ def plan_cache(context_len: Any, new_len: Any, page_table: Any, free_pages: Any,
     live entries are positions `pool_state[0]` to `pool_state[1]` (modulo its length), and written into `page_table`
     [batch, entries]; the pages of finished requests go back to the ring's end and are handed out from the next step on.
     Fills `plan`, whose `context_len` and `pool_state` are the next step's inputs (with another plan: outputs never share
-    memory with inputs or with one another). A step that does not fit is refused whole: `plan.pool_state[2]` is then not 0 and no row has a
-    slot."""
+    memory with inputs or with one another). A step that does not fit is refused whole: `plan.pool_state[2]` is then not 0 and
+    no row has a slot.
+
+    A request holds the pages that its context reaches. Where tokens are taken back (drafts that were not kept), cut
+    `plan.context_len` and, before the next step, put the ids of the pages behind the last token into the ring at position
+    `plan.pool_state[1]`, which grows by their number."""
     calls.cache_plan(*_all_raw(context_len, new_len, page_table, free_pages, pool_state, *plan), page_size, num_pages, _stream(stream))
     return plan
 
@@ -323,8 +327,12 @@ def cache_attention(q: Any, cache: PagedCache, page_table: Any, context_len: Any
     (rows `row_start[b]` to `row_start[b + 1]`) stands at position `context_len[b]` - n + i and sees the keys up to it, its
     own included: one row a request for plain decoding, a few for drafted tokens, many for a prompt or a chunk of one, mixed
     in one call. `scale` defaults to 1/sqrt(d). `max_new` is the most rows any request has (one with more, or with rows
-    beyond q's, is not computed and reported), contexts are clamped to `max_context`. Rows that see no key get zeros; rows behind the last request are
-    left as they were."""
+    beyond q's, is not computed and reported). `max_context` is the longest context: a longer
+    one is cut to it without a report, as if the request ended there. Rows that see no key get zeros; rows behind the last request are left as
+    they were. `out` may be q itself.
+
+    Sums and softmax statistics are f32; weights are rounded to f16, where rows are many (prompts) a value times its page's scale
+    too, with eleven bits for weights down to 2^-20 of a row's largest and for values down to 2^-22 of the largest scale."""
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
     calls.cache_attention(*_all_raw(q, *cache, page_table, context_len, row_start, out), scale * _LOG2_E, max_new, max_context,
                           _raw(workspace), _stream(stream))

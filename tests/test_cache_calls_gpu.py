@@ -1,4 +1,4 @@
-"""Calls of the paged 8-bit cache that its documentation allows: memory side by side."""
+"""Calls of the paged 8-bit cache that its documentation allows: memory side by side, attention in place, contexts that are cut."""
 
 from __future__ import annotations
 
@@ -7,7 +7,7 @@ import pytest
 
 from krn_b200 import ops
 from tests import cache_reference as ref
-from tests.test_cache_gpu import plan_case
+from tests.test_cache_gpu import Server, attention_case, exact_check, plan_case, run_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -47,3 +47,55 @@ def test_plan_in_memory_side_by_side(cuda) -> None:
         np.testing.assert_array_equal(got.cpu().numpy(), expected)
     np.testing.assert_array_equal(context.cpu().numpy(), case["context"])
     np.testing.assert_array_equal(new.cpu().numpy(), case["new"])
+
+
+@pytest.mark.parametrize("dtype,context,new,page,heads,group,d", [
+    ("bfloat16", [300, 65], [1, 1], 64, 2, 4, 128), ("float16", [5000, 700], [3, 2], 16, 1, 4, 64),  # streamed, whole and in pieces
+    ("bfloat16", [500, 130], [200, 70], 32, 2, 4, 128), ("float16", [6000], [90], 64, 1, 4, 128),   # tiled, whole and in shares
+    ("bfloat16", [2900, 80, 700], [150, 1, 2], 64, 2, 4, 64)])                                      # side by side
+def test_attention_in_place(cuda, dtype, context, new, page, heads, group, d) -> None:
+    """`out` may be q itself: a row of q is read by those only that write it."""
+    torch = cuda
+    case = attention_case(torch, np.random.default_rng(61), dtype, context, new, page, heads, group, d)
+    want = run_attention(torch, case)
+    q, rows = case["q"].clone(), sum(new)
+    cache = ops.PagedCache(*(torch.from_numpy(x).cuda() for x in (*case["codes"], *case["scales"])))
+    table, lengths, start = (torch.from_numpy(case[x]).cuda() for x in ("table", "context", "start"))
+    given = dict(max_new=max(new), max_context=table.shape[1] * page)
+    workspace = torch.empty(ops.cache_attention_workspace(len(new), len(q), heads * group, heads, d, **given), dtype=torch.uint8,
+                            device="cuda")
+    ops.cache_attention(q, cache, table, lengths, start, q, workspace=workspace, **given)
+    assert torch.equal(q[:rows], want[:rows]) and torch.equal(q[rows:], case["q"][rows:])
+
+
+def test_drafted_tokens_that_are_not_kept(cuda) -> None:
+    """Each step brings up to four tokens a request, of which some are kept: the context is cut, and a page that it no longer
+    reaches goes back to the ring. No page is lost, and the outputs are those over the tokens that were kept."""
+    torch, rng = cuda, np.random.default_rng(62)
+    batch, page, pages = 5, 16, 40
+    server = Server(torch, batch, 60, page=page, pages=pages, width=6, max_new=20)
+    new = [20, 15, 1, 16, 3]
+    for step in range(14):
+        server.inputs(rng, new)
+        server.out.fill_(7.0)
+        plan = server.step()
+        assert plan.pool_state[2].item() == 0
+        assert plan.context_len.tolist() == [len(h) for h in server.held]
+        server.check(new)
+        exact_check(server, plan, new)
+        cut = [int(rng.integers(0, n)) if step else 0 for n in new]
+        for b, n in enumerate(cut):
+            del server.held[b][len(server.held[b]) - n:]
+        before, after = plan.context_len.clone(), plan.context_len - torch.tensor(cut, dtype=torch.int32, device="cuda")
+        left, right = (after + page - 1) // page, (before + page - 1) // page
+        entry = torch.arange(server.table.shape[1], device="cuda")
+        back = server.table[(entry >= left[:, None]) & (entry < right[:, None])]
+        given = plan.pool_state[1].item()
+        server.ring[(given + torch.arange(len(back), device="cuda")) % pages] = back
+        plan.pool_state[1] += len(back)
+        plan.context_len.copy_(after)
+        state = plan.pool_state.tolist()
+        free = server.ring[(state[0] + torch.arange(state[1] - state[0], device="cuda")) % pages].tolist()
+        held = server.table[entry < left[:, None]].tolist()
+        assert sorted(free + held) == list(range(pages))
+        new = [int(n) for n in rng.integers(1, 5, batch)]
