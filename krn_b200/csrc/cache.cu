@@ -6,15 +6,10 @@
 //
 // The reference has neither (its roadmap lists paged attention); the rounding to e4m3 is its narrowing rule, nearest even
 // and saturating (src/krn/compiler/narrow.py:94-105).
-#include "host.cuh"
-
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
+#include "cache.cuh"
 
 namespace krnb {
 namespace {
-
-constexpr int kErrDeviceIndex = 6;  // mirrors KRN_B200_ERR_DEVICE_INDEX in include/krn_b200.h
 
 enum Site { kSitePlanPage = 41, kSiteAppendSlot = 42 };
 
@@ -234,15 +229,6 @@ struct AppendParams {
   int rows, runs_len, heads, page_shift, num_pages;
 };
 
-template <bool BF16>
-__device__ __forceinline__ float2 unpack(uint32_t w) {
-  if constexpr (BF16) {
-    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-  } else {
-    return __half22float2(*reinterpret_cast<const __half2*>(&w));
-  }
-}
-
 // The least power of two 2^k, k >= kLeastExponent, with a <= 448 * 2^k, read off a's exponent: 448 = 1.75 * 2^8.
 __device__ __forceinline__ float scale_of(float a) {
   const uint32_t bits = __float_as_uint(a);
@@ -258,8 +244,7 @@ __device__ __forceinline__ uint32_t codes_of(float2 v) {
 }
 
 __device__ __forceinline__ uint32_t rescale_two(uint32_t codes, float ratio) {
-  uint32_t h;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(uint16_t(codes)));
+  const uint32_t h = halves_of(codes);
   const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h));
   uint16_t r;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(v.y * ratio), "f"(v.x * ratio));
@@ -436,14 +421,6 @@ bool overlaps_table(const Span& a, const void* table, int64_t count, int64_t byt
   return false;
 }
 
-bool page_size_ok(int64_t page_size) { return page_size >= 16 && page_size <= 256 && (page_size & (page_size - 1)) == 0; }
-
-int shift_of(int64_t page_size) {
-  int s = 0;
-  while ((int64_t(1) << s) < page_size) ++s;
-  return s;
-}
-
 }  // namespace
 }  // namespace krnb
 
@@ -460,10 +437,7 @@ extern "C" int krn_b200_cache_plan(const int32_t* context_len, const int32_t* ne
                                    int64_t table_pitch, int64_t capacity, int64_t page_size, int64_t num_pages, int64_t rows,
                                    int64_t runs_len, void* stream_handle) {
   using namespace krnb;
-  if (!page_size_ok(page_size)) {
-    return fail(KRN_B200_ERR_UNSUPPORTED, "page size %lld is not available on sm_100a: pages are 16, 32, 64, 128 or 256 tokens. "
-                "Instead: use one of them", (long long)page_size);
-  }
+  if (int rc = check_page_size(page_size)) return rc;
   if (batch < 0 || max_pages <= 0 || capacity <= 0 || num_pages <= 0 || rows < 0 || table_pitch < max_pages) {
     return fail(KRN_B200_ERR_INVALID_ARGUMENT, "bad extents (batch %lld, %lld table entries at pitch %lld, ring of %lld, %lld "
                 "pages, %lld rows)", (long long)batch, (long long)max_pages, (long long)table_pitch, (long long)capacity,
@@ -535,10 +509,7 @@ extern "C" int krn_b200_cache_append(int type, const void* k, const void* v, con
     return fail(KRN_B200_ERR_UNSUPPORTED, "head dimension %lld is not available on sm_100a. Instead: use d = 64 or d = 128",
                 (long long)d);
   }
-  if (!page_size_ok(page_size)) {
-    return fail(KRN_B200_ERR_UNSUPPORTED, "page size %lld is not available on sm_100a: pages are 16, 32, 64, 128 or 256 tokens. "
-                "Instead: use one of them", (long long)page_size);
-  }
+  if (int rc = check_page_size(page_size)) return rc;
   if (rows < 0 || runs_len < 0 || heads <= 0 || num_pages <= 0) {
     return fail(KRN_B200_ERR_INVALID_ARGUMENT, "bad extents (%lld rows, %lld runs, %lld heads, %lld pages)", (long long)rows,
                 (long long)runs_len, (long long)heads, (long long)num_pages);

@@ -43,12 +43,6 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
   return y;
 }
 
-__device__ __forceinline__ uint4 ld_shared_16(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
-  return v;
-}
-
 __device__ __forceinline__ uint2 ld_shared_8(uint32_t addr) {
   uint2 v;
   asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
@@ -748,10 +742,7 @@ extern "C" int krn_b200_cache_attn(int type, const void* q, const void* k_pages,
     return fail(KRN_B200_ERR_UNSUPPORTED, "head dimension %lld is not available on sm_100a: tiles are built from 64- or 128-byte "
                 "rows. Instead: use d = 64 or d = 128", (long long)d);
   }
-  if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1)) != 0) {
-    return fail(KRN_B200_ERR_UNSUPPORTED, "page size %lld is not available on sm_100a: pages are 16, 32, 64, 128 or 256 tokens. "
-                "Instead: use one of them", (long long)page_size);
-  }
+  if (int rc = check_page_size(page_size)) return rc;
   if (batch < 0 || rows < 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0 || num_pages <= 0 || max_pages <= 0 ||
       table_pitch < max_pages || max_new <= 0 || max_context <= 0) {
     return fail(KRN_B200_ERR_INVALID_ARGUMENT, "bad extents (batch %lld, %lld rows, %lld / %lld heads, %lld pages, table of %lld, "
@@ -817,8 +808,7 @@ extern "C" int krn_b200_cache_attn(int type, const void* q, const void* k_pages,
   p.kv_heads = int(kv_heads);
   p.group = int(q_heads / kv_heads);
   p.group_inverse = uint32_t((65536 + p.group - 1) / p.group);
-  p.page_shift = 0;
-  while ((int64_t(1) << p.page_shift) < page_size) ++p.page_shift;
+  p.page_shift = shift_of(page_size);
   p.num_pages = int(num_pages);
   p.max_new = int(max_new < rows ? max_new : rows);
   p.max_context = int(max_context);

@@ -1,14 +1,9 @@
-// What the two paths of attention over the paged 8-bit cache share: arguments, the rule that parts them, conversions.
+// What the two paths of attention over the paged 8-bit cache share: arguments and the rule that parts them.
 #pragma once
 
-#include "host.cuh"
-
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
+#include "cache.cuh"
 
 namespace krnb {
-
-constexpr int kErrDeviceIndex = 6;  // mirrors KRN_B200_ERR_DEVICE_INDEX in include/krn_b200.h
 
 enum CacheAttnSite { kSitePage = 51, kSiteRows = 52, kSiteTile = 53, kSiteKeys = 54, kSiteValues = 55,
                      kSiteScores = 57, kSiteWeights = 58, kSiteOutput = 59, kSiteRoom = 60, kSiteRead = 61 };
@@ -56,20 +51,10 @@ __device__ __forceinline__ void report_rows(const CacheAttnParams& a, int b, Dev
   if (n > 0 && !rows_ok(a, b, n)) report_failure(status, kErrDeviceIndex, kSiteRows, uint32_t(n));
 }
 
-template <bool BF16>
-__device__ __forceinline__ float2 unpack(uint32_t w) {
-  if constexpr (BF16) {
-    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-  } else {
-    return __half22float2(*reinterpret_cast<const __half2*>(&w));
-  }
-}
-
-// Two e4m3 codes in the low 16 bits, as f16.
-__device__ __forceinline__ uint32_t halves_of(uint32_t codes) {
-  uint32_t h2;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"(uint16_t(codes)));
-  return h2;
+__device__ __forceinline__ uint4 ld_shared_16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
 }
 
 // Boxes of `tokens` rows of one head.

@@ -96,12 +96,6 @@ __device__ __forceinline__ void st_shared_16(uint32_t addr, uint32_t x, uint32_t
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 
-__device__ __forceinline__ uint4 ld_shared_16(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
-  return v;
-}
-
 // One lane polls, the warp follows. (For a warp that has others of its kind to wait with, polling with every lane is faster:
 // 3170 against 3450 cycles a key tile for the softmax warps.)
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, DeviceStatus* status, int site) {
