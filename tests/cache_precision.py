@@ -83,7 +83,7 @@ def judge(got, out, spread):
     """(the worst row's error in units of T, all rows' error in units of all rows' T)."""
     wrong = np.sqrt(((got - out) ** 2).sum(axis=2))
     rows = np.divide(wrong, spread, out=np.where(wrong > 0, np.inf, 0.0), where=spread > 0)
-    return float(rows.max()), float(np.sqrt((wrong ** 2).sum() / (spread ** 2).sum()))
+    return float(rows.max()), float(np.linalg.norm(wrong) / (np.linalg.norm(spread) or 1.0))  # outputs may be zeros, exactly
 
 
 def holds(worst, together) -> bool:
