@@ -33,10 +33,12 @@
 // because one sets the pace: it spends over a hundred cycles on each wait and about 80 on each product, 2030 cycles a query
 // and key tile in a trace, of which the tensor cores work 1024.
 //
-// A step of both query tiles takes 3170 cycles, of which the exponentials need 2048 (16 a cycle) and the products, whose
-// operands come out of shared memory at its full rate beside the conversion's traffic, about 2580. A prompt of 8192 tokens, 8 kv
-// heads of 128, group 4: 500 to 530 us = 1040 TFLOP/s under the power limit. Two threads a query row (16 softmax warps of 104
-// registers) shorten the chain of a query tile and not the step: 72 against 69 us for four chunks of 512 over 4096 tokens.
+// A step of both query tiles takes 3170 cycles in a trace, of which the exponentials need 2048 (16 a cycle) and the products about
+// 2580 from issue to end, 2048 by arithmetic; counters have tensor cores and special-function units busy for 60 % of the active
+// cycles each, the set-up of a block included. That the products wait for shared memory, which they read beside the conversion's
+// traffic, is a guess. A prompt of 8192 tokens, 8 kv heads of 128, group 4: 465 to 545 us by the box = 1180 to 1010 TFLOP/s under the
+// power limit; f16, with a product and a half for the scores: 510 to 550; d = 64: 410 to 460. Two threads a query row (16 softmax
+// warps of 104 registers) shorten the chain of a query tile and not the step: 72 against 69 us for four chunks of 512 over 4096.
 #include "cache_attn.cuh"
 
 namespace krnb {
