@@ -79,7 +79,7 @@ def expected(dtype, q, *cache, page, scale):
     return out, spread
 
 
-def judge(got, out, spread):
+def deviations(got, out, spread):
     """(the worst row's error in units of T, all rows' error in units of all rows' T)."""
     wrong = np.sqrt(((got - out) ** 2).sum(axis=2))
     rows = np.divide(wrong, spread, out=np.where(wrong > 0, np.inf, 0.0), where=spread > 0)

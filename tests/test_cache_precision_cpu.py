@@ -44,10 +44,10 @@ def case(rng, dtype, context, new, page, heads, group, d, sink=0.0, outlier=0.0)
     return q, (*codes, *scales, table, context.astype(np.int32), start)
 
 
-def judged(rng, dtype, shape, scale=1.0, sink=0.0, outlier=0.0, **mistake):
+def deviations(rng, dtype, shape, scale=1.0, sink=0.0, outlier=0.0, **mistake):
     q, cache = case(rng, dtype, *shape, sink=sink, outlier=outlier)
     given = dict(page=shape[2], scale=scale / math.sqrt(shape[5]))
-    return precision.judge(precision.modelled(dtype, q, *cache, **given, **mistake), *precision.expected(dtype, q, *cache, **given))
+    return precision.deviations(precision.modelled(dtype, q, *cache, **given, **mistake), *precision.expected(dtype, q, *cache, **given))
 
 
 SHAPES = [([300], [20], 16, 1, 4, 128), ([1000, 90], [9, 30], 64, 2, 2, 64), ([4000], [12], 64, 1, 4, 128)]
@@ -83,46 +83,46 @@ def test_query_parts(dtype) -> None:
 @pytest.mark.parametrize("shape", SHAPES)
 @pytest.mark.parametrize("scale", [1.0, 3.0])
 def test_roundings_pass(dtype, shape, scale) -> None:
-    assert precision.holds(*judged(np.random.default_rng(3), dtype, shape, scale))
+    assert precision.holds(*deviations(np.random.default_rng(3), dtype, shape, scale))
 
 
 @BOTH
 @pytest.mark.parametrize("sink", [12.0, 18.0, 22.0, 24.0])
 def test_roundings_pass_beside_a_sink(dtype, sink) -> None:
-    assert precision.holds(*judged(np.random.default_rng(4), dtype, SHAPES[0], sink=sink))
-    assert precision.holds(*judged(np.random.default_rng(5), dtype, SHAPES[2], sink=sink))
+    assert precision.holds(*deviations(np.random.default_rng(4), dtype, SHAPES[0], sink=sink))
+    assert precision.holds(*deviations(np.random.default_rng(5), dtype, SHAPES[2], sink=sink))
 
 
 @BOTH
 @pytest.mark.parametrize("outlier", [4.0, 8.0, 10.0, 12.0])
 def test_roundings_pass_with_a_large_element(dtype, outlier) -> None:
-    assert precision.holds(*judged(np.random.default_rng(6), dtype, SHAPES[0], outlier=outlier))
+    assert precision.holds(*deviations(np.random.default_rng(6), dtype, SHAPES[0], outlier=outlier))
 
 
 @BOTH
 @pytest.mark.parametrize("shape", SHAPES)
 def test_a_lost_part_of_the_query_does_not_pass(dtype, shape) -> None:
     parts = 1 if dtype == "bfloat16" else 2
-    assert not precision.holds(*judged(np.random.default_rng(7), dtype, shape, 3.0, parts=parts))
+    assert not precision.holds(*deviations(np.random.default_rng(7), dtype, shape, 3.0, parts=parts))
 
 
 @BOTH
 @pytest.mark.parametrize("by", [1.02, 0.98])
 @pytest.mark.parametrize("shape", SHAPES)
 def test_a_fiftieth_does_not_pass(dtype, shape, by) -> None:
-    assert not precision.holds(*judged(np.random.default_rng(8), dtype, shape, by=by))
+    assert not precision.holds(*deviations(np.random.default_rng(8), dtype, shape, by=by))
 
 
 @BOTH
 @pytest.mark.parametrize("sink", [22.0, 24.0])
 def test_weights_that_are_not_lifted_do_not_pass_beside_a_sink(dtype, sink) -> None:
     """Of 22 octaves on: at 18 they lose less than bf16's own rounding."""
-    assert not precision.holds(*judged(np.random.default_rng(9), dtype, SHAPES[0], sink=sink, lift=0))
-    assert not precision.holds(*judged(np.random.default_rng(10), dtype, SHAPES[2], sink=sink, lift=0))
+    assert not precision.holds(*deviations(np.random.default_rng(9), dtype, SHAPES[0], sink=sink, lift=0))
+    assert not precision.holds(*deviations(np.random.default_rng(10), dtype, SHAPES[2], sink=sink, lift=0))
 
 
 @BOTH
 @pytest.mark.parametrize("outlier", [10.0, 12.0])
 def test_parts_of_e4m3_alone_do_not_pass_with_a_large_element(dtype, outlier) -> None:
     e4m3 = lambda x: ref.DECODE[ref.encode(x)]  # noqa: E731
-    assert not precision.holds(*judged(np.random.default_rng(11), dtype, SHAPES[0], outlier=outlier, last=e4m3, scale=4.0))
+    assert not precision.holds(*deviations(np.random.default_rng(11), dtype, SHAPES[0], outlier=outlier, last=e4m3, scale=4.0))

@@ -26,7 +26,7 @@ def check(torch, rng, dtype, shape, scale=1.0, **what):
                             dtype=torch.uint8, device="cuda")
     ops.cache_attention(dq, ops.PagedCache(*pools), table, lengths, start, out, max_new=most, max_context=longest, workspace=workspace,
                         scale=scale)
-    worst, together = precision.judge(out.double().cpu().numpy(), *precision.expected(dtype, q, *cache, page=page, scale=scale))
+    worst, together = precision.deviations(out.double().cpu().numpy(), *precision.expected(dtype, q, *cache, page=page, scale=scale))
     assert precision.holds(worst, together), (worst, together)
 
 
